@@ -590,6 +590,60 @@ int spc_sparse_conv_products(spc_stream_t stream, int dtype, const void* x, cons
                              int64_t n_in, int64_t cin, int64_t cout, const spc_conv_epilogue* epi,
                              void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------
+ * Row layer norm of any width and its gradient.
+ * ------------------------------------------------------------------------ */
+
+/* What a layer norm applies behind (x - mean) / sqrt(var + eps): the optional
+ * gamma / beta [c] in param_dtype, then the optional modulation by the row's
+ * batch item b, * (1 + scale[b]) + shift[b] (scale and shift together: n_batch
+ * rows of c values in mod_dtype, mod_stride elements apart, so the halves of
+ * one Linear's output serve as they are), then SiLU if silu is set.  Rows of
+ * item b are [offsets[b], offsets[b+1]) (offsets: device int64 [n_batch + 1],
+ * ascending, 8-byte aligned; NULL with n_batch 1: every row; only with scale
+ * and shift).  Rows before offsets[0] and from offsets[n_batch] on belong to
+ * no item: their outputs are zeros and they add to no sum.  Pointers need
+ * only their elements' alignment; rows whose width, strides and addresses are
+ * multiples of 16 bytes are the fast ones. */
+typedef struct {
+    const void* gamma;
+    const void* beta;
+    const void* scale;
+    const void* shift;
+    const int64_t* offsets;
+    int64_t n_batch;
+    int64_t mod_stride;
+    int32_t param_dtype;
+    int32_t mod_dtype;
+    int32_t silu;
+    float eps;
+} spc_layer_norm_params;
+
+/* y [n, c] (contiguous, dtype) from x [n, c] whose rows are x_stride elements
+ * apart; mean and biased variance over a row in F32 (mean first, then the
+ * squares of the differences), every step in F32, rounded once to dtype.
+ * (spc_layernorm_silu rounds between the steps, as the block's tensors do.)
+ * stats: f32 [n, 2], (mean, 1 / sqrt(var + eps)) of every row of an item, for
+ * the gradient, or NULL.  y may be x when x_stride is c.  c <= 8192, n_batch
+ * <= 65535. */
+int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
+                   int64_t c, const spc_layer_norm_params* params, void* y, float* stats);
+
+/* The gradient of spc_layer_norm for dy [n, c] (rows dy_stride apart), from x
+ * and the stats it wrote: dx [n, c] (contiguous, dtype; NULL: not wanted; dx
+ * may be dy or x when its stride is c), dgamma / dbeta [c] in param_dtype,
+ * dscale / dshift [n_batch, c] (contiguous) in mod_dtype (NULL: not wanted).
+ * The roundings of the forward pass are not differentiated.  Sums over rows
+ * are F32 over chunks of rows, then over the chunks, in a fixed order: equal
+ * calls give equal bits.  workspace: spc_layer_norm_backward_workspace_bytes
+ * (n_batch 1 without a modulation), 4-byte aligned, needed for the parameters'
+ * gradients only. */
+size_t spc_layer_norm_backward_workspace_bytes(int dtype, int64_t n, int64_t c, int64_t n_batch);
+int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
+                            const void* x, int64_t x_stride, const float* stats, int64_t n, int64_t c,
+                            const spc_layer_norm_params* params, void* dx, void* dgamma, void* dbeta,
+                            void* dscale, void* dshift, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -117,8 +117,22 @@ def lib() -> ctypes.CDLL:
     L.spc_conv_products_workspace_bytes.argtypes = [_I64, _I64]
     L.spc_sparse_conv_products.argtypes = [_P, _INT, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                            ctypes.POINTER(ConvEpilogue), _P, _SZ]
+    L.spc_layer_norm.argtypes = [_P, _INT, _P, _I64, _I64, _I64, ctypes.POINTER(LayerNormParams), _P,
+                                 _P]
+    L.spc_layer_norm_backward_workspace_bytes.restype = _SZ
+    L.spc_layer_norm_backward_workspace_bytes.argtypes = [_INT, _I64, _I64, _I64]
+    L.spc_layer_norm_backward.argtypes = [_P, _INT, _P, _I64, _P, _I64, _P, _I64, _I64,
+                                          ctypes.POINTER(LayerNormParams), _P, _P, _P, _P, _P, _P,
+                                          _SZ]
     _lib = L
     return L
+
+
+class LayerNormParams(ctypes.Structure):
+    """spc_layer_norm_params (include/sam3d_spconv_amd.h)."""
+    _fields_ = [("gamma", _P), ("beta", _P), ("scale", _P), ("shift", _P), ("offsets", _P),
+                ("n_batch", _I64), ("mod_stride", _I64), ("param_dtype", _I32),
+                ("mod_dtype", _I32), ("silu", _I32), ("eps", ctypes.c_float)]
 
 
 EPI_NONE, EPI_RESIDUAL, EPI_NORM_MOD_SILU = 0, 1, 2
@@ -152,6 +166,33 @@ def _need_gpu(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("sparse-conv kernels run on the GPU only; got a CPU tensor")
+
+
+def _one_device(x: torch.Tensor, *others) -> torch.device:
+    """x's device; every tensor of the call has to be there."""
+    for t in (x, *others):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"tensors on {x.device} and {t.device} in one call")
+    _need_gpu(x)
+    return x.device
+
+
+class _on:
+    """Makes `device` the current one for a call (its default stream is the
+    null stream, which means the current device's)."""
+
+    def __init__(self, device: torch.device):
+        self._device, self._was = device.index, None
+
+    def __enter__(self):
+        was = torch.cuda.current_device()
+        if was != self._device:
+            self._was = was
+            torch.cuda.set_device(self._device)
+
+    def __exit__(self, *exc):
+        if self._was is not None:
+            torch.cuda.set_device(self._was)
 
 
 def dtype_code(dt: torch.dtype) -> int:
@@ -716,6 +757,134 @@ def layernorm_mod_silu(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor
                                       scale.shape[0], _ptr(out))
     _check("spc_layernorm_mod_silu", st)
     return out
+
+
+def _strided_rows(x: torch.Tensor, name: str):
+    """(x, row stride): x [n, c] as it is when its rows are contiguous."""
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be [n, c], got {tuple(x.shape)}")
+    n, c = x.shape
+    if c > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, (x.stride(0) if n > 1 else c)
+
+
+def _param_pair(a, b, width: int, names: str):
+    """Two parameter tensors [width] (or None) in one dtype the kernels read."""
+    for t in (a, b):
+        if t is not None and t.shape != (width,):
+            raise ValueError(f"{names} must be [{width}], got {tuple(t.shape)}")
+    dts = {t.dtype for t in (a, b) if t is not None}
+    if len(dts) > 1 or not dts <= {torch.float32, torch.float16, torch.bfloat16}:
+        a, b = (None if t is None else t.to(torch.float32) for t in (a, b))
+    return tuple(None if t is None else t.contiguous() for t in (a, b))
+
+
+def _layer_norm_params(x, weight, bias, eps, scale, shift, offsets, silu):
+    """(spc_layer_norm_params, tensors it points into, items)."""
+    c = x.shape[1]
+    weight, bias = _param_pair(weight, bias, c, "weight / bias")
+    p = LayerNormParams(silu=int(bool(silu)), eps=float(eps), n_batch=1)
+    for t, name in ((weight, "gamma"), (bias, "beta")):
+        if t is not None:
+            setattr(p, name, t.data_ptr())
+            p.param_dtype = dtype_code(t.dtype)
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift go together")
+    if scale is None:
+        if offsets is not None:
+            raise ValueError("offsets need scale and shift")
+        return p, (weight, bias)
+    if scale.dim() != 2 or scale.shape != shift.shape or scale.shape[1] != c:
+        raise ValueError(f"scale / shift must be [n_batch, {c}], got {tuple(scale.shape)} and "
+                         f"{tuple(shift.shape)}")
+    if scale.dtype != shift.dtype or scale.dtype not in (torch.float32, torch.float16,
+                                                         torch.bfloat16):
+        scale, shift = scale.to(torch.float32), shift.to(torch.float32)
+    if scale.stride() != shift.stride() or (c > 1 and scale.stride(1) != 1):
+        scale, shift = scale.contiguous(), shift.contiguous()
+    nb = scale.shape[0]
+    if offsets is not None:
+        if offsets.dtype != torch.int64 or offsets.shape != (nb + 1,):
+            raise ValueError(f"offsets must be int64 [{nb + 1}]")
+        offsets = offsets.contiguous()
+        p.offsets = offsets.data_ptr()
+    elif nb != 1:
+        raise ValueError("more than one item needs offsets")
+    p.scale, p.shift, p.n_batch = scale.data_ptr(), shift.data_ptr(), nb
+    p.mod_stride, p.mod_dtype = scale.stride(0), dtype_code(scale.dtype)
+    return p, (weight, bias, scale, shift, offsets)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-6, *,
+               scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
+               offsets: torch.Tensor | None = None, silu: bool = False,
+               return_stats: bool = False, out: torch.Tensor | None = None):
+    """LayerNorm over the rows of x [n, c] (spc_layer_norm; c <= 8192, rows at
+    any stride): the affine weight / bias [c] if given, then * (1 + scale[b])
+    + shift[b] by the row's batch item b if given ([n_batch, c]; rows of item b
+    are offsets[b] .. offsets[b+1], device int64, rows of no item come out as
+    zeros; without offsets one item of all rows), then SiLU.  F32 throughout,
+    rounded once to x's dtype.  return_stats: also f32 [n, 2] (mean, 1 / sqrt(
+    var + eps)), what layer_norm_backward reads.  out: contiguous [n, c] (may
+    be x).  Not recorded for gradients: SparseLayerNorm32 is."""
+    dev = _one_device(x, weight, bias, scale, shift, offsets, out)
+    dt = dtype_code(x.dtype)
+    x, stride = _strided_rows(x, "x")
+    n, c = x.shape
+    p, keep = _layer_norm_params(x, weight, bias, eps, scale, shift, offsets, silu)
+    if out is None:
+        out = torch.empty((n, c), dtype=x.dtype, device=dev)
+    elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of x's shape and dtype")
+    # rows of no item have no statistics: zeros, not what the memory held
+    stats = None if not return_stats else (torch.empty if offsets is None else torch.zeros)(
+        (n, 2), dtype=torch.float32, device=dev)
+    with _on(dev):
+        st = lib().spc_layer_norm(_stream(dev), dt, _ptr(x), stride, n, c, ctypes.byref(p),
+                                  _ptr(out), _ptr(stats))
+    _check("spc_layer_norm", st)
+    del keep  # alive until queued
+    return (out, stats) if return_stats else out
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor,
+                        weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                        scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
+                        offsets: torch.Tensor | None = None, silu: bool = False,
+                        need=(True, True, True, True, True)):
+    """(dx, dweight, dbias, dscale, dshift) of layer_norm for the gradient dy
+    [n, c] of its output, from x and the stats of that call with the same
+    arguments (spc_layer_norm_backward).  None for parameters that are not
+    given or whose place in `need` is false; a gradient has its parameter's
+    dtype.  Deterministic."""
+    dev = _one_device(x, dy, stats, weight, bias, scale, shift, offsets)
+    dt = dtype_code(x.dtype)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and dtype")
+    x, xs = _strided_rows(x, "x")
+    dy, dys = _strided_rows(dy, "dy")
+    n, c = x.shape
+    if stats.shape != (n, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError("stats must be contiguous float32 [n, 2]")
+    p, keep = _layer_norm_params(x, weight, bias, 0.0, scale, shift, offsets, silu)
+    params = keep[:4] if scale is not None else (*keep, None, None)
+    dx = torch.empty((n, c), dtype=x.dtype, device=dev) if need[0] else None
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None and k else None
+             for t, k in zip(params, need[1:])]
+    ws, nbytes = None, 0
+    with _on(dev):
+        if any(g is not None for g in grads):
+            nbytes = lib().spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
+            ws = _workspace(nbytes, dev)
+        st = lib().spc_layer_norm_backward(_stream(dev), dt, _ptr(dy), dys, _ptr(x), xs, _ptr(stats),
+                                           n, c, ctypes.byref(p), _ptr(dx), *map(_ptr, grads),
+                                           _ptr(ws), nbytes)
+    _check("spc_layer_norm_backward", st)
+    given = (weight, bias, scale, shift)
+    return (dx, *(g if g is None or g.dtype == t.dtype else g.to(t.dtype)
+                  for g, t in zip(grads, given)))
 
 
 def spconv_f16_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,

@@ -43,7 +43,7 @@ __all__ = [
     "SparseTensor", "SparseTensorData", "sparse_batch_broadcast", "sparse_batch_op",
     "sparse_cat", "sparse_unbind", "SparseConv3d", "SparseInverseConv3d",
     "SparseDownsample", "SparseUpsample", "SparseSubdivide", "SparseLinear",
-    "SparseGroupNorm32", "SparseSiLU",
+    "SparseGroupNorm32", "SparseLayerNorm32", "SparseSiLU",
 ]
 
 BACKEND = "hip"
@@ -836,6 +836,13 @@ def batch_offsets(x: SparseTensor) -> torch.Tensor:
     return torch.tensor(offs, dtype=torch.int64).to(x.feats.device, non_blocking=True)
 
 
+def _item_offsets(x: SparseTensor) -> torch.Tensor:
+    """batch_offsets(x), kept with the coordinates per layout (a copy from the
+    host, which a captured graph cannot hold)."""
+    rows = tuple((sl.start, sl.stop) for sl in x.layout)
+    return x.data.cached(("offsets", rows), lambda c: batch_offsets(x))
+
+
 def max_item_rows(x: SparseTensor) -> int:
     """Rows of the largest batch item (from the layout, no device sync)."""
     return max((sl.stop - sl.start for sl in x.layout), default=0)
@@ -852,6 +859,58 @@ class SparseGroupNorm32(nn.GroupNorm):
         return input.replace(nat.group_norm_silu(input.feats, batch_offsets(input), self.num_groups,
                                                  self.weight, self.bias, self.eps, silu=False,
                                                  max_rows=max_item_rows(input)))
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """nat.layer_norm with its gradient (x's statistics are kept, the
+    normalised rows are not)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, scale, shift, offsets, eps, silu):
+        y, stats = nat.layer_norm(x, weight, bias, eps, scale=scale, shift=shift, offsets=offsets,
+                                  silu=silu, return_stats=True)
+        ctx.save_for_backward(x, stats, weight, bias, scale, shift, offsets)
+        ctx.silu = silu
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, stats, weight, bias, scale, shift, offsets = ctx.saved_tensors
+        grads = nat.layer_norm_backward(dy, x, stats, weight, bias, scale=scale, shift=shift,
+                                        offsets=offsets, silu=ctx.silu,
+                                        need=ctx.needs_input_grad[:5])
+        return (*grads, None, None, None)
+
+
+class SparseLayerNorm32(nn.LayerNorm):
+    """LayerNorm over the channels of each row, computed in F32 and rounded
+    once to the feature dtype, with its gradient (spc_layer_norm,
+    spc_layer_norm_backward).  forward(x, scale, shift, silu) also applies a
+    modulation * (1 + scale[b]) + shift[b] by the row's batch item
+    ([x.shape[0], channels], for instance the halves of a Linear's output) and
+    SiLU in the same pass; gradients go to the feats, weight, bias, scale and
+    shift.  Once differentiable."""
+
+    def __init__(self, channels: int, eps: float = 1e-6, elementwise_affine: bool = True,
+                 bias: bool = True):
+        super().__init__(channels, eps, elementwise_affine, bias)
+
+    def forward(self, input: SparseTensor, scale: Optional[torch.Tensor] = None,
+                shift: Optional[torch.Tensor] = None, silu: bool = False) -> SparseTensor:
+        x, offsets = input.feats, None
+        if x.dim() != 2 or x.shape[1] != self.normalized_shape[0]:
+            raise ValueError(f"expected feats [N, {self.normalized_shape[0]}], got {tuple(x.shape)}")
+        if scale is not None:
+            if scale.dim() != 2 or scale.shape[0] != input.shape[0]:
+                raise ValueError(f"scale / shift must be [{input.shape[0]}, {x.shape[1]}], got "
+                                 f"{tuple(scale.shape)}")
+            offsets = _item_offsets(input)
+        args = (x, self.weight, self.bias, scale, shift)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+            return input.replace(_LayerNormFn.apply(*args, offsets, self.eps, silu))
+        return input.replace(nat.layer_norm(x, self.weight, self.bias, self.eps, scale=scale,
+                                            shift=shift, offsets=offsets, silu=silu))
 
 
 class SparseSiLU(nn.SiLU):
