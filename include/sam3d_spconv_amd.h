@@ -644,6 +644,44 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
                             const spc_layer_norm_params* params, void* dx, void* dgamma, void* dbeta,
                             void* dscale, void* dshift, void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------
+ * Linear products with 4-bit weights (a quantised checkpoint's modulation and
+ * skip Linears).
+ * ------------------------------------------------------------------------ */
+
+/* Q4_0 blocks (GGUF tensor type 2): 32 weights along the input features in 18
+ * bytes, an f16 scale d and 16 bytes of four-bit q (byte j: weight j in its
+ * low, weight 16 + j in its high half), w = d (q - 8).
+ * spc_q4_0_quantize: n F32 weights (a multiple of 32, 16-byte aligned) to
+ * blocks; d = (the value of largest magnitude) / -8 rounded to f16, q =
+ * floor(w / d + 8.5) held to 0..15. */
+int spc_q4_0_quantize(spc_stream_t stream, const float* w, int64_t n, uint8_t* blocks);
+
+/* The blocks of a Linear's weight [out_features, in_features] (in_features a
+ * multiple of 32) laid out for the products: transpose 0 for spc_linear_q4_0,
+ * 1 for spc_linear_q4_0_input_grad.  packed: spc_linear_q4_0_packed_bytes
+ * (0: unsupported shape), 16-byte aligned; once per weight. */
+size_t spc_linear_q4_0_packed_bytes(int64_t out_features, int64_t in_features, int transpose);
+int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out_features,
+                         int64_t in_features, int transpose, void* packed);
+
+/* y [m, out_features] = x W^T + bias for x [m, in_features] in dtype (rows
+ * x_stride elements apart), y contiguous in dtype, bias [out_features] in
+ * bias_dtype or NULL.  Weights enter exactly, sums are F32, one rounding to
+ * dtype at the end; a row with an infinity or NaN comes out as NaNs.  m up to
+ * 1,048,560; made for few rows (the weights' bytes are the cost up to some
+ * 64), right for any.  16-byte aligned rows are the fast ones. */
+int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
+                    const void* packed, int64_t out_features, int64_t in_features, const void* bias,
+                    int bias_dtype, void* y);
+
+/* dx [m, in_features] = dy W for dy [m, out_features] (rows dy_stride apart),
+ * packed with transpose 1.  dy times a scale enters with 16 bits (F32 rows:
+ * 24), sums are F32. */
+int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
+                               int64_t m, const void* packed, int64_t out_features,
+                               int64_t in_features, void* dx);
+
 #ifdef __cplusplus
 }
 #endif

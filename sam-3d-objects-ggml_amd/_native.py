@@ -124,6 +124,12 @@ def lib() -> ctypes.CDLL:
     L.spc_layer_norm_backward.argtypes = [_P, _INT, _P, _I64, _P, _I64, _P, _I64, _I64,
                                           ctypes.POINTER(LayerNormParams), _P, _P, _P, _P, _P, _P,
                                           _SZ]
+    L.spc_q4_0_quantize.argtypes = [_P, _P, _I64, _P]
+    L.spc_linear_q4_0_packed_bytes.restype = _SZ
+    L.spc_linear_q4_0_packed_bytes.argtypes = [_I64, _I64, _INT]
+    L.spc_linear_q4_0_pack.argtypes = [_P, _P, _I64, _I64, _INT, _P]
+    L.spc_linear_q4_0.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P, _INT, _P]
+    L.spc_linear_q4_0_input_grad.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P]
     _lib = L
     return L
 
@@ -937,6 +943,96 @@ def q8_0_dequant(blocks: torch.Tensor, dtype: torch.dtype = torch.float32) -> to
                                 _ptr(out))
     _check("spc_q8_0_dequant", st)
     return out
+
+
+def q4_0_quantize(w: torch.Tensor) -> torch.Tensor:
+    """float32 weights (numel % 32 == 0, blocks along the last, contiguous
+    dimension) -> Q4_0 blocks (uint8, 18 bytes per block; spc_q4_0_quantize)."""
+    dev = _one_device(w)
+    w = w.detach().to(torch.float32).contiguous()
+    n = w.numel()
+    out = torch.empty(n // 32 * 18, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        st = lib().spc_q4_0_quantize(_stream(dev), _ptr(w), n, _ptr(out))
+    _check("spc_q4_0_quantize", st)
+    return out
+
+
+@dataclass
+class Q4Weights:
+    """A Linear's Q4_0 weight laid out for the products (spc_linear_q4_0_pack)."""
+
+    data: torch.Tensor  # uint8
+    out_features: int
+    in_features: int
+    transpose: bool     # for linear_q4_0_input_grad
+
+
+def pack_q4_0(blocks: torch.Tensor, *, out_features: int, in_features: int,
+              transpose: bool = False) -> Q4Weights:
+    """Q4_0 blocks (uint8, rows [out_features, in_features / 32 * 18]) -> the
+    operand of linear_q4_0, or with transpose of linear_q4_0_input_grad."""
+    dev = _one_device(blocks)
+    L = lib()
+    nbytes = L.spc_linear_q4_0_packed_bytes(int(out_features), int(in_features), int(bool(transpose)))
+    if not nbytes:
+        raise ValueError(f"unsupported shape [{out_features}, {in_features}]: in_features must be a "
+                         "multiple of 32")
+    if blocks.dtype != torch.uint8 or blocks.numel() != out_features * (in_features // 32) * 18:
+        raise ValueError(f"expected {out_features * (in_features // 32) * 18} Q4_0 bytes (uint8)")
+    blocks = blocks.contiguous()
+    data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        st = L.spc_linear_q4_0_pack(_stream(dev), _ptr(blocks), int(out_features), int(in_features),
+                                    int(bool(transpose)), _ptr(data))
+    _check("spc_linear_q4_0_pack", st)
+    return Q4Weights(data, int(out_features), int(in_features), bool(transpose))
+
+
+def linear_q4_0(x: torch.Tensor, w: Q4Weights, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """x [m, in_features] times Q4_0 weights, + bias (spc_linear_q4_0): y [m,
+    out_features] in x's dtype.  Not recorded for gradients: Q4Linear is."""
+    dev = _one_device(x, w.data, bias)
+    dt = dtype_code(x.dtype)
+    if w.transpose:
+        raise ValueError("these weights are packed for linear_q4_0_input_grad")
+    x, stride = _strided_rows(x, "x")
+    if x.shape[1] != w.in_features:
+        raise ValueError(f"expected x [m, {w.in_features}], got {tuple(x.shape)}")
+    bdt = F32
+    if bias is not None:
+        if bias.shape != (w.out_features,):
+            raise ValueError(f"bias must be [{w.out_features}], got {tuple(bias.shape)}")
+        if bias.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            bias = bias.to(torch.float32)
+        bias, bdt = bias.contiguous(), dtype_code(bias.dtype)
+    m = x.shape[0]
+    y = torch.empty((m, w.out_features), dtype=x.dtype, device=dev)
+    with _on(dev):
+        st = lib().spc_linear_q4_0(_stream(dev), dt, _ptr(x), stride, m, _ptr(w.data), w.out_features,
+                                   w.in_features, _ptr(bias), bdt, _ptr(y))
+    _check("spc_linear_q4_0", st)
+    return y
+
+
+def linear_q4_0_input_grad(dy: torch.Tensor, w: Q4Weights) -> torch.Tensor:
+    """dy [m, out_features] times the weights (packed with transpose): the
+    gradient [m, in_features] of linear_q4_0's x, in dy's dtype
+    (spc_linear_q4_0_input_grad)."""
+    dev = _one_device(dy, w.data)
+    dt = dtype_code(dy.dtype)
+    if not w.transpose:
+        raise ValueError("these weights are not packed with transpose")
+    dy, stride = _strided_rows(dy, "dy")
+    if dy.shape[1] != w.out_features:
+        raise ValueError(f"expected dy [m, {w.out_features}], got {tuple(dy.shape)}")
+    m = dy.shape[0]
+    dx = torch.empty((m, w.in_features), dtype=dy.dtype, device=dev)
+    with _on(dev):
+        st = lib().spc_linear_q4_0_input_grad(_stream(dev), dt, _ptr(dy), stride, m, _ptr(w.data),
+                                              w.out_features, w.in_features, _ptr(dx))
+    _check("spc_linear_q4_0_input_grad", st)
+    return dx
 
 
 def scatter_mean(features: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor,

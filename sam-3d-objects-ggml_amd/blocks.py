@@ -26,7 +26,7 @@ import torch
 import torch.nn as nn
 
 from . import _native as nat
-from .sparse import (SparseConv3d, SparseDownsample, SparseGroupNorm32, SparseLinear, SparseSiLU,
+from .sparse import (Q4Linear, SparseConv3d, SparseDownsample, SparseGroupNorm32, SparseLinear, SparseSiLU,
                      SparseSubdivide, SparseTensor, SparseUpsample, _LONG_PLAN, _pad32, _run,
                      _subm_map, batch_offsets, max_item_rows)
 
@@ -74,8 +74,9 @@ class SparseResBlock3d(nn.Module):
         self.conv2 = SparseConv3d(self.out_channels, self.out_channels, 3)
         for p in self.conv2.parameters():  # zero_module (modules/utils.py)
             p.detach().zero_()
-        self.emb_layers = nn.Sequential(nn.SiLU(), nn.Linear(emb_channels, 2 * self.out_channels,
-                                                             bias=True))
+        # nn.Linear, or Q4_0 blocks once loaded (Q4Linear.load_q4_0)
+        self.emb_layers = nn.Sequential(nn.SiLU(), Q4Linear(emb_channels, 2 * self.out_channels,
+                                                            bias=True))
         self.skip_connection = (SparseLinear(channels, self.out_channels)
                                 if channels != self.out_channels else nn.Identity())
         self.updown = None

@@ -28,6 +28,10 @@ layouts the converter writes:
 F32 / F16 / BF16 tensors become the module's parameters; Q8_0 tensors
 (34-byte blocks along ne[0]) are attached as blocks (`load_q8_0`), which the
 bf16 path dequantises inside the GEMM.
+
+`load_linear` does the same for a Linear (ne = (in, out)): Q4_0 tensors
+(18-byte blocks along ne[0]) are attached to a Q4Linear / SparseLinear as
+blocks (`load_q4_0`), which its product reads as they are.
 """
 from __future__ import annotations
 
@@ -285,6 +289,43 @@ def load_sparse_conv(module, reader: GGUFReader, name: str, layout: Optional[str
             if conv.bias is None:
                 raise GGUFError(f"{bname}: the conv was built without a bias")
             conv.bias.copy_(b.to(conv.bias.dtype))
+
+
+def load_linear(module, reader: GGUFReader, name: str) -> None:
+    """Loads `<name>.weight` (ne = (in, out)) and `<name>.bias` when present
+    into an nn.Linear, for instance a residual block's `emb_layers[1]`
+    (`<block>.emb_layers.1`).  F32 / F16 / BF16 tensors become the parameter,
+    Q8_0 tensors are dequantised into it once; Q4_0 tensors stay blocks and
+    need a Q4Linear (or SparseLinear)."""
+    import torch
+
+    n_in, n_out = module.in_features, module.out_features
+    wname, bname = name + ".weight", name + ".bias"
+    t = reader.info(wname)
+    if tuple(t.ne) != (n_in, n_out):
+        raise GGUFError(f"{wname}: ggml ne {t.ne}, the Linear has ({n_in}, {n_out})")
+    b = None
+    if bname in reader:
+        b = _float_tensor(reader, bname)
+        if module.bias is None:
+            raise GGUFError(f"{bname}: the Linear was built without a bias")
+        if b.numel() != n_out:
+            raise GGUFError(f"{bname}: {b.numel()} values, the Linear has {n_out} outputs")
+    with torch.no_grad():
+        if t.ggml_type == GGML_Q4_0:
+            if not hasattr(module, "load_q4_0"):
+                raise GGUFError(f"{wname}: Q4_0 needs a Q4Linear or SparseLinear")
+            module.load_q4_0(torch.from_numpy(np.array(reader.raw(wname))))
+        else:
+            if t.ggml_type == GGML_Q8_0:
+                w = _dequant_q8_0_cpu(torch.from_numpy(np.array(reader.raw(wname))))
+            else:
+                w = _float_tensor(reader, wname)
+            module.weight.copy_(w.reshape(n_out, n_in).to(module.weight.dtype))
+            if hasattr(module, "drop_q4_0"):
+                module.drop_q4_0()
+        if b is not None:
+            module.bias.copy_(b.to(module.bias.dtype))
 
 
 def _dequant_q8_0_cpu(blocks):

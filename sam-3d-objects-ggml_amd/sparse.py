@@ -43,7 +43,7 @@ __all__ = [
     "SparseTensor", "SparseTensorData", "sparse_batch_broadcast", "sparse_batch_op",
     "sparse_cat", "sparse_unbind", "SparseConv3d", "SparseInverseConv3d",
     "SparseDownsample", "SparseUpsample", "SparseSubdivide", "SparseLinear",
-    "SparseGroupNorm32", "SparseLayerNorm32", "SparseSiLU",
+    "Q4Linear", "SparseGroupNorm32", "SparseLayerNorm32", "SparseSiLU",
 ]
 
 BACKEND = "hip"
@@ -818,7 +818,93 @@ class SparseInverseConv3d(nn.Module, _ConvCore):
 # ---------------------------------------------------------------------------
 # spatial ops (SP/spatial.py)
 # ---------------------------------------------------------------------------
-class SparseLinear(nn.Linear):
+class _Q4LinearFn(torch.autograd.Function):
+    """nat.linear_q4_0 with the gradients of the rows and the bias."""
+
+    @staticmethod
+    def forward(ctx, x, bias, linear):
+        ctx.linear, ctx.blocks = linear, linear._q4
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return nat.linear_q4_0(x, linear._q4_operand(x.device, False), bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        dx = db = None
+        if ctx.needs_input_grad[0]:
+            if ctx.linear._q4 is not ctx.blocks:
+                raise RuntimeError("the Q4_0 weights were replaced between forward and backward")
+            dx = nat.linear_q4_0_input_grad(dy, ctx.linear._q4_operand(dy.device, True))
+        if ctx.needs_input_grad[1]:
+            db = dy.float().sum(0).to(ctx.bias_dtype)
+        return dx, db, None
+
+
+class Q4Linear(nn.Linear):
+    """nn.Linear whose weight may be Q4_0 blocks (load_q4_0, quantize_q4_0):
+    without them nn.Linear itself; with them spc_linear_q4_0 on GPU rows of
+    any leading dimensions, with gradients for the rows (through the frozen
+    blocks, spc_linear_q4_0_input_grad) and the bias.  The float parameter is
+    left as is and then neither read nor given a gradient; the blocks are not
+    part of the state dict.  Made for few rows: a modulation, a token."""
+
+    _q4 = None          # blocks, uint8 [out_features, in_features / 32 * 18]
+
+    def load_q4_0(self, blocks: torch.Tensor) -> None:
+        """Uses Q4_0 blocks (uint8, 18 bytes each, rows [out_features,
+        in_features]) as the weight."""
+        n = self.out_features * self.in_features
+        if self.in_features % 32:
+            raise ValueError(f"Q4_0 needs in_features a multiple of 32, not {self.in_features}")
+        if blocks.dtype != torch.uint8 or blocks.numel() != n // 32 * 18:
+            raise ValueError(f"expected {n // 32 * 18} Q4_0 bytes (uint8) for this Linear")
+        # a copy: the packed operands are made from it when first needed
+        self._q4 = blocks.detach().clone(memory_format=torch.contiguous_format)
+        self._q4_packed = {}
+
+    def quantize_q4_0(self) -> torch.Tensor:
+        """Quantises the current weight on the GPU, uses it, and returns the
+        blocks."""
+        if self.in_features % 32:
+            raise ValueError(f"Q4_0 needs in_features a multiple of 32, not {self.in_features}")
+        blocks = nat.q4_0_quantize(self.weight)
+        self.load_q4_0(blocks)
+        return blocks
+
+    def drop_q4_0(self) -> None:
+        """Back to the float parameter."""
+        self._q4, self._q4_packed = None, {}
+
+    def _q4_operand(self, device, transpose: bool) -> nat.Q4Weights:
+        key = (device, transpose)
+        w = self._q4_packed.get(key)
+        if w is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Q4_0 weights are laid out by the first call (and the first "
+                                   "backward pass): run one before capturing a graph")
+            w = nat.pack_q4_0(self._q4.to(device), out_features=self.out_features,
+                              in_features=self.in_features, transpose=transpose)
+            # once: later calls may come on other streams
+            torch.cuda.current_stream(device).synchronize()
+            self._q4_packed[key] = w
+        return w
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if self._q4 is None:
+            return super().forward(input)
+        nat._need_gpu(input)
+        if input.shape[-1] != self.in_features:
+            raise ValueError(f"expected input [..., {self.in_features}], got {tuple(input.shape)}")
+        x = input.reshape(-1, self.in_features)
+        if torch.is_grad_enabled() and (x.requires_grad or
+                                        (self.bias is not None and self.bias.requires_grad)):
+            y = _Q4LinearFn.apply(x, self.bias, self)
+        else:
+            y = nat.linear_q4_0(x, self._q4_operand(x.device, False), self.bias)
+        return y.view(*input.shape[:-1], self.out_features)
+
+
+class SparseLinear(Q4Linear):
     """nn.Linear over the feats of a SparseTensor (SP/linear.py:9-15)."""
 
     def forward(self, input: SparseTensor) -> SparseTensor:

@@ -1,0 +1,129 @@
+"""Q4_0 Linears: host checks, module bookkeeping and the GGUF loader (no GPU)."""
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+from gguf_writer import bf16_bytes, f32_bytes, write_gguf
+from q4_reference import dequant, gradient, parts, product, random_blocks
+
+
+def test_reference_products():
+    b = random_blocks(5, 64, 0)
+    d, q = parts(b)
+    assert q.min() >= -8 and q.max() <= 7
+    raw = b.numpy()
+    assert float(q[2, 33]) == float(raw[2, 1, 2 + 1] & 15) - 8       # byte 1, low half
+    assert float(q[2, 32 + 17]) == float(raw[2, 1, 2 + 1] >> 4) - 8  # byte 1, high half
+    w = dequant(b)
+    assert torch.equal(w[2, 32:64], q[2, 32:64] * d[2, 1])
+    x, dy = torch.randn(3, 64), torch.randn(3, 5)
+    torch.testing.assert_close(product(x, b)[0], x.double() @ w.t())
+    torch.testing.assert_close(gradient(dy, b)[0], dy.double() @ w)
+
+
+def test_host_validation(spc):
+    nat = spc._native
+    L = nat.lib()
+    fake = 1 << 12
+    assert L.spc_linear_q4_0_packed_bytes(16, 128, 0) == 16 * 128 * 18 // 32
+    assert L.spc_linear_q4_0_packed_bytes(17, 32, 0) == 2 * 16 * 128 * 18 // 32   # padded tiles
+    assert L.spc_linear_q4_0_packed_bytes(128, 32, 1) == 128 * 32 * 18 // 32
+    for out, inp in ((0, 32), (1, 0), (1, 33), (-1, 32), (1 << 31, 32), (1, 1 << 31)):
+        assert L.spc_linear_q4_0_packed_bytes(out, inp, 0) == 0
+        assert L.spc_linear_q4_0_pack(None, fake, out, inp, 0, fake) == nat.BAD_SHAPE
+    assert L.spc_linear_q4_0_pack(None, None, 16, 32, 0, fake) == nat.BAD_ARG
+    assert L.spc_linear_q4_0_pack(None, fake, 16, 32, 0, fake + 8) == nat.BAD_ARG
+    assert L.spc_q4_0_quantize(None, fake, 33, fake) == nat.BAD_ARG
+    assert L.spc_q4_0_quantize(None, fake + 4, 32, fake) == nat.BAD_ARG
+    assert L.spc_q4_0_quantize(None, None, 0, None) == nat.OK
+
+    def run(fn, dtype=nat.BF16, x=fake, stride=64, m=1, w=fake, y=fake):
+        if fn == "y":
+            return L.spc_linear_q4_0(None, dtype, x, stride, m, w, 64, 64, None, 0, y)
+        return L.spc_linear_q4_0_input_grad(None, dtype, x, stride, m, w, 64, 64, y)
+
+    for fn in ("y", "dx"):
+        assert run(fn, m=0, x=None, w=None, y=None) == nat.OK
+        assert run(fn, m=-1) == nat.BAD_SHAPE and run(fn, m=65535 * 16 + 1) == nat.BAD_SHAPE
+        assert run(fn, stride=-1) == nat.BAD_SHAPE
+        assert run(fn, dtype=nat.Q8_0) == nat.BAD_ARG
+        assert run(fn, x=None) == nat.BAD_ARG and run(fn, w=None) == nat.BAD_ARG
+        assert run(fn, x=fake + 1) == nat.BAD_ARG and run(fn, w=fake + 8) == nat.BAD_ARG
+        assert run(fn, y=fake + 2, dtype=nat.F32) == nat.BAD_ARG
+        assert b"misaligned" in L.spc_last_error()
+    assert L.spc_linear_q4_0(None, nat.BF16, fake, 64, 1, fake, 64, 64, fake, 9, fake) == nat.BAD_ARG
+    assert L.spc_linear_q4_0(None, nat.BF16, fake, 64, 1, fake, 64, 64, fake + 2, 0, fake) == nat.BAD_ARG
+
+
+def test_cpu_tensors_are_rejected(spc):
+    nat = spc._native
+    b = random_blocks(20, 64, 1)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        nat.pack_q4_0(b, out_features=20, in_features=64)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        nat.q4_0_quantize(torch.zeros(32))
+
+
+def test_module_is_nn_linear_until_blocks_are_loaded(spc):
+    torch.manual_seed(4)
+    plain = torch.nn.Linear(64, 20)
+    torch.manual_seed(4)
+    lin = spc.sparse.Q4Linear(64, 20)
+    assert isinstance(lin, torch.nn.Linear) and list(lin.state_dict()) == list(plain.state_dict())
+    x = torch.randn(3, 64)
+    assert torch.equal(lin(x), plain(x))
+    lin.load_q4_0(random_blocks(20, 64, 1))
+    assert list(lin.state_dict()) == list(plain.state_dict())
+    with pytest.raises(RuntimeError, match="GPU only"):
+        lin(x)
+    lin.drop_q4_0()
+    assert torch.equal(lin(x), plain(x))
+    for bad in (torch.zeros(720 - 18, dtype=torch.uint8), torch.zeros(720, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            lin.load_q4_0(bad)
+
+
+def test_gguf_linear(spc, orc, tmp_path):
+    gg = importlib.import_module(spc.__name__ + ".gguf")
+    rng = np.random.default_rng(0)
+    w = rng.standard_normal((40, 64)).astype(np.float32)
+    bias = rng.standard_normal(40).astype(np.float32)
+    blocks = random_blocks(40, 64, 3)
+    q8 = orc.q8_0_quantize(w)
+    p = str(tmp_path / "m.gguf")
+    write_gguf(p, [], [
+        ("f.weight", "F32", (64, 40), f32_bytes(w)), ("f.bias", "F32", (40,), f32_bytes(bias)),
+        ("h.weight", "BF16", (64, 40), bf16_bytes(w)),
+        ("q4.weight", "Q4_0", (64, 40), blocks.numpy().tobytes()),
+        ("q4.bias", "BF16", (40,), bf16_bytes(bias)),
+        ("q8.weight", "Q8_0", (64, 40), q8.tobytes()),
+        ("t.weight", "F32", (40, 64), f32_bytes(w)),
+        ("b.weight", "F32", (64, 40), f32_bytes(w)), ("b.bias", "F32", (39,), f32_bytes(bias[:39])),
+    ])
+    lin = spc.sparse.Q4Linear(64, 40)
+    with gg.GGUFReader(p) as r:
+        gg.load_linear(lin, r, "q4")
+        assert torch.equal(lin._q4.view(40, 2, 18), blocks)
+        assert torch.equal(lin.bias.detach(), torch.from_numpy(bias).bfloat16().float())
+        gg.load_linear(lin, r, "f")
+        assert lin._q4 is None
+        assert np.array_equal(lin.weight.detach().numpy(), w)
+        assert np.array_equal(lin.bias.detach().numpy(), bias)
+        plain = torch.nn.Linear(64, 40)
+        gg.load_linear(plain, r, "h")
+        assert torch.equal(plain.weight.detach(), torch.from_numpy(w).bfloat16().float())
+        gg.load_linear(plain, r, "q8")
+        assert float((plain.weight.detach() - torch.from_numpy(w)).abs().max()) < 0.02
+        with pytest.raises(gg.GGUFError, match="Q4Linear"):
+            gg.load_linear(plain, r, "q4")
+        for name in ("t", "b"):
+            before = lin.weight.detach().clone()
+            with pytest.raises(gg.GGUFError):
+                gg.load_linear(lin, r, name)
+            assert torch.equal(lin.weight.detach(), before)
+        with pytest.raises(gg.GGUFError):
+            gg.load_linear(torch.nn.Linear(64, 40, bias=False), r, "f")
+        with pytest.raises(KeyError):
+            gg.load_linear(lin, r, "none")
