@@ -595,16 +595,16 @@ int spc_sparse_conv_products(spc_stream_t stream, int dtype, const void* x, cons
  * ------------------------------------------------------------------------ */
 
 /* What a layer norm applies behind (x - mean) / sqrt(var + eps): the optional
- * gamma / beta [c] in param_dtype, then the optional modulation by the row's
- * batch item b, * (1 + scale[b]) + shift[b] (scale and shift together: n_batch
- * rows of c values in mod_dtype, mod_stride elements apart, so the halves of
+ * gamma / beta [c] in param_dtype (F32 or the rows' dtype), then the optional
+ * modulation by the row's batch item b, * (1 + scale[b]) + shift[b] (scale and
+ * shift together: n_batch rows of c values in mod_dtype, F32 or the rows',
+ * mod_stride elements apart, so the halves of
  * one Linear's output serve as they are), then SiLU if silu is set.  Rows of
  * item b are [offsets[b], offsets[b+1]) (offsets: device int64 [n_batch + 1],
  * ascending, 8-byte aligned; NULL with n_batch 1: every row; only with scale
  * and shift).  Rows before offsets[0] and from offsets[n_batch] on belong to
  * no item: their outputs are zeros and they add to no sum.  Pointers need
- * only their elements' alignment; rows whose width, strides and addresses are
- * multiples of 16 bytes are the fast ones. */
+ * only their elements' alignment, widths and strides none. */
 typedef struct {
     const void* gamma;
     const void* beta;

@@ -176,29 +176,23 @@ def _need_gpu(*ts: torch.Tensor) -> None:
 
 def _one_device(x: torch.Tensor, *others) -> torch.device:
     """x's device; every tensor of the call has to be there."""
-    for t in (x, *others):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"tensors on {x.device} and {t.device} in one call")
-    _need_gpu(x)
-    return x.device
+    dev = x.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    if dev.type != "cuda":
+        _need_gpu(x)
+    return dev
 
 
-class _on:
-    """Makes `device` the current one for a call (its default stream is the
-    null stream, which means the current device's)."""
-
-    def __init__(self, device: torch.device):
-        self._device, self._was = device.index, None
-
-    def __enter__(self):
-        was = torch.cuda.current_device()
-        if was != self._device:
-            self._was = was
-            torch.cuda.set_device(self._device)
-
-    def __exit__(self, *exc):
-        if self._was is not None:
-            torch.cuda.set_device(self._was)
+def _launch(fn, dev: torch.device, *args) -> int:
+    """fn(current stream of dev, *args) with dev the current device (its default
+    stream is the null stream, which means the current device's)."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    with torch.cuda.device(index):
+        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 def dtype_code(dt: torch.dtype) -> int:
@@ -766,60 +760,64 @@ def layernorm_mod_silu(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor
 
 
 def _strided_rows(x: torch.Tensor, name: str):
-    """(x, row stride): x [n, c] as it is when its rows are contiguous."""
+    """(x, n, c, row stride): x [n, c] as it is when its rows are contiguous."""
     if x.dim() != 2:
         raise ValueError(f"{name} must be [n, c], got {tuple(x.shape)}")
     n, c = x.shape
-    if c > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    return x, (x.stride(0) if n > 1 else c)
+    stride, inner = x.stride()
+    if inner != 1 and c > 1:
+        x, stride = x.contiguous(), c
+    return x, n, c, stride if n > 1 else c
 
 
-def _param_pair(a, b, width: int, names: str):
-    """Two parameter tensors [width] (or None) in one dtype the kernels read."""
+def _param_pair(a, b, width: int, names: str, dtype: torch.dtype):
+    """Two parameter tensors [width] (or None), both float32 or both `dtype`."""
     for t in (a, b):
         if t is not None and t.shape != (width,):
             raise ValueError(f"{names} must be [{width}], got {tuple(t.shape)}")
     dts = {t.dtype for t in (a, b) if t is not None}
-    if len(dts) > 1 or not dts <= {torch.float32, torch.float16, torch.bfloat16}:
+    if len(dts) > 1 or not dts <= {torch.float32, dtype}:
         a, b = (None if t is None else t.to(torch.float32) for t in (a, b))
     return tuple(None if t is None else t.contiguous() for t in (a, b))
 
 
-def _layer_norm_params(x, weight, bias, eps, scale, shift, offsets, silu):
-    """(spc_layer_norm_params, tensors it points into, items)."""
-    c = x.shape[1]
-    weight, bias = _param_pair(weight, bias, c, "weight / bias")
-    p = LayerNormParams(silu=int(bool(silu)), eps=float(eps), n_batch=1)
-    for t, name in ((weight, "gamma"), (bias, "beta")):
-        if t is not None:
-            setattr(p, name, t.data_ptr())
-            p.param_dtype = dtype_code(t.dtype)
-    if (scale is None) != (shift is None):
-        raise ValueError("scale and shift go together")
-    if scale is None:
+def _layer_norm_params(x, c, weight, bias, eps, scale, shift, offsets, silu):
+    """(spc_layer_norm_params, tensors it points into)."""
+    f32, dt = torch.float32, x.dtype
+    gp = bp = sp = hp = op = None
+    pdt = mdt = nb = 1
+    ms = 0
+    if weight is not None or bias is not None:
+        weight, bias = _param_pair(weight, bias, c, "weight / bias", dt)
+        gp, bp = _ptr(weight), _ptr(bias)
+        pdt = dtype_code((weight if weight is not None else bias).dtype)
+    if scale is not None or shift is not None:
+        if scale is None or shift is None:
+            raise ValueError("scale and shift go together")
+        if scale.dim() != 2 or scale.shape != shift.shape or scale.shape[1] != c:
+            raise ValueError(f"scale / shift must be [n_batch, {c}], got {tuple(scale.shape)} and "
+                             f"{tuple(shift.shape)}")
+        mdt = scale.dtype
+        if mdt != shift.dtype or (mdt != f32 and mdt != dt):
+            scale, shift, mdt = scale.to(f32), shift.to(f32), f32
+        mdt = dtype_code(mdt)
+        st = scale.stride()
+        if st != shift.stride() or (c > 1 and st[1] != 1):
+            scale, shift = scale.contiguous(), shift.contiguous()
+            st = scale.stride()
+        nb, ms = scale.shape[0], st[0]
         if offsets is not None:
-            raise ValueError("offsets need scale and shift")
-        return p, (weight, bias)
-    if scale.dim() != 2 or scale.shape != shift.shape or scale.shape[1] != c:
-        raise ValueError(f"scale / shift must be [n_batch, {c}], got {tuple(scale.shape)} and "
-                         f"{tuple(shift.shape)}")
-    if scale.dtype != shift.dtype or scale.dtype not in (torch.float32, torch.float16,
-                                                         torch.bfloat16):
-        scale, shift = scale.to(torch.float32), shift.to(torch.float32)
-    if scale.stride() != shift.stride() or (c > 1 and scale.stride(1) != 1):
-        scale, shift = scale.contiguous(), shift.contiguous()
-    nb = scale.shape[0]
-    if offsets is not None:
-        if offsets.dtype != torch.int64 or offsets.shape != (nb + 1,):
-            raise ValueError(f"offsets must be int64 [{nb + 1}]")
-        offsets = offsets.contiguous()
-        p.offsets = offsets.data_ptr()
-    elif nb != 1:
-        raise ValueError("more than one item needs offsets")
-    p.scale, p.shift, p.n_batch = scale.data_ptr(), shift.data_ptr(), nb
-    p.mod_stride, p.mod_dtype = scale.stride(0), dtype_code(scale.dtype)
-    return p, (weight, bias, scale, shift, offsets)
+            if offsets.dtype != torch.int64 or offsets.shape != (nb + 1,):
+                raise ValueError(f"offsets must be int64 [{nb + 1}]")
+            offsets = offsets.contiguous()
+            op = offsets.data_ptr()
+        elif nb != 1:
+            raise ValueError("more than one item needs offsets")
+        sp, hp = scale.data_ptr(), shift.data_ptr()
+    elif offsets is not None:
+        raise ValueError("offsets need scale and shift")
+    return (LayerNormParams(gp, bp, sp, hp, op, nb, ms, pdt, mdt, 1 if silu else 0, eps),
+            (weight, bias, scale, shift, offsets))
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -837,20 +835,19 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     be x).  Not recorded for gradients: SparseLayerNorm32 is."""
     dev = _one_device(x, weight, bias, scale, shift, offsets, out)
     dt = dtype_code(x.dtype)
-    x, stride = _strided_rows(x, "x")
-    n, c = x.shape
-    p, keep = _layer_norm_params(x, weight, bias, eps, scale, shift, offsets, silu)
+    x, n, c, stride = _strided_rows(x, "x")
+    p, keep = _layer_norm_params(x, c, weight, bias, eps, scale, shift, offsets, silu)
     if out is None:
-        out = torch.empty((n, c), dtype=x.dtype, device=dev)
+        out = x.new_empty((n, c))
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of x's shape and dtype")
     # rows of no item have no statistics: zeros, not what the memory held
     stats = None if not return_stats else (torch.empty if offsets is None else torch.zeros)(
         (n, 2), dtype=torch.float32, device=dev)
-    with _on(dev):
-        st = lib().spc_layer_norm(_stream(dev), dt, _ptr(x), stride, n, c, ctypes.byref(p),
-                                  _ptr(out), _ptr(stats))
-    _check("spc_layer_norm", st)
+    st = _launch(lib().spc_layer_norm, dev, dt, x.data_ptr(), stride, n, c, p, out.data_ptr(),
+                 _ptr(stats))
+    if st:
+        _check("spc_layer_norm", st)
     del keep  # alive until queued
     return (out, stats) if return_stats else out
 
@@ -869,25 +866,21 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor,
     dt = dtype_code(x.dtype)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("dy must have x's shape and dtype")
-    x, xs = _strided_rows(x, "x")
-    dy, dys = _strided_rows(dy, "dy")
-    n, c = x.shape
+    x, n, c, xs = _strided_rows(x, "x")
+    dy, _, _, dys = _strided_rows(dy, "dy")
     if stats.shape != (n, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("stats must be contiguous float32 [n, 2]")
-    p, keep = _layer_norm_params(x, weight, bias, 0.0, scale, shift, offsets, silu)
-    params = keep[:4] if scale is not None else (*keep, None, None)
-    dx = torch.empty((n, c), dtype=x.dtype, device=dev) if need[0] else None
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if t is not None and k else None
-             for t, k in zip(params, need[1:])]
+    p, keep = _layer_norm_params(x, c, weight, bias, 0.0, scale, shift, offsets, silu)
+    dx = x.new_empty((n, c)) if need[0] else None
+    grads = [t.new_empty(t.shape) if t is not None and k else None for t, k in zip(keep, need[1:])]
     ws, nbytes = None, 0
-    with _on(dev):
-        if any(g is not None for g in grads):
-            nbytes = lib().spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
-            ws = _workspace(nbytes, dev)
-        st = lib().spc_layer_norm_backward(_stream(dev), dt, _ptr(dy), dys, _ptr(x), xs, _ptr(stats),
-                                           n, c, ctypes.byref(p), _ptr(dx), *map(_ptr, grads),
-                                           _ptr(ws), nbytes)
-    _check("spc_layer_norm_backward", st)
+    if any(g is not None for g in grads):
+        nbytes = lib().spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
+        ws = _workspace(nbytes, dev)
+    st = _launch(lib().spc_layer_norm_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs,
+                 stats.data_ptr(), n, c, p, _ptr(dx), *map(_ptr, grads), _ptr(ws), nbytes)
+    if st:
+        _check("spc_layer_norm_backward", st)
     given = (weight, bias, scale, shift)
     return (dx, *(g if g is None or g.dtype == t.dtype else g.to(t.dtype)
                   for g, t in zip(grads, given)))
@@ -952,8 +945,7 @@ def q4_0_quantize(w: torch.Tensor) -> torch.Tensor:
     w = w.detach().to(torch.float32).contiguous()
     n = w.numel()
     out = torch.empty(n // 32 * 18, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = lib().spc_q4_0_quantize(_stream(dev), _ptr(w), n, _ptr(out))
+    st = _launch(lib().spc_q4_0_quantize, dev, _ptr(w), n, _ptr(out))
     _check("spc_q4_0_quantize", st)
     return out
 
@@ -982,9 +974,8 @@ def pack_q4_0(blocks: torch.Tensor, *, out_features: int, in_features: int,
         raise ValueError(f"expected {out_features * (in_features // 32) * 18} Q4_0 bytes (uint8)")
     blocks = blocks.contiguous()
     data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = L.spc_linear_q4_0_pack(_stream(dev), _ptr(blocks), int(out_features), int(in_features),
-                                    int(bool(transpose)), _ptr(data))
+    st = _launch(L.spc_linear_q4_0_pack, dev, _ptr(blocks), int(out_features), int(in_features),
+                 int(bool(transpose)), _ptr(data))
     _check("spc_linear_q4_0_pack", st)
     return Q4Weights(data, int(out_features), int(in_features), bool(transpose))
 
@@ -996,8 +987,8 @@ def linear_q4_0(x: torch.Tensor, w: Q4Weights, bias: torch.Tensor | None = None)
     dt = dtype_code(x.dtype)
     if w.transpose:
         raise ValueError("these weights are packed for linear_q4_0_input_grad")
-    x, stride = _strided_rows(x, "x")
-    if x.shape[1] != w.in_features:
+    x, m, k, stride = _strided_rows(x, "x")
+    if k != w.in_features:
         raise ValueError(f"expected x [m, {w.in_features}], got {tuple(x.shape)}")
     bdt = F32
     if bias is not None:
@@ -1006,12 +997,11 @@ def linear_q4_0(x: torch.Tensor, w: Q4Weights, bias: torch.Tensor | None = None)
         if bias.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             bias = bias.to(torch.float32)
         bias, bdt = bias.contiguous(), dtype_code(bias.dtype)
-    m = x.shape[0]
-    y = torch.empty((m, w.out_features), dtype=x.dtype, device=dev)
-    with _on(dev):
-        st = lib().spc_linear_q4_0(_stream(dev), dt, _ptr(x), stride, m, _ptr(w.data), w.out_features,
-                                   w.in_features, _ptr(bias), bdt, _ptr(y))
-    _check("spc_linear_q4_0", st)
+    y = x.new_empty((m, w.out_features))
+    st = _launch(lib().spc_linear_q4_0, dev, dt, x.data_ptr(), stride, m, w.data.data_ptr(),
+                 w.out_features, w.in_features, _ptr(bias), bdt, y.data_ptr())
+    if st:
+        _check("spc_linear_q4_0", st)
     return y
 
 
@@ -1023,15 +1013,14 @@ def linear_q4_0_input_grad(dy: torch.Tensor, w: Q4Weights) -> torch.Tensor:
     dt = dtype_code(dy.dtype)
     if not w.transpose:
         raise ValueError("these weights are not packed with transpose")
-    dy, stride = _strided_rows(dy, "dy")
-    if dy.shape[1] != w.out_features:
+    dy, m, o, stride = _strided_rows(dy, "dy")
+    if o != w.out_features:
         raise ValueError(f"expected dy [m, {w.out_features}], got {tuple(dy.shape)}")
-    m = dy.shape[0]
-    dx = torch.empty((m, w.in_features), dtype=dy.dtype, device=dev)
-    with _on(dev):
-        st = lib().spc_linear_q4_0_input_grad(_stream(dev), dt, _ptr(dy), stride, m, _ptr(w.data),
-                                              w.out_features, w.in_features, _ptr(dx))
-    _check("spc_linear_q4_0_input_grad", st)
+    dx = dy.new_empty((m, w.in_features))
+    st = _launch(lib().spc_linear_q4_0_input_grad, dev, dt, dy.data_ptr(), stride, m,
+                 w.data.data_ptr(), w.out_features, w.in_features, dx.data_ptr())
+    if st:
+        _check("spc_linear_q4_0_input_grad", st)
     return dx
 
 

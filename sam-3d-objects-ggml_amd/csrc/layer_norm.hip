@@ -9,22 +9,24 @@ namespace spc {
 namespace {
 
 // Rows a block takes.  Forward: up to 2,048 blocks (eight to a CU), each with
-// as many rounds of its teams as that leaves.  Backward: half as many, since
-// every block ends by writing its channels' two sums.
+// as many rounds of its teams as that leaves.  Backward: a quarter, since
+// every block ends by writing its channels' two sums, which the second kernel
+// reads again (62,710 x 512 bf16: 40.4 + 6.4 us with 1,024 blocks, 39.7 + 4.1).
 inline int64_t ln_rows_per(int64_t n, int teams, int64_t blocks) {
     const int64_t rounds = std::max<int64_t>(1, ceil_div(n, blocks * teams));
     return rounds * teams;
 }
 constexpr int64_t kLnForwardBlocks = 2048;
-constexpr int64_t kLnBackwardBlocks = 1024;
+constexpr int64_t kLnBackwardBlocks = 512;
 
-// Sums the slots of each item's chunks (32 channels and all of an item's
-// slots a block, in a fixed order) and forms the parameters' gradients from
+// Sums the slots of each item's chunks (16 channels and all of an item's
+// slots a block, in a fixed order; eight slots in flight a thread: the pass is
+// the latency of its loads) and forms the parameters' gradients from
 // A = sum dz h, B = sum dz:
 //   modulated: dscale = gamma A + beta B, dshift = B, and for the weight and
 //   bias (1 + scale) A, (1 + scale) B into `sums`, added over the items by
 //   ln_sum_items_kernel;  affine alone: dgamma = A, dbeta = B.
-constexpr int kLnFinalChannels = 32, kLnFinalThreads = 1024;
+constexpr int kLnFinalChannels = 16, kLnFinalThreads = 1024;
 
 struct LnFinal {
     const float* part;
@@ -45,37 +47,49 @@ __device__ __forceinline__ void ln_put(void* p, int dt, int64_t i, float v) {
 }
 
 __global__ __launch_bounds__(kLnFinalThreads) void ln_finalize_kernel(LnFinal p) {
-    constexpr int L = kLnFinalThreads / kLnFinalChannels;
-    __shared__ float ls[2][L][kLnFinalChannels];
+    constexpr int C = kLnFinalChannels, L = kLnFinalThreads / C, W = kLnFinalThreads / 64, DEEP = 8;
+    __shared__ float ls[2][W][C];
     const int64_t item = blockIdx.y;
-    const int cl = threadIdx.x % kLnFinalChannels, l = threadIdx.x / kLnFinalChannels;
-    const int ch = blockIdx.x * kLnFinalChannels + cl;
+    const int cl = threadIdx.x % C, l = threadIdx.x / C;
+    const int ch = blockIdx.x * C + cl;
     const int64_t lo = p.off ? min(max(p.off[item], (int64_t)0), p.n) : 0;
     const int64_t hi = p.off ? min(max(p.off[item + 1], (int64_t)0), p.n) : p.n;
     float a = 0.0f, b = 0.0f;
     if (lo < hi && ch < p.c) {
         const int64_t j1 = (hi - 1) / p.rows_per;
-#pragma unroll 4
-        for (int64_t j = lo / p.rows_per + l; j <= j1; j += L) {
-            const float* s = p.part + (j + item) * 2 * p.c + ch;
-            a += s[0];
-            b += s[p.c];
-        }
-    }
-    ls[0][l][cl] = a;
-    ls[1][l][cl] = b;
-    __syncthreads();
+        for (int64_t j = lo / p.rows_per + l; j <= j1; j += DEEP * L) {
+            float u[DEEP], v[DEEP];
 #pragma unroll
-    for (int w = L / 2; w > 0; w >>= 1) {
-        if (l < w) {
-            ls[0][l][cl] += ls[0][l + w][cl];
-            ls[1][l][cl] += ls[1][l + w][cl];
+            for (int i = 0; i < DEEP; ++i) {
+                const int64_t jj = j + i * L;
+                const float* s = p.part + (min(jj, j1) + item) * 2 * p.c + ch;
+                u[i] = jj <= j1 ? s[0] : 0.0f;
+                v[i] = jj <= j1 ? s[p.c] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                a += u[i];
+                b += v[i];
+            }
         }
-        __syncthreads();
     }
+#pragma unroll
+    for (int o = C; o < 64; o <<= 1) {
+        a += __shfl_xor(a, o);
+        b += __shfl_xor(b, o);
+    }
+    if ((threadIdx.x & 63) < C) {
+        ls[0][threadIdx.x >> 6][cl] = a;
+        ls[1][threadIdx.x >> 6][cl] = b;
+    }
+    __syncthreads();
     if (l != 0 || ch >= p.c) return;
-    a = ls[0][0][cl];
-    b = ls[1][0][cl];
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        a += ls[0][w][cl];
+        b += ls[1][w][cl];
+    }
     if (p.scale) {
         const float g = p.gamma ? ln_param(p.gamma, p.p_dtype, ch) : 1.0f;
         const float t = p.beta ? ln_param(p.beta, p.p_dtype, ch) : 0.0f;
@@ -126,8 +140,9 @@ int ln_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t 
         return SPC_BAD_ARG;
     }
     const bool affine = q->gamma || q->beta, mod = q->scale || q->shift;
-    if ((affine && !ln_float_dtype(q->param_dtype)) || (mod && !ln_float_dtype(q->mod_dtype))) {
-        set_last_error("%s: unknown parameter dtype", fn);
+    auto known = [&](int dt) { return dt == SPC_F32 || dt == dtype; };
+    if ((affine && !known(q->param_dtype)) || (mod && !known(q->mod_dtype))) {
+        set_last_error("%s: parameters must be F32 or of the rows' dtype", fn);
         return SPC_BAD_ARG;
     }
     if (mod && (!q->scale || !q->shift || q->n_batch < 1 || q->n_batch > 65535 || q->mod_stride < 0 ||
@@ -193,7 +208,7 @@ int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stri
     }
     p.y = y;
     p.stats = stats;
-    p.rows_per = (int)ln_rows_per(n, ln_teams(dtype, p.c), kLnForwardBlocks);
+    p.rows_per = (int)ln_rows_per(n, ln_teams(dtype, p.c, false), kLnForwardBlocks);
     const unsigned blocks = (unsigned)ceil_div(n, p.rows_per);
     const hipError_t e = dtype == SPC_BF16  ? ln_forward_bf16(s, p, blocks)
                          : dtype == SPC_F16 ? ln_forward_f16(s, p, blocks)
@@ -204,7 +219,7 @@ int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stri
 size_t spc_layer_norm_backward_workspace_bytes(int dtype, int64_t n, int64_t c, int64_t n_batch) {
     if (!ln_float_dtype(dtype) || n < 0 || n > INT32_MAX || c <= 0 || c > kLnMaxC || n_batch < 1 || n_batch > 65535)
         return 0;
-    const int64_t slots = ln_backward_chunks(n, ln_teams(dtype, (int)c)) + n_batch;
+    const int64_t slots = ln_backward_chunks(n, ln_teams(dtype, (int)c, true)) + n_batch;
     return (size_t)((slots + n_batch) * 2 * c * (int64_t)sizeof(float));
 }
 
@@ -231,7 +246,7 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
         return SPC_BAD_ARG;
     }
     if (!dx && !sums) return SPC_OK;
-    const int teams = ln_teams(dtype, p.c);
+    const int teams = ln_teams(dtype, p.c, true);
     const int64_t chunks = ln_backward_chunks(n, teams);
     if (sums) {
         if (!workspace || off(workspace, 4) ||

@@ -35,10 +35,10 @@ struct LnArgs {
     int64_t dy_stride;
     int64_t n;
     int c;
-    const void* gamma;  // p_dtype [c] or null
+    const void* gamma;  // p_dtype (F32 or the rows') [c] or null
     const void* beta;
     int p_dtype;
-    const void* scale;  // m_dtype, rows of c `m_stride` apart, or null
+    const void* scale;  // m_dtype (F32 or the rows'), rows of c `m_stride` apart, or null
     const void* shift;
     int64_t m_stride;
     int m_dtype;
@@ -52,7 +52,6 @@ struct LnArgs {
     float* part;         // [chunks + items][2][c], or null
 };
 
-// U elements of 16 bytes (U = all of them), 4 or 2.
 template <int DT>
 struct LnElem {
     static constexpr int V = DT == SPC_F32 ? 4 : 8;  // elements in 16 bytes
@@ -70,68 +69,75 @@ struct LnElem {
 template <>
 struct LnElem<SPC_F32> {
     static constexpr int V = 4;
-    using S = float;
+    using S = uint32_t;
 };
+
+// Element e of a lane's vector k is channel (lane + T k) V + e: the team's
+// vectors lie side by side, so its loads and stores are one contiguous run.
+// Rows need only their elements' alignment (gfx950 loads 16 bytes from any
+// address); a width that is no multiple of V leaves one lane of the team with
+// a part of a vector, `tail` = c % V elements, which it takes in pairs (TAIL).
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(2)));
+
+template <typename S, int V>
+__device__ __forceinline__ void ln_load_tail(u32x4 (&w)[V * (int)sizeof(S) / 16], const S* q, int tail) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4 / (int)sizeof(S)) {
+        constexpr int P = 4 / (int)sizeof(S);  // elements a word
+        uint32_t v = 0;
+        if (e + P <= tail) v = *reinterpret_cast<const u32_any*>(q + e);
+        else if (e < tail) v = *reinterpret_cast<const uint16_t*>(q + e);
+        w[e / P / 4][e / P % 4] = v;
+    }
+}
+
+// V elements of size S, `left` of them (> 0) inside the width.
+template <typename S, int V, bool TAIL>
+__device__ __forceinline__ void ln_load_vector(u32x4 (&w)[V * (int)sizeof(S) / 16], const S* q, int left,
+                                               int tail) {
+    if (!TAIL || left >= V) {
+#pragma unroll
+        for (int i = 0; i < V * (int)sizeof(S) / 16; ++i)
+            w[i] = *reinterpret_cast<const u32x4_any*>(q + i * (16 / (int)sizeof(S)));
+    } else {
+        ln_load_tail<S, V>(w, q, tail);
+    }
+}
 
 // A row's elements as they were loaded (16 bytes a vector, NV of them).
 template <int NV>
 struct LnRaw {
-    u32x4 v[NV];
+    u32x4 v[NV][1];
 };
 
-// Where a team's lane holds element e of its vector k: units of U elements
-// lie next to each other across the lanes, so every load and store of a team
-// is one contiguous run (U = V: 16-byte words; rows whose width or address
-// they do not divide: 4- or 2-byte units).
-template <int T, int V, int U>
-__device__ __forceinline__ int ln_channel(int lane, int k, int e) {
-    return (lane + T * ((k * V + e) / U)) * U + e % U;
-}
-
-template <int DT, int T, int NV, int U>
+template <int DT, int T, int NV, bool TAIL>
 __device__ __forceinline__ LnRaw<NV> ln_load(const void* base, int64_t at, int c, int lane, bool on) {
     constexpr int V = LnElem<DT>::V;
+    using S = typename LnElem<DT>::S;
+    const S* row = static_cast<const S*>(base) + at;
     LnRaw<NV> r;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        r.v[k] = u32x4{0, 0, 0, 0};
-        if constexpr (U == V) {
-            const int ch = ln_channel<T, V, U>(lane, k, 0);
-            if (on && ch < c)
-                r.v[k] = *reinterpret_cast<const u32x4*>(
-                    static_cast<const typename LnElem<DT>::S*>(base) + at + ch);
-        } else {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if constexpr (DT == SPC_F32 || U == 2) {
-                    const int ch = ln_channel<T, V, U>(lane, k, w * V / 4);
-                    if (on && ch < c)
-                        r.v[k][w] = *reinterpret_cast<const uint32_t*>(
-                            static_cast<const typename LnElem<DT>::S*>(base) + at + ch);
-                } else {
-                    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-                    const int c0 = ln_channel<T, V, U>(lane, k, 2 * w);
-                    const int c1 = ln_channel<T, V, U>(lane, k, 2 * w + 1);
-                    const uint32_t a = on && c0 < c ? p[c0] : 0u;
-                    const uint32_t b = on && c1 < c ? p[c1] : 0u;
-                    r.v[k][w] = a | (b << 16);
-                }
-            }
-        }
+        const int ch = (lane + T * k) * V;
+        r.v[k][0] = u32x4{0, 0, 0, 0};
+        if (on && ch < c) ln_load_vector<S, V, TAIL>(r.v[k], row + ch, c - ch, c % V);
     }
     return r;
 }
 
 template <int DT, int NV>
 __device__ __forceinline__ float ln_get(const LnRaw<NV>& r, int k, int e) {
-    if constexpr (DT == SPC_F32) return __uint_as_float(r.v[k][e]);
-    else return e & 1 ? LnElem<DT>::hi(r.v[k][e / 2]) : LnElem<DT>::lo(r.v[k][e / 2]);
+    if constexpr (DT == SPC_F32) return __uint_as_float(r.v[k][0][e]);
+    else return e & 1 ? LnElem<DT>::hi(r.v[k][0][e / 2]) : LnElem<DT>::lo(r.v[k][0][e / 2]);
 }
 
-template <int DT, int T, int NV, int U>
+template <int DT, int T, int NV, bool TAIL>
 __device__ __forceinline__ void ln_store(void* base, int64_t at, int c, int lane,
                                          const float (&o)[NV][LnElem<DT>::V]) {
-    constexpr int V = LnElem<DT>::V;
+    constexpr int V = LnElem<DT>::V, P = DT == SPC_F32 ? 1 : 2;
+    using S = typename LnElem<DT>::S;
+    S* row = static_cast<S*>(base) + at;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         u32x4 q;
@@ -140,65 +146,110 @@ __device__ __forceinline__ void ln_store(void* base, int64_t at, int c, int lane
             if constexpr (DT == SPC_F32) q[w] = __float_as_uint(o[k][w]);
             else q[w] = LnElem<DT>::bits(o[k][2 * w]) | (LnElem<DT>::bits(o[k][2 * w + 1]) << 16);
         }
-        auto* p = static_cast<typename LnElem<DT>::S*>(base) + at;
-        if constexpr (U == V) {
-            const int ch = ln_channel<T, V, U>(lane, k, 0);
-            if (ch < c) __builtin_nontemporal_store(q, reinterpret_cast<u32x4*>(p + ch));
-        } else {
+        const int ch = (lane + T * k) * V;
+        if (TAIL ? ch + V <= c : ch < c) {
+            __builtin_nontemporal_store(q, reinterpret_cast<u32x4_any*>(row + ch));
+        } else if (TAIL && ch < c) {
+            const int tail = c % V;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if constexpr (DT == SPC_F32 || U == 2) {
-                    const int ch = ln_channel<T, V, U>(lane, k, w * V / 4);
-                    if (ch < c) *reinterpret_cast<uint32_t*>(p + ch) = q[w];
-                } else {
-                    const int c0 = ln_channel<T, V, U>(lane, k, 2 * w);
-                    const int c1 = ln_channel<T, V, U>(lane, k, 2 * w + 1);
-                    if (c0 < c) p[c0] = (uint16_t)q[w];
-                    if (c1 < c) p[c1] = (uint16_t)(q[w] >> 16);
-                }
+            for (int e = 0; e < V; e += P) {
+                if (e + P <= tail) *reinterpret_cast<u32_any*>(row + ch + e) = q[e / P];
+                else if (e < tail) row[ch + e] = (S)q[e / P];
             }
         }
     }
 }
 
-// Element i of a parameter stored as dtype dt.
+// Element i of a parameter stored as F32, or as the rows are.
 __device__ __forceinline__ float ln_param(const void* p, int dt, int64_t i) {
     if (dt == SPC_F32) return static_cast<const float*>(p)[i];
     const uint16_t b = static_cast<const uint16_t*>(p)[i];
     return dt == SPC_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
 }
 
-// The lane's coefficients for item b.
-template <int T, int NV, int V, int U>
+// A lane's share of a parameter as loaded.  Loading and converting are apart
+// so that every load of a block's coefficients is under way before the first
+// is waited for: converted where they were loaded, each element's load was a
+// latency of its own (one row of 1,024, modulated: 7.2 us, 3.4 apart; 62,710
+// rows x 128 bf16 with SiLU: 19.3 and 8.8).
+template <int DT, int T, int NV, bool TAIL>
+struct LnParam {
+    static constexpr int V = LnElem<DT>::V;
+    using S = typename LnElem<DT>::S;
+    u32x4 w[NV][V / 4];  // F32: V words; as the rows: 16 bytes
+
+    __device__ __forceinline__ void load(const void* p, bool f32, int64_t at, int c, int lane) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int ch = (lane + T * k) * V;
+            if (ch < c) {
+                // (unsigned: a scalar base and a 32-bit offset)
+                if (DT == SPC_F32 || f32)
+                    ln_load_vector<uint32_t, V, TAIL>(w[k], static_cast<const uint32_t*>(p) + at + (uint32_t)ch,
+                                                      c - ch, c % V);
+                else
+                    ln_load_vector<S, V, TAIL>(reinterpret_cast<u32x4(&)[1]>(w[k]),
+                                               static_cast<const S*>(p) + at + (uint32_t)ch, c - ch, c % V);
+            }
+        }
+    }
+    // f(k, e, value) for every element
+    template <typename F>
+    __device__ __forceinline__ void each(bool f32, F&& f) const {
+        if (DT == SPC_F32 || f32) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) f(k, e, __uint_as_float(w[k][e / 4][e % 4]));
+        } else if constexpr (DT != SPC_F32) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    f(k, e, e & 1 ? LnElem<DT>::hi(w[k][0][e / 2]) : LnElem<DT>::lo(w[k][0][e / 2]));
+        }
+    }
+};
+
+// The lane's coefficients for item b (past the width: finite).
+template <int DT, int T, int NV, bool TAIL>
 __device__ __forceinline__ void ln_coefficients(const LnArgs& p, int64_t b, int lane,
-                                                float (&a)[NV][V], float (&k0)[NV][V]) {
+                                                float (&a)[NV][LnElem<DT>::V],
+                                                float (&k0)[NV][LnElem<DT>::V]) {
+    constexpr int V = LnElem<DT>::V;
+    const bool pf = p.p_dtype == SPC_F32, mf = p.m_dtype == SPC_F32;
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const int ch = ln_channel<T, V, U>(lane, k, e);
-            float g = 1.0f, t = 0.0f;
-            if (ch < p.c) {
-                if (p.gamma) g = ln_param(p.gamma, p.p_dtype, ch);
-                if (p.beta) t = ln_param(p.beta, p.p_dtype, ch);
-                if (p.scale) {
-                    const float s = 1.0f + ln_param(p.scale, p.m_dtype, b * p.m_stride + ch);
-                    g *= s;
-                    t = t * s + ln_param(p.shift, p.m_dtype, b * p.m_stride + ch);
-                }
-            }
-            a[k][e] = g;
-            k0[k][e] = t;
+            a[k][e] = 1.0f;
+            k0[k][e] = 0.0f;
         }
+    {
+        LnParam<DT, T, NV, TAIL> g{}, t{};
+        if (p.gamma) g.load(p.gamma, pf, 0, p.c, lane);
+        if (p.beta) t.load(p.beta, pf, 0, p.c, lane);
+        if (p.gamma) g.each(pf, [&](int k, int e, float v) { a[k][e] = v; });
+        if (p.beta) t.each(pf, [&](int k, int e, float v) { k0[k][e] = v; });
+    }
+    if (p.scale) {
+        LnParam<DT, T, NV, TAIL> s{}, h{};
+        s.load(p.scale, mf, b * p.m_stride, p.c, lane);
+        h.load(p.shift, mf, b * p.m_stride, p.c, lane);
+        s.each(mf, [&](int k, int e, float v) {
+            a[k][e] *= 1.0f + v;
+            k0[k][e] *= 1.0f + v;
+        });
+        h.each(mf, [&](int k, int e, float v) { k0[k][e] += v; });
+    }
 }
 
-// Sum over the T lanes of a team (T = 256: over the block's four waves too,
-// through one of two LDS slots in turn, so one barrier a sum is enough: a
-// thread that writes a slot again has passed the barrier behind which every
-// thread read it).  Every step adds a lane's value and its partner's, so all
-// lanes end with the same bits.  Lane exchanges are DPP moves and permlane
-// swaps within the register file; the same steps as LDS permutes were what
-// bound narrow rows.
+// Sum over the T lanes of a team (T > 64: over its waves too, through one of
+// two LDS slots in turn, so one barrier a sum is enough: a thread that writes a
+// slot again has passed the barrier behind which every thread read it).  Every
+// step adds a lane's value and its partner's, so all lanes end with the same
+// bits.  Lane exchanges are DPP moves and permlane swaps within the register
+// file.
 template <int T>
 __device__ __forceinline__ float wave_part_sum(float v) {
     constexpr int W = T > 64 ? 64 : T;
@@ -223,17 +274,26 @@ __device__ __forceinline__ float wave_part_sum(float v) {
     return v;
 }
 
-struct LnBlockSum {
+struct LnTeamSum {
     float (*slot)[2][4];  // LDS [2 slots][2 values][4 waves]
     int turn = 0;
+    // the team's waves' values of one slot row
+    template <int T>
+    __device__ __forceinline__ float waves(const float* s) const {
+        if constexpr (T == 128) {
+            const int w = threadIdx.x >> 6 & 2;
+            return s[w] + s[w + 1];
+        } else {
+            return (s[0] + s[1]) + (s[2] + s[3]);
+        }
+    }
     template <int T>
     __device__ __forceinline__ float sum(float v) {
         v = wave_part_sum<T>(v);
         if constexpr (T > 64) {
-            float(*s)[4] = slot[turn];
-            if ((threadIdx.x & 63) == 0) s[0][threadIdx.x >> 6] = v;
+            if ((threadIdx.x & 63) == 0) slot[turn][0][threadIdx.x >> 6] = v;
             __syncthreads();
-            v = (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
+            v = waves<T>(slot[turn][0]);
             turn ^= 1;
         }
         return v;
@@ -243,18 +303,25 @@ struct LnBlockSum {
         v = wave_part_sum<T>(v);
         u = wave_part_sum<T>(u);
         if constexpr (T > 64) {
-            float(*s)[4] = slot[turn];
             if ((threadIdx.x & 63) == 0) {
-                s[0][threadIdx.x >> 6] = v;
-                s[1][threadIdx.x >> 6] = u;
+                slot[turn][0][threadIdx.x >> 6] = v;
+                slot[turn][1][threadIdx.x >> 6] = u;
             }
             __syncthreads();
-            v = (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
-            u = (s[1][0] + s[1][1]) + (s[1][2] + s[1][3]);
+            v = waves<T>(slot[turn][0]);
+            u = waves<T>(slot[turn][1]);
             turn ^= 1;
         }
     }
 };
+
+// 1 / sqrt(v) by the hardware's instruction (one unit in the last place);
+// it takes subnormals for zero, so tiny values are scaled by a power of 4.
+__device__ __forceinline__ float ln_rsqrt(float v) {
+    const bool tiny = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p100f : v);
+    return tiny ? r * 0x1p50f : r;
+}
 
 // sigmoid(z); F32 rows take the correctly scaled exponential, 16-bit rows the
 // hardware's (its error grows as |z| 2^-24, far below half their last bit).
@@ -264,52 +331,101 @@ __device__ __forceinline__ float ln_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// Last item i in [0, nb) with off[i] <= row (0 if there is none).
-__device__ __forceinline__ int64_t ln_item(const int64_t* off, int64_t nb, int64_t row) {
-    int64_t lo = 0, hi = nb;
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (off[mid] <= row) lo = mid;
-        else hi = mid;
+// The items' row offsets: up to 63 items in one load a wave, a lane each, so
+// that finding a block's first item and its bounds costs one latency; more by
+// a binary search.
+struct LnItems {
+    const int64_t* off;
+    int64_t nb;
+    int64_t mine = 0;
+    __device__ __forceinline__ LnItems(const int64_t* o, int64_t n) : off(o), nb(n) {
+        if (off && nb < 64) mine = off[min((int64_t)(threadIdx.x & 63), nb)];
     }
-    return lo;
+    __device__ __forceinline__ int64_t at(int64_t i) const {
+        if (nb >= 64) return off[i];
+        const int l = (int)i;
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)mine, l);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)mine >> 32), l);
+        return (int64_t)(((uint64_t)hi << 32) | lo);
+    }
+    // Last item i in [0, nb) with off[i] <= row (0 if there is none).
+    __device__ __forceinline__ int64_t find(int64_t row) const {
+        if (nb < 64) {
+            const uint64_t m = __ballot((int64_t)(threadIdx.x & 63) < nb && mine <= row);
+            return m ? 63 - __builtin_clzll(m) : 0;
+        }
+        int64_t lo = 0, hi = nb;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (off[mid] <= row) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+
+// Adds the squares of the lane's values inside the width.
+template <int DT, int T, int NV, bool TAIL>
+__device__ __forceinline__ void ln_squares(const float (&v)[NV][LnElem<DT>::V], int c, int lane,
+                                           float& s) {
+    constexpr int V = LnElem<DT>::V;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int left = c - (lane + T * k) * V;
+        float q = 0.0f;
+        if (!TAIL) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) q += v[k][e] * v[k][e];
+            s += left > 0 ? q : 0.0f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += e < left ? v[k][e] * v[k][e] : 0.0f;
+        }
+    }
 }
 
-// Zeros for the rows [lo, hi), which belong to no item.
-template <int DT, int T, int NV, int U>
-__device__ __forceinline__ void ln_zero_rows(const LnArgs& p, int64_t lo, int64_t hi, int lane) {
+// Zeros for the chunk's rows that belong to no item: [lo, first) and [end, hi).
+template <int DT, int T, int NV, bool TAIL>
+__device__ __forceinline__ void ln_zero_rows(const LnArgs& p, int64_t lo, int64_t first, int64_t end,
+                                             int64_t hi, int lane) {
     constexpr int TPB = kLnThreads / T;
+    if ((lo == first && end >= hi) || !p.y) return;
     const float z[NV][LnElem<DT>::V] = {};
-    for (int64_t row = lo + threadIdx.x / T; row < hi; row += TPB) {
-        if (p.y) ln_store<DT, T, NV, U>(p.y, row * p.c, p.c, lane, z);
-    }
+    for (int64_t row = lo + threadIdx.x / T; row < hi; row += TPB)
+        if (row < first || row >= end) ln_store<DT, T, NV, TAIL>(p.y, row * p.c, p.c, lane, z);
 }
 
-template <int DT, int T, int NV, int U>
+template <int DT, int T, int NV, bool TAIL, bool SILU>
 __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
     constexpr int V = LnElem<DT>::V, TPB = kLnThreads / T;
     __shared__ float slots[2][2][4];
-    LnBlockSum team{slots};
+    LnTeamSum team{slots};
     const int lane = threadIdx.x % T;
     const int64_t lo = (int64_t)blockIdx.x * p.rows_per;
     const int64_t hi = min(p.n, lo + p.rows_per);
     const float inv_c = 1.0f / (float)p.c;
-    int64_t item = 0, first = lo;
+    const LnItems items(p.off, p.nb);
+    // the chunk's first rows: under way before the offsets are known
+    int64_t row = lo + threadIdx.x / T;
+    LnRaw<NV> next = ln_load<DT, T, NV, TAIL>(p.x, row * p.x_stride, p.c, lane, row < hi);
+    int64_t item = 0, first = lo, loaded = lo;
     if (p.off) {
-        item = ln_item(p.off, p.nb, lo);
-        first = min(max(p.off[0], lo), hi);
-        ln_zero_rows<DT, T, NV, U>(p, lo, first, lane);
+        item = items.find(lo);
+        first = min(max(items.at(0), lo), hi);
     }
+    const int64_t begin = first;
     for (; first < hi && item < p.nb; ++item) {
-        const int64_t last = p.off ? min(hi, p.off[item + 1]) : hi;
+        const int64_t last = p.off ? min(hi, items.at(item + 1)) : hi;
         if (last <= first) continue;
+        row = first + threadIdx.x / T;
+        if (first != loaded)
+            next = ln_load<DT, T, NV, TAIL>(p.x, row * p.x_stride, p.c, lane, row < last);
+        loaded = -1;
         float a[NV][V], k0[NV][V];
-        ln_coefficients<T, NV, V, U>(p, item, lane, a, k0);
-        int64_t row = first + threadIdx.x / T;
-        LnRaw<NV> next = ln_load<DT, T, NV, U>(p.x, row * p.x_stride, p.c, lane, row < last);
+        ln_coefficients<DT, T, NV, TAIL>(p, item, lane, a, k0);
         for (int64_t base = first; base < last; base += TPB, row += TPB) {
             const LnRaw<NV> cur = next;
-            next = ln_load<DT, T, NV, U>(p.x, (row + TPB) * p.x_stride, p.c, lane, row + TPB < last);
+            next = ln_load<DT, T, NV, TAIL>(p.x, (row + TPB) * p.x_stride, p.c, lane, row + TPB < last);
             float v[NV][V];
             float s = 0.0f;
 #pragma unroll
@@ -321,23 +437,21 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    v[k][e] -= mean;
-                    if (ln_channel<T, V, U>(lane, k, e) < p.c) s += v[k][e] * v[k][e];
-                }
-            const float r = 1.0f / sqrtf(team.template sum<T>(s) * inv_c + p.eps);
+                for (int e = 0; e < V; ++e) v[k][e] -= mean;
+            ln_squares<DT, T, NV, TAIL>(v, p.c, lane, s);
+            const float r = ln_rsqrt(team.template sum<T>(s) * inv_c + p.eps);
             if (row < last) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
                     for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * r * a[k][e] + k0[k][e];
-                if (p.silu) {
+                if constexpr (SILU) {
 #pragma unroll
                     for (int k = 0; k < NV; ++k)
 #pragma unroll
                         for (int e = 0; e < V; ++e) v[k][e] *= ln_sigmoid<DT>(v[k][e]);
                 }
-                ln_store<DT, T, NV, U>(p.y, row * p.c, p.c, lane, v);
+                ln_store<DT, T, NV, TAIL>(p.y, row * p.c, p.c, lane, v);
                 if (p.stats && lane == 0) {
                     p.stats[2 * row] = mean;
                     p.stats[2 * row + 1] = r;
@@ -346,7 +460,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
         }
         first = last;
     }
-    if (p.off) ln_zero_rows<DT, T, NV, U>(p, first, hi, lane);
+    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane);
 }
 
 // Adds a segment's sums over the block's teams and writes them to the slot of
@@ -354,11 +468,13 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
 // one segment to the next, so the slots are distinct and at most chunks +
 // items.  Lanes of one wave first, then the waves through LDS, in a fixed
 // order.
-template <int T, int NV, int V, int U>
+template <int T, int NV, int V>
 __device__ __forceinline__ void ln_flush(const LnArgs& p, int64_t slot, int lane, float* lds,
                                          float (&sum)[NV][V], int which) {
     float* out = p.part + (slot * 2 + which) * p.c;
-    if constexpr (T <= 64) {
+    if constexpr (T < 256) {
+        constexpr int W = T * NV * V;              // channels a team covers
+        constexpr int COPIES = T > 64 ? 2 : 4;     // teams left once a wave's are added
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -366,51 +482,70 @@ __device__ __forceinline__ void ln_flush(const LnArgs& p, int64_t slot, int lane
 #pragma unroll
                 for (int o = T; o < 64; o <<= 1) sum[k][e] += __shfl_xor(sum[k][e], o);
             }
-        constexpr int W = T * NV * V;  // channels a team covers
         __syncthreads();
-        if ((threadIdx.x & 63) < T) {
+        if (T >= 64 || (threadIdx.x & 63) < T) {
+            float* mine = lds + threadIdx.x / (T > 64 ? T : 64) * W;
 #pragma unroll
             for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    lds[(threadIdx.x >> 6) * W + ln_channel<T, V, U>(lane, k, e)] = sum[k][e];
+                for (int e = 0; e < V; ++e) mine[(lane + T * k) * V + e] = sum[k][e];
         }
         __syncthreads();
-        for (int ch = threadIdx.x; ch < p.c; ch += kLnThreads)
-            out[ch] = (lds[ch] + lds[W + ch]) + (lds[2 * W + ch] + lds[3 * W + ch]);
+        for (int ch = threadIdx.x; ch < p.c; ch += kLnThreads) {
+            float v = lds[ch] + lds[W + ch];
+            if constexpr (COPIES == 4) v += lds[2 * W + ch] + lds[3 * W + ch];
+            out[ch] = v;
+        }
     } else {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int ch = ln_channel<T, V, U>(lane, k, e);
+                const int ch = (lane + T * k) * V + e;
                 if (ch < p.c) out[ch] = sum[k][e];
             }
     }
 }
 
 // SUMS: the parameters' sums too.
-template <int DT, int T, int NV, int U, bool SUMS>
+template <int DT, int T, int NV, bool TAIL, bool SILU, bool SUMS>
 __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(LnArgs p) {
     constexpr int V = LnElem<DT>::V, TPB = kLnThreads / T;
     __shared__ float slots[2][2][4];
-    __shared__ float lds[SUMS && T <= 64 ? 4 * T * NV * V : 1];
-    LnBlockSum team{slots};
+    __shared__ float lds[SUMS && T < 256 ? (T > 64 ? 2 : 4) * T * NV * V : 1];
+    LnTeamSum team{slots};
     const int lane = threadIdx.x % T;
     const int64_t lo = (int64_t)blockIdx.x * p.rows_per;
     const int64_t hi = min(p.n, lo + p.rows_per);
     const float inv_c = 1.0f / (float)p.c;
-    int64_t item = 0, first = lo;
+    const LnItems items(p.off, p.nb);
+    LnRaw<NV> nx, ny;
+    float nm, nr;
+    auto fetch = [&](int64_t r, bool in) __attribute__((always_inline)) {
+        nx = ln_load<DT, T, NV, TAIL>(p.x, r * p.x_stride, p.c, lane, in);
+        ny = ln_load<DT, T, NV, TAIL>(p.dy, r * p.dy_stride, p.c, lane, in);
+        nm = in ? p.stats[2 * r] : 0.0f;
+        nr = in ? p.stats[2 * r + 1] : 0.0f;
+    };
+    // the chunk's first rows: under way before the offsets are known
+    int64_t row = lo + threadIdx.x / T;
+    fetch(row, row < hi);
+    int64_t item = 0, first = lo, loaded = lo;
     if (p.off) {
-        item = ln_item(p.off, p.nb, lo);
-        first = min(max(p.off[0], lo), hi);
-        ln_zero_rows<DT, T, NV, U>(p, lo, first, lane);
+        item = items.find(lo);
+        first = min(max(items.at(0), lo), hi);
     }
+    const int64_t begin = first;
     for (; first < hi && item < p.nb; ++item) {
-        const int64_t last = p.off ? min(hi, p.off[item + 1]) : hi;
+        const int64_t last = p.off ? min(hi, items.at(item + 1)) : hi;
         if (last <= first) continue;
+        row = first + threadIdx.x / T;
+        bool on = row < last;
+        // (an item that ends inside the chunk must not sum the next one's rows)
+        if (first != loaded || last < hi) fetch(row, on);
+        loaded = -1;
         float a[NV][V], k0[NV][V];
-        ln_coefficients<T, NV, V, U>(p, item, lane, a, k0);
+        ln_coefficients<DT, T, NV, TAIL>(p, item, lane, a, k0);
         float sa[SUMS ? NV : 1][V], sb[SUMS ? NV : 1][V];
         if constexpr (SUMS) {
 #pragma unroll
@@ -418,20 +553,12 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(LnArgs p) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) sa[k][e] = sb[k][e] = 0.0f;
         }
-        int64_t row = first + threadIdx.x / T;
-        bool on = row < last;
-        LnRaw<NV> nx = ln_load<DT, T, NV, U>(p.x, row * p.x_stride, p.c, lane, on);
-        LnRaw<NV> ny = ln_load<DT, T, NV, U>(p.dy, row * p.dy_stride, p.c, lane, on);
-        float nm = on ? p.stats[2 * row] : 0.0f, nr = on ? p.stats[2 * row + 1] : 0.0f;
         for (int64_t base = first; base < last; base += TPB, row += TPB) {
             const LnRaw<NV> cx = nx, cy = ny;
             const float mean = nm, r = nr;
             const bool now = on;
             on = row + TPB < last;
-            nx = ln_load<DT, T, NV, U>(p.x, (row + TPB) * p.x_stride, p.c, lane, on);
-            ny = ln_load<DT, T, NV, U>(p.dy, (row + TPB) * p.dy_stride, p.c, lane, on);
-            nm = on ? p.stats[2 * (row + TPB)] : 0.0f;
-            nr = on ? p.stats[2 * (row + TPB) + 1] : 0.0f;
+            fetch(row + TPB, on);
             float h[NV][V], g[NV][V];
             float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -442,7 +569,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(LnArgs p) {
                     h[k][e] = (ln_get<DT>(cx, k, e) - mean) * r;
                     g[k][e] = ln_get<DT>(cy, k, e);
                 }
-            if (p.silu) {
+            if constexpr (SILU) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -472,95 +599,93 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(LnArgs p) {
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
                     for (int e = 0; e < V; ++e) g[k][e] = r * (g[k][e] - s1 - h[k][e] * s2);
-                if (now) ln_store<DT, T, NV, U>(p.y, row * p.c, p.c, lane, g);
+                if (now) ln_store<DT, T, NV, TAIL>(p.y, row * p.c, p.c, lane, g);
             }
         }
         if constexpr (SUMS) {
-            ln_flush<T, NV, V, U>(p, blockIdx.x + item, lane, lds, sa, 0);
-            ln_flush<T, NV, V, U>(p, blockIdx.x + item, lane, lds, sb, 1);
+            ln_flush<T, NV, V>(p, blockIdx.x + item, lane, lds, sa, 0);
+            ln_flush<T, NV, V>(p, blockIdx.x + item, lane, lds, sb, 1);
         }
         first = last;
     }
-    if (p.off) ln_zero_rows<DT, T, NV, U>(p, first, hi, lane);
+    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane);
 }
 
-// Team width and vectors a lane for c channels: f(T, NV).  A wave takes up to
-// 16 elements a lane, wider rows the whole block.
-template <int DT, int U, typename F>
+// Lanes of a team and vectors a lane for c channels: f(T, NV).  As many rows to
+// a wave as fit, then up to 32 elements a lane (forward) before a row is shared
+// by waves, which costs a barrier a sum (2,048 channels bf16, 31,355 rows: 62 us
+// by four waves a row, 48 by one).  The gradient holds twice the registers a
+// channel, so half the elements a lane.
+template <int DT, bool BACKWARD, typename F>
 hipError_t ln_dispatch(int c, F&& f) {
-    constexpr int V = LnElem<DT>::V;
+    constexpr int V = LnElem<DT>::V, Q = DT == SPC_F32 ? 2 : 1;
     const int nvec = (c + V - 1) / V;
 #define SPC_LN(T, NV) return f(std::integral_constant<int, T>{}, std::integral_constant<int, NV>{})
-    if constexpr (U == V) {
-        if (nvec <= 4) SPC_LN(4, 1);
-        if (nvec <= 8) SPC_LN(8, 1);
-    }
+    if (nvec <= 4) SPC_LN(4, 1);
+    if (nvec <= 8) SPC_LN(8, 1);
     if (nvec <= 16) SPC_LN(16, 1);
     if (nvec <= 32) SPC_LN(32, 1);
     if (nvec <= 64) SPC_LN(64, 1);
+    if (nvec <= 96 && DT != SPC_F32) SPC_LN(32, 3);
     if (nvec <= 128) SPC_LN(64, 2);
     if constexpr (DT == SPC_F32) {
+        if (nvec <= 192) SPC_LN(64, 3);
         if (nvec <= 256) SPC_LN(64, 4);
-        if (nvec <= 512) SPC_LN(256, 2);
-        if (nvec <= 1024) SPC_LN(256, 4);
-        SPC_LN(256, 8);
-    } else {
-        if (nvec <= 256) SPC_LN(256, 1);
-        if (nvec <= 512) SPC_LN(256, 2);
-        SPC_LN(256, 4);
     }
+    if constexpr (!BACKWARD) {
+        if (nvec <= 192 * Q) SPC_LN(64, 3 * Q);
+        if (nvec <= 256 * Q) SPC_LN(64, 4 * Q);
+    } else {
+        if (nvec <= 256 * Q) SPC_LN(128, 2 * Q);
+    }
+    if (nvec <= 512 * Q) SPC_LN(256, 2 * Q);
+    SPC_LN(256, 4 * Q);
 #undef SPC_LN
 }
 
-// Elements a load takes: 16 bytes where the width, the strides and every
-// address allow, else 4 bytes, else one element.
-inline int ln_unit(const LnArgs& p, int esize, bool backward) {
-    auto fits = [&](int64_t bytes) {
-        auto ok = [&](const void* q) { return (uintptr_t)q % bytes == 0; };
-        const int64_t u = bytes / esize;
-        return u >= 1 && p.c % u == 0 && p.x_stride % u == 0 && ok(p.x) && ok(p.y) &&
-               (!backward || (p.dy_stride % u == 0 && ok(p.dy)));
-    };
-    return fits(16) ? 16 / esize : fits(4) ? 4 / esize : 1;
+// Rows a block works on at once.
+inline int ln_teams(int dtype, int c, bool backward) {
+    auto f = [](auto t, auto) { return (hipError_t)(kLnThreads / decltype(t)::value); };
+    if (dtype == SPC_F32)
+        return (int)(backward ? ln_dispatch<SPC_F32, true>(c, f) : ln_dispatch<SPC_F32, false>(c, f));
+    return (int)(backward ? ln_dispatch<SPC_BF16, true>(c, f) : ln_dispatch<SPC_BF16, false>(c, f));
 }
 
-template <int DT, int U>
-hipError_t ln_forward_u(hipStream_t s, const LnArgs& p, unsigned blocks) {
-    return ln_dispatch<DT, U>(p.c, [&](auto t, auto nv) {
-        ln_forward_kernel<DT, decltype(t)::value, decltype(nv)::value, U>
-            <<<blocks, kLnThreads, 0, s>>>(p);
-        return hipGetLastError();
-    });
-}
-
-template <int DT, int U>
-hipError_t ln_backward_u(hipStream_t s, const LnArgs& p, unsigned blocks) {
-    return ln_dispatch<DT, U>(p.c, [&](auto t, auto nv) {
-        constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
-        if (p.part) ln_backward_kernel<DT, T, NV, U, true><<<blocks, kLnThreads, 0, s>>>(p);
-        else ln_backward_kernel<DT, T, NV, U, false><<<blocks, kLnThreads, 0, s>>>(p);
-        return hipGetLastError();
-    });
+// f(TAIL, SILU) for p
+template <int V, typename F>
+void ln_flags(const LnArgs& p, F&& f) {
+    if (p.c % V) {
+        if (p.silu) f(std::true_type{}, std::true_type{});
+        else f(std::true_type{}, std::false_type{});
+    } else {
+        if (p.silu) f(std::false_type{}, std::true_type{});
+        else f(std::false_type{}, std::false_type{});
+    }
 }
 
 template <int DT>
 hipError_t ln_forward(hipStream_t s, const LnArgs& p, unsigned blocks) {
-    constexpr int V = LnElem<DT>::V;
-    const int u = ln_unit(p, 16 / V, false);
-    if (u == V) return ln_forward_u<DT, V>(s, p, blocks);
-    if constexpr (DT != SPC_F32)
-        if (u == 2) return ln_forward_u<DT, 2>(s, p, blocks);
-    return ln_forward_u<DT, 1>(s, p, blocks);
+    return ln_dispatch<DT, false>(p.c, [&](auto t, auto nv) {
+        constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
+        ln_flags<LnElem<DT>::V>(p, [&](auto tail, auto silu) {
+            ln_forward_kernel<DT, T, NV, decltype(tail)::value, decltype(silu)::value>
+                <<<blocks, kLnThreads, 0, s>>>(p);
+        });
+        return hipGetLastError();
+    });
 }
 
 template <int DT>
 hipError_t ln_backward(hipStream_t s, const LnArgs& p, unsigned blocks) {
-    constexpr int V = LnElem<DT>::V;
-    const int u = ln_unit(p, 16 / V, true);
-    if (u == V) return ln_backward_u<DT, V>(s, p, blocks);
-    if constexpr (DT != SPC_F32)
-        if (u == 2) return ln_backward_u<DT, 2>(s, p, blocks);
-    return ln_backward_u<DT, 1>(s, p, blocks);
+    return ln_dispatch<DT, true>(p.c, [&](auto t, auto nv) {
+        constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
+        ln_flags<LnElem<DT>::V>(p, [&](auto tail, auto silu) {
+            constexpr bool TL = decltype(tail)::value, SI = decltype(silu)::value;
+            if (p.part) ln_backward_kernel<DT, T, NV, TL, SI, true><<<blocks, kLnThreads, 0, s>>>(p);
+            else ln_backward_kernel<DT, T, NV, TL, SI, false><<<blocks, kLnThreads, 0, s>>>(p);
+        });
+        return hipGetLastError();
+    });
 }
 
 // One file a dtype (layer_norm_bf16.hip, layer_norm_f16.hip, layer_norm_f32.hip).
@@ -570,15 +695,5 @@ hipError_t ln_forward_f32(hipStream_t s, const LnArgs& p, unsigned blocks);
 hipError_t ln_backward_bf16(hipStream_t s, const LnArgs& p, unsigned blocks);
 hipError_t ln_backward_f16(hipStream_t s, const LnArgs& p, unsigned blocks);
 hipError_t ln_backward_f32(hipStream_t s, const LnArgs& p, unsigned blocks);
-
-// Rows a block's four waves work on at once.
-inline int ln_teams(int dtype, int c) {
-    const int v = dtype == SPC_F32 ? 4 : 8;
-    const int nvec = (c + v - 1) / v;
-    int t = 4;
-    while (t < nvec && t < 64) t <<= 1;
-    const int wave_max = dtype == SPC_F32 ? 256 : 128;
-    return nvec > wave_max ? 1 : kLnThreads / t;
-}
 
 }  // namespace spc

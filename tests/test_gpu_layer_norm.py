@@ -45,10 +45,10 @@ def _run(nat, dev, name, x, w, b, scale, shift, dy, offsets=None, silu=False, ep
     torch.cuda.synchronize()
     ref = Reference(x, w, b, eps, scale, shift, None if offsets is None else _items(offsets, n), silu)
     check(f"{name} y", y, *ref.forward())
-    # a row's way into a sum: the rounds of a block's team (1,024 blocks of at
-    # least one row), its lanes and waves (10), its share of 1,024 chunks (32)
+    # a row's way into a sum: the rounds of a block's team (512 blocks of at
+    # least one row), its lanes and waves (10), its share of 512 chunks (8)
     # and a tree (5)
-    outs = ref.backward(dy, -(-n // 1024) + 50)
+    outs = ref.backward(dy, -(-n // 512) + 50)
     want = [True, w is not None, b is not None, scale is not None, scale is not None]
     for gname, on, got, (val, bound), t in zip(("dx", "dweight", "dbias", "dscale", "dshift"), want,
                                                grads, outs, (x, w, b, scale, shift)):
