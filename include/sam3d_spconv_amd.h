@@ -668,7 +668,9 @@ int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out
 /* y [m, out_features] = x W^T + bias for x [m, in_features] in dtype (rows
  * x_stride elements apart), y contiguous in dtype, bias [out_features] in
  * bias_dtype or NULL.  Weights enter exactly, sums are F32, one rounding to
- * dtype at the end; a row with an infinity or NaN comes out as NaNs.  m up to
+ * dtype at the end (F32 rows enter as three 8-bit parts, of which those below
+ * 2^-126 are taken as zero); a row with an infinity or NaN comes out as NaNs, the
+ * others as without it.  m up to
  * 1,048,560; made for few rows (the weights' bytes are the cost up to some
  * 64), right for any.  16-byte aligned rows are the fast ones. */
 int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
@@ -676,11 +678,19 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
                     int bias_dtype, void* y);
 
 /* dx [m, in_features] = dy W for dy [m, out_features] (rows dy_stride apart),
- * packed with transpose 1.  dy times a scale enters with 16 bits (F32 rows:
- * 24), sums are F32. */
+ * packed with transpose 1.  Sums are F32, one rounding to dtype at the end.
+ * F32 rows: the weights enter exactly, dy times a scale in F32, as three parts.  16-bit rows:
+ * the weights enter as f16(d (q - 8)) (at most 2^-11 of a weight), bf16 rows
+ * with what lies above 2^-28 of the row's largest value.  A row with an
+ * infinity or NaN comes out non-finite, the others as without it.
+ * workspace: spc_linear_q4_0_input_grad_workspace_bytes (0 for most calls;
+ * large products of bf16 rows move them to f16 there first), 16-byte aligned. */
+size_t spc_linear_q4_0_input_grad_workspace_bytes(int dtype, int64_t m, int64_t out_features,
+                                                  int64_t in_features);
 int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                                int64_t m, const void* packed, int64_t out_features,
-                               int64_t in_features, void* dx);
+                               int64_t in_features, void* dx, void* workspace,
+                               size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

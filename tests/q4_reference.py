@@ -52,15 +52,24 @@ def product(x, blocks, bias=None):
 
 
 def gradient(dy, blocks):
-    """(dx, bound before the output's rounding) for dy [m, out]; dy d as two
-    bf16 parts: 2^-15, or three for F32: 2^-24 (the product's rounding)."""
+    """(dx, bound before the output's rounding) for dy [m, out].
+
+    F32 rows: dy d rounded once (u), three parts against 16 + q and -24 as
+    above.  16-bit rows: the weights rounded to f16 (2^-11 of each; subnormal
+    ones are multiples of their scale's last bit, so exact), bf16 rows without
+    what lies below 2^-28 of the row's largest value; one instruction a group
+    of 32."""
     f32 = dy.dtype == torch.float32
+    bf16 = dy.dtype == torch.bfloat16
     dy = dy.detach().cpu().double()
     w = dequant(blocks)
     d = parts(blocks)[0].abs().repeat_interleave(32, 1)
-    n = 3 if f32 else 2
     # eight waves share the summed features: instructions on one accumulator
-    chain = n * (-(-w.shape[0] // 128) // 8 + 1) * 4
-    e = (U if f32 else 2.0 ** -15) * (dy.abs() @ w.abs()) \
-        + 2 * (32 + chain + 12) * U * 79 * (dy.abs() @ d)
+    chain = (3 if f32 else 1) * (-(-w.shape[0] // 128) // 8 + 1) * 4
+    if f32:
+        e = U * (dy.abs() @ w.abs()) + 2 * (32 + chain + 12) * U * 79 * (dy.abs() @ d)
+    else:
+        e = (2.0 ** -11 + 2 * (32 + chain + 12) * U) * (dy.abs() @ w.abs())
+        if bf16 and dy.numel():
+            e = e + 2.0 ** -28 * dy.abs().amax(1, keepdim=True) * w.abs().sum(0)
     return dy @ w, e

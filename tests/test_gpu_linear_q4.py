@@ -32,7 +32,8 @@ def _randn(shape, seed, dt, dev):
 @pytest.mark.parametrize("out,inp", [(1, 32), (17, 64), (50, 160), (300, 384)])
 def test_unit_rows_give_the_weights(spc, dev, dt, out, inp):
     """Rows of the identity: d (q - 8) is exact in F32, so every weight comes
-    back at its place bit for bit (rounded once to 16-bit outputs)."""
+    back at its place bit for bit (rounded once to 16-bit outputs; the gradient
+    of 16-bit rows takes them as f16)."""
     nat = spc._native
     blocks = random_blocks(out, inp, out + inp)
     fwd, bwd = _both(nat, blocks, dev)
@@ -40,7 +41,7 @@ def test_unit_rows_give_the_weights(spc, dev, dt, out, inp):
     y = nat.linear_q4_0(torch.eye(inp, dtype=DT[dt], device=dev), fwd)
     assert torch.equal(y.cpu(), w.t().to(DT[dt]))
     dx = nat.linear_q4_0_input_grad(torch.eye(out, dtype=DT[dt], device=dev), bwd)
-    assert torch.equal(dx.cpu(), w.to(DT[dt]))
+    assert torch.equal(dx.cpu(), (w if dt == "f32" else w.half()).to(DT[dt]))
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
@@ -118,7 +119,7 @@ def test_infinite_rows_stay_alone(spc, dev, dt):
     assert torch.equal(y2[keep], y[keep]) and bool(y2[~keep].isnan().all())
     keep = torch.ones(20, dtype=torch.bool, device=dev)
     keep[2] = keep[9] = False
-    assert torch.equal(dx2[keep], dx[keep]) and bool(dx2[~keep].isnan().all())
+    assert torch.equal(dx2[keep], dx[keep]) and not bool(dx2[~keep].isfinite().any())
 
 
 def test_large_and_small_magnitudes(spc, dev):
@@ -131,6 +132,56 @@ def test_large_and_small_magnitudes(spc, dev):
         check(f"y {s}", nat.linear_q4_0(x * s, fwd), *product(x * s, blocks), torch.float32)
         check(f"dx {s}", nat.linear_q4_0_input_grad(dy * s, bwd), *gradient(dy * s, blocks),
               torch.float32)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("out,inp", [(2500, 96), (2051, 15_456)])
+def test_gradient_rows_of_any_range(spc, dev, dt, out, inp):
+    """Rows whose magnitudes lie anywhere and change along the row by 2^20 and
+    more: zeros first, growing, falling, single large and single tiny values.
+    The second shape moves bf16 rows to f16 ahead of the product."""
+    nat = spc._native
+    moved = nat.lib().spc_linear_q4_0_input_grad_workspace_bytes(nat.dtype_code(DT[dt]), 19, out, inp)
+    assert (moved > 0) == (dt == "bf16" and inp > 10_000)
+    blocks = random_blocks(out, inp, 8)
+    _, bwd = _both(nat, blocks, dev)
+    g = torch.Generator().manual_seed(3)
+    dy = torch.randn(19, out, generator=g)
+    n = torch.arange(out)
+    dy[0] = 0
+    dy[1, :2000] = 0
+    dy[2] *= 2.0 ** (n / 60 - 20)                 # grows 2^41
+    dy[3] *= 2.0 ** (20 - n / 60)
+    dy[4] *= torch.where(n % 128 == 5, 1e6, 1e-6)
+    dy[5] *= 1e30
+    dy[6] *= 1e-30
+    dy[7] *= 1e-38                                # bf16 and F32 subnormals among them
+    dy[8] = 0
+    dy[8, out - 1] = 3e38
+    dy[9] = 0
+    dy[9, 1300] = 1e-39
+    dy[10, 1200:1400] *= 1e9
+    dy[11] *= 2.0 ** (n % 130 - 65).float()       # every group spans 2^130
+    dy[12] *= 3.0 ** (n // 128 % 20 - 10).float()
+    dy = dy.to(DT[dt]).to(dev)
+    dx, bound = gradient(dy, blocks)
+    if dt == "f32":
+        # parts of dy d below 2^-126 count as zero: of an element's three cuts
+        # (each below 2^-7 of the one before) less than 2^-125 in all, times |q - 8|
+        # <= 8; the two sums (16 + q, -24) lose the same parts
+        bound = bound + out * 2.0 ** -122
+    got = nat.linear_q4_0_input_grad(dy, bwd)
+    check(f"any range {dt}", got, dx, bound, DT[dt])
+    # strided rows, at an odd element; alone, a row is as among the others up to
+    # the order of its sums
+    wide = torch.cat([dy[:, :1], dy, dy[:, :3]], 1)
+    check(f"any range {dt} strided", nat.linear_q4_0_input_grad(wide[:, 1:out + 1], bwd), dx, bound,
+          DT[dt])
+    check(f"any range {dt} row", nat.linear_q4_0_input_grad(dy[4:5], bwd), dx[4:5], bound[4:5], DT[dt])
+    dy[3, 7], dy[5, out - 1] = float("inf"), float("nan")
+    bad = nat.linear_q4_0_input_grad(dy, bwd)
+    keep = [i for i in range(19) if i not in (3, 5)]
+    assert torch.equal(bad[keep], got[keep]) and not bool(bad[[3, 5]].isfinite().any())
 
 
 def test_quantize(spc, dev):
