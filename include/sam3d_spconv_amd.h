@@ -672,7 +672,7 @@ int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out
  * 2^-126 are taken as zero); a row with an infinity or NaN comes out as NaNs, the
  * others as without it.  m up to
  * 1,048,560; made for few rows (the weights' bytes are the cost up to some
- * 64), right for any.  16-byte aligned rows are the fast ones. */
+ * 64), right for any. */
 int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
                     const void* packed, int64_t out_features, int64_t in_features, const void* bias,
                     int bias_dtype, void* y);
@@ -682,15 +682,10 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
  * F32 rows: the weights enter exactly, dy times a scale in F32, as three parts.  16-bit rows:
  * the weights enter as f16(d (q - 8)) (at most 2^-11 of a weight), bf16 rows
  * with what lies above 2^-28 of the row's largest value.  A row with an
- * infinity or NaN comes out non-finite, the others as without it.
- * workspace: spc_linear_q4_0_input_grad_workspace_bytes (0 for most calls;
- * large products of bf16 rows move them to f16 there first), 16-byte aligned. */
-size_t spc_linear_q4_0_input_grad_workspace_bytes(int dtype, int64_t m, int64_t out_features,
-                                                  int64_t in_features);
+ * infinity or NaN comes out non-finite, the others as without it. */
 int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                                int64_t m, const void* packed, int64_t out_features,
-                               int64_t in_features, void* dx, void* workspace,
-                               size_t workspace_bytes);
+                               int64_t in_features, void* dx);
 
 #ifdef __cplusplus
 }

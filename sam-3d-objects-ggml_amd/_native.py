@@ -129,9 +129,7 @@ def lib() -> ctypes.CDLL:
     L.spc_linear_q4_0_packed_bytes.argtypes = [_I64, _I64, _INT]
     L.spc_linear_q4_0_pack.argtypes = [_P, _P, _I64, _I64, _INT, _P]
     L.spc_linear_q4_0.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P, _INT, _P]
-    L.spc_linear_q4_0_input_grad_workspace_bytes.restype = _SZ
-    L.spc_linear_q4_0_input_grad_workspace_bytes.argtypes = [_INT, _I64, _I64, _I64]
-    L.spc_linear_q4_0_input_grad.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _SZ]
+    L.spc_linear_q4_0_input_grad.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P]
     _lib = L
     return L
 
@@ -1019,11 +1017,8 @@ def linear_q4_0_input_grad(dy: torch.Tensor, w: Q4Weights) -> torch.Tensor:
     if o != w.out_features:
         raise ValueError(f"expected dy [m, {w.out_features}], got {tuple(dy.shape)}")
     dx = dy.new_empty((m, w.in_features))
-    L = lib()
-    nbytes = L.spc_linear_q4_0_input_grad_workspace_bytes(dt, m, w.out_features, w.in_features)
-    ws = _workspace(nbytes, dev) if nbytes else None
-    st = _launch(L.spc_linear_q4_0_input_grad, dev, dt, dy.data_ptr(), stride, m, w.data.data_ptr(),
-                 w.out_features, w.in_features, dx.data_ptr(), _ptr(ws), nbytes)
+    st = _launch(lib().spc_linear_q4_0_input_grad, dev, dt, dy.data_ptr(), stride, m,
+                 w.data.data_ptr(), w.out_features, w.in_features, dx.data_ptr())
     if st:
         _check("spc_linear_q4_0_input_grad", st)
     return dx

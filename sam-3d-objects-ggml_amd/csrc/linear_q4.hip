@@ -13,7 +13,10 @@
 //
 // Forward, one 16x16x32 product covers exactly one block of every column; its
 // F32 result times d is added to the F32 accumulator, so no weight is ever
-// rounded.  F32 rows run as three bf16 parts that add up to them exactly.
+// rounded.  F32 rows run as three bf16 parts that add up to them exactly, and
+// on (q - 8) / 16 itself, three instructions a weight: the two sums above
+// cancel to a fifth of themselves, which 16-bit outputs do not see and F32
+// ones do (one row, 1024 -> 2048: off by 1.3e-6 of the output's size, 9.5e-8 so).
 // For the gradient the scale varies along the summed index.  F32 rows are
 // multiplied by it first (F32) and run as three bf16 parts; for 16-bit rows the
 // weights are, as f16(d (q - 8)).
@@ -26,6 +29,9 @@
 #include "common.h"
 
 namespace spc {
+
+// (gfx950 loads 16 bytes from any address)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 namespace {
 
@@ -169,6 +175,20 @@ __device__ __forceinline__ floatx4 q4_mfma(u32x4 a, u32x4 b, floatx4 c) {
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// (q - 8) / 16 of a word's weights as bf16: the conversion of four-bit
+// integers, whose results end in zeros, so the cut to bf16 is exact.
+__device__ __forceinline__ u32x4 q4_expand_signed(uint32_t w) {
+    w ^= 0x88888888u;  // q - 8 as four bits of two's complement
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_amdgcn_cvt_off_f32_i4(w >> (4 * i));
+        const float b = __builtin_amdgcn_cvt_off_f32_i4(w >> (4 * i + 16));
+        r[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    return r;
+}
+
 template <bool F16>
 __device__ __forceinline__ u32x4 q4_minus_24() {
     constexpr uint32_t v = F16 ? 0xce00ce00u : 0xc1c0c1c0u;
@@ -183,73 +203,6 @@ __device__ __forceinline__ float q4_rest(float v) {
     return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
 }
 
-// Eight F32 values as three bf16 operands that add up to them: cuts of eight
-// bits each, and the last one's rest is nothing.
-__device__ __forceinline__ void q4_split(const float (&v)[8], u32x4 (&p)[3]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float a = v[2 * i], b = v[2 * i + 1];
-#pragma unroll
-        for (int s = 0; s < 3; ++s) {
-            p[s][i] = q4_high_pair(a, b);
-            a = q4_rest(a);
-            b = q4_rest(b);
-        }
-    }
-}
-
-// Eight consecutive elements of a row as loaded.
-template <int DT>
-struct Q4Row {
-    u32x4 w[DT == SPC_F32 ? 2 : 1];
-};
-// The lane's elements of one group: for each of its four instructions j eight,
-// from 128 g + 32 j + 8 (lane / 16) on, of a row of `sum` elements at `row`.
-// WIDE: 16-byte loads without a branch; in a last, partial group those past the
-// end become the row's last eight, which meet weights of scale 0.
-template <int DT, bool WIDE>
-__device__ __forceinline__ void q4_load_rows(Q4Row<DT> (&r)[4], const char* row, int g, int sum) {
-    constexpr int NW = DT == SPC_F32 ? 2 : 1, ES = DT == SPC_F32 ? 4 : 2;
-    const int k0 = 8 * ((threadIdx.x & 63) / 16);
-    if constexpr (WIDE) {
-        const char* p = row + (int64_t)g * kQ4Group * ES;
-        if ((g + 1) * kQ4Group <= sum) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < NW; ++i)
-                    r[j].w[i] = *reinterpret_cast<const u32x4*>(p + (k0 + 32 * j) * ES + 16 * i);
-        } else {
-            const int last = sum - 8 - g * kQ4Group;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < NW; ++i)
-                    r[j].w[i] = *reinterpret_cast<const u32x4*>(p + min(k0 + 32 * j, last) * ES + 16 * i);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < NW; ++i) r[j].w[i] = u32x4{0, 0, 0, 0};
-            const int64_t k = (int64_t)g * kQ4Group + 32 * j + k0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (k + e >= sum) break;
-                if constexpr (DT == SPC_F32)
-                    r[j].w[e / 4][e % 4] = reinterpret_cast<const uint32_t*>(row)[k + e];
-                else
-                    r[j].w[0][e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(row)[k + e]
-                                        << (16 * (e & 1));
-            }
-        }
-    }
-}
-__device__ __forceinline__ void q4_row_floats(const Q4Row<SPC_F32>& r, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.w[e / 4][e % 4]);
-}
-
 struct Q4Args {
     const void* x;       // rows [m, sum], x_stride elements apart
     int64_t x_stride;
@@ -259,8 +212,6 @@ struct Q4Args {
     const uint16_t* scales;
     const void* bias;    // [cols] or null
     int bias_dtype;
-    const float* factor; // [m]: x is f16 rows times these
-    bool wide;           // rows take 16-byte loads
     void* y;             // [m, cols]
 };
 
@@ -271,13 +222,102 @@ __device__ __forceinline__ void q4_store(void* y, int64_t at, float v) {
     else static_cast<uint16_t*>(y)[at] = f32_to_f16_bits(v);
 }
 
+// ---- rows -------------------------------------------------------------------
+// A step's rows: 128 summed features of ROWS rows, 16 bytes a lane and load, a
+// row in consecutive lanes (LANES of them; PER elements each), kept by a wave
+// for itself: loaded ahead, turned into operands once an element, written to
+// its part of LDS and read back as the matrix instructions want them (lane l:
+// row l % 16, features 32 j + 8 (l / 16) ..+ 7).  Loaded in that order
+// instead, four neighbouring lanes are in four rows, a load is 64 accesses of
+// the cache, and sixteen rows cost three times the weights (16 bf16 rows,
+// 16,384 -> 4096: 19.7 us, 13.2 through LDS); few rows are few loads, and their
+// conversion is done for ROWS rows, not for sixteen.
+template <int DT, int ROWS>
+struct Q4Rows {
+    static constexpr int ES = DT == SPC_F32 ? 4 : 2, PER = 16 / ES, LANES = kQ4Group / PER;
+    static constexpr int NI = ROWS * LANES / 64;         // loads a lane
+    static constexpr int STRIDE = kQ4Group * 2 + 16;     // bytes of an operand row in LDS
+    static constexpr int MT = (ROWS + 15) / 16;          // 16-row tiles
+    const char* row[NI];
+
+    __device__ __forceinline__ static int lane() { return threadIdx.x & 63; }
+    __device__ __forceinline__ static int chunk() { return lane() % LANES; }
+    // the row (of ROWS) of load i
+    __device__ __forceinline__ static int in_tile(int i) { return i * (64 / LANES) + lane() / LANES; }
+
+    // Rows past the last repeat it; their results are not stored.
+    __device__ __forceinline__ Q4Rows(const void* x, int64_t x_stride, int64_t row0, int64_t m) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            row[i] = static_cast<const char*>(x) +
+                     (min(row0 + in_tile(i), m - 1) * x_stride + chunk() * PER) * ES;
+    }
+    // Zeros past the end of a row of `sum` elements.
+    __device__ __forceinline__ void load(u32x4 (&v)[NI], int g, int sum) const {
+        const int64_t at = (int64_t)g * kQ4Group * ES;
+        if ((g + 1) * kQ4Group <= sum) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) v[i] = *reinterpret_cast<const u32x4_any*>(row[i] + at);
+        } else {
+            const int left = sum - g * kQ4Group - chunk() * PER;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                v[i] = u32x4{0, 0, 0, 0};
+                if (left >= PER) {
+                    v[i] = *reinterpret_cast<const u32x4_any*>(row[i] + at);
+                } else if (left > 0) {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) {
+                        if (e >= left) break;
+                        if constexpr (DT == SPC_F32)
+                            v[i][e] = reinterpret_cast<const uint32_t*>(row[i] + at)[e];
+                        else
+                            v[i][e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(row[i] + at)[e]
+                                           << (16 * (e & 1));
+                    }
+                }
+            }
+        }
+    }
+    // One 16-bit operand: the loads as they are.
+    __device__ __forceinline__ static void put(char* lds, int i, u32x4 v) {
+        *reinterpret_cast<u32x4*>(lds + in_tile(i) * STRIDE + chunk() * 16) = v;
+    }
+    // Four F32 values as three bf16 operands that add up to them: cuts of eight
+    // bits each, and the last one's rest is nothing.
+    __device__ __forceinline__ static void put_parts(char* lds, int i, float (&f)[4]) {
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            *reinterpret_cast<u32x2*>(lds + (s * ROWS + in_tile(i)) * STRIDE + chunk() * 8) =
+                u32x2{q4_high_pair(f[0], f[1]), q4_high_pair(f[2], f[3])};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = q4_rest(f[e]);
+        }
+    }
+    // Operand `part` of row tile a for instruction j (fewer than 16 rows repeat).
+    __device__ __forceinline__ static u32x4 get(const char* lds, int part, int a, int j) {
+        const int r = ROWS >= 16 ? 16 * a + lane() % 16 : lane() % ROWS;
+        return *reinterpret_cast<const u32x4*>(lds + (part * ROWS + r) * STRIDE +
+                                               (4 * j + lane() / 16) * 16);
+    }
+};
+
+// A wave's own LDS, written and read back by different lanes of it: its LDS
+// operations complete in order, so only the compiler has to keep theirs.
+__device__ __forceinline__ void q4_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Adds the W waves' accumulators and stores: tiles [MT][NT] of 16 rows x 16
-// columns; lane l of a tile holds column l % 16, rows 4 (l / 16) + i.
+// columns; lane l of a tile holds column l % 16, rows 4 (l / 16) + i.  lds is
+// the block's, whatever it held.
 template <int DT, int MT, int NT, int W>
 __device__ __forceinline__ void q4_finish(const Q4Args& p, floatx4 (&acc)[MT][NT], int64_t row0,
                                           int64_t col0, floatx4* lds) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int TILES = MT * NT;
+    __syncthreads();
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -304,10 +344,17 @@ __device__ __forceinline__ void q4_finish(const Q4Args& p, floatx4 (&acc)[MT][NT
     }
 }
 
+// Bytes of a block's LDS: the waves' rows (and, for the gradient, scales and
+// row factors), then the accumulators.
+constexpr size_t q4_lds(size_t wave_bytes, int tiles, int w) {
+    return wave_bytes * w > (size_t)tiles * w * 1024 ? wave_bytes * w : (size_t)tiles * w * 1024;
+}
+
 // A block's W waves take the groups of 128 summed features in turn, each with
 // its next step of weights and rows under way: f(step) for every step of this
 // wave.  (Two or three steps under way measured slower: 8192 -> 16,384, one
-// bf16 row, 16.2 / 17.3 us with one / two; the waves hide each other's loads.)
+// bf16 row, 16.2 / 17.3 us with one / two; two buffers in turn instead of a move
+// 14.8 / 15.4: the waves hide each other's loads.)
 template <int W, typename Step, typename Load, typename F>
 __device__ __forceinline__ void q4_pipeline(int groups, Load&& load, F&& f) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -320,40 +367,33 @@ __device__ __forceinline__ void q4_pipeline(int groups, Load&& load, F&& f) {
     }
 }
 
-// The lane's rows: row0 + 16 a + lane % 16, those past the last repeat it
-// (their results are not stored).
-template <int DT, int MT>
-__device__ __forceinline__ void q4_rows(const Q4Args& p, int64_t row0, const char* (&row)[MT]) {
-#pragma unroll
-    for (int a = 0; a < MT; ++a)
-        row[a] = static_cast<const char*>(p.x) +
-                 min(row0 + 16 * a + (threadIdx.x & 15), p.m - 1) * p.x_stride * (DT == SPC_F32 ? 4 : 2);
-}
-
-// y = x W^T: a block's W waves share 16 NT columns and 16 MT rows.
-template <int DT, int MT, int NT, int W, bool WIDE>
+// y = x W^T: a block's W waves share 16 NT columns and ROWS rows.
+template <int DT, int ROWS, int NT, int W>
 __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
     constexpr bool F16 = DT == SPC_F16;
     constexpr int PARTS = DT == SPC_F32 ? 3 : 1;
-    __shared__ floatx4 lds[W * MT * NT * 64];
+    typedef Q4Rows<DT, ROWS> R;
+    constexpr int MT = R::MT;
+    constexpr size_t WAVE = PARTS * ROWS * R::STRIDE;
+    __shared__ __attribute__((aligned(16))) char lds[q4_lds(WAVE, MT * NT, W)];
     const uint32_t lane = threadIdx.x & 63;
-    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * 16 * MT;
+    char* mine = lds + (threadIdx.x >> 6) * WAVE;
+    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * ROWS;
     struct Step {
         u32x4 q[NT];
         u32x2 d[NT];
-        Q4Row<DT> x[MT][4];
+        u32x4 x[R::NI];
     };
-    const char* row[MT];
-    q4_rows<DT, MT>(p, row0, row);
+    const R rows(p.x, p.x_stride, row0, p.m);
     auto load = [&](Step& s, int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
+            // (tiles past the last repeat it; their results are not stored)
             const int64_t t = min(tile0 + b, p.col_tiles - 1) * p.groups + g;
             s.q[b] = (reinterpret_cast<const u32x4*>(p.quants) + t * 64)[lane];
             s.d[b] = (reinterpret_cast<const u32x2*>(p.scales) + t * 16)[lane % 16];
         }
-#pragma unroll
-        for (int a = 0; a < MT; ++a) q4_load_rows<DT, WIDE>(s.x[a], row[a], g, p.sum);
+        rows.load(s.x, g, p.sum);
     };
     floatx4 acc[MT][NT];
 #pragma unroll
@@ -362,27 +402,40 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
         for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0, 0, 0, 0};
     const uint32_t one = q4_one<F16>();
     q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
+        q4_wave_sync();
+#pragma unroll
+        for (int i = 0; i < R::NI; ++i) {
+            if constexpr (PARTS == 1) {
+                R::put(mine, i, s.x[i]);
+            } else {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(s.x[i][e]);
+                R::put_parts(mine, i, f);
+            }
+        }
+        q4_wave_sync();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             u32x4 xp[MT][PARTS];
             floatx4 off[MT];
 #pragma unroll
             for (int a = 0; a < MT; ++a) {
-                if constexpr (PARTS == 1) {
-                    xp[a][0] = s.x[a][j].w[0];
-                } else {
-                    float v[8];
-                    q4_row_floats(s.x[a][j], v);
-                    q4_split(v, xp[a]);
-                }
                 off[a] = floatx4{0, 0, 0, 0};
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) off[a] = q4_mfma<F16>(xp[a][q], q4_minus_24<F16>(), off[a]);
+                for (int q = 0; q < PARTS; ++q) xp[a][q] = R::get(mine, q, a, j);
+                if constexpr (PARTS == 1) off[a] = q4_mfma<F16>(xp[a][0], q4_minus_24<F16>(), off[a]);
             }
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                const u32x4 w = q4_expand<F16>(s.q[b][j], one);
-                const float d = f16_bits_to_f32((uint16_t)(s.d[b][j / 2] >> (16 * (j & 1))));
+                float d = f16_bits_to_f32((uint16_t)(s.d[b][j / 2] >> (16 * (j & 1))));
+                u32x4 w;
+                if constexpr (PARTS == 1) {
+                    w = q4_expand<F16>(s.q[b][j], one);
+                } else {
+                    w = q4_expand_signed(s.q[b][j]);
+                    d *= 16.0f;
+                }
 #pragma unroll
                 for (int a = 0; a < MT; ++a) {
                     floatx4 t = off[a];
@@ -393,107 +446,84 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
             }
         }
     });
-    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, lds);
-}
-
-// Eight scales for each of a group's four instructions, from 128 in one load:
-// lane i of the wave's 16-lane row r holds scales 8 (i + r) .. + 7, so what the
-// row needs for instruction j (from 32 j + 8 r on) is in its lane 4 j.  Four
-// loads instead, 16 lanes to an address, cost the vector memory path as much as
-// 4 KB (64 cycles a step; it bound one row: 4096 -> 16,384 16.6 us, XX).
-__device__ __forceinline__ u32x4 q4_load_scales(const uint16_t* d) {
-    const uint32_t lane = threadIdx.x & 63;
-    return reinterpret_cast<const u32x4*>(d)[(lane + lane / 16) & 15];
-}
-template <int J>
-__device__ __forceinline__ u32x4 q4_scales(u32x4 d) {
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int v = (int)d[i];
-        r[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, v, 0x150 + 4 * J, 0xf, 0xf, true);
-    }
-    return r;
-}
-__device__ __forceinline__ u32x4 q4_scales(u32x4 d, int j) {  // j unrolled
-    return j == 0 ? q4_scales<0>(d) : j == 1 ? q4_scales<1>(d) : j == 2 ? q4_scales<2>(d) : q4_scales<3>(d);
+    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 // dx = dy W of F32 rows: 16 NT input features (NT 1 or 2: within one block of
-// scales) and 16 MT rows a block.
-template <int MT, int NT, int W, bool WIDE>
+// scales) and ROWS rows a block.  dy times the scale (F32) enters as three parts.
+template <int ROWS, int NT, int W>
 __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
-    constexpr int DT = SPC_F32;
-    __shared__ floatx4 lds[W * MT * NT * 64];
+    typedef Q4Rows<SPC_F32, ROWS> R;
+    constexpr int MT = R::MT;
+    constexpr size_t WAVE = 3 * ROWS * R::STRIDE;
+    __shared__ __attribute__((aligned(16))) char lds[q4_lds(WAVE, MT * NT, W)];
     const uint32_t lane = threadIdx.x & 63;
-    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * 16 * MT;
+    char* mine = lds + (threadIdx.x >> 6) * WAVE;
+    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * ROWS;
     struct Step {
         u32x4 q[NT];
-        u32x4 d;     // scales along the summed features
-        Q4Row<DT> x[MT][4];
+        u32x2 d;  // the scales of this lane's four summed features
+        u32x4 x[R::NI];
     };
-    const char* row[MT];
-    q4_rows<DT, MT>(p, row0, row);
+    const R rows(p.x, p.x_stride, row0, p.m);
     const uint16_t* scales = p.scales + tile0 / 2 * p.groups * kQ4Group;
     auto load = [&](Step& s, int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < NT; ++b)
             s.q[b] = (reinterpret_cast<const u32x4*>(p.quants) + ((tile0 + b) * p.groups + g) * 64)[lane];
-        s.d = q4_load_scales(scales + (int64_t)g * kQ4Group);
-#pragma unroll
-        for (int a = 0; a < MT; ++a) q4_load_rows<DT, WIDE>(s.x[a], row[a], g, p.sum);
+        s.d = reinterpret_cast<const u32x2*>(scales + (int64_t)g * kQ4Group)[lane % 32];
+        rows.load(s.x, g, p.sum);
     };
-    floatx4 acc[MT][NT], off[MT];
+    floatx4 acc[MT][NT];
 #pragma unroll
-    for (int a = 0; a < MT; ++a) {
-        off[a] = floatx4{0, 0, 0, 0};
+    for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0, 0, 0, 0};
-    }
-    const uint32_t one = q4_one<false>();
     q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
+        q4_wave_sync();
+#pragma unroll
+        for (int i = 0; i < R::NI; ++i) {
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                f[e] = __uint_as_float(s.x[i][e]) *
+                       f16_bits_to_f32((uint16_t)(s.d[e / 2] >> (16 * (e & 1))));
+            R::put_parts(mine, i, f);
+        }
+        q4_wave_sync();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             u32x4 w[NT];
 #pragma unroll
-            for (int b = 0; b < NT; ++b) w[b] = q4_expand<false>(s.q[b][j], one);
-            const u32x4 d = q4_scales(s.d, j);
+            for (int b = 0; b < NT; ++b) w[b] = q4_expand_signed(s.q[b][j]);
 #pragma unroll
-            for (int a = 0; a < MT; ++a) {
-                float v[8];
-                q4_row_floats(s.x[a][j], v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    v[e] *= f16_bits_to_f32((uint16_t)(d[e / 2] >> (16 * (e & 1))));
-                u32x4 xp[3];
-                q4_split(v, xp);
+            for (int a = 0; a < MT; ++a)
 #pragma unroll
                 for (int q = 0; q < 3; ++q) {
-                    off[a] = q4_mfma<false>(xp[q], q4_minus_24<false>(), off[a]);
+                    const u32x4 xp = R::get(mine, q, a, j);
 #pragma unroll
-                    for (int b = 0; b < NT; ++b) acc[a][b] = q4_mfma<false>(xp[q], w[b], acc[a][b]);
+                    for (int b = 0; b < NT; ++b) acc[a][b] = q4_mfma<false>(xp, w[b], acc[a][b]);
                 }
-            }
         }
     });
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] += off[a];
-    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, lds);
+        for (int b = 0; b < NT; ++b) acc[a][b] *= 16.0f;
+    q4_finish<SPC_F32, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 // ---- the gradient of 16-bit rows -------------------------------------------
 // Multiplying the rows by a scale that differs for every 32 columns costs six
-// instructions an element and block of columns, and their split into two parts
-// three matrix instructions a tile, which bound 16-bit rows
-// (16 rows, 4096 -> 16,384: 23 us of a floor of 8).  Here the weights take the
-// scale, f16(d (q - 8)), rounded to 11 bits -- at most 2^-11 of a weight, an
-// eighth of a bf16 output's own rounding and as much as an f16 output's -- and
-// the rows enter as f16 whatever their columns: f16 rows as they are, bf16 rows
-// with their exponents moved into f16's range by a power of two that each wave
-// chooses for each row from what it has seen of it (exact for values down to
-// 2^-27 of the row's largest; of smaller ones less than 2^-28 of it is lost).
+// instructions an element and block of columns, and their split into parts
+// three matrix instructions a tile, which bound 16-bit rows (16 rows, 4096 ->
+// 16,384: 23 us of a floor of 8).  Here the weights take the scale, f16(d (q -
+// 8)), rounded to 11 bits -- at most 2^-11 of a weight, an eighth of a bf16
+// output's own rounding and as much as an f16 output's -- and the rows enter as
+// f16 whatever their columns: f16 rows as they are, bf16 rows with their
+// exponents moved into f16's range by a power of two that each wave chooses for
+// each row from what it has seen of it (exact for values down to 2^-27 of the
+// row's largest; of smaller ones less than 2^-28 of it is lost).
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -515,34 +545,39 @@ __device__ __forceinline__ u32x4 q4_expand_scaled(uint32_t w, u32x4 d, uint32_t 
 
 // A row's exponent bias: what is taken off its bf16 exponents to make f16's.
 // The row's largest value seen so far has f16 exponent 28 when the bias is
-// set, so it may grow by 2^2 before the bias has to move.
+// set, so it may grow by 2^2 before the bias has to move.  A step only looks
+// for values past that in its lane; the row's maximum is formed when one is
+// found (every step: 16 rows, 4096 -> 16,384, 22.5 us, 21.0 so).
 struct Q4Bias {
-    uint32_t top = 0;  // largest magnitude seen, bf16 bits
+    u16x2 seen = {0, 0};   // the lane's largest magnitudes, bf16 bits
+    u16x2 limit = {0, 0};  // largest that fits; 0 until the row has one but 0
     int bias = 0;
 
-    // Takes a group's elements in (all lanes of a row agree); true if the bias
-    // moves, by `*by`.
-    __device__ __forceinline__ bool see(const Q4Row<SPC_BF16> (&r)[4], int* by) {
+    // Takes a step's elements in; true if one does not fit.
+    __device__ __forceinline__ bool see(u32x4 v) {
         u16x2 m = {0, 0};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, r[j].w[0][i] & 0x7fff7fffu));
-        uint32_t t = max((uint32_t)m.x, (uint32_t)m.y);
-        // over the four lanes of a row
-        const auto s = __builtin_amdgcn_permlane16_swap(t, t, false, false);
-        t = max(s[0], s[1]);
-        const auto u = __builtin_amdgcn_permlane32_swap(t, t, false, false);
-        t = max(u[0], u[1]);
-        const uint32_t had = top;
-        top = max(top, t);
-        const int e = (int)(top >> 7);
-        const bool move = e - bias > 30 || (had == 0 && top != 0);
-        const int to = move ? max(e - 28, 0) : bias;
-        *by = to - bias;
+        for (int i = 0; i < 4; ++i)
+            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+        seen = __builtin_elementwise_max(seen, m);
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(m, limit)) != 0;
+    }
+    // The largest magnitude the row's 16 lanes have seen.
+    __device__ __forceinline__ int top() const {
+        int t = max((int)seen.x, (int)seen.y);
+        t = max(t, __builtin_amdgcn_update_dpp(0, t, 0xB1, 0xf, 0xf, true));    // lane ^ 1
+        t = max(t, __builtin_amdgcn_update_dpp(0, t, 0x4E, 0xf, 0xf, true));    // lane ^ 2
+        t = max(t, __builtin_amdgcn_update_dpp(0, t, 0x141, 0xf, 0xf, true));   // mirror in 8
+        return max(t, __builtin_amdgcn_update_dpp(0, t, 0x140, 0xf, 0xf, true));  // in 16
+    }
+    // Moves the bias if the row needs it; by how much.
+    __device__ __forceinline__ int move() {
+        const int t = top(), e = t >> 7;
+        const int to = e > bias + 30 || (limit.x == 0 && t != 0) ? max(e - 28, 0) : bias;
+        const int by = to - bias;
         bias = to;
-        return move;
+        if (t != 0) limit = (u16x2)(uint16_t)(((bias + 31) << 7) - 1);
+        return by;
     }
     // bf16 -> f16 with the bias taken off; what falls below f16's range is 0
     // (or, in the last binade, loses its leading bit).
@@ -560,189 +595,153 @@ struct Q4Bias {
     // What a sum of the moved values is to be multiplied by; NaN for a row
     // with an infinity or NaN.
     __device__ __forceinline__ float factor() const {
-        return top >= 0x7f80u ? __builtin_nanf("") : ldexpf(1.0f, bias - 112);
+        return top() >= 0x7f80 ? __builtin_nanf("") : ldexpf(1.0f, bias - 112);
     }
 };
 
-// bf16 rows to f16 rows ahead of the product, for products so large that
-// moving the exponents in every column's wave costs more than a kernel: a
-// block a row, the bias from the whole row (largest value to f16 exponent 28),
-// its factor beside it.  Rows of `ld` elements, those past n zero.
-constexpr int kQ4RowThreads = 1024;
-__global__ __launch_bounds__(kQ4RowThreads) void q4_rows_kernel(const uint16_t* __restrict__ x,
-                                                                int64_t x_stride, int n, int ld,
-                                                                uint16_t* __restrict__ y,
-                                                                float* __restrict__ factor) {
-    __shared__ uint32_t ws[kQ4RowThreads / 64];
-    const uint16_t* row = x + (int64_t)blockIdx.x * x_stride;
-    uint32_t top = 0;
-    for (int i = threadIdx.x; i < n; i += kQ4RowThreads) top = max(top, (uint32_t)row[i] & 0x7fffu);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kQ4RowThreads / 64; ++w) top = max(top, ws[w]);
-    Q4Bias b;
-    b.top = top;
-    b.bias = max((int)(top >> 7) - 28, 0);
-    if (threadIdx.x == 0) factor[blockIdx.x] = b.factor();
-    for (int i = 8 * threadIdx.x; i < ld; i += 8 * kQ4RowThreads) {
-        u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i + e < n) v[e / 2] |= (uint32_t)row[i + e] << (16 * (e & 1));
-        *reinterpret_cast<u32x4*>(y + (int64_t)blockIdx.x * ld + i) = b.f16(v);
-    }
-}
-
-// dx = dy W of 16-bit rows: 16 NT input features and 16 MT rows a block.  MOVED:
-// rows of q4_rows_kernel (OT the output's type).
-template <int OT, bool MOVED, int MT, int NT, int W, bool WIDE>
+// dx = dy W of 16-bit rows: 16 NT input features (NT 1 or 2: within one block
+// of scales) and ROWS rows a block.
+template <int DT, int ROWS, int NT, int W>
 __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
-    constexpr int DT = MOVED ? SPC_F16 : OT;
-    constexpr int KB = (NT + 1) / 2;  // blocks of scales
-    __shared__ floatx4 lds[W * MT * NT * 64];
+    typedef Q4Rows<DT, ROWS> R;
+    constexpr int MT = R::MT, NI = R::NI;
+    constexpr size_t SCALES = ROWS * R::STRIDE, FACTORS = SCALES + kQ4Group * 2;
+    constexpr size_t WAVE = FACTORS + (ROWS * 4 + 15) / 16 * 16;
+    __shared__ __attribute__((aligned(16))) char lds[q4_lds(WAVE, MT * NT, W)];
     const uint32_t lane = threadIdx.x & 63;
-    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * 16 * MT;
+    char* mine = lds + (threadIdx.x >> 6) * WAVE;
+    u32x4* scales = reinterpret_cast<u32x4*>(mine + SCALES);  // [16]
+    const int64_t tile0 = (int64_t)blockIdx.x * NT, row0 = (int64_t)blockIdx.y * ROWS;
     struct Step {
         u32x4 q[NT];
-        u32x4 d[KB];  // scales along the summed features
-        Q4Row<DT> x[MT][4];
+        u32x4 d;  // scales 8 (lane % 16) .. + 7 along the summed features
+        u32x4 x[NI];
     };
-    const char* row[MT];
-    q4_rows<DT, MT>(p, row0, row);
-    const int64_t last = p.col_tiles - 1;
+    const R rows(p.x, p.x_stride, row0, p.m);
+    const uint16_t* all_scales = p.scales + tile0 / 2 * p.groups * kQ4Group;
     auto load = [&](Step& s, int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < NT; ++b)
-            s.q[b] = (reinterpret_cast<const u32x4*>(p.quants) +
-                      (min(tile0 + b, last) * p.groups + g) * 64)[lane];
-#pragma unroll
-        for (int k = 0; k < KB; ++k)
-            s.d[k] = q4_load_scales(p.scales + (min(tile0 + 2 * k, last) / 2 * p.groups + g) * kQ4Group);
-#pragma unroll
-        for (int a = 0; a < MT; ++a) q4_load_rows<DT, WIDE>(s.x[a], row[a], g, p.sum);
+            s.q[b] = (reinterpret_cast<const u32x4*>(p.quants) + ((tile0 + b) * p.groups + g) * 64)[lane];
+        s.d = reinterpret_cast<const u32x4*>(all_scales + (int64_t)g * kQ4Group)[lane % 16];
+        rows.load(s.x, g, p.sum);
     };
     floatx4 acc[MT][NT];
-    Q4Bias bias[MT];
+    Q4Bias bias[NI];
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0, 0, 0, 0};
-    // the accumulator rows' factors: row 4 (lane / 16) + i is lane row's % 16
-    auto scale_rows = [&](int a, float f) __attribute__((always_inline)) {
+    // multiplies the accumulators' rows by the factors f(i) of the loads' rows
+    auto scale_rows = [&](auto&& f) __attribute__((always_inline)) {
+        float* fs = reinterpret_cast<float*>(mine + FACTORS);
+        q4_wave_sync();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float fi = __shfl(f, 4 * (lane / 16) + i);
+        for (int i = 0; i < NI; ++i)
+            if (R::chunk() == 0) fs[R::in_tile(i)] = f(i);
+        q4_wave_sync();
 #pragma unroll
-            for (int b = 0; b < NT; ++b) acc[a][b][i] *= fi;
-        }
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float fi = fs[(16 * a + 4 * (lane / 16) + i) % ROWS];
+#pragma unroll
+                for (int b = 0; b < NT; ++b) acc[a][b][i] *= fi;
+            }
     };
     const uint32_t one = q4_one<true>();
     q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
         if constexpr (DT == SPC_BF16) {
+            bool over = false;
 #pragma unroll
-            for (int a = 0; a < MT; ++a) {
-                int by;
-                const bool move = bias[a].see(s.x[a], &by);
-                if (__any(move)) scale_rows(a, ldexpf(1.0f, -by));
+            for (int i = 0; i < NI; ++i) over |= bias[i].see(s.x[i]);
+            if (__any(over)) {
+                float f[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) f[i] = ldexpf(1.0f, -bias[i].move());
+                scale_rows([&](int i) { return f[i]; });
             }
         }
+        q4_wave_sync();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) R::put(mine, i, DT == SPC_BF16 ? bias[i].f16(s.x[i]) : s.x[i]);
+        if (lane < 16) scales[lane] = s.d;
+        q4_wave_sync();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             u32x4 x[MT];
 #pragma unroll
-            for (int a = 0; a < MT; ++a)
-                x[a] = DT == SPC_BF16 ? bias[a].f16(s.x[a][j].w[0]) : s.x[a][j].w[0];
-            u32x4 d[KB];
-#pragma unroll
-            for (int k = 0; k < KB; ++k) d[k] = q4_scales(s.d[k], j);
+            for (int a = 0; a < MT; ++a) x[a] = R::get(mine, 0, a, j);
+            const u32x4 d = scales[4 * j + lane / 16];
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                const u32x4 w = q4_expand_scaled(s.q[b][j], d[b / 2], one);
+                const u32x4 w = q4_expand_scaled(s.q[b][j], d, one);
 #pragma unroll
                 for (int a = 0; a < MT; ++a) acc[a][b] = q4_mfma<true>(x[a], w, acc[a][b]);
             }
         }
     });
-    if constexpr (MOVED || DT == SPC_BF16) {
+    if constexpr (DT == SPC_BF16) {
+        float f[NI];
 #pragma unroll
-        for (int a = 0; a < MT; ++a) {
-            float f;
-            if constexpr (MOVED) f = p.factor[min(row0 + 16 * a + lane % 16, p.m - 1)];
-            else f = bias[a].factor();
-            scale_rows(a, f);
-        }
+        for (int i = 0; i < NI; ++i) f[i] = bias[i].factor();
+        scale_rows([&](int i) { return f[i]; });
     }
-    q4_finish<OT, MT, NT, W>(p, acc, row0, tile0 * 16, lds);
+    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
-template <int DT, int MT, int NT, int W>
+template <int DT, int ROWS, int NT, int W>
 void q4_forward_launch(hipStream_t s, const Q4Args& p) {
-    const dim3 grid((unsigned)ceil_div(p.col_tiles, NT), (unsigned)ceil_div(p.m, 16 * MT));
-    if (p.wide) q4_forward_kernel<DT, MT, NT, W, true><<<grid, 64 * W, 0, s>>>(p);
-    else q4_forward_kernel<DT, MT, NT, W, false><<<grid, 64 * W, 0, s>>>(p);
+    const dim3 grid((unsigned)ceil_div(p.col_tiles, NT), (unsigned)ceil_div(p.m, ROWS));
+    q4_forward_kernel<DT, ROWS, NT, W><<<grid, 64 * W, 0, s>>>(p);
 }
 
-template <int DT, int MT, int NT, int W>
+template <int DT, int ROWS, int NT, int W>
 void q4_grad_launch(hipStream_t s, const Q4Args& p) {
-    const dim3 grid((unsigned)ceil_div(p.col_tiles, NT), (unsigned)ceil_div(p.m, 16 * MT));
-    if constexpr (DT == SPC_F32) {
-        if (p.wide) q4_grad_kernel<MT, NT, W, true><<<grid, 64 * W, 0, s>>>(p);
-        else q4_grad_kernel<MT, NT, W, false><<<grid, 64 * W, 0, s>>>(p);
-    } else {
-        if (DT == SPC_BF16 && p.factor)
-            q4_grad16_kernel<DT, DT == SPC_BF16, MT, NT, W, true><<<grid, 64 * W, 0, s>>>(p);
-        else if (p.wide) q4_grad16_kernel<DT, false, MT, NT, W, true><<<grid, 64 * W, 0, s>>>(p);
-        else q4_grad16_kernel<DT, false, MT, NT, W, false><<<grid, 64 * W, 0, s>>>(p);
-    }
+    const dim3 grid((unsigned)(p.col_tiles / NT), (unsigned)ceil_div(p.m, ROWS));
+    if constexpr (DT == SPC_F32) q4_grad_kernel<ROWS, NT, W><<<grid, 64 * W, 0, s>>>(p);
+    else q4_grad16_kernel<DT, ROWS, NT, W><<<grid, 64 * W, 0, s>>>(p);
+}
+
+// f(ROWS) with the fewest rows a block that hold m, at most 32 (F32, whose
+// three operands take as much LDS as that: 16).
+template <int DT, typename F>
+void q4_row_tile(int64_t m, F&& f) {
+    if (m <= 4) f(std::integral_constant<int, 4>{});
+    else if (m <= 8) f(std::integral_constant<int, 8>{});
+    else if (m <= 16 || DT == SPC_F32) f(std::integral_constant<int, 16>{});
+    else if constexpr (DT != SPC_F32) f(std::integral_constant<int, 32>{});
+}
+
+// Two column tiles a wave where that leaves a block for every CU: each reads
+// (and converts) the rows half as often.  us with one / two: 8192 -> 16,384, one
+// bf16 row 15.1 / 14.8, eight 17.6 / 16.3, sixteen 22.4 / 17.9, two F32 rows
+// 26.7 / 20.4; 4096 -> 4096 (256 tiles), one 4.5 / 5.4, forty 13.1 / 9.9; the
+// gradient of 8192 -> 16,384, one 20.1 / 18.6, sixteen 34.5 / 25.8, of 4096 ->
+// 16,384 (256 tiles), sixteen 21.6 / 25.1.  Four tiles gain 1 us at F32 and
+// lose elsewhere.
+template <int ROWS>
+inline bool q4_two_tiles(const Q4Args& p) {
+    return p.col_tiles * ceil_div(p.m, ROWS) >= 512;
 }
 
 template <int DT>
 hipError_t q4_forward(hipStream_t s, const Q4Args& p) {
-    // F32 rows hold three operands each: two row tiles at most
-    // More column tiles a wave read the rows (and split F32 ones) less often, as
-    // long as 256 blocks are left for the CUs.  us with 1 / 2 / 4 tiles: 8192 ->
-    // 16,384, one bf16 row 16.2 / 15.0 / 15.7, eight 25.6 / 18.0 / 16.3, sixteen
-    // 36.0 / 22.3 / 17.5, two F32 rows 36.7 / 28.3 / 22.6; 4096 -> 8192, one
-    // 6.8 / 6.4 / 8.7, sixteen 11.8 / 8.5 / 9.9; 4096 -> 4096, one 4.6 / 5.4 / 7.8.
-    if (p.m <= 16) {
-        if (p.col_tiles >= 1024 && (p.m > 4 || DT == SPC_F32)) q4_forward_launch<DT, 1, 4, 8>(s, p);
-        else if (p.col_tiles >= 512) q4_forward_launch<DT, 1, 2, 8>(s, p);
-        else q4_forward_launch<DT, 1, 1, 8>(s, p);
-    } else if (p.m <= 32 || DT == SPC_F32) {
-        q4_forward_launch<DT, 2, 1, 8>(s, p);
-    } else if constexpr (DT != SPC_F32) {
-        q4_forward_launch<DT, 4, 1, 8>(s, p);
-    }
+    q4_row_tile<DT>(p.m, [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value;
+        if (q4_two_tiles<ROWS>(p)) q4_forward_launch<DT, ROWS, 2, 8>(s, p);
+        else q4_forward_launch<DT, ROWS, 1, 8>(s, p);
+    });
     return hipGetLastError();
 }
 
-// bf16 rows moved to f16 ahead of the product (q4_rows_kernel): from XX column
-// tiles times groups on.
-inline bool q4_moves_rows(int dtype, const Q4Layout& l) {
-    return dtype == SPC_BF16 && l.col_tiles * l.groups >= 16384;
-}
-
 template <int DT>
-hipError_t q4_grad(hipStream_t s, Q4Args p, void* workspace) {
-    if (workspace) {
-        const int ld = (p.sum + 7) / 8 * 8;
-        float* factor = static_cast<float*>(workspace);
-        uint16_t* rows = reinterpret_cast<uint16_t*>(factor + (p.m + 3) / 4 * 4);
-        q4_rows_kernel<<<(unsigned)p.m, kQ4RowThreads, 0, s>>>(static_cast<const uint16_t*>(p.x),
-                                                               p.x_stride, p.sum, ld, rows, factor);
-        p.x = rows;
-        p.x_stride = p.sum = ld;
-        p.factor = factor;
-    }
-    if (p.m <= 16) {
-        if (p.col_tiles >= 512) q4_grad_launch<DT, 1, 2, 8>(s, p);
-        else q4_grad_launch<DT, 1, 1, 8>(s, p);
-    } else {
-        q4_grad_launch<DT, 2, 2, 8>(s, p);
-    }
+hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
+    q4_row_tile<DT>(p.m, [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value;
+        if (q4_two_tiles<ROWS>(p)) q4_grad_launch<DT, ROWS, 2, 8>(s, p);
+        else q4_grad_launch<DT, ROWS, 1, 8>(s, p);
+    });
     return hipGetLastError();
 }
 
@@ -784,7 +783,6 @@ int q4_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t 
     p->col_tiles = l.col_tiles;
     p->quants = static_cast<const uint32_t*>(packed);
     p->scales = reinterpret_cast<const uint16_t*>(static_cast<const char*>(packed) + l.quant_bytes);
-    p->wide = (uintptr_t)x % 16 == 0 && x_stride * e % 16 == 0 && l.sum % 8 == 0;
     p->y = y;
     return SPC_OK;
 }
@@ -857,35 +855,18 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
     return e == hipSuccess ? SPC_OK : hip_status(e, "spc_linear_q4_0 launch");
 }
 
-size_t spc_linear_q4_0_input_grad_workspace_bytes(int dtype, int64_t m, int64_t out_features,
-                                                  int64_t in_features) {
-    if (m < 1 || m > (int64_t)65535 * 16 ||
-        spc_linear_q4_0_packed_bytes(out_features, in_features, 1) == 0)
-        return 0;
-    if (!q4_moves_rows(dtype, q4_layout(out_features, in_features, true))) return 0;
-    return (size_t)((m + 3) / 4 * 16 + m * ((out_features + 7) / 8 * 16));
-}
-
 int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                                int64_t m, const void* packed, int64_t out_features,
-                               int64_t in_features, void* dx, void* workspace,
-                               size_t workspace_bytes) {
-    const char* fn = "spc_linear_q4_0_input_grad";
+                               int64_t in_features, void* dx) {
     Q4Args p;
-    const int st = q4_args(fn, dtype, dy, dy_stride, m, packed, out_features, in_features, true, dx, &p);
+    const int st = q4_args("spc_linear_q4_0_input_grad", dtype, dy, dy_stride, m, packed, out_features,
+                           in_features, true, dx, &p);
     if (st != SPC_OK) return st;
     if (m == 0) return SPC_OK;
-    const size_t need =
-        spc_linear_q4_0_input_grad_workspace_bytes(dtype, m, out_features, in_features);
-    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) {
-        set_last_error("%s: workspace missing, misaligned (16 bytes) or too small", fn);
-        return SPC_BAD_ARG;
-    }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    void* ws = need ? workspace : nullptr;
-    const hipError_t e = dtype == SPC_BF16  ? q4_grad<SPC_BF16>(s, p, ws)
-                         : dtype == SPC_F16 ? q4_grad<SPC_F16>(s, p, ws)
-                                            : q4_grad<SPC_F32>(s, p, ws);
+    const hipError_t e = dtype == SPC_BF16  ? q4_grad<SPC_BF16>(s, p)
+                         : dtype == SPC_F16 ? q4_grad<SPC_F16>(s, p)
+                                            : q4_grad<SPC_F32>(s, p);
     return e == hipSuccess ? SPC_OK : hip_status(e, "spc_linear_q4_0_input_grad launch");
 }
 

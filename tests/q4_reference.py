@@ -2,10 +2,10 @@
 kernels' F32 sums.
 
 u = 2^-24.  A matrix instruction adds 32 exact products to its accumulator with
-at most 32 roundings, each at most 2 u (a cut) of the magnitudes so far.  The
-weights enter as 16 + q beside a sum of -24, so a block's magnitudes are at most
-sum |x| d (31 + 24 + 24).  F32 rows enter as three parts that add up exactly, so
-three instructions each.
+at most 32 roundings, each at most 2 u (a cut) of the magnitudes so far.  Under
+16-bit rows the weights enter as 16 + q beside a sum of -24, so a block's
+magnitudes are at most sum |x| d (31 + 24 + 24).  F32 rows enter as three parts
+that add up exactly, so three instructions each, on the weights themselves.
 """
 import numpy as np
 import torch
@@ -38,12 +38,13 @@ def dequant(blocks):
 
 def product(x, blocks, bias=None):
     """(y, bound before the output's rounding) for x [m, in]."""
+    f32 = x.dtype == torch.float32
     x = x.detach().cpu().double()
     w = dequant(blocks)
     d = parts(blocks)[0].abs().repeat_interleave(32, 1)
-    n = 3 if x.abs().numel() and not torch.equal(x, x.to(torch.bfloat16).double()) else 1
     y = x @ w.t()
-    e = 2 * 32 * n * U * 79 * (x.abs() @ d.t()) + (w.shape[1] // 32 + 12) * U * (x.abs() @ w.abs().t())
+    e = 2 * 96 * U * (x.abs() @ w.abs().t()) if f32 else 2 * 32 * U * 79 * (x.abs() @ d.t())
+    e = e + (w.shape[1] // 32 + 12) * U * (x.abs() @ w.abs().t())
     if bias is not None:
         bias = bias.detach().cpu().double()
         y = y + bias
@@ -54,8 +55,7 @@ def product(x, blocks, bias=None):
 def gradient(dy, blocks):
     """(dx, bound before the output's rounding) for dy [m, out].
 
-    F32 rows: dy d rounded once (u), three parts against 16 + q and -24 as
-    above.  16-bit rows: the weights rounded to f16 (2^-11 of each; subnormal
+    F32 rows: dy d rounded once (u), three parts as above.  16-bit rows: the weights rounded to f16 (2^-11 of each; subnormal
     ones are multiples of their scale's last bit, so exact), bf16 rows without
     what lies below 2^-28 of the row's largest value; one instruction a group
     of 32."""
@@ -63,13 +63,9 @@ def gradient(dy, blocks):
     bf16 = dy.dtype == torch.bfloat16
     dy = dy.detach().cpu().double()
     w = dequant(blocks)
-    d = parts(blocks)[0].abs().repeat_interleave(32, 1)
     # eight waves share the summed features: instructions on one accumulator
     chain = (3 if f32 else 1) * (-(-w.shape[0] // 128) // 8 + 1) * 4
-    if f32:
-        e = U * (dy.abs() @ w.abs()) + 2 * (32 + chain + 12) * U * 79 * (dy.abs() @ d)
-    else:
-        e = (2.0 ** -11 + 2 * (32 + chain + 12) * U) * (dy.abs() @ w.abs())
-        if bf16 and dy.numel():
-            e = e + 2.0 ** -28 * dy.abs().amax(1, keepdim=True) * w.abs().sum(0)
+    e = ((U if f32 else 2.0 ** -11) + 2 * (32 + chain + 12) * U) * (dy.abs() @ w.abs())
+    if bf16 and dy.numel():
+        e = e + 2.0 ** -28 * dy.abs().amax(1, keepdim=True) * w.abs().sum(0)
     return dy @ w, e

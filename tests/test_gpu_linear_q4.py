@@ -138,11 +138,8 @@ def test_large_and_small_magnitudes(spc, dev):
 @pytest.mark.parametrize("out,inp", [(2500, 96), (2051, 15_456)])
 def test_gradient_rows_of_any_range(spc, dev, dt, out, inp):
     """Rows whose magnitudes lie anywhere and change along the row by 2^20 and
-    more: zeros first, growing, falling, single large and single tiny values.
-    The second shape moves bf16 rows to f16 ahead of the product."""
+    more: zeros first, growing, falling, single large and single tiny values."""
     nat = spc._native
-    moved = nat.lib().spc_linear_q4_0_input_grad_workspace_bytes(nat.dtype_code(DT[dt]), 19, out, inp)
-    assert (moved > 0) == (dt == "bf16" and inp > 10_000)
     blocks = random_blocks(out, inp, 8)
     _, bwd = _both(nat, blocks, dev)
     g = torch.Generator().manual_seed(3)
@@ -168,7 +165,7 @@ def test_gradient_rows_of_any_range(spc, dev, dt, out, inp):
     if dt == "f32":
         # parts of dy d below 2^-126 count as zero: of an element's three cuts
         # (each below 2^-7 of the one before) less than 2^-125 in all, times |q - 8|
-        # <= 8; the two sums (16 + q, -24) lose the same parts
+        # <= 8
         bound = bound + out * 2.0 ** -122
     got = nat.linear_q4_0_input_grad(dy, bwd)
     check(f"any range {dt}", got, dx, bound, DT[dt])

@@ -42,7 +42,7 @@ def test_host_validation(spc):
     def run(fn, dtype=nat.BF16, x=fake, stride=64, m=1, w=fake, y=fake):
         if fn == "y":
             return L.spc_linear_q4_0(None, dtype, x, stride, m, w, 64, 64, None, 0, y)
-        return L.spc_linear_q4_0_input_grad(None, dtype, x, stride, m, w, 64, 64, y, None, 0)
+        return L.spc_linear_q4_0_input_grad(None, dtype, x, stride, m, w, 64, 64, y)
 
     for fn in ("y", "dx"):
         assert run(fn, m=0, x=None, w=None, y=None) == nat.OK
@@ -53,15 +53,6 @@ def test_host_validation(spc):
         assert run(fn, x=fake + 1) == nat.BAD_ARG and run(fn, w=fake + 8) == nat.BAD_ARG
         assert run(fn, y=fake + 2, dtype=nat.F32) == nat.BAD_ARG
         assert b"misaligned" in L.spc_last_error()
-    # large products of bf16 rows need a workspace
-    need = L.spc_linear_q4_0_input_grad_workspace_bytes(nat.BF16, 3, 16384, 8192)
-    assert need >= 3 * (4 + 2 * 16384)
-    assert L.spc_linear_q4_0_input_grad_workspace_bytes(nat.F32, 3, 16384, 8192) == 0
-    assert L.spc_linear_q4_0_input_grad_workspace_bytes(nat.BF16, 3, 64, 64) == 0
-    for ws, size in ((None, need), (fake + 4, need), (fake, need - 1)):
-        assert L.spc_linear_q4_0_input_grad(None, nat.BF16, fake, 16384, 3, fake, 16384, 8192, fake, ws,
-                                            size) == nat.BAD_ARG
-    assert b"workspace" in L.spc_last_error()
     assert L.spc_linear_q4_0(None, nat.BF16, fake, 64, 1, fake, 64, 64, fake, 9, fake) == nat.BAD_ARG
     assert L.spc_linear_q4_0(None, nat.BF16, fake, 64, 1, fake, 64, 64, fake + 2, 0, fake) == nat.BAD_ARG
 
