@@ -623,8 +623,8 @@ typedef struct {
  * apart; mean and biased variance over a row in F32 (mean first, then the
  * squares of the differences), every step in F32, rounded once to dtype.
  * (spc_layernorm_silu rounds between the steps, as the block's tensors do.)
- * stats: f32 [n, 2], (mean, 1 / sqrt(var + eps)) of every row of an item, for
- * the gradient, or NULL.  y may be x when x_stride is c.  c <= 8192, n_batch
+ * stats: f32 [n, 2], (mean, 1 / sqrt(var + eps)) of every row (zeros for rows
+ * of no item), for the gradient, or NULL.  y may be x when x_stride is c.  c <= 8192, n_batch
  * <= 65535. */
 int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
                    int64_t c, const spc_layer_norm_params* params, void* y, float* stats);

@@ -770,6 +770,14 @@ def _strided_rows(x: torch.Tensor, name: str):
     return x, n, c, stride if n > 1 else c
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two strided tensors meet."""
+    def end(t):
+        return t.data_ptr() + t.element_size() * (
+            1 + sum((k - 1) * st for k, st in zip(t.shape, t.stride())))
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+
+
 def _param_pair(a, b, width: int, names: str, dtype: torch.dtype):
     """Two parameter tensors [width] (or None), both float32 or both `dtype`."""
     for t in (a, b):
@@ -841,9 +849,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         out = x.new_empty((n, c))
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of x's shape and dtype")
-    # rows of no item have no statistics: zeros, not what the memory held
-    stats = None if not return_stats else (torch.empty if offsets is None else torch.zeros)(
-        (n, 2), dtype=torch.float32, device=dev)
+    elif n and not (out.data_ptr() == x.data_ptr() and stride == c) and _overlap(out, x):
+        raise ValueError("out must be x or lie apart from it")
+    stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if return_stats else None
     st = _launch(lib().spc_layer_norm, dev, dt, x.data_ptr(), stride, n, c, p, out.data_ptr(),
                  _ptr(stats))
     if st:

@@ -384,15 +384,19 @@ __device__ __forceinline__ void ln_squares(const float (&v)[NV][LnElem<DT>::V], 
     }
 }
 
-// Zeros for the chunk's rows that belong to no item: [lo, first) and [end, hi).
+// Zeros for the chunk's rows that belong to no item: [lo, first) and [end, hi)
+// (of the forward pass their statistics too).
 template <int DT, int T, int NV, bool TAIL>
 __device__ __forceinline__ void ln_zero_rows(const LnArgs& p, int64_t lo, int64_t first, int64_t end,
-                                             int64_t hi, int lane) {
+                                             int64_t hi, int lane, float* stats) {
     constexpr int TPB = kLnThreads / T;
-    if ((lo == first && end >= hi) || !p.y) return;
+    if (lo == first && end >= hi) return;
     const float z[NV][LnElem<DT>::V] = {};
-    for (int64_t row = lo + threadIdx.x / T; row < hi; row += TPB)
-        if (row < first || row >= end) ln_store<DT, T, NV, TAIL>(p.y, row * p.c, p.c, lane, z);
+    for (int64_t row = lo + threadIdx.x / T; row < hi; row += TPB) {
+        if (row >= first && row < end) continue;
+        if (p.y) ln_store<DT, T, NV, TAIL>(p.y, row * p.c, p.c, lane, z);
+        if (stats && lane == 0) stats[2 * row] = stats[2 * row + 1] = 0.0f;
+    }
 }
 
 template <int DT, int T, int NV, bool TAIL, bool SILU>
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
         }
         first = last;
     }
-    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane);
+    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane, p.stats);
 }
 
 // Adds a segment's sums over the block's teams and writes them to the slot of
@@ -608,7 +612,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(LnArgs p) {
         }
         first = last;
     }
-    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane);
+    if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane, nullptr);
 }
 
 // Lanes of a team and vectors a lane for c channels: f(T, NV).  As many rows to

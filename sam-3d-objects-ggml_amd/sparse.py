@@ -922,11 +922,23 @@ def batch_offsets(x: SparseTensor) -> torch.Tensor:
     return torch.tensor(offs, dtype=torch.int64).to(x.feats.device, non_blocking=True)
 
 
-def _item_offsets(x: SparseTensor) -> torch.Tensor:
-    """batch_offsets(x), kept with the coordinates per layout (a copy from the
-    host, which a captured graph cannot hold)."""
+def _item_offsets(x: SparseTensor) -> Optional[torch.Tensor]:
+    """batch_offsets(x), kept with the coordinates per layout (None: one item
+    of all rows)."""
     rows = tuple((sl.start, sl.stop) for sl in x.layout)
-    return x.data.cached(("offsets", rows), lambda c: batch_offsets(x))
+    if rows == ((0, x.feats.shape[0]),):
+        return None
+
+    def build(c):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the items' row offsets are copied from the host by the first call on "
+                               "these coordinates: run one before capturing a graph")
+        offs = batch_offsets(x)
+        # once: later calls may come on other streams
+        torch.cuda.current_stream(offs.device).synchronize()
+        return offs
+
+    return x.data.cached(("offsets", rows), build)
 
 
 def max_item_rows(x: SparseTensor) -> int:
@@ -976,7 +988,8 @@ class SparseLayerNorm32(nn.LayerNorm):
     modulation * (1 + scale[b]) + shift[b] by the row's batch item
     ([x.shape[0], channels], for instance the halves of a Linear's output) and
     SiLU in the same pass; gradients go to the feats, weight, bias, scale and
-    shift.  Once differentiable."""
+    shift.  With a modulation, rows outside x's layout come out as zeros.  Once
+    differentiable."""
 
     def __init__(self, channels: int, eps: float = 1e-6, elementwise_affine: bool = True,
                  bias: bool = True):

@@ -154,6 +154,34 @@ def test_in_place_and_out(spc, dev):
     assert nat.layer_norm(y, w, b, out=y) is y and torch.equal(y, want)
 
 
+def test_overlapping_out_is_refused(spc, dev):
+    nat = spc._native
+    buf = torch.randn(40, 64, device=dev)
+    for x, out in [(buf[1:], buf[:-1]), (buf[:20, :32], buf.view(-1)[:640].view(20, 32))]:
+        with pytest.raises(ValueError, match="apart"):
+            nat.layer_norm(x, out=out)
+    a, b = buf[:20], buf[20:]
+    assert torch.equal(nat.layer_norm(a, out=b), nat.layer_norm(a))
+
+
+def test_padding_rows_do_not_matter(spc, dev):
+    """Rows of no item: whatever they hold (NaN here) reaches neither the
+    others nor a sum."""
+    nat = spc._native
+    n, c = 300, 136
+    x, w, b, sc, sh, dy = _inputs(dev, torch.bfloat16, n, c, 2, items=3)
+    offsets = [20, 100, 100, 250]
+    kw = dict(scale=sc, shift=sh, offsets=torch.tensor(offsets, device=dev), silu=True)
+    y, st = nat.layer_norm(x, w, b, return_stats=True, **kw)
+    g = nat.layer_norm_backward(dy, x, st, w, b, **kw)
+    out = _items(offsets, n) < 0
+    x[out.to(dev)] = float("nan")
+    dy[out.to(dev)] = float("inf")
+    y2, st2 = nat.layer_norm(x, w, b, return_stats=True, **kw)
+    g2 = nat.layer_norm_backward(dy, x, st2, w, b, **kw)
+    assert all(torch.equal(p, q) for p, q in zip((y, st, *g), (y2, st2, *g2)))
+
+
 def test_equal_calls_equal_bits(spc, dev):
     nat = spc._native
     x, w, b, sc, sh, dy = _inputs(dev, torch.bfloat16, 5000, 320, 1, items=3)
@@ -344,6 +372,29 @@ def test_graph_capture(spc, dev):
         want = step()
         for _, out in graphs:
             assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_module_capture(spc, dev):
+    """The module in a graph: its items' offsets come from a call before."""
+    c, counts = 64, [30, 20]
+    x, _, _, sc, sh, _ = _inputs(dev, torch.bfloat16, 50, c, 3, items=2)
+    ln = spc.sparse.SparseLayerNorm32(c).to(dev)
+    t = _tensor(spc, dev, x, counts)
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                ln(t, sc, sh)
+        torch.cuda.synchronize()
+        ln(t, sc, sh)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ln(t, sc, sh).feats
+        for _ in range(3):
+            x.copy_(torch.randn(50, c, device=dev))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, ln(t, sc, sh).feats)
 
 
 def test_offset_past_32_bits(spc, dev):
