@@ -879,13 +879,15 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor,
     if stats.shape != (n, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("stats must be contiguous float32 [n, 2]")
     p, keep = _layer_norm_params(x, c, weight, bias, 0.0, scale, shift, offsets, silu)
-    dx = x.new_empty((n, c)) if need[0] else None
-    grads = [t.new_empty(t.shape) if t is not None and k else None for t, k in zip(keep, need[1:])]
-    ws, nbytes = None, 0
+    contiguous = torch.contiguous_format
+    dx = torch.empty_like(x, memory_format=contiguous) if need[0] else None
+    grads = [None if t is None or not k else torch.empty_like(t, memory_format=contiguous)
+             for t, k in zip(keep, need[1:])]
+    L, ws, nbytes = lib(), None, 0
     if any(g is not None for g in grads):
-        nbytes = lib().spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
-        ws = _workspace(nbytes, dev)
-    st = _launch(lib().spc_layer_norm_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs,
+        nbytes = L.spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    st = _launch(L.spc_layer_norm_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs,
                  stats.data_ptr(), n, c, p, _ptr(dx), *map(_ptr, grads), _ptr(ws), nbytes)
     if st:
         _check("spc_layer_norm_backward", st)

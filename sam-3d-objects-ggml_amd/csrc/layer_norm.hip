@@ -41,11 +41,6 @@ struct LnFinal {
     float* sums;  // [items][2][c] or null
 };
 
-__device__ __forceinline__ void ln_put(void* p, int dt, int64_t i, float v) {
-    if (dt == SPC_F32) static_cast<float*>(p)[i] = v;
-    else static_cast<uint16_t*>(p)[i] = dt == SPC_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-}
-
 __global__ __launch_bounds__(kLnFinalThreads) void ln_finalize_kernel(LnFinal p) {
     constexpr int C = kLnFinalChannels, L = kLnFinalThreads / C, W = kLnFinalThreads / 64, DEEP = 8;
     __shared__ float ls[2][W][C];
@@ -181,6 +176,12 @@ int ln_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t 
     return SPC_OK;
 }
 
+// Whether one block takes all rows, its sums being the gradients: that saves the
+// second kernel (3 us) and its launch (3 us of the host).  Up to four rounds of a
+// block's teams, two where a row takes half a block or more (us alone / with the
+// second kernel: 16 x 192 4.1 / 6.4, 16 x 1024 7.0 / 7.3, 8 x 2048 8.6 / 7.9).
+inline bool ln_one_block(int64_t n, int teams) { return n > 0 && n <= (teams > 2 ? 4 : 2) * teams; }
+
 // Chunks the backward's row pass makes of n rows.
 inline int64_t ln_backward_chunks(int64_t n, int teams) {
     return ceil_div(n, ln_rows_per(n, teams, kLnBackwardBlocks));
@@ -217,7 +218,8 @@ int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stri
 }
 
 size_t spc_layer_norm_backward_workspace_bytes(int dtype, int64_t n, int64_t c, int64_t n_batch) {
-    if (!ln_float_dtype(dtype) || n < 0 || n > INT32_MAX || c <= 0 || c > kLnMaxC || n_batch < 1 || n_batch > 65535)
+    if (!ln_float_dtype(dtype) || n < 0 || n > INT32_MAX || c <= 0 || c > kLnMaxC || n_batch < 1 ||
+        n_batch > 65535)
         return 0;
     const int64_t slots = ln_backward_chunks(n, ln_teams(dtype, (int)c, true)) + n_batch;
     return (size_t)((slots + n_batch) * 2 * c * (int64_t)sizeof(float));
@@ -248,27 +250,33 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
     if (!dx && !sums) return SPC_OK;
     const int teams = ln_teams(dtype, p.c, true);
     const int64_t chunks = ln_backward_chunks(n, teams);
-    if (sums) {
-        if (!workspace || off(workspace, 4) ||
-            workspace_bytes < spc_layer_norm_backward_workspace_bytes(dtype, n, c, p.nb)) {
-            set_last_error("%s: workspace missing, misaligned or too small", fn);
-            return SPC_BAD_ARG;
-        }
+    // (offsets: rows of no item, and an empty item's zeros, are the second kernel's)
+    const bool alone = sums && ln_one_block(n, teams) && affine != mod && !p.off;
+    if (sums && (!workspace || off(workspace, 4) ||
+                 workspace_bytes < spc_layer_norm_backward_workspace_bytes(dtype, n, c, p.nb))) {
+        set_last_error("%s: workspace missing, misaligned or too small", fn);
+        return SPC_BAD_ARG;
+    }
+    if (alone) {
+        p.grad_a = mod ? dscale : dgamma;
+        p.grad_b = mod ? dshift : dbeta;
+        p.grad_dtype = mod ? p.m_dtype : p.p_dtype;
+    } else if (sums) {
         p.part = static_cast<float*>(workspace);
     }
     p.y = dx;
     p.dy = dy;
     p.dy_stride = dy_stride;
     p.stats = const_cast<float*>(stats);
-    p.rows_per = (int)ln_rows_per(n, teams, kLnBackwardBlocks);
+    p.rows_per = (int)ln_rows_per(n, teams, alone ? 1 : kLnBackwardBlocks);
     if (n > 0) {
-        const unsigned blocks = (unsigned)chunks;
+        const unsigned blocks = alone ? 1 : (unsigned)chunks;
         const hipError_t err = dtype == SPC_BF16  ? ln_backward_bf16(s, p, blocks)
                                : dtype == SPC_F16 ? ln_backward_f16(s, p, blocks)
                                                   : ln_backward_f32(s, p, blocks);
         if (err != hipSuccess) return hip_status(err, "spc_layer_norm_backward launch");
     }
-    if (!sums) return SPC_OK;
+    if (!sums || alone) return SPC_OK;
     LnFinal f{};
     f.part = p.part;
     f.off = p.off;

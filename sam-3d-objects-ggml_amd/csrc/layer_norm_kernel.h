@@ -50,6 +50,11 @@ struct LnArgs {
     void* y;             // y, or dx (null: only the sums)
     float* stats;        // [n, 2] mean, r: written (or null), or read
     float* part;         // [chunks + items][2][c], or null
+    // instead of `part`, where there is one chunk and one item: A and B as the
+    // parameters' gradients themselves
+    void* grad_a;
+    void* grad_b;
+    int grad_dtype;
 };
 
 template <int DT>
@@ -467,6 +472,11 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(LnArgs p) {
     if (p.off) ln_zero_rows<DT, T, NV, TAIL>(p, lo, begin, first, hi, lane, p.stats);
 }
 
+__device__ __forceinline__ void ln_put(void* p, int dt, int64_t i, float v) {
+    if (dt == SPC_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = dt == SPC_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+}
+
 // Adds a segment's sums over the block's teams and writes them to the slot of
 // (chunk, item): chunk + item, since along the rows either index grows from
 // one segment to the next, so the slots are distinct and at most chunks +
@@ -476,6 +486,11 @@ template <int T, int NV, int V>
 __device__ __forceinline__ void ln_flush(const LnArgs& p, int64_t slot, int lane, float* lds,
                                          float (&sum)[NV][V], int which) {
     float* out = p.part + (slot * 2 + which) * p.c;
+    void* grad = which ? p.grad_b : p.grad_a;
+    auto put = [&](int ch, float v) __attribute__((always_inline)) {
+        if (p.part) out[ch] = v;
+        else if (grad) ln_put(grad, p.grad_dtype, ch, v);
+    };
     if constexpr (T < 256) {
         constexpr int W = T * NV * V;              // channels a team covers
         constexpr int COPIES = T > 64 ? 2 : 4;     // teams left once a wave's are added
@@ -498,7 +513,7 @@ __device__ __forceinline__ void ln_flush(const LnArgs& p, int64_t slot, int lane
         for (int ch = threadIdx.x; ch < p.c; ch += kLnThreads) {
             float v = lds[ch] + lds[W + ch];
             if constexpr (COPIES == 4) v += lds[2 * W + ch] + lds[3 * W + ch];
-            out[ch] = v;
+            put(ch, v);
         }
     } else {
 #pragma unroll
@@ -506,7 +521,7 @@ __device__ __forceinline__ void ln_flush(const LnArgs& p, int64_t slot, int lane
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int ch = (lane + T * k) * V + e;
-                if (ch < p.c) out[ch] = sum[k][e];
+                if (ch < p.c) put(ch, sum[k][e]);
             }
     }
 }
@@ -685,7 +700,8 @@ hipError_t ln_backward(hipStream_t s, const LnArgs& p, unsigned blocks) {
         constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
         ln_flags<LnElem<DT>::V>(p, [&](auto tail, auto silu) {
             constexpr bool TL = decltype(tail)::value, SI = decltype(silu)::value;
-            if (p.part) ln_backward_kernel<DT, T, NV, TL, SI, true><<<blocks, kLnThreads, 0, s>>>(p);
+            if (p.part || p.grad_a || p.grad_b)
+                ln_backward_kernel<DT, T, NV, TL, SI, true><<<blocks, kLnThreads, 0, s>>>(p);
             else ln_backward_kernel<DT, T, NV, TL, SI, false><<<blocks, kLnThreads, 0, s>>>(p);
         });
         return hipGetLastError();

@@ -217,6 +217,28 @@ def test_need(spc, dev):
             assert (p is None) if not k else torch.equal(p, q)
 
 
+@pytest.mark.parametrize("n", [1, 4, 5, 30])
+@pytest.mark.parametrize("c", [8, 72, 600, 1024, 2048, 3000, 8192])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_few_rows(spc, dev, dt, c, n):
+    """Calls that one block takes, whose sums are the gradients, and their
+    neighbours."""
+    nat = spc._native
+    x, w, b, _, _, dy = _inputs(dev, DT[dt], n, c, n)
+    _run(nat, dev, f"{dt} {n}x{c}", x, w, b, None, None, dy)
+    wanted = nat.layer_norm_backward(dy, x, nat.layer_norm(x, w, b, return_stats=True)[1], w, b)
+    for need in [(0, 1, 0), (0, 0, 1), (1, 0, 1), (1, 1, 0)]:
+        got = nat.layer_norm_backward(dy, x, nat.layer_norm(x, w, b, return_stats=True)[1], w, b,
+                                      need=(*need, 1, 1))
+        assert got[3:] == (None, None)
+        for k, p, q in zip(need, got, wanted):
+            assert (p is None) if not k else torch.equal(p, q)
+    x, _, _, sc, sh, dy = _inputs(dev, DT[dt], n, c, n + 1, items=1, affine=False)
+    _run(nat, dev, f"{dt} mod {n}x{c}", x, None, None, sc, sh, dy, silu=True)
+    _run(nat, dev, f"{dt} mod offsets {n}x{c}", x, None, None, sc, sh, dy, [0, n], silu=True)
+    _run(nat, dev, f"{dt} empty item {n}x{c}", x, None, None, sc, sh, dy, [0, 0], silu=True)
+
+
 def test_large_offset_and_special_rows(spc, dev):
     """Rows far from zero; a constant row; rows with an infinity or a NaN stay
     alone with it."""
