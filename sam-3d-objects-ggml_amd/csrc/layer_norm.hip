@@ -8,16 +8,22 @@ namespace spc {
 
 namespace {
 
-// Rows a block takes.  Forward: up to 2,048 blocks (eight to a CU), each with
-// as many rounds of its teams as that leaves.  Backward: a quarter, since
-// every block ends by writing its channels' two sums, which the second kernel
-// reads again (62,710 x 512 bf16: 40.4 + 6.4 us with 1,024 blocks, 39.7 + 4.1).
-inline int64_t ln_rows_per(int64_t n, int teams, int64_t blocks) {
-    const int64_t rounds = std::max<int64_t>(1, ceil_div(n, blocks * teams));
-    return rounds * teams;
+// Rows a block takes, a number of rounds of its teams.  Forward: up to four, so
+// that the coefficients' loads and the first rows' latency are shared, as long
+// as three blocks to a CU are left (us with 1 / 2 / 4 / 8 rounds: 62,710 x 128
+// bf16 9.5 / 7.6 / 7.2 / -, x 512 29 / - / 22.0 / 21.6, x 1024 53 / - / 46.3 / 50.2;
+// 11,774 x 2048 modulated 26.0 / 20.4 / 18.5 (3) / -).
+inline int64_t ln_forward_rows(int64_t n, int teams) {
+    return std::min<int64_t>(4, std::max<int64_t>(1, ceil_div(n, teams) / 768)) * teams;
 }
-constexpr int64_t kLnForwardBlocks = 2048;
+
+// Backward: 512 blocks, since every block ends by writing its channels' two
+// sums, which the second kernel reads again (62,710 x 512 bf16: 40.4 + 6.4 us
+// with 1,024 blocks, 39.7 + 4.1).
 constexpr int64_t kLnBackwardBlocks = 512;
+inline int64_t ln_backward_rows(int64_t n, int teams) {
+    return std::max<int64_t>(1, ceil_div(n, kLnBackwardBlocks * teams)) * teams;
+}
 
 // Sums the slots of each item's chunks (16 channels and all of an item's
 // slots a block, in a fixed order; eight slots in flight a thread: the pass is
@@ -184,7 +190,7 @@ inline bool ln_one_block(int64_t n, int teams) { return n > 0 && n <= (teams > 2
 
 // Chunks the backward's row pass makes of n rows.
 inline int64_t ln_backward_chunks(int64_t n, int teams) {
-    return ceil_div(n, ln_rows_per(n, teams, kLnBackwardBlocks));
+    return ceil_div(n, ln_backward_rows(n, teams));
 }
 
 }  // namespace
@@ -209,7 +215,7 @@ int spc_layer_norm(spc_stream_t stream, int dtype, const void* x, int64_t x_stri
     }
     p.y = y;
     p.stats = stats;
-    p.rows_per = (int)ln_rows_per(n, ln_teams(dtype, p.c, false), kLnForwardBlocks);
+    p.rows_per = (int)ln_forward_rows(n, ln_teams(dtype, p.c, false));
     const unsigned blocks = (unsigned)ceil_div(n, p.rows_per);
     const hipError_t e = dtype == SPC_BF16  ? ln_forward_bf16(s, p, blocks)
                          : dtype == SPC_F16 ? ln_forward_f16(s, p, blocks)
@@ -268,7 +274,7 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
     p.dy = dy;
     p.dy_stride = dy_stride;
     p.stats = const_cast<float*>(stats);
-    p.rows_per = (int)ln_rows_per(n, teams, alone ? 1 : kLnBackwardBlocks);
+    p.rows_per = (int)(alone ? n : ln_backward_rows(n, teams));
     if (n > 0) {
         const unsigned blocks = alone ? 1 : (unsigned)chunks;
         const hipError_t err = dtype == SPC_BF16  ? ln_backward_bf16(s, p, blocks)
