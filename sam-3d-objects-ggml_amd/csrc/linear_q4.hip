@@ -518,29 +518,37 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 // instructions an element and block of columns, and their split into parts
 // three matrix instructions a tile, which bound 16-bit rows (16 rows, 4096 ->
 // 16,384: 23 us of a floor of 8).  Here the weights take the scale, f16(d (q -
-// 8)), rounded to 11 bits -- at most 2^-11 of a weight, an eighth of a bf16
-// output's own rounding and as much as an f16 output's -- and the rows enter as
-// f16 whatever their columns: f16 rows as they are, bf16 rows with their
-// exponents moved into f16's range by a power of two that each wave chooses for
-// each row from what it has seen of it (exact for values down to 2^-27 of the
-// row's largest; of smaller ones less than 2^-28 of it is lost).
+// 8)), and the rows enter as f16 whatever their columns.
+//
+// f16 rows enter as they are, and so that no weight's rounding adds to the
+// output's own, what f16(d (q - 8)) leaves over is a second operand: a multiple
+// of d's last bit below 2^-11 of the weight, so an f16 too (outputs off by
+// 2.1e-4 of their size with it, 2.7e-4 without, as much as the plain form's).
+// Under bf16 rows it stays out: at most 2^-11 of a weight, an eighth of a bf16
+// output's rounding.  bf16 rows have their exponents moved into f16's range by
+// a power of two that each wave chooses for each row from what it has seen of
+// it (exact for values down to 2^-27 of the row's largest; of smaller ones less
+// than 2^-28 of it is lost).
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-// The eight weights of a word times their eight scales.
-__device__ __forceinline__ u32x4 q4_expand_scaled(uint32_t w, u32x4 d, uint32_t one) {
+// The eight weights of a word times their eight scales, rounded, and (PARTS 2)
+// what the rounding left over.
+template <int PARTS>
+__device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t one, u32x4 (&r)[PARTS]) {
     const u32x4 q = q4_expand<true>(w, one);  // 16 + q
-    u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         // (copies: a bit cast of a vector's element takes the vector's first)
         const uint32_t qi = q[i], di = d[i];
-        const f16x2 t = (__builtin_bit_cast(f16x2, qi) - (f16x2)(_Float16)24.0f) *
-                        __builtin_bit_cast(f16x2, di);
-        r[i] = __builtin_bit_cast(uint32_t, t);
+        const f16x2 v = __builtin_bit_cast(f16x2, qi) - (f16x2)(_Float16)24.0f;
+        const f16x2 s = __builtin_bit_cast(f16x2, di);
+        const f16x2 t = v * s;
+        r[0][i] = __builtin_bit_cast(uint32_t, t);
+        if constexpr (PARTS == 2)
+            r[1][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, s, -t));
     }
-    return r;
 }
 
 // A row's exponent bias: what is taken off its bf16 exponents to make f16's.
@@ -604,7 +612,7 @@ struct Q4Bias {
 template <int DT, int ROWS, int NT, int W>
 __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
     typedef Q4Rows<DT, ROWS> R;
-    constexpr int MT = R::MT, NI = R::NI;
+    constexpr int MT = R::MT, NI = R::NI, PARTS = DT == SPC_F16 ? 2 : 1;
     constexpr size_t SCALES = ROWS * R::STRIDE, FACTORS = SCALES + kQ4Group * 2;
     constexpr size_t WAVE = FACTORS + (ROWS * 4 + 15) / 16 * 16;
     __shared__ __attribute__((aligned(16))) char lds[q4_lds(WAVE, MT * NT, W)];
@@ -675,9 +683,12 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
             const u32x4 d = scales[4 * j + lane / 16];
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                const u32x4 w = q4_expand_scaled(s.q[b][j], d, one);
+                u32x4 w[PARTS];
+                q4_expand_scaled<PARTS>(s.q[b][j], d, one, w);
 #pragma unroll
-                for (int a = 0; a < MT; ++a) acc[a][b] = q4_mfma<true>(x[a], w, acc[a][b]);
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) acc[a][b] = q4_mfma<true>(x[a], w[q], acc[a][b]);
             }
         }
     });

@@ -55,17 +55,18 @@ def product(x, blocks, bias=None):
 def gradient(dy, blocks):
     """(dx, bound before the output's rounding) for dy [m, out].
 
-    F32 rows: dy d rounded once (u), three parts as above.  16-bit rows: the weights rounded to f16 (2^-11 of each; subnormal
-    ones are multiples of their scale's last bit, so exact), bf16 rows without
-    what lies below 2^-28 of the row's largest value; one instruction a group
-    of 32."""
+    F32 rows: dy d rounded once (u), three parts as above.  f16 rows: the weights
+    exactly, as f16(w) and the rest, two instructions a group of 32.  bf16 rows:
+    the weights rounded to f16 (2^-11 of each; subnormal ones are multiples of
+    their scale's last bit, so exact), without what lies below 2^-28 of the row's
+    largest value."""
     f32 = dy.dtype == torch.float32
     bf16 = dy.dtype == torch.bfloat16
     dy = dy.detach().cpu().double()
     w = dequant(blocks)
     # eight waves share the summed features: instructions on one accumulator
-    chain = (3 if f32 else 1) * (-(-w.shape[0] // 128) // 8 + 1) * 4
-    e = ((U if f32 else 2.0 ** -11) + 2 * (32 + chain + 12) * U) * (dy.abs() @ w.abs())
+    chain = (3 if f32 else 1 if bf16 else 2) * (-(-w.shape[0] // 128) // 8 + 1) * 4
+    e = ((U if f32 else 2.0 ** -11 if bf16 else 0.0) + 2 * (32 + chain + 12) * U) * (dy.abs() @ w.abs())
     if bf16 and dy.numel():
         e = e + 2.0 ** -28 * dy.abs().amax(1, keepdim=True) * w.abs().sum(0)
     return dy @ w, e

@@ -33,7 +33,7 @@ def _randn(shape, seed, dt, dev):
 def test_unit_rows_give_the_weights(spc, dev, dt, out, inp):
     """Rows of the identity: d (q - 8) is exact in F32, so every weight comes
     back at its place bit for bit (rounded once to 16-bit outputs; the gradient
-    of 16-bit rows takes them as f16)."""
+    of bf16 rows takes them as f16)."""
     nat = spc._native
     blocks = random_blocks(out, inp, out + inp)
     fwd, bwd = _both(nat, blocks, dev)
@@ -41,7 +41,7 @@ def test_unit_rows_give_the_weights(spc, dev, dt, out, inp):
     y = nat.linear_q4_0(torch.eye(inp, dtype=DT[dt], device=dev), fwd)
     assert torch.equal(y.cpu(), w.t().to(DT[dt]))
     dx = nat.linear_q4_0_input_grad(torch.eye(out, dtype=DT[dt], device=dev), bwd)
-    assert torch.equal(dx.cpu(), (w if dt == "f32" else w.half()).to(DT[dt]))
+    assert torch.equal(dx.cpu(), (w.half() if dt == "bf16" else w).to(DT[dt]))
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
