@@ -658,7 +658,7 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
 int spc_q4_0_quantize(spc_stream_t stream, const float* w, int64_t n, uint8_t* blocks);
 
 /* The blocks of a Linear's weight [out_features, in_features] (in_features a
- * multiple of 32) laid out for the products: transpose 0 for spc_linear_q4_0,
+ * multiple of 32, both up to 2^27) laid out for the products: transpose 0 for spc_linear_q4_0,
  * 1 for spc_linear_q4_0_input_grad.  packed: spc_linear_q4_0_packed_bytes
  * (0: unsupported shape), 16-byte aligned; once per weight. */
 size_t spc_linear_q4_0_packed_bytes(int64_t out_features, int64_t in_features, int transpose);

@@ -13,8 +13,10 @@ namespace {
 // as three blocks to a CU are left (us with 1 / 2 / 4 / 8 rounds: 62,710 x 128
 // bf16 9.5 / 7.6 / 7.2 / -, x 512 29 / - / 22.0 / 21.6, x 1024 53 / - / 46.3 / 50.2;
 // 11,774 x 2048 modulated 26.0 / 20.4 / 18.5 (3) / -).
+// A launch holds below 2^32 threads, so rows past 2^23 blocks take more rounds.
 inline int64_t ln_forward_rows(int64_t n, int teams) {
-    return std::min<int64_t>(4, std::max<int64_t>(1, ceil_div(n, teams) / 768)) * teams;
+    const int64_t rounds = std::min<int64_t>(4, std::max<int64_t>(1, ceil_div(n, teams) / 768));
+    return std::max(rounds, ceil_div(n, (int64_t)teams << 23)) * teams;
 }
 
 // Backward: 512 blocks, since every block ends by writing its channels' two

@@ -756,10 +756,17 @@ hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
     return hipGetLastError();
 }
 
+// Up to 2^27 features: a launch holds below 2^32 threads, 512 for 32 columns.
+constexpr int64_t kQ4MaxFeatures = 1 << 27;
+
+bool q4_known(int64_t out, int64_t in) {
+    return out >= 1 && in >= 32 && in % 32 == 0 && out <= kQ4MaxFeatures && in <= kQ4MaxFeatures;
+}
+
 int q4_shape(const char* fn, int64_t out, int64_t in) {
-    if (out < 1 || in < 32 || in % 32 || out > INT32_MAX - 127 || in > INT32_MAX - 127) {
-        set_last_error("%s: unsupported shape out_features=%lld in_features=%lld (a multiple of 32)",
-                       fn, (long long)out, (long long)in);
+    if (!q4_known(out, in)) {
+        set_last_error("%s: unsupported shape out_features=%lld in_features=%lld (a multiple of 32, "
+                       "both up to 2^27)", fn, (long long)out, (long long)in);
         return SPC_BAD_SHAPE;
     }
     return SPC_OK;
@@ -819,9 +826,7 @@ int spc_q4_0_quantize(spc_stream_t stream, const float* w, int64_t n, uint8_t* b
 }
 
 size_t spc_linear_q4_0_packed_bytes(int64_t out_features, int64_t in_features, int transpose) {
-    if (out_features < 1 || in_features < 32 || in_features % 32 || out_features > INT32_MAX - 127 ||
-        in_features > INT32_MAX - 127)
-        return 0;
+    if (!q4_known(out_features, in_features)) return 0;
     const Q4Layout l = q4_layout(out_features, in_features, transpose != 0);
     return (size_t)(l.quant_bytes + l.scale_bytes);
 }

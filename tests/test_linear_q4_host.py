@@ -127,3 +127,17 @@ def test_gguf_linear(spc, orc, tmp_path):
             gg.load_linear(torch.nn.Linear(64, 40, bias=False), r, "f")
         with pytest.raises(KeyError):
             gg.load_linear(lin, r, "none")
+
+
+def test_features_past_a_launch_are_refused(spc):
+    """512 threads for every 16 or 32 columns have to stay below 2^32 threads."""
+    L = spc._native.lib()
+    top = 1 << 27
+    for out, inp, t in ((top, 32, 0), (32, top, 1)):
+        assert L.spc_linear_q4_0_packed_bytes(out, inp, t) > 0
+    fake = 1 << 12
+    for out, inp in ((top + 1, 32), (32, top + 32)):
+        assert L.spc_linear_q4_0_packed_bytes(out, inp, 0) == 0
+        assert L.spc_linear_q4_0_pack(None, fake, out, inp, 0, fake) == spc._native.BAD_SHAPE
+        assert L.spc_linear_q4_0(None, 0, fake, inp, 1, fake, out, inp, None, 0,
+                                 fake) == spc._native.BAD_SHAPE
