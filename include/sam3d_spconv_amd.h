@@ -598,8 +598,8 @@ int spc_sparse_conv_products(spc_stream_t stream, int dtype, const void* x, cons
  * gamma / beta [c] in param_dtype (F32 or the rows' dtype), then the optional
  * modulation by the row's batch item b, * (1 + scale[b]) + shift[b] (scale and
  * shift together: n_batch rows of c values in mod_dtype, F32 or the rows',
- * mod_stride elements apart, so the halves of
- * one Linear's output serve as they are), then SiLU if silu is set.  Rows of
+ * mod_stride elements apart, so the halves of one Linear's output serve as they
+ * are), then SiLU if silu is set.  Rows of
  * item b are [offsets[b], offsets[b+1]) (offsets: device int64 [n_batch + 1],
  * ascending, 8-byte aligned; NULL with n_batch 1: every row; only with scale
  * and shift).  Rows before offsets[0] and from offsets[n_batch] on belong to
@@ -670,9 +670,8 @@ int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out
  * bias_dtype or NULL.  Weights enter exactly, sums are F32, one rounding to
  * dtype at the end (F32 rows enter as three 8-bit parts, of which those below
  * 2^-126 are taken as zero); a row with an infinity or NaN comes out as NaNs, the
- * others as without it.  m up to
- * 1,048,560; made for few rows (the weights' bytes are the cost up to some
- * 64), right for any. */
+ * others as without it.  m up to 1,048,560; made for few rows (the weights'
+ * bytes are the cost up to some 64), right for any. */
 int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
                     const void* packed, int64_t out_features, int64_t in_features, const void* bias,
                     int bias_dtype, void* y);
@@ -682,11 +681,20 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
  * F32 rows: the weights enter exactly, dy times a scale in F32, as three parts.
  * f16 rows: the weights enter exactly, the rows as they are.  bf16 rows: the
  * weights enter as f16(d (q - 8)) (at most 2^-11 of a weight), the rows with
- * what lies above 2^-28 of the row's largest value. A row with an
- * infinity or NaN comes out non-finite, the others as without it. */
+ * what lies above 2^-28 of the row's largest value.  Under 16-bit rows weights
+ * past f16's 65,504 are infinite.  A row with an infinity or NaN comes out
+ * non-finite, the others as without it. */
 int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                                int64_t m, const void* packed, int64_t out_features,
                                int64_t in_features, void* dx);
+
+/* dbias [out_features] in bias_dtype: the sums of dy's columns, F32 in a fixed
+ * order.  workspace: spc_linear_q4_0_bias_grad_workspace_bytes (none up to 512
+ * rows), 4-byte aligned. */
+size_t spc_linear_q4_0_bias_grad_workspace_bytes(int64_t m, int64_t out_features);
+int spc_linear_q4_0_bias_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
+                              int64_t m, int64_t out_features, int bias_dtype, void* dbias,
+                              void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

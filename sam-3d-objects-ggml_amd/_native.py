@@ -130,6 +130,9 @@ def lib() -> ctypes.CDLL:
     L.spc_linear_q4_0_pack.argtypes = [_P, _P, _I64, _I64, _INT, _P]
     L.spc_linear_q4_0.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P, _INT, _P]
     L.spc_linear_q4_0_input_grad.argtypes = [_P, _INT, _P, _I64, _I64, _P, _I64, _I64, _P]
+    L.spc_linear_q4_0_bias_grad_workspace_bytes.restype = _SZ
+    L.spc_linear_q4_0_bias_grad_workspace_bytes.argtypes = [_I64, _I64]
+    L.spc_linear_q4_0_bias_grad.argtypes = [_P, _INT, _P, _I64, _I64, _I64, _INT, _P, _P, _SZ]
     _lib = L
     return L
 
@@ -1032,6 +1035,26 @@ def linear_q4_0_input_grad(dy: torch.Tensor, w: Q4Weights) -> torch.Tensor:
     if st:
         _check("spc_linear_q4_0_input_grad", st)
     return dx
+
+
+def linear_q4_0_bias_grad(dy: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The gradient [out_features] of linear_q4_0's bias, in `dtype`: the sums
+    of dy's columns in F32 (spc_linear_q4_0_bias_grad).  Deterministic."""
+    dev = _one_device(dy)
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        return linear_q4_0_bias_grad(dy).to(dtype)
+    dt, bdt = dtype_code(dy.dtype), dtype_code(dtype)
+    dy, m, o, stride = _strided_rows(dy, "dy")
+    L, ws = lib(), None
+    nbytes = L.spc_linear_q4_0_bias_grad_workspace_bytes(m, o)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    db = torch.empty(o, dtype=dtype, device=dev)
+    st = _launch(L.spc_linear_q4_0_bias_grad, dev, dt, dy.data_ptr(), stride, m, o, bdt, db.data_ptr(),
+                 _ptr(ws), nbytes)
+    if st:
+        _check("spc_linear_q4_0_bias_grad", st)
+    return db
 
 
 def scatter_mean(features: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor,

@@ -756,8 +756,65 @@ hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
     return hipGetLastError();
 }
 
+// ---- the bias' gradient -----------------------------------------------------
+// Sums of the rows' columns, F32 in a fixed order: 32 columns and 512 rows a
+// block, 16 rows a thread (eight under way), then the lanes of a wave, then the
+// waves through LDS; more than 512 rows by the same kernel again over the
+// blocks' sums.  (Queued calls, us, 16-bit rows, beside a library's cast, sum
+// and cast: 16 x 2048 6.9 / 14.5, 5,000 x 130 11.3 / 17, 62,710 x 1024 65 / 126.
+// The sum was the one step of the pass that could record a memory node into a
+// captured graph.)
+constexpr int kQ4SumCols = 32, kQ4SumThreads = 1024, kQ4SumRows = 512;
+
+__device__ __forceinline__ float q4_element(const void* p, int dt, int64_t i) {
+    if (dt == SPC_F32) return static_cast<const float*>(p)[i];
+    const uint16_t b = static_cast<const uint16_t*>(p)[i];
+    return dt == SPC_BF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+}
+
+__global__ __launch_bounds__(kQ4SumThreads) void q4_column_sums_kernel(const void* x, int dtype,
+                                                                       int64_t stride, int64_t m,
+                                                                       int64_t rows_per, int64_t cols,
+                                                                       void* out, int out_dtype) {
+    constexpr int C = kQ4SumCols, L = kQ4SumThreads / C, W = kQ4SumThreads / 64, DEEP = 8;
+    __shared__ float ls[W][C];
+    const int cl = threadIdx.x % C, l = threadIdx.x / C;
+    const int64_t col = (int64_t)blockIdx.x * C + cl;
+    const int64_t lo = (int64_t)blockIdx.y * rows_per, hi = min(m, lo + rows_per);
+    float s = 0.0f;
+    if (col < cols)
+        for (int64_t r = lo + l; r < hi; r += DEEP * L) {
+            float v[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) {
+                const int64_t at = r + i * L;
+                v[i] = q4_element(x, dtype, min(at, hi - 1) * stride + col);
+                if (at >= hi) v[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) s += v[i];
+        }
+    s += __shfl_xor(s, C);
+    if ((threadIdx.x & 63) < C) ls[threadIdx.x >> 6][cl] = s;
+    __syncthreads();
+    if (l != 0 || col >= cols) return;
+    s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) s += ls[w][cl];
+    const int64_t at = (int64_t)blockIdx.y * cols + col;
+    if (out_dtype == SPC_F32) q4_store<SPC_F32>(out, at, s);
+    else if (out_dtype == SPC_BF16) q4_store<SPC_BF16>(out, at, s);
+    else q4_store<SPC_F16>(out, at, s);
+}
+
+// Blocks along the rows: at most a y-dimension's, of more rows where that is few.
+inline int64_t q4_sum_rows(int64_t m) { return std::max<int64_t>(kQ4SumRows, ceil_div(m, kQ4SumRows)); }
+
+inline bool q4_float_dtype(int dt) { return dt == SPC_F32 || dt == SPC_F16 || dt == SPC_BF16; }
+
 // Up to 2^27 features: a launch holds below 2^32 threads, 512 for 32 columns.
 constexpr int64_t kQ4MaxFeatures = 1 << 27;
+constexpr int64_t kQ4MaxRows = 65535 * 16;  // a launch's y dimension, 16 rows a block
 
 bool q4_known(int64_t out, int64_t in) {
     return out >= 1 && in >= 32 && in % 32 == 0 && out <= kQ4MaxFeatures && in <= kQ4MaxFeatures;
@@ -777,11 +834,12 @@ int q4_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t 
             int64_t out, int64_t in, bool transpose, void* y, Q4Args* p) {
     const int st = q4_shape(fn, out, in);
     if (st != SPC_OK) return st;
-    if (m < 0 || m > (int64_t)65535 * 16 || x_stride < 0) {
-        set_last_error("%s: unsupported rows m=%lld (0 to %d)", fn, (long long)m, 65535 * 16);
+    if (m < 0 || m > kQ4MaxRows || x_stride < 0) {
+        set_last_error("%s: unsupported rows m=%lld (0 to %lld)", fn, (long long)m,
+                       (long long)kQ4MaxRows);
         return SPC_BAD_SHAPE;
     }
-    if (dtype != SPC_F32 && dtype != SPC_F16 && dtype != SPC_BF16) {
+    if (!q4_float_dtype(dtype)) {
         set_last_error("%s: unknown dtype %d", fn, dtype);
         return SPC_BAD_ARG;
     }
@@ -856,7 +914,7 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
     Q4Args p;
     const int st = q4_args(fn, dtype, x, x_stride, m, packed, out_features, in_features, false, y, &p);
     if (st != SPC_OK) return st;
-    if (bias && ((bias_dtype != SPC_F32 && bias_dtype != SPC_F16 && bias_dtype != SPC_BF16) ||
+    if (bias && (!q4_float_dtype(bias_dtype) ||
                  (uintptr_t)bias % (bias_dtype == SPC_F32 ? 4 : 2))) {
         set_last_error("%s: unknown bias dtype or misaligned bias", fn);
         return SPC_BAD_ARG;
@@ -884,6 +942,43 @@ int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, i
                          : dtype == SPC_F16 ? q4_grad<SPC_F16>(s, p)
                                             : q4_grad<SPC_F32>(s, p);
     return e == hipSuccess ? SPC_OK : hip_status(e, "spc_linear_q4_0_input_grad launch");
+}
+
+size_t spc_linear_q4_0_bias_grad_workspace_bytes(int64_t m, int64_t out_features) {
+    if (m < 0 || m > kQ4MaxRows || out_features < 1 || out_features > kQ4MaxFeatures) return 0;
+    return m <= kQ4SumRows ? 0 : (size_t)(ceil_div(m, q4_sum_rows(m)) * out_features * 4);
+}
+
+int spc_linear_q4_0_bias_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
+                              int64_t m, int64_t out_features, int bias_dtype, void* dbias,
+                              void* workspace, size_t workspace_bytes) {
+    const char* fn = "spc_linear_q4_0_bias_grad";
+    if (m < 0 || m > kQ4MaxRows || dy_stride < 0 || out_features < 1 || out_features > kQ4MaxFeatures) {
+        set_last_error("%s: unsupported shape m=%lld out_features=%lld", fn, (long long)m,
+                       (long long)out_features);
+        return SPC_BAD_SHAPE;
+    }
+    const size_t need = spc_linear_q4_0_bias_grad_workspace_bytes(m, out_features);
+    if (!q4_float_dtype(dtype) || !q4_float_dtype(bias_dtype) || (m > 0 && !dy) || !dbias ||
+        (uintptr_t)dy % (dtype == SPC_F32 ? 4 : 2) || (uintptr_t)dbias % (bias_dtype == SPC_F32 ? 4 : 2) ||
+        workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 4))) {
+        set_last_error("%s: unknown dtype, null or misaligned pointer, or workspace too small", fn);
+        return SPC_BAD_ARG;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const unsigned cb = (unsigned)ceil_div(out_features, kQ4SumCols);
+    if (need) {
+        const int64_t per = q4_sum_rows(m), parts = ceil_div(m, per);
+        q4_column_sums_kernel<<<dim3(cb, (unsigned)parts), kQ4SumThreads, 0, s>>>(
+            dy, dtype, dy_stride, m, per, out_features, workspace, SPC_F32);
+        q4_column_sums_kernel<<<cb, kQ4SumThreads, 0, s>>>(workspace, SPC_F32, out_features, parts, parts,
+                                                           out_features, dbias, bias_dtype);
+    } else {
+        q4_column_sums_kernel<<<cb, kQ4SumThreads, 0, s>>>(dy, dtype, dy_stride, m, std::max<int64_t>(m, 1),
+                                                           out_features, dbias, bias_dtype);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? SPC_OK : hip_status(e, "spc_linear_q4_0_bias_grad launch");
 }
 
 }  // extern "C"

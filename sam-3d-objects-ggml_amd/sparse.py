@@ -836,7 +836,7 @@ class _Q4LinearFn(torch.autograd.Function):
                 raise RuntimeError("the Q4_0 weights were replaced between forward and backward")
             dx = nat.linear_q4_0_input_grad(dy, ctx.linear._q4_operand(dy.device, True))
         if ctx.needs_input_grad[1]:
-            db = dy.float().sum(0).to(ctx.bias_dtype)
+            db = nat.linear_q4_0_bias_grad(dy, ctx.bias_dtype)
         return dx, db, None
 
 

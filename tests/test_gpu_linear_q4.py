@@ -230,6 +230,35 @@ def test_equal_calls_streams_and_graphs(spc, dev):
         assert all(torch.equal(p, q) for p, q in zip(out, step()))
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,o", [(0, 5), (1, 1), (3, 33), (31, 130), (512, 64), (513, 31), (5000, 130),
+                                 (262_200, 3)])
+def test_bias_gradient(spc, dev, dt, m, o):
+    """Column sums of strided rows, in every dtype of the bias, a captured one too."""
+    nat = spc._native
+    dy = _randn((m, o + 3), m + o, dt, dev)[:, 1:1 + o]
+    ref = dy.cpu().double()
+    # additions one behind another: a thread's rows, a wave's two lanes and the
+    # sixteen waves, and the second pass over at most 512 blocks' sums
+    per = max(512, -(-m // 512))
+    steps = -(-per // 32) + 17 + 33
+    bound = steps * 2.0 ** -24 * ref.abs().sum(0)
+    for bdt in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
+        db = nat.linear_q4_0_bias_grad(dy, bdt)
+        assert db.dtype == bdt
+        check(f"dbias {bdt}", db, ref.sum(0), bound, torch.float32 if bdt == torch.float64 else bdt)
+    if m:
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = nat.linear_q4_0_bias_grad(dy, dt)
+        for i in range(3):
+            dy.copy_(torch.randn(m, o, device=dev) + i)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, nat.linear_q4_0_bias_grad(dy, dt))
+
+
 def test_refusals(spc, dev):
     nat = spc._native
     blocks = random_blocks(20, 64, 1).to(dev)

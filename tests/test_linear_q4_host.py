@@ -141,3 +141,20 @@ def test_features_past_a_launch_are_refused(spc):
         assert L.spc_linear_q4_0_pack(None, fake, out, inp, 0, fake) == spc._native.BAD_SHAPE
         assert L.spc_linear_q4_0(None, 0, fake, inp, 1, fake, out, inp, None, 0,
                                  fake) == spc._native.BAD_SHAPE
+
+
+def test_bias_gradient_validation(spc):
+    nat = spc._native
+    L = nat.lib()
+    fake = 1 << 12
+    need = L.spc_linear_q4_0_bias_grad_workspace_bytes
+    assert need(0, 8) == need(512, 8) == need(-1, 8) == 0
+    assert need(513, 8) == 2 * 8 * 4 and need(65535 * 16, 8) == 512 * 8 * 4
+
+    def run(dt=nat.BF16, dy=fake, stride=8, m=4, o=8, bdt=nat.F32, out=fake, ws=None, nbytes=0):
+        return L.spc_linear_q4_0_bias_grad(None, dt, dy, stride, m, o, bdt, out, ws, nbytes)
+
+    assert run(m=-1) == run(m=65535 * 16 + 1) == run(o=0) == run(stride=-1) == nat.BAD_SHAPE
+    assert run(dt=nat.Q8_0) == run(bdt=nat.Q8_0) == run(dy=None) == run(out=None) == nat.BAD_ARG
+    assert run(dy=fake + 1) == run(out=fake + 2) == run(m=513) == nat.BAD_ARG
+    assert run(m=513, ws=fake, nbytes=63) == run(m=513, ws=fake + 1, nbytes=64) == nat.BAD_ARG
