@@ -26,8 +26,9 @@ Supported convolutions (what the SAM 3D models instantiate):
                                      lexicographic (b, x/2, y/2, z/2) order
                                      (SRC/sparse_ops.cpp:27-81)
 Anything else raises NotImplementedError.  Channel counts that are not
-multiples of 32 are zero-padded around the kernel.  The modules are
-forward-only (inference): the conv's backward raises.
+multiples of 32 are zero-padded around the kernel.  The convolutions are
+forward-only (inference): their backward raises.  SparseLayerNorm32 and Q4Linear
+(a Linear on 4-bit blocks) have gradients.
 """
 from __future__ import annotations
 
@@ -818,6 +819,26 @@ class SparseInverseConv3d(nn.Module, _ConvCore):
 # ---------------------------------------------------------------------------
 # spatial ops (SP/spatial.py)
 # ---------------------------------------------------------------------------
+def _eager_leaves(*ts) -> list:
+    """The gradient accumulators of the leaves among ts, to be held until the
+    op is recorded.  An accumulator belongs to the stream of the first graph it
+    is part of; a backward pass captured while an eager graph keeps it alive
+    would leave the capture, and that ends the process.  So eager graphs mark
+    theirs and a capture that meets a mark is refused."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    nodes = []
+    for t in ts:
+        if t is not None and t.requires_grad and t.is_leaf:
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            if not capturing:
+                node.metadata["eager"] = True
+            elif "eager" in node.metadata:
+                raise RuntimeError("an eager graph of these tensors is alive: drop its outputs and "
+                                   "losses before capturing a forward and backward pass")
+            nodes.append(node)
+    return nodes
+
+
 class _Q4LinearFn(torch.autograd.Function):
     """nat.linear_q4_0 with the gradients of the rows and the bias."""
 
@@ -846,7 +867,10 @@ class Q4Linear(nn.Linear):
     any leading dimensions, with gradients for the rows (through the frozen
     blocks, spc_linear_q4_0_input_grad) and the bias.  The float parameter is
     left as is and then neither read nor given a gradient; the blocks are not
-    part of the state dict.  Made for few rows: a modulation, a token."""
+    part of the state dict.  Made for few rows: a modulation, a token.  The
+    blocks are laid out by the first call and the first backward pass; a
+    captured graph reads that memory, so load and drop blocks only once such
+    graphs are done with.  Capturing a backward pass: as SparseLayerNorm32."""
 
     _q4 = None          # blocks, uint8 [out_features, in_features / 32 * 18]
 
@@ -898,7 +922,9 @@ class Q4Linear(nn.Linear):
         x = input.reshape(-1, self.in_features)
         if torch.is_grad_enabled() and (x.requires_grad or
                                         (self.bias is not None and self.bias.requires_grad)):
+            held = _eager_leaves(input, self.bias)
             y = _Q4LinearFn.apply(x, self.bias, self)
+            del held
         else:
             y = nat.linear_q4_0(x, self._q4_operand(x.device, False), self.bias)
         return y.view(*input.shape[:-1], self.out_features)
@@ -989,7 +1015,8 @@ class SparseLayerNorm32(nn.LayerNorm):
     ([x.shape[0], channels], for instance the halves of a Linear's output) and
     SiLU in the same pass; gradients go to the feats, weight, bias, scale and
     shift.  With a modulation, rows outside x's layout come out as zeros.  Once
-    differentiable."""
+    differentiable.  A forward and backward pass may be captured into a graph,
+    both in the one capture, once no eager graph of the same leaves is alive."""
 
     def __init__(self, channels: int, eps: float = 1e-6, elementwise_affine: bool = True,
                  bias: bool = True):
@@ -1007,7 +1034,10 @@ class SparseLayerNorm32(nn.LayerNorm):
             offsets = _item_offsets(input)
         args = (x, self.weight, self.bias, scale, shift)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-            return input.replace(_LayerNormFn.apply(*args, offsets, self.eps, silu))
+            held = _eager_leaves(*args)
+            y = _LayerNormFn.apply(*args, offsets, self.eps, silu)
+            del held
+            return input.replace(y)
         return input.replace(nat.layer_norm(x, self.weight, self.bias, self.eps, scale=scale,
                                             shift=shift, offsets=offsets, silu=silu))
 

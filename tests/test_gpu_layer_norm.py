@@ -1,6 +1,8 @@
 """The general row layer norm and its gradient (nat.layer_norm,
 nat.layer_norm_backward, SparseLayerNorm32) against 64 bits.  Bounds:
 tests/norm_reference.py."""
+import copy
+
 import pytest
 import torch
 
@@ -417,6 +419,62 @@ def test_module_capture(spc, dev):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, ln(t, sc, sh).feats)
+
+
+def test_training_pass_capture(spc, dev):
+    """Forward and backward of norm and 4-bit Linear in one graph, replayed on
+    new values with eager work between; refused while an eager graph of the
+    same leaves is alive."""
+    c, e, counts = 64, 32, [30, 20]
+    sp = spc.sparse
+    lin = sp.Q4Linear(e, 2 * c).to(dev)
+    lin.quantize_q4_0()
+    ln = sp.SparseLayerNorm32(c).to(dev)
+    x = torch.randn(50, c, device=dev, requires_grad=True)
+    emb = torch.randn(2, e, device=dev, requires_grad=True)
+    dy = torch.randn(50, c, device=dev)
+    t = _tensor(spc, dev, x.detach(), counts)
+
+    def run(x, emb, ln, lin):
+        scale, shift = lin(emb).chunk(2, 1)
+        return ln(t.replace(x), scale, shift, silu=True).feats
+
+    leaves = [x, emb, ln.weight, ln.bias, lin.bias]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):          # first calls: operands, offsets
+        y = run(x, emb, ln, lin)
+        y.backward(dy)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for fn in (lambda: ln(t), lambda: lin(emb)):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                fn()
+        torch.cuda.synchronize()
+    del y
+    for p in leaves:
+        p.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = run(x, emb, ln, lin)
+        y.backward(dy)
+    grads = [p.grad for p in leaves]
+    # eager results from other leaves of the same values
+    ln2, lin2 = copy.deepcopy(ln), copy.deepcopy(lin)
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(50, c, device=dev) + i)
+            emb.copy_(torch.randn(2, e, device=dev))
+        dy.copy_(torch.randn(50, c, device=dev))
+        g.replay()
+        torch.cuda.synchronize()
+        x2, emb2 = (v.detach().clone().requires_grad_() for v in (x, emb))
+        y2 = run(x2, emb2, ln2, lin2)
+        want = torch.autograd.grad(y2, [x2, emb2, ln2.weight, ln2.bias, lin2.bias], dy)
+        assert torch.equal(y, y2)
+        for p, q in zip(grads, want):
+            assert torch.equal(p, q)
 
 
 def test_offset_past_32_bits(spc, dev):
