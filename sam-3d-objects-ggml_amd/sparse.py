@@ -883,8 +883,9 @@ class Q4Linear(nn.Linear):
         if blocks.dtype != torch.uint8 or blocks.numel() != n // 32 * 18:
             raise ValueError(f"expected {n // 32 * 18} Q4_0 bytes (uint8) for this Linear")
         # a copy: the packed operands are made from it when first needed
-        self._q4 = blocks.detach().clone(memory_format=torch.contiguous_format)
-        self._q4_packed = {}
+        blocks = blocks.detach().clone(memory_format=torch.contiguous_format)
+        self.drop_q4_0()
+        self._q4 = blocks
 
     def quantize_q4_0(self) -> torch.Tensor:
         """Quantises the current weight on the GPU, uses it, and returns the
@@ -897,6 +898,8 @@ class Q4Linear(nn.Linear):
 
     def drop_q4_0(self) -> None:
         """Back to the float parameter."""
+        for device in {device for device, _ in getattr(self, "_q4_packed", ())}:
+            torch.cuda.synchronize(device)  # products on any stream may still read them
         self._q4, self._q4_packed = None, {}
 
     def _q4_operand(self, device, transpose: bool) -> nat.Q4Weights:

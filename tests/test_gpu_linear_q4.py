@@ -315,6 +315,31 @@ def test_module(spc, dev):
     assert torch.equal(lin(x), plain)
 
 
+def test_blocks_dropped_under_a_queued_product(spc, dev):
+    """The laid out weights outlive products that other streams have queued."""
+    lin = spc.sparse.Q4Linear(1024, 1024, bias=False).to(dev)
+    blocks = lin.quantize_q4_0()
+    x = _randn((3, 1024), 1, torch.bfloat16, dev)
+    big = torch.randn(8192, 8192, device=dev)
+    out = torch.empty_like(big)
+    for drop in (lin.drop_q4_0, lambda: lin.load_q4_0(blocks)):
+        lin.load_q4_0(blocks)
+        with torch.no_grad():
+            want = lin(x)
+        torch.cuda.synchronize()
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s), torch.no_grad():
+            for _ in range(4):
+                torch.mm(big, big, out=out)
+            y = lin(x)
+        size = lin._q4_operand(x.device, False).data.numel()
+        drop()
+        junk = [torch.full((size,), 0x3c, dtype=torch.uint8, device=dev) for _ in range(4)]
+        s.synchronize()
+        assert torch.equal(y, want)
+        del junk
+
+
 def test_first_call_in_a_capture_is_refused(spc, dev):
     lin = spc.sparse.Q4Linear(64, 32).to(dev)
     lin.quantize_q4_0()
