@@ -177,35 +177,34 @@ def _need_gpu(*ts: torch.Tensor) -> None:
             raise RuntimeError("sparse-conv kernels run on the GPU only; got a CPU tensor")
 
 
-def _one_device(x: torch.Tensor, *others) -> torch.device:
-    """x's device; every tensor of the call has to be there."""
-    dev = x.device
+def _one_device(x: torch.Tensor, *others) -> int:
+    """The GPU x is on; every tensor of the call has to be there."""
+    dev = x.get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
-    if dev.type != "cuda":
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {x.device} and {t.device} in one call")
+    if not x.is_cuda:
         _need_gpu(x)
     return dev
 
 
-def _launch(fn, dev: torch.device, *args) -> int:
+def _launch(fn, dev: int, *args) -> int:
     """fn(current stream of dev, *args) with dev the current device (its default
     stream is the null stream, which means the current device's)."""
-    index = dev.index
-    if torch.cuda.current_device() == index:
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
-    with torch.cuda.device(index):
-        return fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    if torch.cuda.current_device() == dev:
+        return fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    with torch.cuda.device(dev):
+        return fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+
+
+_DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
 def dtype_code(dt: torch.dtype) -> int:
-    if dt == torch.float32:
-        return F32
-    if dt == torch.float16:
-        return F16
-    if dt == torch.bfloat16:
-        return BF16
-    raise TypeError(f"unsupported feature dtype {dt}")
+    code = _DTYPE_CODES.get(dt)
+    if code is None:
+        raise TypeError(f"unsupported feature dtype {dt}")
+    return code
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor:
@@ -783,35 +782,38 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _param_pair(a, b, width: int, names: str, dtype: torch.dtype):
     """Two parameter tensors [width] (or None), both float32 or both `dtype`."""
+    f32, dts = torch.float32, []
     for t in (a, b):
-        if t is not None and t.shape != (width,):
-            raise ValueError(f"{names} must be [{width}], got {tuple(t.shape)}")
-    dts = {t.dtype for t in (a, b) if t is not None}
-    if len(dts) > 1 or not dts <= {torch.float32, dtype}:
-        a, b = (None if t is None else t.to(torch.float32) for t in (a, b))
-    return tuple(None if t is None else t.contiguous() for t in (a, b))
+        if t is not None:
+            if t.dim() != 1 or t.numel() != width:
+                raise ValueError(f"{names} must be [{width}], got {tuple(t.shape)}")
+            dts.append(t.dtype)
+    if dts[0] is not dts[-1] or (dts[0] is not f32 and dts[0] is not dtype):
+        a, b = (None if t is None else t.to(f32) for t in (a, b))
+    return (None if a is None else a.contiguous()), (None if b is None else b.contiguous())
 
 
 def _layer_norm_params(x, c, weight, bias, eps, scale, shift, offsets, silu):
     """(spc_layer_norm_params, tensors it points into)."""
-    f32, dt = torch.float32, x.dtype
     gp = bp = sp = hp = op = None
     pdt = mdt = nb = 1
     ms = 0
     if weight is not None or bias is not None:
-        weight, bias = _param_pair(weight, bias, c, "weight / bias", dt)
-        gp, bp = _ptr(weight), _ptr(bias)
-        pdt = dtype_code((weight if weight is not None else bias).dtype)
+        weight, bias = _param_pair(weight, bias, c, "weight / bias", x.dtype)
+        if bias is not None:
+            bp, pdt = bias.data_ptr(), _DTYPE_CODES[bias.dtype]
+        if weight is not None:
+            gp, pdt = weight.data_ptr(), _DTYPE_CODES[weight.dtype]
     if scale is not None or shift is not None:
         if scale is None or shift is None:
             raise ValueError("scale and shift go together")
         if scale.dim() != 2 or scale.shape != shift.shape or scale.shape[1] != c:
             raise ValueError(f"scale / shift must be [n_batch, {c}], got {tuple(scale.shape)} and "
                              f"{tuple(shift.shape)}")
-        mdt = scale.dtype
-        if mdt != shift.dtype or (mdt != f32 and mdt != dt):
+        f32, mdt = torch.float32, scale.dtype
+        if mdt is not shift.dtype or (mdt is not f32 and mdt is not x.dtype):
             scale, shift, mdt = scale.to(f32), shift.to(f32), f32
-        mdt = dtype_code(mdt)
+        mdt = _DTYPE_CODES[mdt]
         st = scale.stride()
         if st != shift.stride() or (c > 1 and st[1] != 1):
             scale, shift = scale.contiguous(), shift.contiguous()
@@ -849,7 +851,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     x, n, c, stride = _strided_rows(x, "x")
     p, keep = _layer_norm_params(x, c, weight, bias, eps, scale, shift, offsets, silu)
     if out is None:
-        out = x.new_empty((n, c))
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous, of x's shape and dtype")
     elif n and not (out.data_ptr() == x.data_ptr() and stride == c) and _overlap(out, x):
@@ -861,6 +863,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
         _check("spc_layer_norm", st)
     del keep  # alive until queued
     return (out, stats) if return_stats else out
+
+
+_NO_GRADS = [None] * 4
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor,
@@ -882,21 +887,25 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, stats: torch.Tensor,
     if stats.shape != (n, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
         raise ValueError("stats must be contiguous float32 [n, 2]")
     p, keep = _layer_norm_params(x, c, weight, bias, 0.0, scale, shift, offsets, silu)
-    contiguous = torch.contiguous_format
-    dx = torch.empty_like(x, memory_format=contiguous) if need[0] else None
-    grads = [None if t is None or not k else torch.empty_like(t, memory_format=contiguous)
-             for t, k in zip(keep, need[1:])]
+    grads, ptrs = [], []
+    for t, k in zip((x, *keep), need):
+        g = None
+        if t is not None and k:
+            g = torch.empty_like(t, memory_format=torch.contiguous_format)
+        grads.append(g)
+        ptrs.append(None if g is None else g.data_ptr())
     L, ws, nbytes = lib(), None, 0
-    if any(g is not None for g in grads):
+    if ptrs[1:] != _NO_GRADS:
         nbytes = L.spc_layer_norm_backward_workspace_bytes(dt, n, c, p.n_batch)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     st = _launch(L.spc_layer_norm_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs,
-                 stats.data_ptr(), n, c, p, _ptr(dx), *map(_ptr, grads), _ptr(ws), nbytes)
+                 stats.data_ptr(), n, c, p, *ptrs, _ptr(ws), nbytes)
     if st:
         _check("spc_layer_norm_backward", st)
-    given = (weight, bias, scale, shift)
-    return (dx, *(g if g is None or g.dtype == t.dtype else g.to(t.dtype)
-                  for g, t in zip(grads, given)))
+    for i, t in enumerate((weight, bias, scale, shift), 1):
+        if t is not None and t is not keep[i - 1] and grads[i] is not None:
+            grads[i] = grads[i].to(t.dtype)  # (a copy in F32 was the parameter)
+    return tuple(grads)
 
 
 def spconv_f16_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
