@@ -310,13 +310,15 @@ __device__ __forceinline__ void q4_wave_sync() {
 }
 
 // Adds the W waves' accumulators and stores: tiles [MT][NT] of 16 rows x 16
-// columns; lane l of a tile holds column l % 16, rows 4 (l / 16) + i.  lds is
-// the block's, whatever it held.
-template <int DT, int MT, int NT, int W>
+// columns; lane l of a tile holds column l % 16, rows 4 (l / 16) + i.  Of a block
+// of fewer than 16 rows the tile's others repeat them.  lds is the block's,
+// whatever it held.
+template <int DT, int ROWS, int MT, int NT, int W>
 __device__ __forceinline__ void q4_finish(const Q4Args& p, floatx4 (&acc)[MT][NT], int64_t row0,
                                           int64_t col0, floatx4* lds) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int TILES = MT * NT;
+    const int64_t end = min(p.m, row0 + ROWS);
     __syncthreads();
 #pragma unroll
     for (int a = 0; a < MT; ++a)
@@ -339,7 +341,7 @@ __device__ __forceinline__ void q4_finish(const Q4Args& p, floatx4 (&acc)[MT][NT
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t row = row0 + 16 * a + 4 * (lane / 16) + i;
-            if (row < p.m) q4_store<DT>(p.y, row * p.cols + col, v[i] + bias);
+            if (row < end) q4_store<DT>(p.y, row * p.cols + col, v[i] + bias);
         }
     }
 }
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
             }
         }
     });
-    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
+    q4_finish<DT, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 // dx = dy W of F32 rows: 16 NT input features (NT 1 or 2: within one block of
@@ -510,7 +512,7 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] *= 16.0f;
-    q4_finish<SPC_F32, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
+    q4_finish<SPC_F32, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 // ---- the gradient of 16-bit rows -------------------------------------------
@@ -698,7 +700,7 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
         for (int i = 0; i < NI; ++i) f[i] = bias[i].factor();
         scale_rows([&](int i) { return f[i]; });
     }
-    q4_finish<DT, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
+    q4_finish<DT, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 template <int DT, int ROWS, int NT, int W>
@@ -714,13 +716,25 @@ void q4_grad_launch(hipStream_t s, const Q4Args& p) {
     else q4_grad16_kernel<DT, ROWS, NT, W><<<grid, 64 * W, 0, s>>>(p);
 }
 
-// f(ROWS) with the fewest rows a block that hold m, at most 32 (F32, whose
-// three operands take as much LDS as that: 16).
+// f(ROWS) with the fewest rows a block that hold m or leave a CU to every block, at
+// most 32 (F32, whose three operands take as much LDS as that: 16): beyond a few
+// rows a block's time is its rows' conversion, while other CUs would stand
+// idle.  us with the fewest that hold m / that spread: forward, thirty bf16 rows
+// 8192 -> 1024 11.0 / 6.7, 1024 -> 1024 4.3 / 3.8, sixteen F32 rows 4096 -> 1024
+// 9.2 / 6.3; gradient, thirty bf16 rows of 1024 -> 16,384 28 / 13.8, sixteen 17.8 /
+// 12.0.  Past a block to a CU it loses (sixteen bf16 rows, 8192 -> 4096 8.6 / 9.6,
+// gradient of 4096 -> 16,384 18.8 / 20.0), but half the most rows do not (thirty
+// bf16 rows, 4096 -> 4096 8.1 / 7.1, gradient of 4096 -> 8192 17.6 / 14.4; sixteen
+// F32 rows, gradient of 4096 -> 4096 10.5 / 9.1).
 template <int DT, typename F>
-void q4_row_tile(int64_t m, F&& f) {
-    if (m <= 4) f(std::integral_constant<int, 4>{});
-    else if (m <= 8) f(std::integral_constant<int, 8>{});
-    else if (m <= 16 || DT == SPC_F32) f(std::integral_constant<int, 16>{});
+void q4_row_tile(const Q4Args& p, F&& f) {
+    auto fits = [&](int rows) {
+        const int blocks = rows < (DT == SPC_F32 ? 8 : 16) ? 256 : 512;
+        return p.m <= rows || p.col_tiles * ceil_div(p.m, rows) <= blocks;
+    };
+    if (fits(4)) f(std::integral_constant<int, 4>{});
+    else if (fits(8)) f(std::integral_constant<int, 8>{});
+    else if (fits(16) || DT == SPC_F32) f(std::integral_constant<int, 16>{});
     else if constexpr (DT != SPC_F32) f(std::integral_constant<int, 32>{});
 }
 
@@ -736,11 +750,26 @@ inline bool q4_two_tiles(const Q4Args& p) {
     return p.col_tiles * ceil_div(p.m, ROWS) >= 512;
 }
 
+// Sixteen waves a block instead of eight for one tile of long sums: hardly a CU
+// has a second block to hide the loads' latency.  us with eight / sixteen: one
+// bf16 row, 8192 -> 1024 5.8 / 5.5, 16,384 -> 4096 10.3 / 9.4, eight F32 rows,
+// 8192 -> 1024 11.0 / 10.2; shorter sums the same or slower (2048 -> 1024 3.5 /
+// 3.6); sixteen rows, gradient of 4096 -> 16,384 21.4 / 20.4, of 4096 -> 8192
+// 12.3 / 12.5.  More rows have no registers left (thirty, gradient of 1024 ->
+// 8192: 17 / 72, spilled).
+template <int DT, int ROWS>
+constexpr int kQ4MoreWaves = ROWS <= (DT == SPC_F32 ? 8 : 16) ? 16 : 8;
+template <int ROWS>
+inline bool q4_long_sum(const Q4Args& p) {
+    return p.groups >= (ROWS <= 8 ? 64 : 128);
+}
+
 template <int DT>
 hipError_t q4_forward(hipStream_t s, const Q4Args& p) {
-    q4_row_tile<DT>(p.m, [&](auto rows) {
-        constexpr int ROWS = decltype(rows)::value;
+    q4_row_tile<DT>(p, [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value, W = kQ4MoreWaves<DT, ROWS>;
         if (q4_two_tiles<ROWS>(p)) q4_forward_launch<DT, ROWS, 2, 8>(s, p);
+        else if (q4_long_sum<ROWS>(p)) q4_forward_launch<DT, ROWS, 1, W>(s, p);
         else q4_forward_launch<DT, ROWS, 1, 8>(s, p);
     });
     return hipGetLastError();
@@ -748,9 +777,10 @@ hipError_t q4_forward(hipStream_t s, const Q4Args& p) {
 
 template <int DT>
 hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
-    q4_row_tile<DT>(p.m, [&](auto rows) {
-        constexpr int ROWS = decltype(rows)::value;
+    q4_row_tile<DT>(p, [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value, W = kQ4MoreWaves<DT, ROWS>;
         if (q4_two_tiles<ROWS>(p)) q4_grad_launch<DT, ROWS, 2, 8>(s, p);
+        else if (q4_long_sum<ROWS>(p)) q4_grad_launch<DT, ROWS, 1, W>(s, p);
         else q4_grad_launch<DT, ROWS, 1, 8>(s, p);
     });
     return hipGetLastError();

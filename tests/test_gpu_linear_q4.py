@@ -230,6 +230,22 @@ def test_equal_calls_streams_and_graphs(spc, dev):
         assert all(torch.equal(p, q) for p, q in zip(out, step()))
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("out,inp,m", [
+    (8200, 64, 3), (8200, 64, 9), (16_500, 32, 16),             # long sums of the gradient
+    (40, 8224, 2), (20, 16_416, 13),                            # and of the forward pass
+    (1040, 96, 7), (2100, 96, 11), (4100, 64, 17), (4100, 64, 30), (64, 4128, 31), (70, 128, 200)])
+def test_row_tiles(spc, dev, dt, out, inp, m):
+    """Row counts around the blocks' 4, 8, 16 and 32 rows, where the columns are
+    few, many, or the summed features long."""
+    nat = spc._native
+    blocks = random_blocks(out, inp, m)
+    fwd, bwd = _both(nat, blocks, dev)
+    x, dy = _randn((m, inp), 1, DT[dt], dev), _randn((m, out), 2, DT[dt], dev)
+    check("y", nat.linear_q4_0(x, fwd), *product(x, blocks), DT[dt])
+    check("dx", nat.linear_q4_0_input_grad(dy, bwd), *gradient(dy, blocks), DT[dt])
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,o", [(0, 5), (1, 1), (3, 33), (31, 130), (512, 64), (513, 31), (5000, 130),
                                  (262_200, 3)])
