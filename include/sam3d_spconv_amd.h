@@ -680,9 +680,9 @@ int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_str
  * packed with transpose 1.  Sums are F32, one rounding to dtype at the end.
  * F32 rows: the weights enter exactly, dy times a scale in F32, as three parts.
  * f16 rows: the weights enter exactly, the rows as they are.  bf16 rows: the
- * weights enter as f16(d (q - 8)) (at most 2^-11 of a weight), the rows with
- * what lies above 2^-28 of the row's largest value.  Under 16-bit rows weights
- * past f16's 65,504 are infinite.  A row with an infinity or NaN comes out
+ * weights enter as f16(d (q - 8)) (at most 2^-11 of a weight), the rows as they
+ * are.  Under 16-bit rows weights past f16's 65,504 are infinite (their products
+ * infinite or NaN).  A row with an infinity or NaN comes out
  * non-finite, the others as without it. */
 int spc_linear_q4_0_input_grad(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                                int64_t m, const void* packed, int64_t out_features,

@@ -19,7 +19,7 @@
 // ones do (one row, 1024 -> 2048: off by 1.3e-6 of the output's size, 9.5e-8 so).
 // For the gradient the scale varies along the summed index.  F32 rows are
 // multiplied by it first (F32) and run as three bf16 parts; for 16-bit rows the
-// weights are, as f16(d (q - 8)).
+// weights are, as one or two operands.
 //
 // The weights are laid out once (spc_linear_q4_0_pack) in the order the lanes
 // want them: for 16 columns and 128 summed features a lane's 16 bytes are its
@@ -527,17 +527,29 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 // of d's last bit below 2^-11 of the weight, so an f16 too (outputs off by
 // 2.1e-4 of their size with it, 2.7e-4 without, as much as the plain form's).
 // Under bf16 rows it stays out: at most 2^-11 of a weight, an eighth of a bf16
-// output's rounding.  bf16 rows have their exponents moved into f16's range by
-// a power of two that each wave chooses for each row from what it has seen of
-// it (exact for values down to 2^-27 of the row's largest; of smaller ones less
-// than 2^-28 of it is lost).
+// output's rounding.
+//
+// bf16 rows have a range that f16 has not, and a value may not vanish under its
+// row's largest: where the large ones meet zero weights it is the result.  Two ways:
+// - raw: the rows as they are, f16(d (q - 8)) as two bf16 operands, cut and the
+//   three bits below the cut: exact for every bf16, for twelve instructions a
+//   pair of weights where one operand takes four;
+// - moved: the rows' exponents moved into f16's range by a power of two that each
+//   wave chooses for each row from what it has seen of it, eleven instructions a
+//   pair of row elements; a step with a value that does not fit (below 2^-27 of
+//   its row's largest) goes raw.
+// The first falls on a block's 16 NT columns, the second on its ROWS rows, so
+// rows are moved where they are few (us raw / moved: one row, 16,384 -> 8192
+// 28.2 / 17.8, eight, 8192 -> 1024 9.4 / 7.7, sixteen by two tiles, 8192 ->
+// 16,384 31.3 / 29.4, by one, 16,384 -> 4096 21.2 / 22.7, thirty, 22.4 / 27.0).
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // The eight weights of a word times their eight scales, rounded, and (PARTS 2)
 // what the rounding left over.
-template <int PARTS>
+// BF16: the rounded weight as two bf16 operands.
+template <bool BF16, int PARTS>
 __device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t one, u32x4 (&r)[PARTS]) {
     const u32x4 q = q4_expand<true>(w, one);  // 16 + q
 #pragma unroll
@@ -547,9 +559,15 @@ __device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t o
         const f16x2 v = __builtin_bit_cast(f16x2, qi) - (f16x2)(_Float16)24.0f;
         const f16x2 s = __builtin_bit_cast(f16x2, di);
         const f16x2 t = v * s;
-        r[0][i] = __builtin_bit_cast(uint32_t, t);
-        if constexpr (PARTS == 2)
-            r[1][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, s, -t));
+        if constexpr (BF16) {
+            const float a = (float)t.x, b = (float)t.y;
+            r[0][i] = q4_high_pair(a, b);
+            r[1][i] = q4_high_pair(q4_rest(a), q4_rest(b));
+        } else {
+            r[0][i] = __builtin_bit_cast(uint32_t, t);
+            if constexpr (PARTS == 2)
+                r[1][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, s, -t));
+        }
     }
 }
 
@@ -561,6 +579,7 @@ __device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t o
 struct Q4Bias {
     u16x2 seen = {0, 0};   // the lane's largest magnitudes, bf16 bits
     u16x2 limit = {0, 0};  // largest that fits; 0 until the row has one but 0
+    u16x2 least = {0, 0};  // smallest but 0 that fits, less one
     int bias = 0;
 
     // Takes a step's elements in; true if one does not fit.
@@ -571,6 +590,15 @@ struct Q4Bias {
             m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
         seen = __builtin_elementwise_max(seen, m);
         return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(m, limit)) != 0;
+    }
+    // Whether an element but 0 is too small to fit.
+    __device__ __forceinline__ bool small(u32x4 v) const {
+        u16x2 m = {0xffff, 0xffff};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (zeros become the largest)
+            m = __builtin_elementwise_min(
+                m, (u16x2)(__builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu) - (u16x2){1, 1}));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(least, m)) != 0;
     }
     // The largest magnitude the row's 16 lanes have seen.
     __device__ __forceinline__ int top() const {
@@ -587,10 +615,11 @@ struct Q4Bias {
         const int by = to - bias;
         bias = to;
         if (t != 0) limit = (u16x2)(uint16_t)(((bias + 31) << 7) - 1);
+        // (without a bias subnormals are f16's)
+        least = (u16x2)(uint16_t)(bias ? ((bias + 1) << 7) - 1 : 0);
         return by;
     }
-    // bf16 -> f16 with the bias taken off; what falls below f16's range is 0
-    // (or, in the last binade, loses its leading bit).
+    // bf16 -> f16 with the bias taken off, for elements that fit.
     __device__ __forceinline__ u32x4 f16(u32x4 v) const {
         const u16x2 off = (u16x2)(uint16_t)(bias << 7);
         u32x4 r;
@@ -614,7 +643,8 @@ struct Q4Bias {
 template <int DT, int ROWS, int NT, int W>
 __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
     typedef Q4Rows<DT, ROWS> R;
-    constexpr int MT = R::MT, NI = R::NI, PARTS = DT == SPC_F16 ? 2 : 1;
+    constexpr bool MOVED = DT == SPC_BF16 && ROWS < 16 * NT;
+    constexpr int MT = R::MT, NI = R::NI;
     constexpr size_t SCALES = ROWS * R::STRIDE, FACTORS = SCALES + kQ4Group * 2;
     constexpr size_t WAVE = FACTORS + (ROWS * 4 + 15) / 16 * 16;
     __shared__ __attribute__((aligned(16))) char lds[q4_lds(WAVE, MT * NT, W)];
@@ -636,12 +666,13 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
         s.d = reinterpret_cast<const u32x4*>(all_scales + (int64_t)g * kQ4Group)[lane % 16];
         rows.load(s.x, g, p.sum);
     };
-    floatx4 acc[MT][NT];
+    // (moved rows: acc in units of their biases)
+    floatx4 acc[MT][NT], raw[MT][NT];
     Q4Bias bias[NI];
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0, 0, 0, 0};
+        for (int b = 0; b < NT; ++b) acc[a][b] = raw[a][b] = floatx4{0, 0, 0, 0};
     // multiplies the accumulators' rows by the factors f(i) of the loads' rows
     auto scale_rows = [&](auto&& f) __attribute__((always_inline)) {
         float* fs = reinterpret_cast<float*>(mine + FACTORS);
@@ -660,23 +691,10 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
             }
     };
     const uint32_t one = q4_one<true>();
-    q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
-        if constexpr (DT == SPC_BF16) {
-            bool over = false;
-#pragma unroll
-            for (int i = 0; i < NI; ++i) over |= bias[i].see(s.x[i]);
-            if (__any(over)) {
-                float f[NI];
-#pragma unroll
-                for (int i = 0; i < NI; ++i) f[i] = ldexpf(1.0f, -bias[i].move());
-                scale_rows([&](int i) { return f[i]; });
-            }
-        }
-        q4_wave_sync();
-#pragma unroll
-        for (int i = 0; i < NI; ++i) R::put(mine, i, DT == SPC_BF16 ? bias[i].f16(s.x[i]) : s.x[i]);
-        if (lane < 16) scales[lane] = s.d;
-        q4_wave_sync();
+    // a step's products of the rows in LDS, as f16 or bf16, added to `to`
+    auto products = [&](const Step& s, auto bf16, floatx4 (&to)[MT][NT]) __attribute__((always_inline)) {
+        constexpr bool BF16 = decltype(bf16)::value;
+        constexpr int PARTS = BF16 || DT == SPC_F16 ? 2 : 1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             u32x4 x[MT];
@@ -686,19 +704,48 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
                 u32x4 w[PARTS];
-                q4_expand_scaled<PARTS>(s.q[b][j], d, one, w);
+                q4_expand_scaled<BF16, PARTS>(s.q[b][j], d, one, w);
 #pragma unroll
                 for (int a = 0; a < MT; ++a)
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) acc[a][b] = q4_mfma<true>(x[a], w[q], acc[a][b]);
+                    for (int q = 0; q < PARTS; ++q) to[a][b] = q4_mfma<!BF16>(x[a], w[q], to[a][b]);
             }
         }
+    };
+    q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
+        bool small = false;
+        if constexpr (MOVED) {
+            bool over = false;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) over |= bias[i].see(s.x[i]);
+            if (__any(over)) {
+                float f[NI];
+#pragma unroll
+                for (int i = 0; i < NI; ++i) f[i] = ldexpf(1.0f, -bias[i].move());
+                scale_rows([&](int i) { return f[i]; });
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i) small |= bias[i].small(s.x[i]);
+            small = __any(small);
+        }
+        q4_wave_sync();
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            R::put(mine, i, MOVED && !small ? bias[i].f16(s.x[i]) : s.x[i]);
+        if (lane < 16) scales[lane] = s.d;
+        q4_wave_sync();
+        if (MOVED && small) products(s, std::true_type{}, raw);
+        else products(s, std::bool_constant<DT == SPC_BF16 && !MOVED>{}, acc);
     });
-    if constexpr (DT == SPC_BF16) {
+    if constexpr (MOVED) {
         float f[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) f[i] = bias[i].factor();
         scale_rows([&](int i) { return f[i]; });
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[a][b] += raw[a][b];
     }
     q4_finish<DT, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }

@@ -1,0 +1,50 @@
+"""4-bit products of rows whose values lie far apart: what a value contributes
+does not depend on the largest one of its row.
+
+u = 2^-24; a matrix instruction adds 32 exact products with at most 32 roundings
+of 2 u each (a cut) of the magnitudes so far, a chain of instructions on one
+accumulator one more each; see q4_reference."""
+import pytest
+import torch
+
+from norm_reference import U, check
+from q4_reference import dequant, random_blocks
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def _gradient(dy, blocks):
+    """(dx, bound before the output's rounding), relative to sum |dy w| alone: a
+    value on zero weights adds nothing to it.  F32 rows times the scale round
+    once (u); bf16 rows meet f16(w), 2^-11 at most.  Up to three operands, eight
+    waves or more; parts of F32 products below 2^-126 count as zero (2^-122 an
+    element, q4_reference)."""
+    d, w = dy.detach().cpu().double(), dequant(blocks)
+    weights = {torch.float32: U, torch.bfloat16: 2.0 ** -11, torch.float16: 0.0}[dy.dtype]
+    chain = 3 * (-(-w.shape[0] // 128) // 8 + 1) * 4
+    e = (weights + 2 * (32 + chain + 16) * U) * (d.abs() @ w.abs())
+    return d @ w, e + (w.shape[0] * 2.0 ** -122 if dy.dtype == torch.float32 else 0.0)
+
+
+# blocks of 4, 8, 16 and 32 rows, of one and two column tiles, eight and sixteen waves
+@pytest.mark.parametrize("out,inp,m", [
+    (256, 64, 1), (2500, 96, 1), (2500, 96, 7), (16_500, 32, 4), (16_500, 64, 30), (300, 8256, 3),
+    (300, 4096, 6), (300, 4096, 16), (300, 4096, 30), (8200, 4096, 13), (16_500, 4096, 16),
+    (300, 2048, 90), (300, 8256, 40)])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_gradient_under_large_values_on_zero_weights(spc, dev, dt, out, inp, m):
+    """Rows whose large values stand where every weight is zero: the others'
+    products are the result, down to a type's last binade."""
+    blocks = random_blocks(out, inp, out + inp)
+    dead = torch.randperm(out, generator=torch.Generator().manual_seed(1))[:out // 50 + 1]
+    blocks[dead, :, 2:] = 0x88
+    bwd = spc._native.pack_q4_0(blocks.to(dev), out_features=out, in_features=inp, transpose=True)
+    dy = torch.randn(m, out, generator=torch.Generator().manual_seed(2))
+    for large, scale in [(1e4, 1e-4)] + ([] if dt == "f16" else [(1e30, 1e-3), (1e37, 1e-20)]):
+        x = dy * scale
+        x[:, dead] = large
+        x = x.to(DT[dt]).to(dev)
+        check(f"dx {dt} {large} over {scale}", spc._native.linear_q4_0_input_grad(x, bwd),
+              *_gradient(x, blocks), DT[dt])
