@@ -669,8 +669,9 @@ int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out
  * x_stride elements apart), y contiguous in dtype, bias [out_features] in
  * bias_dtype or NULL.  Weights enter exactly, sums are F32, one rounding to
  * dtype at the end (F32 rows enter as three 8-bit parts, of which those below
- * 2^-126 are taken as zero); a row with an infinity or NaN comes out as NaNs, the
- * others as without it.  m up to 1,048,560; made for few rows (the weights'
+ * 2^-126 are taken as zero; of bf16 and F32 rows a block's sum x (q - 8) has to
+ * stay below 2^132, which values up to 2^123 do whatever the weights); a row with
+ * an infinity or NaN comes out as NaNs, the others as without it.  m up to 1,048,560; made for few rows (the weights'
  * bytes are the cost up to some 64), right for any. */
 int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
                     const void* packed, int64_t out_features, int64_t in_features, const void* bias,

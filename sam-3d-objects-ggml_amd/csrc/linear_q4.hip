@@ -6,17 +6,17 @@
 // are read once, as they are, and expanded in registers for the matrix
 // instructions, which take 16 rows at the price of one:
 //
-//   16 + q is the bf16 pattern 0x4180 | q << 3 (f16: 0x4c00 | q << 6), exactly,
-//   so two weights cost one shift and one and-or;
-//   sum x (q - 8) = sum x (16 + q) + sum x (-24), and the second sum is one
-//   more matrix instruction on a constant, shared by all columns.
+//   f16: 16 + q is the pattern 0x4c00 | q << 6, exactly, so two weights are one
+//   shift, one and-or and one subtraction of 24;
+//   bf16: (q - 8) / 16 by the conversion of four-bit integers.
+//
+// ((q - 8) itself, not 16 + q beside a sum of -24 x, though that saves an
+// instruction: a row's large value that meets zero weights would leave its own
+// rounding in every column, or overflow.)
 //
 // Forward, one 16x16x32 product covers exactly one block of every column; its
 // F32 result times d is added to the F32 accumulator, so no weight is ever
-// rounded.  F32 rows run as three bf16 parts that add up to them exactly, and
-// on (q - 8) / 16 itself, three instructions a weight: the two sums above
-// cancel to a fifth of themselves, which 16-bit outputs do not see and F32
-// ones do (one row, 1024 -> 2048: off by 1.3e-6 of the output's size, 9.5e-8 so).
+// rounded.  F32 rows run as three bf16 parts that add up to them exactly.
 // For the gradient the scale varies along the summed index.  F32 rows are
 // multiplied by it first (F32) and run as three bf16 parts; for 16-bit rows the
 // weights are, as one or two operands.
@@ -144,25 +144,26 @@ __global__ __launch_bounds__(256) void q4_quantize_kernel(const float* __restric
 }
 
 // ---- operands -------------------------------------------------------------
-// The patterns' fixed bits: one of the two in a vector register, since an
+// The f16 pattern's fixed bits: one of the two in a vector register, since an
 // instruction reads one scalar operand, and the and-or is one instruction then.
-template <bool F16>
 __device__ __forceinline__ uint32_t q4_one() {
-    uint32_t v = F16 ? 0x4c004c00u : 0x41804180u;
+    uint32_t v = 0x4c004c00u;
     asm("" : "+v"(v));
     return v;
 }
-template <bool F16>
-__device__ __forceinline__ u32x4 q4_expand(uint32_t w, uint32_t one) {
-    if constexpr (F16) {
-        constexpr uint32_t m = 0x03c003c0u;
-        return u32x4{((w << 6) & m) | one, ((w << 2) & m) | one, ((w >> 2) & m) | one,
-                     ((w >> 6) & m) | one};
-    } else {
-        constexpr uint32_t m = 0x00780078u;
-        return u32x4{((w << 3) & m) | one, ((w >> 1) & m) | one, ((w >> 5) & m) | one,
-                     ((w >> 9) & m) | one};
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// (q - 8) of a word's weights as f16.
+__device__ __forceinline__ u32x4 q4_expand_f16(uint32_t w, uint32_t one) {
+    constexpr uint32_t m = 0x03c003c0u;
+    u32x4 r = {((w << 6) & m) | one, ((w << 2) & m) | one, ((w >> 2) & m) | one, ((w >> 6) & m) | one};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t ri = r[i];  // (a copy: a bit cast of a vector's element takes the vector's first)
+        r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, ri) - (f16x2)(_Float16)24.0f);
     }
+    return r;
 }
 
 template <bool F16>
@@ -176,23 +177,29 @@ __device__ __forceinline__ floatx4 q4_mfma(u32x4 a, u32x4 b, floatx4 c) {
 }
 
 // (q - 8) / 16 of a word's weights as bf16: the conversion of four-bit
-// integers, whose results end in zeros, so the cut to bf16 is exact.
+// integers, whose results end in zeros, so the cut to bf16 is exact.  It takes
+// a byte's low half, so every other nibble costs no shift of its own (compiled
+// from shifts: 144 instructions for 64 weights, 112 so).
+template <int BYTE>
+__device__ __forceinline__ float q4_signed(uint32_t w) {
+    float f;
+    if constexpr (BYTE == 0) f = __builtin_amdgcn_cvt_off_f32_i4(w);
+    if constexpr (BYTE == 1)
+        asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+    if constexpr (BYTE == 2)
+        asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+    if constexpr (BYTE == 3)
+        asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+    return f;
+}
 __device__ __forceinline__ u32x4 q4_expand_signed(uint32_t w) {
     w ^= 0x88888888u;  // q - 8 as four bits of two's complement
-    u32x4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = __builtin_amdgcn_cvt_off_f32_i4(w >> (4 * i));
-        const float b = __builtin_amdgcn_cvt_off_f32_i4(w >> (4 * i + 16));
-        r[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-    }
-    return r;
-}
-
-template <bool F16>
-__device__ __forceinline__ u32x4 q4_minus_24() {
-    constexpr uint32_t v = F16 ? 0xce00ce00u : 0xc1c0c1c0u;
-    return u32x4{v, v, v, v};
+    const uint32_t odd = w >> 4;
+    auto pair = [](float a, float b) __attribute__((always_inline)) {
+        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    };
+    return u32x4{pair(q4_signed<0>(w), q4_signed<2>(w)), pair(q4_signed<0>(odd), q4_signed<2>(odd)),
+                 pair(q4_signed<1>(w), q4_signed<3>(w)), pair(q4_signed<1>(odd), q4_signed<3>(odd))};
 }
 
 // The high halves of two F32 words as a bf16 pair (a cut, not a rounding).
@@ -402,7 +409,7 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = floatx4{0, 0, 0, 0};
-    const uint32_t one = q4_one<F16>();
+    const uint32_t one = q4_one();
     q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
         q4_wave_sync();
 #pragma unroll
@@ -426,18 +433,15 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
                 off[a] = floatx4{0, 0, 0, 0};
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) xp[a][q] = R::get(mine, q, a, j);
-                if constexpr (PARTS == 1) off[a] = q4_mfma<F16>(xp[a][0], q4_minus_24<F16>(), off[a]);
+                // (nothing, or NaN where the row has an infinity or NaN)
+                if constexpr (PARTS == 1) off[a] = q4_mfma<F16>(xp[a][0], u32x4{0, 0, 0, 0}, off[a]);
             }
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                float d = f16_bits_to_f32((uint16_t)(s.d[b][j / 2] >> (16 * (j & 1))));
+                const float d = f16_bits_to_f32((uint16_t)(s.d[b][j / 2] >> (16 * (j & 1))));
                 u32x4 w;
-                if constexpr (PARTS == 1) {
-                    w = q4_expand<F16>(s.q[b][j], one);
-                } else {
-                    w = q4_expand_signed(s.q[b][j]);
-                    d *= 16.0f;
-                }
+                if constexpr (F16) w = q4_expand_f16(s.q[b][j], one);
+                else w = q4_expand_signed(s.q[b][j]);
 #pragma unroll
                 for (int a = 0; a < MT; ++a) {
                     floatx4 t = off[a];
@@ -448,6 +452,12 @@ __global__ __launch_bounds__(64 * W) void q4_forward_kernel(Q4Args p) {
             }
         }
     });
+    if constexpr (!F16) {
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) acc[a][b] *= 16.0f;
+    }
     q4_finish<DT, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
@@ -543,7 +553,6 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 // 28.2 / 17.8, eight, 8192 -> 1024 9.4 / 7.7, sixteen by two tiles, 8192 ->
 // 16,384 31.3 / 29.4, by one, 16,384 -> 4096 21.2 / 22.7, thirty, 22.4 / 27.0).
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // The eight weights of a word times their eight scales, rounded, and (PARTS 2)
@@ -551,12 +560,11 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // BF16: the rounded weight as two bf16 operands.
 template <bool BF16, int PARTS>
 __device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t one, u32x4 (&r)[PARTS]) {
-    const u32x4 q = q4_expand<true>(w, one);  // 16 + q
+    const u32x4 q = q4_expand_f16(w, one);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        // (copies: a bit cast of a vector's element takes the vector's first)
         const uint32_t qi = q[i], di = d[i];
-        const f16x2 v = __builtin_bit_cast(f16x2, qi) - (f16x2)(_Float16)24.0f;
+        const f16x2 v = __builtin_bit_cast(f16x2, qi);
         const f16x2 s = __builtin_bit_cast(f16x2, di);
         const f16x2 t = v * s;
         if constexpr (BF16) {
@@ -690,7 +698,7 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
                 for (int b = 0; b < NT; ++b) acc[a][b][i] *= fi;
             }
     };
-    const uint32_t one = q4_one<true>();
+    const uint32_t one = q4_one();
     // a step's products of the rows in LDS, as f16 or bf16, added to `to`
     auto products = [&](const Step& s, auto bf16, floatx4 (&to)[MT][NT]) __attribute__((always_inline)) {
         constexpr bool BF16 = decltype(bf16)::value;

@@ -48,3 +48,35 @@ def test_gradient_under_large_values_on_zero_weights(spc, dev, dt, out, inp, m):
         x = x.to(DT[dt]).to(dev)
         check(f"dx {dt} {large} over {scale}", spc._native.linear_q4_0_input_grad(x, bwd),
               *_gradient(x, blocks), DT[dt])
+
+
+def _product(x, blocks):
+    """(y, bound before the output's rounding), relative to sum |x w| alone: a
+    block's 32 products x (q - 8) are exact, in one matrix instruction (F32 rows:
+    three), then one addition a block and the waves'."""
+    d, w = x.detach().cpu().double(), dequant(blocks)
+    steps = (96 if x.dtype == torch.float32 else 32) * 2 + w.shape[1] // 32 + 17
+    return d @ w.t(), steps * U * (d.abs() @ w.abs().t())
+
+
+@pytest.mark.parametrize("out,inp,m", [
+    (64, 128, 1), (64, 128, 16), (190, 416, 30), (4100, 64, 17), (20, 16_416, 13), (8300, 64, 40),
+    (2100, 96, 100)])
+@pytest.mark.parametrize("dt,large", [("f16", 6e4), ("bf16", 2.0 ** 20), ("bf16", 2e37), ("bf16", 3e38),
+                                      ("f32", 2.0 ** 20), ("f32", 3e38)])
+def test_product_under_large_values_on_zero_weights(spc, dev, dt, large, out, inp, m):
+    """A large value that meets zero weights only leaves no trace, in its
+    block's sums or elsewhere; on other weights it is a term like any."""
+    blocks = random_blocks(out, inp, out + inp)
+    blocks[:, :, 2] = blocks[:, :, 2] & 0xf0 | 8          # weight 0 of every block: zero
+    fwd = spc._native.pack_q4_0(blocks.to(dev), out_features=out, in_features=inp)
+    x = torch.randn(m, inp, generator=torch.Generator().manual_seed(3))
+    x[:, ::32] = torch.where(torch.arange(m)[:, None] % 2 == 0, large, -large)
+    x = x.to(DT[dt]).to(dev)
+    check(f"y {dt} {large}", spc._native.linear_q4_0(x, fwd), *_product(x, blocks), DT[dt])
+    x[:, 5] = large                                       # and on weights of every size
+    y, bound = _product(x, blocks)
+    got = spc._native.linear_q4_0(x, fwd)
+    fits = y.abs() + bound < torch.finfo(DT[dt]).max * 0.99
+    check(f"y {dt} {large} met", torch.where(fits.to(dev), got, 0), torch.where(fits, y, 0),
+          torch.where(fits, bound, 0), DT[dt])
