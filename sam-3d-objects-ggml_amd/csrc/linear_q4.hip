@@ -850,6 +850,9 @@ hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
 // The sum was the one step of the pass that could record a memory node into a
 // captured graph.)
 constexpr int kQ4SumCols = 32, kQ4SumThreads = 1024, kQ4SumRows = 512;
+// Blocks along the columns, each taking every such many-th 32: a launch holds
+// below 2^32 threads.
+constexpr int64_t kQ4SumBlocks = 1 << 21;
 
 __device__ __forceinline__ float q4_element(const void* p, int dt, int64_t i) {
     if (dt == SPC_F32) return static_cast<const float*>(p)[i];
@@ -864,32 +867,36 @@ __global__ __launch_bounds__(kQ4SumThreads) void q4_column_sums_kernel(const voi
     constexpr int C = kQ4SumCols, L = kQ4SumThreads / C, W = kQ4SumThreads / 64, DEEP = 8;
     __shared__ float ls[W][C];
     const int cl = threadIdx.x % C, l = threadIdx.x / C;
-    const int64_t col = (int64_t)blockIdx.x * C + cl;
     const int64_t lo = (int64_t)blockIdx.y * rows_per, hi = min(m, lo + rows_per);
-    float s = 0.0f;
-    if (col < cols)
-        for (int64_t r = lo + l; r < hi; r += DEEP * L) {
-            float v[DEEP];
+    for (int64_t c0 = (int64_t)blockIdx.x * C; c0 < cols; c0 += (int64_t)gridDim.x * C) {
+        const int64_t col = c0 + cl;
+        float s = 0.0f;
+        if (col < cols)
+            for (int64_t r = lo + l; r < hi; r += DEEP * L) {
+                float v[DEEP];
 #pragma unroll
-            for (int i = 0; i < DEEP; ++i) {
-                const int64_t at = r + i * L;
-                v[i] = q4_element(x, dtype, min(at, hi - 1) * stride + col);
-                if (at >= hi) v[i] = 0.0f;
+                for (int i = 0; i < DEEP; ++i) {
+                    const int64_t at = r + i * L;
+                    v[i] = q4_element(x, dtype, min(at, hi - 1) * stride + col);
+                    if (at >= hi) v[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < DEEP; ++i) s += v[i];
             }
+        s += __shfl_xor(s, C);
+        if ((threadIdx.x & 63) < C) ls[threadIdx.x >> 6][cl] = s;
+        __syncthreads();
+        if (l == 0 && col < cols) {
+            s = 0.0f;
 #pragma unroll
-            for (int i = 0; i < DEEP; ++i) s += v[i];
+            for (int w = 0; w < W; ++w) s += ls[w][cl];
+            const int64_t at = (int64_t)blockIdx.y * cols + col;
+            if (out_dtype == SPC_F32) q4_store<SPC_F32>(out, at, s);
+            else if (out_dtype == SPC_BF16) q4_store<SPC_BF16>(out, at, s);
+            else q4_store<SPC_F16>(out, at, s);
         }
-    s += __shfl_xor(s, C);
-    if ((threadIdx.x & 63) < C) ls[threadIdx.x >> 6][cl] = s;
-    __syncthreads();
-    if (l != 0 || col >= cols) return;
-    s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) s += ls[w][cl];
-    const int64_t at = (int64_t)blockIdx.y * cols + col;
-    if (out_dtype == SPC_F32) q4_store<SPC_F32>(out, at, s);
-    else if (out_dtype == SPC_BF16) q4_store<SPC_BF16>(out, at, s);
-    else q4_store<SPC_F16>(out, at, s);
+        __syncthreads();  // (before the sums of the next columns)
+    }
 }
 
 // Blocks along the rows: at most a y-dimension's, of more rows where that is few.
@@ -897,7 +904,8 @@ inline int64_t q4_sum_rows(int64_t m) { return std::max<int64_t>(kQ4SumRows, cei
 
 inline bool q4_float_dtype(int dt) { return dt == SPC_F32 || dt == SPC_F16 || dt == SPC_BF16; }
 
-// Up to 2^27 features: a launch holds below 2^32 threads, 512 for 32 columns.
+// Up to 2^27 features: a launch holds below 2^32 threads, the products' 512 for
+// 16 or 32 columns.
 constexpr int64_t kQ4MaxFeatures = 1 << 27;
 constexpr int64_t kQ4MaxRows = 65535 * 16;  // a launch's y dimension, 16 rows a block
 
@@ -1051,7 +1059,7 @@ int spc_linear_q4_0_bias_grad(spc_stream_t stream, int dtype, const void* dy, in
         return SPC_BAD_ARG;
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const unsigned cb = (unsigned)ceil_div(out_features, kQ4SumCols);
+    const unsigned cb = (unsigned)std::min(ceil_div(out_features, kQ4SumCols), kQ4SumBlocks);
     if (need) {
         const int64_t per = q4_sum_rows(m), parts = ceil_div(m, per);
         q4_column_sums_kernel<<<dim3(cb, (unsigned)parts), kQ4SumThreads, 0, s>>>(

@@ -80,3 +80,13 @@ def test_product_under_large_values_on_zero_weights(spc, dev, dt, large, out, in
     fits = y.abs() + bound < torch.finfo(DT[dt]).max * 0.99
     check(f"y {dt} {large} met", torch.where(fits.to(dev), got, 0), torch.where(fits, y, 0),
           torch.where(fits, bound, 0), DT[dt])
+
+
+@pytest.mark.parametrize("m", [1, 513])
+def test_bias_gradient_of_the_widest_linear(spc, dev, m):
+    """2^27 features, as many as the products take, by one kernel and by two
+    (rows that repeat: the sums are exact)."""
+    o = 1 << 27
+    row = torch.randint(-128, 128, (1, o), device=dev, dtype=torch.int16).to(torch.bfloat16)
+    db = spc._native.linear_q4_0_bias_grad(row.expand(m, o))
+    assert bool((db == row[0].float() * m).all())
