@@ -884,6 +884,8 @@ class Q4Linear(nn.Linear):
             raise ValueError(f"expected {n // 32 * 18} Q4_0 bytes (uint8) for this Linear")
         # a copy: the packed operands are made from it when first needed
         blocks = blocks.detach().clone(memory_format=torch.contiguous_format)
+        if blocks.is_cuda:  # the first call, which lays them out, may come on another stream
+            torch.cuda.current_stream(blocks.device).synchronize()
         self.drop_q4_0()
         self._q4 = blocks
 
