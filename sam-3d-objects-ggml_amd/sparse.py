@@ -819,22 +819,37 @@ class SparseInverseConv3d(nn.Module, _ConvCore):
 # ---------------------------------------------------------------------------
 # spatial ops (SP/spatial.py)
 # ---------------------------------------------------------------------------
+def _accumulator(t: torch.Tensor):
+    return torch.autograd.graph.get_gradient_edge(t).node
+
+
 def _eager_leaves(*ts) -> list:
     """The gradient accumulators of the leaves among ts, to be held until the
     op is recorded.  An accumulator belongs to the stream of the first graph it
     is part of; a backward pass captured while an eager graph keeps it alive
-    would leave the capture, and that ends the process.  So eager graphs mark
-    theirs and a capture that meets a mark is refused."""
+    would leave the capture, and that ends the process.  So a capture takes
+    only accumulators that a call here made, in it or in an earlier capture on
+    the same stream.  Eager calls mark theirs; one that another operator made
+    shows by outliving the reference to it."""
     capturing = torch.cuda.is_current_stream_capturing()
+    stream = torch.cuda.current_stream().cuda_stream if capturing else None
     nodes = []
     for t in ts:
         if t is not None and t.requires_grad and t.is_leaf:
-            node = torch.autograd.graph.get_gradient_edge(t).node
+            node = _accumulator(t)
             if not capturing:
                 node.metadata["eager"] = True
-            elif "eager" in node.metadata:
-                raise RuntimeError("an eager graph of these tensors is alive: drop its outputs and "
-                                   "losses before capturing a forward and backward pass")
+            elif node.metadata.get("captured") != stream:
+                if not node.metadata:
+                    node.metadata["eager"] = True
+                    del node
+                    node = _accumulator(t)
+                if node.metadata:
+                    raise RuntimeError(
+                        "an eager graph of these tensors is alive: drop its outputs and losses before "
+                        "capturing a forward and backward pass (in a capture, leaves that several "
+                        "operators take come here first, or as a view)")
+                node.metadata["captured"] = stream
             nodes.append(node)
     return nodes
 
@@ -924,12 +939,13 @@ class Q4Linear(nn.Linear):
         nat._need_gpu(input)
         if input.shape[-1] != self.in_features:
             raise ValueError(f"expected input [..., {self.in_features}], got {tuple(input.shape)}")
-        x = input.reshape(-1, self.in_features)
-        if torch.is_grad_enabled() and (x.requires_grad or
+        held = None
+        if torch.is_grad_enabled() and (input.requires_grad or
                                         (self.bias is not None and self.bias.requires_grad)):
-            held = _eager_leaves(input, self.bias)
+            held = _eager_leaves(input, self.bias)  # (before the view, which makes them too)
+        x = input.reshape(-1, self.in_features)
+        if held is not None:
             y = _Q4LinearFn.apply(x, self.bias, self)
-            del held
         else:
             y = nat.linear_q4_0(x, self._q4_operand(x.device, False), self.bias)
         return y.view(*input.shape[:-1], self.out_features)
@@ -1021,7 +1037,9 @@ class SparseLayerNorm32(nn.LayerNorm):
     SiLU in the same pass; gradients go to the feats, weight, bias, scale and
     shift.  With a modulation, rows outside x's layout come out as zeros.  Once
     differentiable.  A forward and backward pass may be captured into a graph,
-    both in the one capture, once no eager graph of the same leaves is alive."""
+    both in the one capture, once no eager graph of the same leaves is alive,
+    this operator's or another's (refused otherwise, as are leaves that another
+    operator of the capture took before: pass a view of those)."""
 
     def __init__(self, channels: int, eps: float = 1e-6, elementwise_affine: bool = True,
                  bias: bool = True):

@@ -158,3 +158,38 @@ def test_bias_gradient_validation(spc):
     assert run(dt=nat.Q8_0) == run(bdt=nat.Q8_0) == run(dy=None) == run(out=None) == nat.BAD_ARG
     assert run(dy=fake + 1) == run(out=fake + 2) == run(m=513) == nat.BAD_ARG
     assert run(m=513, ws=fake, nbytes=63) == run(m=513, ws=fake + 1, nbytes=64) == nat.BAD_ARG
+
+
+def test_captures_take_fresh_accumulators_only(spc, monkeypatch):
+    """What a capture makes of leaves that an eager graph of any operator still
+    holds, and of those it has met itself."""
+    held, sp = spc.sparse._eager_leaves, spc.sparse
+
+    def capture(stream):
+        monkeypatch.setattr(sp.torch.cuda, "is_current_stream_capturing", lambda: stream is not None)
+        monkeypatch.setattr(sp.torch.cuda, "current_stream",
+                            lambda *a: type("Stream", (), {"cuda_stream": stream}))
+
+    a, b = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True)
+    y = a * 2                                 # an eager graph of another operator
+    capture(7)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        held(a, b)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        held(a)                               # again: the first refusal left nothing behind
+    del y
+    keep = held(a, b), a * 2, b * 3
+    assert held(a, a) and held(b)             # met before in this capture
+    capture(8)                                # their graph is alive, on another stream
+    with pytest.raises(RuntimeError, match="eager graph"):
+        held(a)
+    capture(7)
+    assert held(a, None, torch.zeros(3), a * 2)
+    del keep
+    capture(None)
+    keep = held(a), a * 2                     # an eager graph of ours
+    capture(7)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        held(b, a)
+    del keep
+    assert held(a)
