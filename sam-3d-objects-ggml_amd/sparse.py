@@ -882,7 +882,9 @@ class Q4Linear(nn.Linear):
     any leading dimensions, with gradients for the rows (through the frozen
     blocks, spc_linear_q4_0_input_grad) and the bias.  The float parameter is
     left as is and then neither read nor given a gradient; the blocks are not
-    part of the state dict.  Made for few rows: a modulation, a token.  The
+    part of the state dict, and load_state_dict refuses a weight that differs
+    from the float parameter while they stand in its place (drop_q4_0 first, or
+    leave the key out).  Made for few rows: a modulation, a token.  The
     blocks are laid out by the first call and the first backward pass; a
     captured graph reads that memory, so load and drop blocks only once such
     graphs are done with.  Capturing a backward pass: as SparseLayerNorm32."""
@@ -932,6 +934,16 @@ class Q4Linear(nn.Linear):
             torch.cuda.current_stream(device).synchronize()
             self._q4_packed[key] = w
         return w
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        w = state_dict.get(prefix + "weight")
+        if self._q4 is not None and w is not None and (
+                w.is_meta or self.weight.is_meta or
+                not torch.equal(w.to(self.weight.device, self.weight.dtype), self.weight)):
+            args[-1].append(f"{prefix}weight: Q4_0 blocks are loaded in this weight's place, it would "
+                            "not be read: call drop_q4_0() first, or leave the key out")
+        else:
+            super()._load_from_state_dict(state_dict, prefix, *args)
 
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         if self._q4 is None:

@@ -193,3 +193,24 @@ def test_captures_take_fresh_accumulators_only(spc, monkeypatch):
         held(b, a)
     del keep
     assert held(a)
+
+
+def test_a_state_dict_does_not_load_behind_blocks(spc):
+    """A weight that would not be read is refused; the module's own state, a
+    state without the weight, and any after drop_q4_0 load as into nn.Linear."""
+    net = torch.nn.Sequential(spc.sparse.Q4Linear(64, 20), torch.nn.SiLU(), spc.sparse.SparseLinear(64, 20))
+    net[0].load_q4_0(random_blocks(20, 64, 1))
+    own, other = net.state_dict(), torch.nn.Sequential(
+        torch.nn.Linear(64, 20), torch.nn.SiLU(), torch.nn.Linear(64, 20)).state_dict()
+    net.load_state_dict({k: v.clone() for k, v in own.items()})
+    with pytest.raises(RuntimeError, match=r"0\.weight: Q4_0 blocks .* drop_q4_0"):
+        net.load_state_dict(other)
+    with pytest.raises(RuntimeError, match="drop_q4_0"):
+        net.load_state_dict(other, strict=False)
+    other["0.bias"] = other["0.bias"] + 1
+    net.load_state_dict({k: v for k, v in other.items() if k != "0.weight"}, strict=False)
+    assert torch.equal(net[0].bias, other["0.bias"]) and net[0]._q4 is not None
+    assert torch.equal(net[2].weight, other["2.weight"])
+    net[0].drop_q4_0()
+    net.load_state_dict(other)
+    assert torch.equal(net[0].weight, other["0.weight"])
