@@ -36,6 +36,7 @@ import math
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad
 import torch.nn as nn
 
 from . import _native as nat
@@ -819,6 +820,14 @@ class SparseInverseConv3d(nn.Module, _ConvCore):
 # ---------------------------------------------------------------------------
 # spatial ops (SP/spatial.py)
 # ---------------------------------------------------------------------------
+def _recorded(*ts) -> bool:
+    """Whether a call on ts is autograd's: a gradient may be asked for, or one
+    of them may be a dual tensor (the functions then raise: they have no
+    forward mode)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+            or torch.autograd.forward_ad._current_level >= 0)
+
+
 def _accumulator(t: torch.Tensor):
     return torch.autograd.graph.get_gradient_edge(t).node
 
@@ -952,8 +961,7 @@ class Q4Linear(nn.Linear):
         if input.shape[-1] != self.in_features:
             raise ValueError(f"expected input [..., {self.in_features}], got {tuple(input.shape)}")
         held = None
-        if torch.is_grad_enabled() and (input.requires_grad or
-                                        (self.bias is not None and self.bias.requires_grad)):
+        if _recorded(input, self.bias):
             held = _eager_leaves(input, self.bias)  # (before the view, which makes them too)
         x = input.reshape(-1, self.in_features)
         if held is not None:
@@ -1068,7 +1076,7 @@ class SparseLayerNorm32(nn.LayerNorm):
                                  f"{tuple(scale.shape)}")
             offsets = _item_offsets(input)
         args = (x, self.weight, self.bias, scale, shift)
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        if _recorded(*args):
             held = _eager_leaves(*args)
             y = _LayerNormFn.apply(*args, offsets, self.eps, silu)
             del held

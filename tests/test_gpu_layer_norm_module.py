@@ -52,3 +52,23 @@ def test_capture_beside_graphs_of_other_operators(spc, dev):
         grads = torch.autograd.grad(want, [x2, ln.weight, ln.bias], dy)
         for _, y, got in graphs:
             assert torch.equal(y, want) and all(torch.equal(p, q) for p, q in zip(got, grads))
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+@pytest.mark.parametrize("which", ["x", "weight", "scale"])
+def test_forward_mode_is_refused(spc, dev, which, mode):
+    """A tangent is not dropped in silence; calls without one work."""
+    fw = torch.autograd.forward_ad
+    ln = spc.sparse.SparseLayerNorm32(64).to(dev).requires_grad_(False)
+    x, mod = torch.randn(6, 64, device=dev), torch.randn(1, 64, device=dev)
+    want = ln(_tensor(spc, dev, x), mod, mod).feats
+    with mode(), fw.dual_level():
+        assert torch.equal(ln(_tensor(spc, dev, x), mod, mod).feats, want)
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        a, m = dual(x) if which == "x" else x, dual(mod) if which == "scale" else mod
+        if which == "weight":
+            w = ln.weight
+            del ln.weight
+            ln.weight = dual(w.detach())
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            ln(_tensor(spc, dev, a), m, mod)

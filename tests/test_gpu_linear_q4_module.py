@@ -38,3 +38,16 @@ def test_blocks_loaded_on_another_stream(spc, dev, load):
     blocks = blocks.cpu().view(512, 32, 18)
     check("y", y, *product(x, blocks), torch.float32)
     check("dx", x.grad, *gradient(dy, blocks), torch.float32)
+
+
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad])
+def test_forward_mode_is_refused(spc, dev, mode):
+    fw = torch.autograd.forward_ad
+    lin = spc.sparse.Q4Linear(64, 32).to(dev).requires_grad_(False)
+    lin.quantize_q4_0()
+    x = torch.randn(2, 64, device=dev)
+    want = lin(x)
+    with mode(), fw.dual_level():
+        assert torch.equal(lin(x), want)
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            lin(fw.make_dual(x, torch.ones_like(x)))
