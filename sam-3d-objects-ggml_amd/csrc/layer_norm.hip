@@ -93,7 +93,11 @@ __global__ __launch_bounds__(kLnFinalThreads) void ln_finalize_kernel(LnFinal p)
         a += ls[0][w][cl];
         b += ls[1][w][cl];
     }
-    if (p.scale) {
+    if (p.scale && lo >= hi) {  // no row met this item's coefficients, whatever they hold
+        if (p.dscale) ln_put(p.dscale, p.m_dtype, item * p.c + ch, 0.0f);
+        if (p.dshift) ln_put(p.dshift, p.m_dtype, item * p.c + ch, 0.0f);
+        if (p.sums) p.sums[item * 2 * p.c + ch] = p.sums[(item * 2 + 1) * p.c + ch] = 0.0f;
+    } else if (p.scale) {
         const float g = p.gamma ? ln_param(p.gamma, p.p_dtype, ch) : 1.0f;
         const float t = p.beta ? ln_param(p.beta, p.p_dtype, ch) : 0.0f;
         if (p.dscale) ln_put(p.dscale, p.m_dtype, item * p.c + ch, g * a + t * b);
