@@ -329,7 +329,8 @@ __device__ __forceinline__ float ln_rsqrt(float v) {
 }
 
 // sigmoid(z); F32 rows take the correctly scaled exponential, 16-bit rows the
-// hardware's (its error grows as |z| 2^-24, far below half their last bit).
+// hardware's (its error grows as |z| 2^-24, far below half their last bit).  A
+// sigmoid below 2^-126 is zero (z < -87.3: |silu| below 1.1e-36).
 template <int DT>
 __device__ __forceinline__ float ln_sigmoid(float z) {
     const float e = DT == SPC_F32 ? expf(-z) : __expf(-z);

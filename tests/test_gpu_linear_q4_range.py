@@ -90,3 +90,34 @@ def test_bias_gradient_of_the_widest_linear(spc, dev, m):
     row = torch.randint(-128, 128, (1, o), device=dev, dtype=torch.int16).to(torch.bfloat16)
     db = spc._native.linear_q4_0_bias_grad(row.expand(m, o))
     assert bool((db == row[0].float() * m).all())
+
+
+def test_elements_past_32_bits(spc, dev):
+    """Rows further apart than 2^31 elements, and outputs of more than 2^32."""
+    nat = spc._native
+    blocks = random_blocks(4128, 32, 7)
+    fwd = nat.pack_q4_0(blocks.to(dev), out_features=4128, in_features=32)
+    wide = random_blocks(16, 4128, 8)
+    bwd = nat.pack_q4_0(wide.to(dev), out_features=16, in_features=4128, transpose=True)
+    ld = (1 << 31) + 8
+    far = torch.empty(2 * ld + 32, dtype=torch.bfloat16, device=dev).as_strided((3, 32), (ld, 1))
+    far.copy_(torch.randn(3, 32, generator=torch.Generator().manual_seed(1)))
+    check("y far", nat.linear_q4_0(far, fwd), *_product(far, blocks), torch.bfloat16)
+    check("dx far", nat.linear_q4_0_input_grad(far[:, :16], bwd), *_gradient(far[:, :16], wide),
+          torch.bfloat16)
+    del far
+    m = 65_535 * 16
+    assert m * 4128 > 1 << 32
+    x = torch.randn(m, 32, device=dev).bfloat16()
+    rows = [0, 1, 31, m // 2 + 5, 1_040_448, 1_040_449, m - 17, m - 1]   # (1,040,447.8: element 2^32)
+    y = nat.linear_q4_0(x, fwd)
+    check("y", y[rows], *_product(x[rows], blocks), torch.bfloat16)
+    db = nat.linear_q4_0_bias_grad(y)
+    for cols in (slice(0, 2), slice(4126, 4128)):
+        want = y[:, cols].double()
+        # a thread's 64 rows of a block's 2,048, lanes, waves, then 512 blocks' sums
+        check("dbias", db[cols], want.sum(0).cpu(), 2.0 ** -24 * 200 * want.abs().sum(0).cpu(),
+              torch.float32)
+    del y
+    dx = nat.linear_q4_0_input_grad(x[:, :16], bwd)
+    check("dx", dx[rows], *_gradient(x[rows, :16], wide), torch.bfloat16)
