@@ -1000,7 +1000,8 @@ def _item_offsets(x: SparseTensor) -> Optional[torch.Tensor]:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the items' row offsets are copied from the host by the first call on "
                                "these coordinates: run one before capturing a graph")
-        offs = batch_offsets(x)
+        with torch.inference_mode(False):  # (a later call may save them for its backward pass)
+            offs = batch_offsets(x)
         # once: later calls may come on other streams
         torch.cuda.current_stream(offs.device).synchronize()
         return offs

@@ -72,3 +72,24 @@ def test_forward_mode_is_refused(spc, dev, which, mode):
             ln.weight = dual(w.detach())
         with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
             ln(_tensor(spc, dev, a), m, mod)
+
+
+def test_training_after_inference_mode(spc, dev):
+    """What a first call in inference mode keeps (offsets, laid out weights)
+    serves a training pass."""
+    sp = spc.sparse
+    ln, lin = sp.SparseLayerNorm32(64).to(dev), sp.Q4Linear(32, 128).to(dev)
+    x = torch.randn(50, 64, device=dev)
+    coords = torch.tensor([[0, i, 0, 0] for i in range(20)] + [[1, i, 0, 0] for i in range(30)],
+                          dtype=torch.int32, device=dev)
+    emb = torch.randn(2, 32, device=dev)
+    t = sp.SparseTensor(x, coords)
+    with torch.inference_mode():
+        lin.quantize_q4_0()
+        want = ln(t, *lin(emb).chunk(2, 1), silu=True).feats
+    emb.requires_grad_()
+    y = ln(t, *lin(emb).chunk(2, 1), silu=True).feats
+    assert torch.equal(y, want)
+    y.square().sum().backward()
+    assert bool(emb.grad.isfinite().all()) and float(emb.grad.abs().max()) > 0
+    assert bool(ln.weight.grad.isfinite().all()) and bool(lin.bias.grad.isfinite().all())
