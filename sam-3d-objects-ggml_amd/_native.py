@@ -965,6 +965,8 @@ def q4_0_quantize(w: torch.Tensor) -> torch.Tensor:
     dimension) -> Q4_0 blocks (uint8, 18 bytes per block; spc_q4_0_quantize)."""
     dev = _one_device(w)
     w = w.detach().to(torch.float32).contiguous()
+    if w.data_ptr() % 16:  # a view at any element
+        w = w.clone()
     n = w.numel()
     out = torch.empty(n // 32 * 18, dtype=torch.uint8, device=dev)
     st = _launch(lib().spc_q4_0_quantize, dev, _ptr(w), n, _ptr(out))

@@ -51,3 +51,13 @@ def test_forward_mode_is_refused(spc, dev, mode):
         assert torch.equal(lin(x), want)
         with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
             lin(fw.make_dual(x, torch.ones_like(x)))
+
+
+def test_weights_at_any_element_are_quantised(spc, dev):
+    """A parameter that is a view into a flat buffer."""
+    flat = torch.randn(64 * 96 + 3, generator=torch.Generator().manual_seed(1)).to(dev)
+    lin = spc.sparse.Q4Linear(96, 64, bias=False).to(dev)
+    want = spc._native.q4_0_quantize(flat[3:].clone().view(64, 96))
+    lin.weight.data = flat[3:].view(64, 96)
+    assert torch.equal(lin.quantize_q4_0(), want)
+    assert torch.equal(spc._native.q4_0_quantize(flat[3:]), want)
