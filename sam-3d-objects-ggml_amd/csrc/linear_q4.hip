@@ -24,6 +24,10 @@
 // The weights are laid out once (spc_linear_q4_0_pack) in the order the lanes
 // want them: for 16 columns and 128 summed features a lane's 16 bytes are its
 // eight weights of four instructions, so a wave's load is one 1 KB run.
+//
+// Times below are a kernel's in a captured graph, rows times weights as in ->
+// out.  The two of a choice were measured side by side; those of the loads'
+// order (16 bf16 rows through LDS, steps under way) on weights as 16 + q.
 #include <algorithm>
 
 #include "common.h"
@@ -550,8 +554,9 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 //   its row's largest) goes raw.
 // The first falls on a block's 16 NT columns, the second on its ROWS rows, so
 // rows are moved where they are few (us raw / moved: one row, 16,384 -> 8192
-// 28.2 / 17.8, eight, 8192 -> 1024 9.4 / 7.7, sixteen by two tiles, 8192 ->
-// 16,384 31.3 / 29.4, by one, 16,384 -> 4096 21.2 / 22.7, thirty, 22.4 / 27.0).
+// 28.2 / 17.8, eight, 1024 -> 8192 9.4 / 7.7, sixteen by two tiles, 16,384 ->
+// 8192 31.3 / 29.4, by one, 4096 -> 16,384 21.2 / 22.7, thirty, 16,384 -> 4096
+// 22.4 / 27.0).
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
@@ -583,7 +588,7 @@ __device__ __forceinline__ void q4_expand_scaled(uint32_t w, u32x4 d, uint32_t o
 // The row's largest value seen so far has f16 exponent 28 when the bias is
 // set, so it may grow by 2^2 before the bias has to move.  A step only looks
 // for values past that in its lane; the row's maximum is formed when one is
-// found (every step: 16 rows, 4096 -> 16,384, 22.5 us, 21.0 so).
+// found.
 struct Q4Bias {
     u16x2 seen = {0, 0};   // the lane's largest magnitudes, bf16 bits
     u16x2 limit = {0, 0};  // largest that fits; 0 until the row has one but 0
@@ -775,12 +780,12 @@ void q4_grad_launch(hipStream_t s, const Q4Args& p) {
 // most 32 (F32, whose three operands take as much LDS as that: 16): beyond a few
 // rows a block's time is its rows' conversion, while other CUs would stand
 // idle.  us with the fewest that hold m / that spread: forward, thirty bf16 rows
-// 8192 -> 1024 11.0 / 6.7, 1024 -> 1024 4.3 / 3.8, sixteen F32 rows 4096 -> 1024
-// 9.2 / 6.3; gradient, thirty bf16 rows of 1024 -> 16,384 28 / 13.8, sixteen 17.8 /
-// 12.0.  Past a block to a CU it loses (sixteen bf16 rows, 8192 -> 4096 8.6 / 9.6,
-// gradient of 4096 -> 16,384 18.8 / 20.0), but half the most rows do not (thirty
-// bf16 rows, 4096 -> 4096 8.1 / 7.1, gradient of 4096 -> 8192 17.6 / 14.4; sixteen
-// F32 rows, gradient of 4096 -> 4096 10.5 / 9.1).
+// 8192 -> 1024 11.4 / 7.2, 1024 -> 1024 4.4 / 3.8, sixteen F32 rows 4096 -> 1024
+// 9.2 / 6.1; gradient, thirty bf16 rows of 1024 -> 16,384 24.8 / 16.2, sixteen 18.0 /
+// 12.6.  Past a block to a CU it loses (sixteen bf16 rows, 8192 -> 4096 9.3 / 11.1,
+// gradient of 4096 -> 16,384 19.6 / 22.4), but half the most rows hardly do (thirty
+// bf16 rows, 4096 -> 4096 8.6 / 7.9, gradient of 4096 -> 8192 15.3 / 16.0; sixteen
+// F32 rows, gradient of 4096 -> 4096 10.2 / 8.9).
 template <int DT, typename F>
 void q4_row_tile(const Q4Args& p, F&& f) {
     auto fits = [&](int rows) {
@@ -795,36 +800,33 @@ void q4_row_tile(const Q4Args& p, F&& f) {
 
 // Two column tiles a wave where that leaves a block for every CU: each reads
 // (and converts) the rows half as often.  us with one / two: 8192 -> 16,384, one
-// bf16 row 15.1 / 14.8, eight 17.6 / 16.3, sixteen 22.4 / 17.9, two F32 rows
-// 26.7 / 20.4; 4096 -> 4096 (256 tiles), one 4.5 / 5.4, forty 13.1 / 9.9; the
-// gradient of 8192 -> 16,384, one 20.1 / 18.6, sixteen 34.5 / 25.8, of 4096 ->
-// 16,384 (256 tiles), sixteen 21.6 / 25.1.  Four tiles gain 1 us at F32 and
-// lose elsewhere.
+// bf16 row 20.3 / 16.7, eight 23.0 / 18.3, sixteen 23.6 / 20.2, two F32 rows
+// 27.8 / 21.6; 4096 -> 4096 (256 tiles), one 4.9 / 6.1, forty 13.9 / 10.5; the
+// gradient of 8192 -> 16,384, one 22.8 / 19.5, sixteen 35.8 / 27.9, of 4096 ->
+// 16,384 (256 tiles), sixteen 19.7 / 26.5.
 template <int ROWS>
 inline bool q4_two_tiles(const Q4Args& p) {
     return p.col_tiles * ceil_div(p.m, ROWS) >= 512;
 }
 
-// Sixteen waves a block instead of eight for one tile of long sums: hardly a CU
-// has a second block to hide the loads' latency.  us with eight / sixteen: one
-// bf16 row, 8192 -> 1024 5.8 / 5.5, 16,384 -> 4096 10.3 / 9.4, eight F32 rows,
-// 8192 -> 1024 11.0 / 10.2; shorter sums the same or slower (2048 -> 1024 3.5 /
-// 3.6); sixteen rows, gradient of 4096 -> 16,384 21.4 / 20.4, of 4096 -> 8192
-// 12.3 / 12.5.  More rows have no registers left (thirty, gradient of 1024 ->
-// 8192: 17 / 72, spilled).
+// Sixteen waves a block instead of eight for one tile of 8192 summed features or
+// more: hardly a CU has a second block to hide the loads' latency.  us with
+// eight / sixteen: one bf16 row, 8192 -> 1024 6.4 / 6.0, 16,384 -> 4096 11.6 / 10.6,
+// eight F32 rows, 8192 -> 1024 8.8 / 8.3; sixteen bf16 rows, 8192 -> 4096 9.3 both,
+// 16,384 -> 4096 15.0 / 13.9, the gradient of 4096 to 8192 12.8 / 12.4, 10,240 14.4 /
+// 13.9, 12,288 16.4 / 15.8, 14,336 18.3 / 17.7, 16,384 20.6 / 19.6; shorter sums the
+// same or slower (2048 -> 1024 3.65 / 3.74).  More rows have no registers left
+// (thirty, spilled, lost four times their time).
 template <int DT, int ROWS>
 constexpr int kQ4MoreWaves = ROWS <= (DT == SPC_F32 ? 8 : 16) ? 16 : 8;
-template <int ROWS>
-inline bool q4_long_sum(const Q4Args& p) {
-    return p.groups >= (ROWS <= 8 ? 64 : 128);
-}
+inline bool q4_long_sum(const Q4Args& p) { return p.groups >= 64; }
 
 template <int DT>
 hipError_t q4_forward(hipStream_t s, const Q4Args& p) {
     q4_row_tile<DT>(p, [&](auto rows) {
         constexpr int ROWS = decltype(rows)::value, W = kQ4MoreWaves<DT, ROWS>;
         if (q4_two_tiles<ROWS>(p)) q4_forward_launch<DT, ROWS, 2, 8>(s, p);
-        else if (q4_long_sum<ROWS>(p)) q4_forward_launch<DT, ROWS, 1, W>(s, p);
+        else if (q4_long_sum(p)) q4_forward_launch<DT, ROWS, 1, W>(s, p);
         else q4_forward_launch<DT, ROWS, 1, 8>(s, p);
     });
     return hipGetLastError();
@@ -835,7 +837,7 @@ hipError_t q4_grad(hipStream_t s, const Q4Args& p) {
     q4_row_tile<DT>(p, [&](auto rows) {
         constexpr int ROWS = decltype(rows)::value, W = kQ4MoreWaves<DT, ROWS>;
         if (q4_two_tiles<ROWS>(p)) q4_grad_launch<DT, ROWS, 2, 8>(s, p);
-        else if (q4_long_sum<ROWS>(p)) q4_grad_launch<DT, ROWS, 1, W>(s, p);
+        else if (q4_long_sum(p)) q4_grad_launch<DT, ROWS, 1, W>(s, p);
         else q4_grad_launch<DT, ROWS, 1, 8>(s, p);
     });
     return hipGetLastError();
