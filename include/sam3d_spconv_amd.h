@@ -654,7 +654,9 @@ int spc_layer_norm_backward(spc_stream_t stream, int dtype, const void* dy, int6
  * low, weight 16 + j in its high half), w = d (q - 8).
  * spc_q4_0_quantize: n F32 weights (a multiple of 32, 16-byte aligned) to
  * blocks; d = (the value of largest magnitude) / -8 rounded to f16, q =
- * floor(w / d + 8.5) held to 0..15. */
+ * floor(w r + 8.5) held to 0..15 with r = 1 / d in F32, d as rounded.  (Not
+ * promised to be the bytes of another quantiser, which may divide by d before
+ * its rounding; any Q4_0 blocks are read alike.) */
 int spc_q4_0_quantize(spc_stream_t stream, const float* w, int64_t n, uint8_t* blocks);
 
 /* The blocks of a Linear's weight [out_features, in_features] (in_features a
@@ -671,8 +673,9 @@ int spc_linear_q4_0_pack(spc_stream_t stream, const uint8_t* blocks, int64_t out
  * dtype at the end (F32 rows enter as three 8-bit parts, of which those below
  * 2^-126 are taken as zero; of bf16 and F32 rows a block's sum x (q - 8) has to
  * stay below 2^132, which values up to 2^123 do whatever the weights); a row with
- * an infinity or NaN comes out as NaNs, the others as without it.  m up to 1,048,560; made for few rows (the weights'
- * bytes are the cost up to some 64), right for any. */
+ * an infinity or NaN comes out as NaNs, the others as without it.  m up to
+ * 1,048,560; made for few rows (the weights' bytes are the cost for one to four of
+ * them, under a large weight), right for any. */
 int spc_linear_q4_0(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t m,
                     const void* packed, int64_t out_features, int64_t in_features, const void* bias,
                     int bias_dtype, void* y);
