@@ -621,16 +621,14 @@ struct Q4Bias {
         t = max(t, __builtin_amdgcn_update_dpp(0, t, 0x141, 0xf, 0xf, true));   // mirror in 8
         return max(t, __builtin_amdgcn_update_dpp(0, t, 0x140, 0xf, 0xf, true));  // in 16
     }
-    // Moves the bias if the row needs it; by how much.
-    __device__ __forceinline__ int move() {
+    // Moves the bias if the row needs it.
+    __device__ __forceinline__ void move() {
         const int t = top(), e = t >> 7;
         const int to = e > bias + 30 || (limit.x == 0 && t != 0) ? max(e - 28, 0) : bias;
-        const int by = to - bias;
         bias = to;
         if (t != 0) limit = (u16x2)(uint16_t)(((bias + 31) << 7) - 1);
         // (without a bias subnormals are f16's)
         least = (u16x2)(uint16_t)(bias ? ((bias + 1) << 7) - 1 : 0);
-        return by;
     }
     // bf16 -> f16 with the bias taken off, for elements that fit.
     __device__ __forceinline__ u32x4 f16(u32x4 v) const {
@@ -679,28 +677,33 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
         s.d = reinterpret_cast<const u32x4*>(all_scales + (int64_t)g * kQ4Group)[lane % 16];
         rows.load(s.x, g, p.sum);
     };
-    // (moved rows: acc in units of their biases)
+    // (moved rows: acc in units of the biases, raw in ones)
     floatx4 acc[MT][NT], raw[MT][NT];
     Q4Bias bias[NI];
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = raw[a][b] = floatx4{0, 0, 0, 0};
-    // multiplies the accumulators' rows by the factors f(i) of the loads' rows
-    auto scale_rows = [&](auto&& f) __attribute__((always_inline)) {
+    // adds acc's rows times the factors of the loads' rows to raw, acc starts again
+    auto flush = [&]() __attribute__((always_inline)) {
         float* fs = reinterpret_cast<float*>(mine + FACTORS);
         q4_wave_sync();
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (R::chunk() == 0) fs[R::in_tile(i)] = f(i);
+        for (int i = 0; i < NI; ++i) {
+            const float f = bias[i].factor();
+            if (R::chunk() == 0) fs[R::in_tile(i)] = f;
+        }
         q4_wave_sync();
 #pragma unroll
         for (int a = 0; a < MT; ++a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float fi = fs[(16 * a + 4 * (lane / 16) + i) % ROWS];
+                const float f = fs[(16 * a + 4 * (lane / 16) + i) % ROWS];
 #pragma unroll
-                for (int b = 0; b < NT; ++b) acc[a][b][i] *= fi;
+                for (int b = 0; b < NT; ++b) {
+                    raw[a][b][i] += acc[a][b][i] * f;
+                    acc[a][b][i] = 0.0f;
+                }
             }
     };
     const uint32_t one = q4_one();
@@ -732,10 +735,10 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) over |= bias[i].see(s.x[i]);
             if (__any(over)) {
-                float f[NI];
+                // (into raw: moved with the biases, what is there could vanish)
+                flush();
 #pragma unroll
-                for (int i = 0; i < NI; ++i) f[i] = ldexpf(1.0f, -bias[i].move());
-                scale_rows([&](int i) { return f[i]; });
+                for (int i = 0; i < NI; ++i) bias[i].move();
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) small |= bias[i].small(s.x[i]);
@@ -750,17 +753,8 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
         if (MOVED && small) products(s, std::true_type{}, raw);
         else products(s, std::bool_constant<DT == SPC_BF16 && !MOVED>{}, acc);
     });
-    if constexpr (MOVED) {
-        float f[NI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) f[i] = bias[i].factor();
-        scale_rows([&](int i) { return f[i]; });
-#pragma unroll
-        for (int a = 0; a < MT; ++a)
-#pragma unroll
-            for (int b = 0; b < NT; ++b) acc[a][b] += raw[a][b];
-    }
-    q4_finish<DT, ROWS, MT, NT, W>(p, acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
+    if constexpr (MOVED) flush();
+    q4_finish<DT, ROWS, MT, NT, W>(p, MOVED ? raw : acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 
 template <int DT, int ROWS, int NT, int W>

@@ -50,6 +50,22 @@ def test_gradient_under_large_values_on_zero_weights(spc, dev, dt, out, inp, m):
               *_gradient(x, blocks), DT[dt])
 
 
+
+@pytest.mark.parametrize("out,inp,m", [(16_500, 32, 4), (16_500, 4096, 16), (2600, 8256, 8), (2600, 8256, 40)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_gradient_before_large_values_on_zero_weights(spc, dev, dt, out, inp, m):
+    """Large values at a row's end only: what was summed before they were met
+    stays."""
+    blocks = random_blocks(out, inp, out)
+    blocks[-3:, :, 2:] = 0x88
+    bwd = spc._native.pack_q4_0(blocks.to(dev), out_features=out, in_features=inp, transpose=True)
+    for large, scale in [(1e5, 1e-5), (1e20, 1e-10), (3e38, 1e-20), (3e38, 1e-30)]:
+        x = torch.randn(m, out, generator=torch.Generator().manual_seed(2)) * scale
+        x[:, -3:] = large
+        x = x.to(DT[dt]).to(dev)
+        check(f"dx {dt} {large} after {scale}", spc._native.linear_q4_0_input_grad(x, bwd),
+              *_gradient(x, blocks), DT[dt])
+
 def _product(x, blocks):
     """(y, bound before the output's rounding), relative to sum |x w| alone: a
     block's 32 products x (q - 8) are exact, in one matrix instruction (F32 rows:
