@@ -128,3 +128,26 @@ def test_every_gradient_of_the_most_items(spc, dev, dt):
     check("dscale", ds[some], *outs[3], torch.float32)
     check("dshift", dh[some], *outs[4], torch.float32)
     assert all(bool((g.cpu()[rows == 0] == 0).all()) for g in (ds, dh))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,c", [(16, 72), (333, 192), (5000, 101), (30_000, 1024)])
+def test_sums_of_whole_gradients_are_exact(spc, dev, dt, n, c):
+    """dbias and dshift of whole numbers up to 128: sums below 2^24, whatever
+    their order, and dweight of rows whose h is +-1 (half the channels each)."""
+    nat = spc._native
+    dy = torch.randint(-128, 129, (n, c), generator=torch.Generator().manual_seed(n)).to(DT[dt])
+    sign = (2.0 * (torch.arange(c) % 2) - 1).expand(n, c)
+    x = (sign * 2.0 ** (torch.arange(n)[:, None] % 5)).to(DT[dt])
+    w, b = torch.ones(c, device=dev), torch.zeros(c, device=dev)
+    _, st = nat.layer_norm(x.to(dev), w, b, 0.0, return_stats=True)
+    _, dw, db, _, _ = nat.layer_norm_backward(dy.to(dev), x.to(dev), st, w, b)
+    assert torch.equal(db.cpu(), dy.float().sum(0))
+    if c % 2 == 0:
+        assert torch.equal(dw.cpu(), (dy.float() * sign).sum(0))
+    cuts = [0, n // 3, n // 3, n]
+    mod = torch.zeros(3, c, device=dev)
+    dh = nat.layer_norm_backward(dy.to(dev), x.to(dev), st, scale=mod, shift=mod,
+                                 offsets=torch.tensor(cuts, device=dev))[4]
+    want = torch.stack([dy[lo:hi].float().sum(0) for lo, hi in zip(cuts, cuts[1:])])
+    assert torch.equal(dh.cpu(), want)

@@ -137,3 +137,44 @@ def test_elements_past_32_bits(spc, dev):
     del y
     dx = nat.linear_q4_0_input_grad(x[:, :16], bwd)
     check("dx", dx[rows], *_gradient(x[rows, :16], wide), torch.bfloat16)
+
+
+@pytest.mark.parametrize("out,inp,m", [(130, 1024, 1), (1024, 192, 6), (1000, 1024, 16), (1024, 4096, 30),
+                                       (70, 96, 200)])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_sums_of_whole_numbers_are_exact(spc, dev, dt, out, inp, m):
+    """Rows of whole numbers up to 128 and scales +-2^-6 .. 2^-3: every sum over
+    1,024 features stays below 2^23 of its last bit, so nothing may be lost before
+    the output's rounding."""
+    nat = spc._native
+    blocks = random_blocks(out, inp, out + m)
+    g = torch.Generator().manual_seed(out)
+    d = 2.0 ** torch.randint(-6, -2, (out, inp // 32), generator=g) * (
+        2 * torch.randint(0, 2, (out, inp // 32), generator=g) - 1)
+    blocks[..., :2] = d.half()[..., None].view(torch.uint8)
+    w = dequant(blocks)
+    kw = dict(out_features=out, in_features=inp)
+    fwd, bwd = nat.pack_q4_0(blocks.to(dev), **kw), nat.pack_q4_0(blocks.to(dev), transpose=True, **kw)
+    x, dy = (torch.randint(-128, 129, (m, k), generator=g).to(DT[dt]) for k in (min(inp, 1024), out))
+    x = torch.cat([x, torch.zeros(m, inp - x.shape[1], dtype=DT[dt])], 1)
+    assert torch.equal(nat.linear_q4_0(x.to(dev), fwd).cpu(), (x.double() @ w.t()).to(DT[dt]))
+    assert torch.equal(nat.linear_q4_0_input_grad(dy.to(dev), bwd).cpu(), (dy.double() @ w).to(DT[dt]))
+    assert torch.equal(nat.linear_q4_0_bias_grad(dy.to(dev)).cpu(), dy.float().sum(0))
+
+
+def test_f32_rows_keep_24_bits(spc, dev):
+    """One value of a row against weights that are powers of two: the product is
+    that value's, all 24 bits of it."""
+    nat = spc._native
+    blocks = random_blocks(64, 128, 3)
+    blocks[..., :2] = torch.tensor([0.125]).half().view(torch.uint8)
+    q = torch.tensor([0, 4, 6, 7, 8, 9, 10, 12])          # q - 8: -8, -4, -2, -1, 0, 1, 2, 4
+    pick = q[torch.randint(0, 8, (2, 64, 4, 16), generator=torch.Generator().manual_seed(1))]
+    blocks[..., 2:] = (pick[0] | pick[1] << 4).to(torch.uint8)
+    w = dequant(blocks)
+    kw = dict(out_features=64, in_features=128)
+    fwd, bwd = nat.pack_q4_0(blocks.to(dev), **kw), nat.pack_q4_0(blocks.to(dev), transpose=True, **kw)
+    for n, run, weights in ((128, lambda t: nat.linear_q4_0(t, fwd), w.t()),
+                            (64, lambda t: nat.linear_q4_0_input_grad(t, bwd), w)):
+        v = torch.randn(n, generator=torch.Generator().manual_seed(n)) * 10.0 ** torch.linspace(-25, 25, n)
+        assert torch.equal(run(torch.diag(v).to(dev)).cpu().double(), v.double()[:, None] * weights)
