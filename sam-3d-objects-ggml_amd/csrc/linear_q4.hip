@@ -550,8 +550,8 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 //   pair of weights where one operand takes four;
 // - moved: the rows' exponents moved into f16's range by a power of two that each
 //   wave chooses for each row from what it has seen of it, eleven instructions a
-//   pair of row elements; a step with a value that does not fit (below 2^-27 of
-//   its row's largest) goes raw.
+//   pair of row elements; a row's step with a value that does not fit (below
+//   2^-27 of its largest) goes raw.
 // The first falls on a block's 16 NT columns, the second on its ROWS rows, so
 // rows are moved where they are few (us raw / moved: one row, 16,384 -> 8192
 // 28.2 / 17.8, eight, 1024 -> 8192 9.4 / 7.7, sixteen by two tiles, 16,384 ->
@@ -621,11 +621,14 @@ struct Q4Bias {
         t = max(t, __builtin_amdgcn_update_dpp(0, t, 0x141, 0xf, 0xf, true));   // mirror in 8
         return max(t, __builtin_amdgcn_update_dpp(0, t, 0x140, 0xf, 0xf, true));  // in 16
     }
-    // Moves the bias if the row needs it.
+    // Whether the row needs another bias; moves it.
+    __device__ __forceinline__ bool must_move() const {
+        const int t = top();
+        return t >> 7 > bias + 30 || (limit.x == 0 && t != 0);
+    }
     __device__ __forceinline__ void move() {
-        const int t = top(), e = t >> 7;
-        const int to = e > bias + 30 || (limit.x == 0 && t != 0) ? max(e - 28, 0) : bias;
-        bias = to;
+        const int t = top();
+        if (must_move()) bias = max((t >> 7) - 28, 0);
         if (t != 0) limit = (u16x2)(uint16_t)(((bias + 31) << 7) - 1);
         // (without a bias subnormals are f16's)
         least = (u16x2)(uint16_t)(bias ? ((bias + 1) << 7) - 1 : 0);
@@ -684,25 +687,26 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
     for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < NT; ++b) acc[a][b] = raw[a][b] = floatx4{0, 0, 0, 0};
-    // adds acc's rows times the factors of the loads' rows to raw, acc starts again
-    auto flush = [&]() __attribute__((always_inline)) {
+    // adds acc's rows, of those loads' rows that f(i) says, times their factors to
+    // raw, and starts them again
+    auto flush = [&](auto&& f) __attribute__((always_inline)) {
         float* fs = reinterpret_cast<float*>(mine + FACTORS);
         q4_wave_sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const float f = bias[i].factor();
-            if (R::chunk() == 0) fs[R::in_tile(i)] = f;
+            const float v = f(i) ? bias[i].factor() : 0.0f;  // (a factor is never 0)
+            if (R::chunk() == 0) fs[R::in_tile(i)] = v;
         }
         q4_wave_sync();
 #pragma unroll
         for (int a = 0; a < MT; ++a)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float f = fs[(16 * a + 4 * (lane / 16) + i) % ROWS];
+                const float v = fs[(16 * a + 4 * (lane / 16) + i) % ROWS];
 #pragma unroll
                 for (int b = 0; b < NT; ++b) {
-                    raw[a][b][i] += acc[a][b][i] * f;
-                    acc[a][b][i] = 0.0f;
+                    raw[a][b][i] = v != 0.0f ? raw[a][b][i] + acc[a][b][i] * v : raw[a][b][i];
+                    acc[a][b][i] = v != 0.0f ? 0.0f : acc[a][b][i];
                 }
             }
     };
@@ -729,31 +733,43 @@ __global__ __launch_bounds__(64 * W) void q4_grad16_kernel(Q4Args p) {
         }
     };
     q4_pipeline<W, Step>(p.groups, load, [&](const Step& s) __attribute__((always_inline)) {
-        bool small = false;
+        bool small[NI] = {}, any_small = false;
         if constexpr (MOVED) {
             bool over = false;
 #pragma unroll
             for (int i = 0; i < NI; ++i) over |= bias[i].see(s.x[i]);
             if (__any(over)) {
                 // (into raw: moved with the biases, what is there could vanish)
-                flush();
+                flush([&](int i) { return bias[i].must_move(); });
 #pragma unroll
                 for (int i = 0; i < NI; ++i) bias[i].move();
             }
+            // a row's 16 lanes decide for it alone, so its result is its own
+            static_assert(R::LANES == 16, "a row's lanes");
 #pragma unroll
-            for (int i = 0; i < NI; ++i) small |= bias[i].small(s.x[i]);
-            small = __any(small);
+            for (int i = 0; i < NI; ++i) {
+                const uint64_t m = __ballot(bias[i].small(s.x[i]));
+                small[i] = (m >> (lane & 48) & 0xffff) != 0;
+                any_small |= m != 0;
+            }
         }
+        const u32x4 zero = {0, 0, 0, 0};
         q4_wave_sync();
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            R::put(mine, i, MOVED && !small ? bias[i].f16(s.x[i]) : s.x[i]);
+            R::put(mine, i, !MOVED ? s.x[i] : small[i] ? zero : bias[i].f16(s.x[i]));
         if (lane < 16) scales[lane] = s.d;
         q4_wave_sync();
-        if (MOVED && small) products(s, std::true_type{}, raw);
-        else products(s, std::bool_constant<DT == SPC_BF16 && !MOVED>{}, acc);
+        products(s, std::bool_constant<DT == SPC_BF16 && !MOVED>{}, acc);
+        if (MOVED && any_small) {
+            q4_wave_sync();
+#pragma unroll
+            for (int i = 0; i < NI; ++i) R::put(mine, i, small[i] ? s.x[i] : zero);
+            q4_wave_sync();
+            products(s, std::true_type{}, raw);
+        }
     });
-    if constexpr (MOVED) flush();
+    if constexpr (MOVED) flush([](int) { return true; });
     q4_finish<DT, ROWS, MT, NT, W>(p, MOVED ? raw : acc, row0, tile0 * 16, reinterpret_cast<floatx4*>(lds));
 }
 

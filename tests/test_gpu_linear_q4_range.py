@@ -66,6 +66,21 @@ def test_gradient_before_large_values_on_zero_weights(spc, dev, dt, out, inp, m)
         check(f"dx {dt} {large} after {scale}", spc._native.linear_q4_0_input_grad(x, bwd),
               *_gradient(x, blocks), DT[dt])
 
+
+@pytest.mark.parametrize("out,inp,m", [(2600, 8256, 4), (16_500, 2048, 7), (2600, 8256, 16), (2600, 2048, 60)])
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+def test_rows_do_not_depend_on_each_other(spc, dev, dt, out, inp, m):
+    """Bit for bit, whatever range the rows beside them have."""
+    blocks = random_blocks(out, inp, out + m)
+    bwd = spc._native.pack_q4_0(blocks.to(dev), out_features=out, in_features=inp, transpose=True)
+    dy = torch.randn(m, out, generator=torch.Generator().manual_seed(m)).to(DT[dt]).to(dev)
+    want = spc._native.linear_q4_0_input_grad(dy, bwd)
+    dy[1::4, ::3] *= 2.0 ** -20 if dt == "f16" else 2.0 ** -60
+    dy[2::4, out // 2:] *= 2.0 ** 10 if dt == "f16" else 2.0 ** 40
+    dy[3, out - 1] = float("inf")
+    got = spc._native.linear_q4_0_input_grad(dy, bwd)
+    assert torch.equal(got[::4], want[::4])
+
 def _product(x, blocks):
     """(y, bound before the output's rounding), relative to sum |x w| alone: a
     block's 32 products x (q - 8) are exact, in one matrix instruction (F32 rows:
