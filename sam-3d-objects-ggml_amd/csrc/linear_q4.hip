@@ -554,8 +554,8 @@ __global__ __launch_bounds__(64 * W) void q4_grad_kernel(Q4Args p) {
 //   2^-27 of its largest) goes raw.
 // The first falls on a block's 16 NT columns, the second on its ROWS rows, so
 // rows are moved where they are few (us raw / moved: one row, 16,384 -> 8192
-// 28.2 / 17.8, eight, 1024 -> 8192 9.4 / 7.7, sixteen by two tiles, 16,384 ->
-// 8192 31.3 / 29.4, by one, 4096 -> 16,384 21.2 / 22.7, thirty, 16,384 -> 4096
+// 28.2 / 17.5, eight, 1024 -> 8192 9.4 / 7.8, sixteen by two tiles, 16,384 ->
+// 8192 31.3 / 30.2, by one, 4096 -> 16,384 21.2 / 22.7, thirty, 16,384 -> 4096
 // 22.4 / 27.0).
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
