@@ -700,6 +700,77 @@ int spc_linear_q4_0_bias_grad(spc_stream_t stream, int dtype, const void* dy, in
                               int64_t m, int64_t out_features, int bias_dtype, void* dbias,
                               void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------------------------
+ * Dropout whose mask is computed, never stored, and low-rank adapters.
+ * ------------------------------------------------------------------------ */
+
+/* y = residual + dropout(x): x [n, c] (rows x_stride elements apart), residual
+ * like it (rows residual_stride apart) or NULL, y [n, c] contiguous, all of
+ * dtype.  Element (row, col) is dropped (counts as zero, whatever it holds)
+ * with probability p, else it is x / (1 - p); F32, one rounding.  p is taken to
+ * the nearest 65536th.  The mask is a function of (seed, row, col, c) alone, so
+ * the same call on a gradient of y is x's gradient: 16 bits of Philox4x32 with
+ * seven rounds, key seed[0], counter (row ceil(c / 8) + col / 8, seed[1]), word
+ * col % 8 / 2, its low half for even columns; kept iff they are at least
+ * p 65536.  seed: two int64 in device memory, read when the kernel runs (a
+ * replayed graph takes what they hold then); NULL with p 0 only.  y may be x or
+ * residual where that is contiguous.  Pointers need only their elements'
+ * alignment. */
+int spc_dropout(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
+                int64_t c, double p, const int64_t* seed, const void* residual,
+                int64_t residual_stride, void* y);
+
+/* Low-rank adapters, by the batch item (request) that a row belongs to: item
+ * i's rows are [offsets[i], offsets[i + 1]) (device int64 [n_items + 1],
+ * ascending; NULL with n_items 1: every row), its adapter is adapters[i]
+ * (device int32 [n_items]; NULL with n_adapters 1: adapter 0), values outside
+ * [0, n_adapters) naming none.  down [n_adapters, rank, in_features], up
+ * [n_adapters, out_features, rank] (contiguous, the rows' dtype), scale f32
+ * [n_adapters] or NULL (1).  p and seed: dropout of the rows in front of the
+ * adapters, spc_dropout's (x [n, in_features]); seed NULL with p 0 only. */
+typedef struct {
+    const void* down;
+    const void* up;
+    const float* scale;
+    const int64_t* offsets;
+    const int32_t* adapters;
+    const int64_t* seed;
+    int64_t n_adapters;
+    int64_t n_items;
+    int64_t in_features;
+    int64_t out_features;
+    int64_t rank;
+    double p;
+} spc_lora_params;
+
+/* y [n, out_features] = base + scale_a (dropout(x) down_a^T) up_a^T, a the
+ * adapter of the row's item; rows without one (or behind the last item, or
+ * before the first) are base.  x [n, in_features] and base (NULL: zeros) with
+ * rows x_stride and base_stride elements apart, y contiguous (may be base where
+ * that is).  hidden: f32 [n, rank], dropout(x) down_a^T (zeros for rows without
+ * an adapter), what the gradient reads, or NULL.  Sums are F32, the hidden rows
+ * are kept in F32; one rounding to dtype.  rank 1 to 128, in_features and
+ * out_features to 2^24, n_items and n_adapters to 65535.  workspace:
+ * spc_lora_workspace_bytes, 16-byte aligned. */
+size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t in_features,
+                                int64_t out_features, int64_t rank, int backward);
+int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
+             const spc_lora_params* params, const void* base, int64_t base_stride, void* y,
+             float* hidden, void* workspace, size_t workspace_bytes);
+
+/* The gradients of spc_lora for dy [n, out_features], from x and the hidden
+ * rows that it wrote, with the same params: dx [n, in_features] = dx_base +
+ * dropout'(scale_a dy up_a down_a) (dx_base: for instance the projection's own,
+ * NULL: zeros; dx contiguous, may be dx_base where that is), ddown and dup like
+ * down and up (zeros for adapters without rows), each NULL if not wanted
+ * (hidden is read for dup only).  Rows without an adapter add to nothing.  Sums
+ * are F32 in a fixed order: equal calls give equal bits.  workspace:
+ * spc_lora_workspace_bytes with backward 1, 16-byte aligned. */
+int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
+                      const void* x, int64_t x_stride, const float* hidden, int64_t n,
+                      const spc_lora_params* params, const void* dx_base, int64_t dx_base_stride,
+                      void* dx, void* ddown, void* dup, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -133,6 +133,13 @@ def lib() -> ctypes.CDLL:
     L.spc_linear_q4_0_bias_grad_workspace_bytes.restype = _SZ
     L.spc_linear_q4_0_bias_grad_workspace_bytes.argtypes = [_I64, _I64]
     L.spc_linear_q4_0_bias_grad.argtypes = [_P, _INT, _P, _I64, _I64, _I64, _INT, _P, _P, _SZ]
+    L.spc_dropout.argtypes = [_P, _INT, _P, _I64, _I64, _I64, ctypes.c_double, _P, _P, _I64, _P]
+    L.spc_lora_workspace_bytes.restype = _SZ
+    L.spc_lora_workspace_bytes.argtypes = [_INT, _I64, _I64, _I64, _I64, _I64, _INT]
+    L.spc_lora.argtypes = [_P, _INT, _P, _I64, _I64, ctypes.POINTER(LoraParams), _P, _I64, _P, _P, _P,
+                           _SZ]
+    L.spc_lora_backward.argtypes = [_P, _INT, _P, _I64, _P, _I64, _P, _I64,
+                                    ctypes.POINTER(LoraParams), _P, _I64, _P, _P, _P, _P, _SZ]
     _lib = L
     return L
 
@@ -142,6 +149,13 @@ class LayerNormParams(ctypes.Structure):
     _fields_ = [("gamma", _P), ("beta", _P), ("scale", _P), ("shift", _P), ("offsets", _P),
                 ("n_batch", _I64), ("mod_stride", _I64), ("param_dtype", _I32),
                 ("mod_dtype", _I32), ("silu", _I32), ("eps", ctypes.c_float)]
+
+
+class LoraParams(ctypes.Structure):
+    """spc_lora_params (include/sam3d_spconv_amd.h)."""
+    _fields_ = [("down", _P), ("up", _P), ("scale", _P), ("offsets", _P), ("adapters", _P),
+                ("seed", _P), ("n_adapters", _I64), ("n_items", _I64), ("in_features", _I64),
+                ("out_features", _I64), ("rank", _I64), ("p", ctypes.c_double)]
 
 
 EPI_NONE, EPI_RESIDUAL, EPI_NORM_MOD_SILU = 0, 1, 2
@@ -1066,6 +1080,179 @@ def linear_q4_0_bias_grad(dy: torch.Tensor, dtype: torch.dtype = torch.float32) 
     if st:
         _check("spc_linear_q4_0_bias_grad", st)
     return db
+
+
+def _dropout_seed(p: float, seed):
+    """seed checked (None: no dropout)."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must lie in [0, 1], got {p}")
+    if p == 0:
+        return None
+    if seed is None or seed.dtype != torch.int64 or seed.shape != (2,):
+        raise ValueError("dropout needs a seed, int64 [2]")
+    return seed.contiguous()
+
+
+def _into(out, like, name: str, *inputs):
+    """out checked: contiguous, of `like`'s shape (n, c) and dtype, one of the
+    inputs (laid out as it is) or apart from them."""
+    shape, dtype = like
+    if out.shape != shape or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous, {list(shape)}, of {name}'s dtype")
+    for t, same in inputs:
+        if t is not None and t.numel() and out.numel() and _overlap(out, t) and not (
+                same and out.data_ptr() == t.data_ptr() and t.is_contiguous()):
+            raise ValueError("out must be an input of its own layout or lie apart from the inputs")
+    return out
+
+
+def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, *,
+            residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """residual + dropout(x) for rows x [n, c] at any stride (spc_dropout): an
+    element is dropped with probability p (to the nearest 65536th; a dropped one
+    counts as zero whatever it holds) or divided by 1 - p.  The mask is computed
+    from seed (device int64 [2], read when the kernel runs) and the element's row
+    and column, so dropout(dy, p, seed) is the gradient of x.  F32, rounded once
+    to x's dtype.  out: contiguous [n, c] (may be x or residual).  Not recorded
+    for gradients: SparseDropout is."""
+    dev = _one_device(x, seed, residual, out)
+    dt = dtype_code(x.dtype)
+    seed = _dropout_seed(p, seed)
+    x, n, c, stride = _strided_rows(x, "x")
+    rs = 0
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError("residual must have x's shape and dtype")
+        residual, _, _, rs = _strided_rows(residual, "residual")
+    if out is None:
+        out = x.new_empty((n, c))
+    else:
+        _into(out, (x.shape, x.dtype), "x", (x, True), (residual, True))
+    if not c:
+        return out
+    st = _launch(lib().spc_dropout, dev, dt, x.data_ptr(), stride, n, c, p, _ptr(seed),
+                 _ptr(residual), rs, out.data_ptr())
+    if st:
+        _check("spc_dropout", st)
+    return out
+
+
+def _lora_params(x, down, up, scale, offsets, adapters, p, seed):
+    """(spc_lora_params, tensors it points into)."""
+    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or \
+            down.shape[1] != up.shape[2]:
+        raise ValueError(f"down / up must be [k, rank, in] and [k, out, rank], got "
+                         f"{tuple(down.shape)} and {tuple(up.shape)}")
+    if down.dtype != x.dtype or up.dtype != x.dtype:
+        raise ValueError("down and up must have the rows' dtype")
+    (k, r, i), o = down.shape, up.shape[1]
+    down, up = down.contiguous(), up.contiguous()
+    if scale is not None:
+        if scale.shape != (k,) or scale.dtype != torch.float32:
+            raise ValueError(f"scale must be float32 [{k}]")
+        scale = scale.contiguous()
+    items = 1
+    if adapters is not None:
+        if adapters.dtype != torch.int32 or adapters.dim() != 1:
+            raise ValueError("adapters must be int32 [n_items]")
+        adapters, items = adapters.contiguous(), adapters.shape[0]
+    elif k != 1:
+        raise ValueError("more than one adapter needs the items' adapters")
+    elif offsets is not None:
+        items = offsets.numel() - 1
+    if offsets is not None:
+        if offsets.dtype != torch.int64 or offsets.shape != (items + 1,):
+            raise ValueError(f"offsets must be int64 [{items + 1}]")
+        offsets = offsets.contiguous()
+    elif items != 1:
+        raise ValueError("more than one item needs offsets")
+    seed = _dropout_seed(p, seed)
+    keep = (down, up, scale, offsets, adapters, seed)
+    return LoraParams(*map(_ptr, keep), k, items, i, o, r, p), keep
+
+
+def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tensor | None = None, *,
+         scale: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
+         adapters: torch.Tensor | None = None, p: float = 0.0, seed: torch.Tensor | None = None,
+         return_hidden: bool = False, out: torch.Tensor | None = None):
+    """base + scale_a (dropout(x) down_a^T) up_a^T [n, out] for rows x [n, in]
+    (spc_lora), a the adapter of the row's batch item: down [k, rank, in], up
+    [k, out, rank], scale float32 [k] (None: 1); item i's rows are offsets[i] ..
+    offsets[i+1] (device int64; None: one item of all rows), its adapter
+    adapters[i] (device int32 [n_items], outside 0 .. k - 1: none; may be left
+    out with one adapter).  Rows without an adapter are base (None: zeros).  p,
+    seed: dropout in front of the adapters, as dropout(x, p, seed).  F32
+    throughout, rounded once to x's dtype.  return_hidden: also float32 [n, rank],
+    dropout(x) down_a^T, what lora_backward reads.  out: contiguous [n, out] (may
+    be base).  Ranks up to 128.  Not recorded for gradients: the Linears'
+    adapters are."""
+    dev = _one_device(x, down, up, base, scale, offsets, adapters, seed, out)
+    dt = dtype_code(x.dtype)
+    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
+    x, n, c, stride = _strided_rows(x, "x")
+    o, r, bs = q.out_features, q.rank, 0
+    if c != q.in_features:
+        raise ValueError(f"expected x [n, {q.in_features}], got {tuple(x.shape)}")
+    if base is not None:
+        if base.shape != (n, o) or base.dtype != x.dtype:
+            raise ValueError(f"base must be [{n}, {o}], of x's dtype")
+        base, _, _, bs = _strided_rows(base, "base")
+    if out is None:
+        out = x.new_empty((n, o))
+    else:
+        _into(out, ((n, o), x.dtype), "x", (x, False), (base, True))
+    hidden = torch.empty((n, r), dtype=torch.float32, device=dev) if return_hidden else None
+    L = lib()
+    nbytes = L.spc_lora_workspace_bytes(dt, n, q.n_items, c, o, r, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    st = _launch(L.spc_lora, dev, dt, x.data_ptr(), stride, n, q, _ptr(base), bs, out.data_ptr(),
+                 _ptr(hidden), ws.data_ptr(), nbytes)
+    if st:
+        _check("spc_lora", st)
+    del keep  # alive until queued
+    return (out, hidden) if return_hidden else out
+
+
+def lora_backward(dy: torch.Tensor, x: torch.Tensor, hidden: torch.Tensor | None,
+                  down: torch.Tensor, up: torch.Tensor, dx_base: torch.Tensor | None = None, *,
+                  scale: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
+                  adapters: torch.Tensor | None = None, p: float = 0.0,
+                  seed: torch.Tensor | None = None, need=(True, True, True)):
+    """(dx, ddown, dup) of lora for the gradient dy [n, out] of its output, from
+    x and the hidden rows of that call with the same arguments
+    (spc_lora_backward); dx_base [n, in] is added to dx (the projection's own
+    gradient of the rows).  None where `need` is false (hidden is read for dup
+    only); adapters without rows get zeros.  Each has its input's dtype.
+    Deterministic."""
+    dev = _one_device(x, dy, hidden, down, up, dx_base, scale, offsets, adapters, seed)
+    dt = dtype_code(x.dtype)
+    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
+    x, n, c, xs = _strided_rows(x, "x")
+    o, r, bs = q.out_features, q.rank, 0
+    if c != q.in_features or dy.shape != (n, o) or dy.dtype != x.dtype:
+        raise ValueError(f"expected x [n, {q.in_features}] and dy [n, {o}] of one dtype, got "
+                         f"{tuple(x.shape)} and {tuple(dy.shape)}")
+    dy, _, _, dys = _strided_rows(dy, "dy")
+    if hidden is not None:
+        if hidden.shape != (n, r) or hidden.dtype != torch.float32 or not hidden.is_contiguous():
+            raise ValueError(f"hidden must be contiguous float32 [{n}, {r}]")
+    elif need[2]:
+        raise ValueError("the gradient of up needs the hidden rows")
+    if dx_base is not None:
+        if dx_base.shape != x.shape or dx_base.dtype != x.dtype:
+            raise ValueError("dx_base must have x's shape and dtype")
+        dx_base, _, _, bs = _strided_rows(dx_base, "dx_base")
+    dx = x.new_empty((n, c)) if need[0] else None
+    ddown, dup = (torch.empty_like(t) if k else None for t, k in zip(keep[:2], need[1:]))
+    L = lib()
+    nbytes = L.spc_lora_workspace_bytes(dt, n, q.n_items, c, o, r, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    st = _launch(L.spc_lora_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs, _ptr(hidden), n,
+                 q, _ptr(dx_base), bs, _ptr(dx), _ptr(ddown), _ptr(dup), ws.data_ptr(), nbytes)
+    if st:
+        _check("spc_lora_backward", st)
+    del keep  # alive until queued
+    return dx, ddown, dup
 
 
 def scatter_mean(features: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor,
