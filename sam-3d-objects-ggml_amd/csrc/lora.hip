@@ -1,144 +1,137 @@
-// lora.hip -- low-rank adapters of many batch items beside a shared projection
-// (spc_lora) and their gradients (spc_lora_backward).  With a the adapter of a
-// row's item, d = dropout (dropout.hip's mask; 1 without),
-//
-//   h = d(x) down_a^T,  y = base + s_a h up_a^T
-//   u = s_a dy up_a,    dx = dx_base + d(u down_a)
-//   ddown_a = sum over a's rows of u^T d(x),  dup_a = s_a sum of dy^T h
+// lora.hip -- entry points of the low-rank adapters and their gradients
+// (kernels: lora_kernel.h).
 #include <algorithm>
 
-#include "rows8.h"
+#include "lora_kernel.h"
 
 namespace spc {
 
 namespace {
 
-constexpr int64_t kLoraMaxRank = 128, kLoraMaxItems = 65535, kLoraMaxAdapters = 65535;
-constexpr int64_t kLoraMaxWidth = 1 << 24;
-
-// Where the items' rows and adapters are.
-struct LoraItems {
-    const int64_t* off;    // [items + 1] or null: one item of all rows
-    const int32_t* which;  // [items] or null: adapter 0
-    int64_t items, adapters, n;
-
-    // The adapter of a row, -1 for none.
-    __device__ int64_t of_row(int64_t row) const {
-        int64_t i = 0;
-        if (off) {
-            int64_t lo = 0, hi = items + 1;  // the number of offsets that are at most `row`
-            while (lo < hi) {
-                const int64_t m = (lo + hi) / 2;
-                if (off[m] <= row) lo = m + 1;
-                else hi = m;
-            }
-            i = lo - 1;
-            if (i < 0 || i >= items) return -1;
-        }
-        const int64_t a = which ? which[i] : 0;
-        return a >= 0 && a < adapters ? a : -1;
-    }
-    __device__ int64_t begin(int64_t i) const { return off ? min(max(off[i], (int64_t)0), n) : 0; }
-    __device__ int64_t end(int64_t i) const { return off ? min(max(off[i + 1], (int64_t)0), n) : n; }
+// Gradients from the slots that the row passes left: adapter a's is the sum over
+// its items and their chunks (slot = chunk + segment), in a fixed order.  A block
+// takes 64 elements, sixteen slots at a time.
+struct LoraSum {
+    const float* part;
+    void* dst;
+    int64_t elements;  // of an adapter
+    int rows_per;
 };
 
 template <int DT>
-__device__ __forceinline__ float lora_get(const void* p, int64_t i) {
-    if constexpr (DT == SPC_F32) return static_cast<const float*>(p)[i];
-    else if constexpr (DT == SPC_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-    else return f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-}
-
-template <int DT>
-__device__ __forceinline__ void lora_put(void* p, int64_t i, float v) {
-    if constexpr (DT == SPC_F32) static_cast<float*>(p)[i] = v;
-    else if constexpr (DT == SPC_BF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16_bits(v);
-    else static_cast<uint16_t*>(p)[i] = f32_to_f16_bits(v);
-}
-
-struct LoraDrop {
-    const int64_t* seed;
-    uint32_t drop;
-    float factor;
-
-    __device__ float apply(float v, int64_t row, int64_t col, int64_t c) const {
-        if (!drop) return v;
-        const u32x4 w = philox7(drop_key(seed), (uint64_t)(row * ((c + 7) / 8) + col / 8));
-        return drop_keeps(w, (int)(col % 8), drop) ? v * factor : 0.0f;
+__global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, LoraSum first, LoraSum second) {
+    __shared__ float ls[16][64];
+    const LoraSum p = blockIdx.y ? second : first;
+    if (!p.dst) return;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x & 63;
+    const int64_t blocks = (p.elements + 63) / 64;
+    for (int64_t w = blockIdx.x; w < blocks * it.adapters; w += gridDim.x) {
+        const int64_t a = w / blocks, first_e = w % blocks * 64, e0 = first_e + 4 * tx;
+        const int left = (int)min(p.elements - e0, (int64_t)4);
+        float s[4] = {0, 0, 0, 0};
+        for (int64_t i0 = 0; i0 < it.items; i0 += 64) {
+            const int64_t i = i0 + lane, v = it.off ? i + 1 : 0;
+            int64_t b = 0, e = 0;
+            if (i < it.items && it.adapter(v) == a) {
+                b = it.begin(v);
+                e = it.end(v);
+            }
+            const int mine0 = (int)(b / p.rows_per), mine1 = (int)((e - 1) / p.rows_per);
+            for (uint64_t m = __ballot(b < e); m; m &= m - 1) {
+                const int k = __builtin_ctzll(m);
+                const int64_t seg = it.off ? i0 + k + 1 : 0;
+                const int64_t j0 = __shfl(mine0, k) + seg, j1 = __shfl(mine1, k) + seg;
+#pragma unroll 4
+                for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16) {
+                    const float* q = p.part + j * p.elements + e0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) s[e] += q[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ls[ty][4 * tx + e] = s[e];
+        __syncthreads();
+        const int64_t at = first_e + threadIdx.x;
+        if (threadIdx.x < 64 && at < p.elements) {
+            float z = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) z += ls[q][threadIdx.x];
+            using S = typename LoraNum<DT>::S;
+            S* d = static_cast<S*>(p.dst) + a * p.elements + at;
+            if constexpr (DT == SPC_F32) *d = __float_as_uint(z);
+            else *d = DT == SPC_BF16 ? f32_to_bf16_bits(z) : f32_to_f16_bits(z);
+        }
+        __syncthreads();
     }
+}
+
+// How a call is split, from its sizes alone.
+struct LoraPlan {
+    int mt, mode;     // mode: kLoraFused, or kLoraShrink and kLoraExpand
+    int64_t tiles;    // tile numbers of the grid
+    int splits, k_per, col_per, col_blocks;
 };
 
-// out[row, j] = s sum over i of d(x)[row, i] w_a(i, j); one block a row.
-template <int DT>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraItems it, const void* x, int64_t stride,
-                                                          int64_t c, const void* w, int64_t w_i, int64_t w_j,
-                                                          int64_t r, const float* scale, LoraDrop d,
-                                                          float* out) {
-    for (int64_t row = blockIdx.x; row < it.n; row += gridDim.x) {
-        const int64_t a = it.of_row(row);
-        for (int64_t j = threadIdx.x / 64; j < r; j += 4) {
-            float sum = 0.0f;
-            if (a >= 0)
-                for (int64_t i = threadIdx.x % 64; i < c; i += 64)
-                    sum += d.apply(lora_get<DT>(x, row * stride + i), row, i, c) *
-                           lora_get<DT>(w, a * c * r + i * w_i + j * w_j);
-            for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-            if (a >= 0 && scale) sum *= scale[a];
-            if (threadIdx.x % 64 == 0) out[row * r + j] = sum;
-        }
+LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
+    LoraPlan q{};
+    const int step = dt == SPC_F32 ? 16 : 32;
+    q.mt = n / items >= 32 ? lora_row_tiles(r) : 1;
+    const int64_t rows = 16 * q.mt, busy = std::max(ceil_div(n, rows), std::min(items, n));
+    q.tiles = items > 1 ? n / rows + items + 3 : ceil_div(n, rows) + 3;
+    q.mode = busy >= 256 || r * c <= 32768 ? kLoraFused : kLoraShrink;
+    auto share = [&](int64_t width, int64_t unit, int64_t want) {  // columns a block
+        const int64_t blocks = std::min(std::max<int64_t>(want / busy, 1), ceil_div(width, unit));
+        return ceil_div(ceil_div(width, blocks), unit) * unit;
+    };
+    q.splits = 1;
+    q.k_per = (int)c;
+    if (q.mode == kLoraShrink) {
+        q.k_per = (int)share(c, 8 * step, 512);
+        q.splits = (int)ceil_div(c, q.k_per);
     }
+    q.col_per = (int)share(o, 4 * step, 512);
+    q.col_blocks = (int)ceil_div(o, q.col_per);
+    return q;
 }
 
-// y[row, i] = base[row, i] + d(s sum over j of h[row, j] w_a(i, j)).
-template <int DT>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraItems it, const float* h, int64_t r,
-                                                          const void* w, int64_t w_i, int64_t w_j,
-                                                          const float* scale, LoraDrop d, const void* base,
-                                                          int64_t base_stride, int64_t c, void* y) {
-    for (int64_t row = blockIdx.x; row < it.n; row += gridDim.x) {
-        const int64_t a = it.of_row(row);
-        for (int64_t i = threadIdx.x; i < c; i += 256) {
-            float sum = 0.0f;
-            if (a >= 0) {
-                for (int64_t j = 0; j < r; ++j) sum += h[row * r + j] * lora_get<DT>(w, a * c * r + i * w_i + j * w_j);
-                if (scale) sum *= scale[a];
-                sum = d.apply(sum, row, i, c);
-            }
-            if (base) {
-                const float b = lora_get<DT>(base, row * base_stride + i);
-                sum = a >= 0 ? sum + b : b;
-            }
-            lora_put<DT>(y, row * c + i, sum);
-        }
-    }
+struct LoraBackPlan {
+    int rows_o, rows_c;         // rows of a chunk
+    int64_t chunks_o, chunks_c, blocks_o, blocks_c;
+    size_t u, pu, pd;           // floats
+};
+
+LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
+    LoraBackPlan q{};
+    const int64_t cols = 4 / lora_rank_waves(r) * lora_wave_cols(dt);
+    q.blocks_o = ceil_div(o, cols);
+    q.blocks_c = ceil_div(c, cols);
+    auto rows = [&](int64_t blocks) {
+        int64_t per = std::max<int64_t>(1, ceil_div(n, std::max<int64_t>(1, 512 / blocks)));
+        if (n / items >= kLoraRows || per >= kLoraRows) per = ceil_div(per, kLoraRows) * kLoraRows;
+        return (int)per;
+    };
+    q.rows_o = rows(q.blocks_o);
+    q.rows_c = rows(q.blocks_c);
+    q.chunks_o = ceil_div(n, q.rows_o);
+    q.chunks_c = ceil_div(n, q.rows_c);
+    q.u = (size_t)(q.blocks_o * n * r);
+    q.pu = (size_t)((q.chunks_o + items + 2) * o * r);
+    q.pd = (size_t)((q.chunks_c + items + 2) * c * r);
+    return q;
 }
 
-// dw_a(i, j) = s_a sum over a's rows of d(x)[row, i] g[row, j]; a thread an
-// element.
-template <int DT>
-__global__ __launch_bounds__(256) void lora_weight_kernel(LoraItems it, const void* x, int64_t stride, int64_t c,
-                                                          const float* g, int64_t r, const float* scale,
-                                                          LoraDrop d, int64_t w_i, int64_t w_j, void* dw) {
-    const int64_t a = blockIdx.y, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= c * r) return;
-    const int64_t i = t / r, j = t % r;
-    double sum = 0.0;
-    for (int64_t k = 0; k < it.items; ++k) {
-        if ((it.which ? it.which[k] : 0) != a) continue;
-        for (int64_t row = it.begin(k); row < it.end(k); ++row)
-            sum += (double)d.apply(lora_get<DT>(x, row * stride + i), row, i, c) * g[row * r + j];
-    }
-    lora_put<DT>(dw, a * c * r + i * w_i + j * w_j, (float)(scale ? sum * scale[a] : sum));
-}
+inline size_t lora_round_up(size_t floats) { return (floats + 63) / 64 * 64; }
 
 // Checks what both entry points share.
 int lora_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t n,
-              const spc_lora_params* q, LoraItems* it, LoraDrop* d) {
-    if (!q || n < 0 || n > INT32_MAX || x_stride < 0 || q->in_features < 1 || q->out_features < 1 ||
+              const spc_lora_params* q, LoraItems* it, uint32_t* drop) {
+    if (!q || n < 0 || n > kLoraMaxRows || x_stride < 0 || q->in_features < 1 || q->out_features < 1 ||
         q->in_features > kLoraMaxWidth || q->out_features > kLoraMaxWidth || q->rank < 1 ||
         q->rank > kLoraMaxRank || q->n_adapters < 1 || q->n_adapters > kLoraMaxAdapters || q->n_items < 1 ||
         q->n_items > kLoraMaxItems) {
-        set_last_error("%s: unsupported shape (below 2^31 rows, widths 1 to 2^24, ranks 1 to 128, 1 to 65535 "
+        set_last_error("%s: unsupported shape (up to 2^27 rows, widths 1 to 2^24, ranks 1 to 128, 1 to 65535 "
                        "adapters and items) or a negative stride", fn);
         return SPC_BAD_SHAPE;
     }
@@ -156,46 +149,14 @@ int lora_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_
     }
     const int64_t e = float_size(dtype);
     auto off = [](const void* p, int64_t by) { return (uintptr_t)p % by != 0; };
-    d->drop = drop_threshold(q->p);
-    d->factor = drop_factor(d->drop);
-    d->seed = q->seed;
-    if (!q->down || !q->up || (d->drop && !q->seed) || (n > 0 && !x) || off(x, e) || off(q->down, e) ||
+    *drop = drop_threshold(q->p);
+    if (!q->down || !q->up || (*drop && !q->seed) || (n > 0 && !x) || off(x, e) || off(q->down, e) ||
         off(q->up, e) || off(q->scale, 4) || off(q->offsets, 8) || off(q->adapters, 4) || off(q->seed, 8)) {
         set_last_error("%s: null or misaligned pointer", fn);
         return SPC_BAD_ARG;
     }
     *it = LoraItems{q->offsets, q->adapters, q->n_items, q->n_adapters, n};
     return SPC_OK;
-}
-
-template <int DT>
-void lora_forward(hipStream_t s, const LoraItems& it, const LoraDrop& d, const void* x, int64_t x_stride,
-                  const spc_lora_params& q, const void* base, int64_t base_stride, void* y, float* hidden) {
-    const unsigned blocks = (unsigned)std::min<int64_t>(it.n, 1 << 16);
-    const int64_t in = q.in_features, out = q.out_features, r = q.rank;
-    lora_shrink_kernel<DT><<<blocks, 256, 0, s>>>(it, x, x_stride, in, q.down, 1, in, r, nullptr, d, hidden);
-    lora_expand_kernel<DT><<<blocks, 256, 0, s>>>(it, hidden, r, q.up, r, 1, q.scale, LoraDrop{}, base,
-                                                  base_stride, out, y);
-}
-
-template <int DT>
-void lora_backward(hipStream_t s, const LoraItems& it, const LoraDrop& d, const void* dy, int64_t dy_stride,
-                   const void* x, int64_t x_stride, const float* hidden, const spc_lora_params& q,
-                   const void* base, int64_t base_stride, void* dx, void* ddown, void* dup, float* u) {
-    const unsigned blocks = (unsigned)std::min<int64_t>(it.n, 1 << 16);
-    const int64_t in = q.in_features, out = q.out_features, r = q.rank;
-    if (blocks && (dx || ddown))
-        lora_shrink_kernel<DT><<<blocks, 256, 0, s>>>(it, dy, dy_stride, out, q.up, r, 1, r, q.scale,
-                                                      LoraDrop{}, u);
-    if (blocks && dx)
-        lora_expand_kernel<DT><<<blocks, 256, 0, s>>>(it, u, r, q.down, 1, in, nullptr, d, base, base_stride,
-                                                      in, dx);
-    if (ddown)
-        lora_weight_kernel<DT><<<dim3((unsigned)ceil_div(in * r, 256), (unsigned)q.n_adapters), 256, 0, s>>>(
-            it, x, x_stride, in, u, r, nullptr, d, 1, in, ddown);
-    if (dup)
-        lora_weight_kernel<DT><<<dim3((unsigned)ceil_div(out * r, 256), (unsigned)q.n_adapters), 256, 0, s>>>(
-            it, dy, dy_stride, out, hidden, r, q.scale, LoraDrop{}, r, 1, dup);
 }
 
 }  // namespace
@@ -208,12 +169,19 @@ extern "C" {
 
 size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t in_features,
                                 int64_t out_features, int64_t rank, int backward) {
-    (void)backward;
-    if (!float_dtype(dtype) || n < 0 || n > INT32_MAX || rank < 1 || rank > kLoraMaxRank || n_items < 1 ||
+    if (!float_dtype(dtype) || n < 0 || n > kLoraMaxRows || rank < 1 || rank > kLoraMaxRank || n_items < 1 ||
         n_items > kLoraMaxItems || in_features < 1 || in_features > kLoraMaxWidth || out_features < 1 ||
         out_features > kLoraMaxWidth)
         return 0;
-    return (size_t)std::max<int64_t>(n, 1) * rank * sizeof(float);
+    size_t floats = 0;
+    if (backward) {
+        const LoraBackPlan b = lora_back_plan(dtype, n, n_items, in_features, out_features, rank);
+        floats = lora_round_up(b.u) + lora_round_up(b.pu) + b.pd;
+    } else {
+        const LoraPlan f = lora_plan(dtype, n, n_items, in_features, out_features, rank);
+        if (f.mode == kLoraShrink) floats = (size_t)f.splits * n * rank;
+    }
+    return std::max<size_t>(floats, 4) * sizeof(float);
 }
 
 int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
@@ -221,14 +189,13 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
              void* workspace, size_t workspace_bytes) {
     const char* fn = "spc_lora";
     hipStream_t s = static_cast<hipStream_t>(stream);
-    LoraItems it;
-    LoraDrop d;
-    const int st = lora_args(fn, dtype, x, x_stride, n, params, &it, &d);
+    LoraArgs p{};
+    const int st = lora_args(fn, dtype, x, x_stride, n, params, &p.it, &p.drop);
     if (st != SPC_OK) return st;
     if (n == 0) return SPC_OK;
     const spc_lora_params& q = *params;
     const int64_t e = float_size(dtype);
-    auto off = [](const void* p, int64_t by) { return (uintptr_t)p % by != 0; };
+    auto off = [](const void* a, int64_t by) { return (uintptr_t)a % by != 0; };
     if (!y || off(y, e) || off(base, e) || off(hidden, 4) || base_stride < 0) {
         set_last_error("%s: null or misaligned pointer, or a negative stride", fn);
         return SPC_BAD_ARG;
@@ -238,11 +205,38 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
-    float* h = hidden ? hidden : static_cast<float*>(workspace);
-    if (dtype == SPC_BF16) lora_forward<SPC_BF16>(s, it, d, x, x_stride, q, base, base_stride, y, h);
-    else if (dtype == SPC_F16) lora_forward<SPC_F16>(s, it, d, x, x_stride, q, base, base_stride, y, h);
-    else lora_forward<SPC_F32>(s, it, d, x, x_stride, q, base, base_stride, y, h);
-    const hipError_t err = hipGetLastError();
+    const LoraPlan f = lora_plan(dtype, n, q.n_items, q.in_features, q.out_features, q.rank);
+    p.x = x;
+    p.xs = x_stride;
+    p.down = q.down;
+    p.up = q.up;
+    p.scale = q.scale;
+    p.base = base;
+    p.bs = base_stride;
+    p.y = y;
+    p.hidden = hidden;
+    p.part = static_cast<float*>(workspace);
+    p.c = (int)q.in_features;
+    p.o = (int)q.out_features;
+    p.r = (int)q.rank;
+    p.k_per = f.k_per;
+    p.splits = f.splits;
+    p.col_per = f.col_per;
+    p.seed = q.seed;
+    p.factor = drop_factor(p.drop);
+    auto launch = [&](int mode, int64_t blocks) {
+        const dim3 grid((unsigned)f.tiles, (unsigned)blocks);
+        return dtype == SPC_BF16  ? lora_forward_bf16(s, p, mode, f.mt, grid)
+               : dtype == SPC_F16 ? lora_forward_f16(s, p, mode, f.mt, grid)
+                                  : lora_forward_f32(s, p, mode, f.mt, grid);
+    };
+    hipError_t err = hipSuccess;
+    if (f.mode == kLoraFused) {
+        err = launch(kLoraFused, f.col_blocks);
+    } else {
+        err = launch(kLoraShrink, f.splits);
+        if (err == hipSuccess) err = launch(kLoraExpand, f.col_blocks);
+    }
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora launch");
 }
 
@@ -252,13 +246,12 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
                       void* workspace, size_t workspace_bytes) {
     const char* fn = "spc_lora_backward";
     hipStream_t s = static_cast<hipStream_t>(stream);
-    LoraItems it;
-    LoraDrop d;
-    const int st = lora_args(fn, dtype, x, x_stride, n, params, &it, &d);
+    LoraBackArgs p{};
+    const int st = lora_args(fn, dtype, x, x_stride, n, params, &p.it, &p.drop);
     if (st != SPC_OK) return st;
     const spc_lora_params& q = *params;
     const int64_t e = float_size(dtype);
-    auto off = [](const void* p, int64_t by) { return (uintptr_t)p % by != 0; };
+    auto off = [](const void* a, int64_t by) { return (uintptr_t)a % by != 0; };
     if ((n > 0 && (!dy || (dup && !hidden))) || off(dy, e) || off(hidden, 4) || off(dx_base, e) || off(dx, e) ||
         off(ddown, e) || off(dup, e) || dy_stride < 0 || dx_base_stride < 0) {
         set_last_error("%s: null or misaligned pointer, or a negative stride", fn);
@@ -270,14 +263,49 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
-    float* u = static_cast<float*>(workspace);
-    if (dtype == SPC_BF16)
-        lora_backward<SPC_BF16>(s, it, d, dy, dy_stride, x, x_stride, hidden, q, dx_base, dx_base_stride, dx, ddown, dup, u);
-    else if (dtype == SPC_F16)
-        lora_backward<SPC_F16>(s, it, d, dy, dy_stride, x, x_stride, hidden, q, dx_base, dx_base_stride, dx, ddown, dup, u);
-    else
-        lora_backward<SPC_F32>(s, it, d, dy, dy_stride, x, x_stride, hidden, q, dx_base, dx_base_stride, dx, ddown, dup, u);
-    const hipError_t err = hipGetLastError();
+    const LoraBackPlan b = lora_back_plan(dtype, n, q.n_items, q.in_features, q.out_features, q.rank);
+    float* ws = static_cast<float*>(workspace);
+    p.dy = dy;
+    p.dys = dy_stride;
+    p.x = x;
+    p.xs = x_stride;
+    p.hidden = hidden;
+    p.down = q.down;
+    p.up = q.up;
+    p.scale = q.scale;
+    p.base = dx_base;
+    p.bs = dx_base_stride;
+    p.dx = dx;
+    p.u = dx || ddown ? ws : nullptr;
+    p.u_parts = (int)b.blocks_o;
+    p.pu = dup ? ws + lora_round_up(b.u) : nullptr;
+    p.pd = ddown ? ws + lora_round_up(b.u) + lora_round_up(b.pu) : nullptr;
+    p.c = (int)q.in_features;
+    p.o = (int)q.out_features;
+    p.r = (int)q.rank;
+    p.seed = q.seed;
+    p.factor = drop_factor(p.drop);
+    hipError_t err = hipSuccess;
+    if (n > 0) {
+        const dim3 out((unsigned)b.blocks_o, (unsigned)b.chunks_o), in((unsigned)b.blocks_c, (unsigned)b.chunks_c);
+        p.rows_per = b.rows_o;
+        err = dtype == SPC_BF16  ? lora_back_out_bf16(s, p, out)
+              : dtype == SPC_F16 ? lora_back_out_f16(s, p, out)
+                                 : lora_back_out_f32(s, p, out);
+        p.rows_per = b.rows_c;
+        if (err == hipSuccess && p.u)
+            err = dtype == SPC_BF16  ? lora_back_in_bf16(s, p, in)
+                  : dtype == SPC_F16 ? lora_back_in_f16(s, p, in)
+                                     : lora_back_in_f32(s, p, in);
+    }
+    if (err == hipSuccess && (ddown || dup)) {
+        const LoraSum d = {p.pd, ddown, q.in_features * q.rank, b.rows_c}, u = {p.pu, dup, q.out_features * q.rank, b.rows_o};
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(std::max(d.elements, u.elements), 64) * q.n_adapters, 1 << 20), 2);
+        if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
+        else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
+        else lora_sum_kernel<SPC_F32><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
+        err = hipGetLastError();
+    }
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
 }
 

@@ -1,0 +1,14 @@
+// lora_bf16.hip -- the adapters' kernels for bf16 rows.
+#include "lora_kernel.h"
+
+namespace spc {
+hipError_t lora_forward_bf16(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid) {
+    return lora_forward<SPC_BF16>(s, p, mode, mt, grid);
+}
+hipError_t lora_back_out_bf16(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
+    return lora_back_out<SPC_BF16>(s, p, grid);
+}
+hipError_t lora_back_in_bf16(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
+    return lora_back_in<SPC_BF16>(s, p, grid);
+}
+}  // namespace spc

@@ -1,0 +1,914 @@
+// lora_kernel.h -- the kernels of the low-rank adapters (spc_lora) and their
+// gradients (spc_lora_backward).  With a the adapter of a row's item, s_a its
+// scale and d the dropout of the rows (rows8.h),
+//
+//   h = d(x) down_a^T,  y = base + s_a h up_a^T
+//   u = s_a dy up_a,    dx = dx_base + d(u down_a)
+//   ddown_a = sum over a's rows of u^T d(x),  dup_a = s_a sum of dy^T h
+//
+// All of it is bound by the rows' bytes (few rows: the adapters'), so every pass
+// reads its rows once and the products run on the matrix instructions, which
+// are far from their limit (rank 16: some 50 operations a byte at most).
+//
+// 16-bit rows meet 16-bit weights exactly (F32 sums).  h and u stay F32, and
+// meet 16-bit operands as two bf16 parts (their sum within 2^-17 of the value,
+// at any magnitude, where one part would be a rounding like the output's); f16
+// operands of those products are two bf16 parts as well, exactly, so that no
+// range but F32's bounds h and u.  F32 rows run on F32 matrix instructions.
+#pragma once
+
+#include "rows8.h"
+
+namespace spc {
+
+constexpr int64_t kLoraMaxRank = 128, kLoraMaxItems = 65535, kLoraMaxAdapters = 65535;
+constexpr int64_t kLoraMaxWidth = 1 << 24, kLoraMaxRows = 1 << 27;
+constexpr int kLoraThreads = 256;
+
+// Where the items' rows and adapters are.  Segment 0 is the rows before the
+// first item, segment i + 1 item i's, the last the rows behind the items.
+struct LoraItems {
+    const int64_t* off;    // [items + 1] or null: one item of all rows
+    const int32_t* which;  // [items] or null: adapter 0
+    int64_t items, adapters, n;
+
+    __device__ __forceinline__ int64_t segments() const { return off ? items + 2 : 1; }
+    __device__ __forceinline__ int64_t begin(int64_t v) const {
+        return v == 0 ? 0 : min(max(off[v - 1], (int64_t)0), n);
+    }
+    __device__ __forceinline__ int64_t end(int64_t v) const {
+        return v + 1 == segments() ? n : min(max(off[v], (int64_t)0), n);
+    }
+    // the segment's adapter, -1 for none
+    __device__ __forceinline__ int64_t adapter(int64_t v) const {
+        if (off) {
+            if (v == 0 || v > items) return -1;
+            --v;
+        }
+        const int64_t a = which ? which[v] : 0;
+        return a >= 0 && a < adapters ? a : -1;
+    }
+    // The last segment v with begin(v) / R + per v <= t (64 probes at a time, by
+    // a whole wave; inside the segments' range whatever the offsets hold).
+    template <int R>
+    __device__ __forceinline__ int64_t find(int64_t t, int64_t per) const {
+        int64_t lo = 0, size = segments();
+        while (size > 1) {
+            const int64_t step = (size + 63) / 64, at = (int64_t)(threadIdx.x & 63) * step;
+            const bool ok = at < size && begin(lo + at) / R + per * (lo + at) <= t;
+            const int64_t past = max(__popcll(__ballot(ok)), 1) - 1;
+            lo += past * step;
+            size = min(step, size - past * step);
+        }
+        return lo;
+    }
+};
+
+struct LoraArgs {
+    LoraItems it;
+    const void* x;
+    int64_t xs;
+    const void* down;
+    const void* up;
+    const float* scale;
+    const void* base;
+    int64_t bs;
+    void* y;
+    float* hidden;
+    float* part;  // [splits][n][r]
+    int c, o, r;  // in_features, out_features, rank
+    int k_per, splits, col_per;
+    const int64_t* seed;
+    uint32_t drop;
+    float factor;
+};
+
+struct LoraBackArgs {
+    LoraItems it;
+    const void* dy;
+    int64_t dys;
+    const void* x;
+    int64_t xs;
+    const float* hidden;
+    const void* down;
+    const void* up;
+    const float* scale;
+    const void* base;  // dx_base
+    int64_t bs;
+    void* dx;
+    float* u;          // [u_parts][n][r]
+    int u_parts;
+    float* pd;         // [slots][r][c], null: not wanted
+    float* pu;         // [slots][o][r]
+    int c, o, r;
+    int rows_per;
+    const int64_t* seed;
+    uint32_t drop;
+    float factor;
+};
+
+// Launches, one for each of the rows' dtypes (lora_bf16.hip, ...).  mt: row tiles
+// of 16 in a block's tile, 1 or lora_row_tiles(rank).
+enum { kLoraFused, kLoraShrink, kLoraExpand };
+#define LORA_LAUNCHERS(D)                                                                             \
+    hipError_t lora_forward_##D(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid);       \
+    hipError_t lora_back_out_##D(hipStream_t s, const LoraBackArgs& p, dim3 grid);                    \
+    hipError_t lora_back_in_##D(hipStream_t s, const LoraBackArgs& p, dim3 grid);
+LORA_LAUNCHERS(bf16)
+LORA_LAUNCHERS(f16)
+LORA_LAUNCHERS(f32)
+#undef LORA_LAUNCHERS
+
+// ranks in tiles of 16: 1, 2, 4 or 8
+inline int lora_rank_tiles(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
+inline int lora_row_tiles(int64_t r) { return r <= 32 ? 4 : 2; }
+// waves of a block along the ranks in the backward kernels (the others along columns)
+inline int lora_rank_waves(int64_t r) { return r <= 32 ? 1 : r <= 64 ? 2 : 4; }
+// columns of one such wave
+inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
+
+// ---------------------------------------------------------------------------
+// operands
+// ---------------------------------------------------------------------------
+template <int DT>
+struct LoraNum {
+    using S = typename RowElem<DT>::S;
+    static constexpr int V = 16 / (int)sizeof(S);  // elements of 16 bytes
+    static constexpr int STEP = 4 * V;             // summed elements of a matrix step
+    static constexpr int PARTS = DT == SPC_F16 ? 2 : 1;   // of a weight or row that meets F32 values
+};
+
+// V elements, those from `left` on zeros.
+template <typename S>
+__device__ __forceinline__ u32x4 lora_load(const S* q, int left) {
+    constexpr int V = 16 / (int)sizeof(S);
+    if (left >= V) return *reinterpret_cast<const u32x4_rows*>(q);
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < V - 1; ++e) {
+        if (e >= left) continue;
+        if constexpr (sizeof(S) == 4) w[e] = q[e];
+        else w[e / 2] |= (uint32_t)q[e] << (16 * (e & 1));
+    }
+    return w;
+}
+
+template <typename S>
+__device__ __forceinline__ void lora_store(S* q, u32x4 w, int left) {
+    constexpr int V = 16 / (int)sizeof(S);
+    if (left >= V) {
+        *reinterpret_cast<u32x4_rows*>(q) = w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V - 1; ++e) {
+        if (e >= left) continue;
+        if constexpr (sizeof(S) == 4) q[e] = w[e];
+        else q[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+// V elements `stride` apart, those from `left` on zeros.
+template <typename S>
+__device__ __forceinline__ u32x4 lora_gather(const S* q, int64_t stride, int left) {
+    constexpr int V = 16 / (int)sizeof(S);
+    u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const S v = e < left ? q[e * stride] : (S)0;
+        if constexpr (sizeof(S) == 4) w[e] = v;
+        else w[e / 2] |= (uint32_t)v << (16 * (e & 1));
+    }
+    return w;
+}
+
+template <int DT>
+__device__ __forceinline__ float lora_value(u32x4 w, int e) {
+    if constexpr (DT == SPC_F32) return __uint_as_float(w[e]);
+    else if constexpr (DT == SPC_BF16)
+        return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    else return f16_bits_to_f32((uint16_t)(w[e / 2] >> (16 * (e & 1))));
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4 lora_round(const float (&v)[LoraNum<DT>::V]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == SPC_F32) w[i] = __float_as_uint(v[i]);
+        else if constexpr (DT == SPC_BF16) w[i] = f32_to_bf16_bits(v[2 * i]) | (uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16;
+        else w[i] = f32_to_f16_bits(v[2 * i]) | (uint32_t)f32_to_f16_bits(v[2 * i + 1]) << 16;
+    }
+    return w;
+}
+
+// 16 x 16 products over STEP summed elements: row operand a (lane % 16 the
+// result's row), column operand b (lane % 16 its column), elements V (lane / 16)
+// on of the step; the result's rows 4 (lane / 16) .. + 3 of column lane % 16.
+template <int DT>
+__device__ __forceinline__ floatx4 lora_mma(u32x4 a, u32x4 b, floatx4 c) {
+    if constexpr (DT == SPC_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       c, 0, 0, 0);
+    } else if constexpr (DT == SPC_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
+                                                      0, 0, 0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+// Two values as bf16 parts: hi cut, lo the nearest of what is left.  (An infinity's
+// rest is NaN, as is a product that it enters.)
+__device__ __forceinline__ void lora_split(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
+    hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
+    lo = f32_to_bf16_bits(a - __uint_as_float(ia & 0xffff0000u)) |
+         (uint32_t)f32_to_bf16_bits(b - __uint_as_float(ib & 0xffff0000u)) << 16;
+}
+
+// F32 values h and u as column operand: 16-bit rows two bf16 parts.
+struct LoraSplit {
+    u32x4 hi, lo;
+};
+__device__ __forceinline__ LoraSplit lora_split8(const float (&v)[8]) {
+    LoraSplit s;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint32_t hi, lo;
+        lora_split(v[2 * q], v[2 * q + 1], hi, lo);
+        s.hi[q] = hi;
+        s.lo[q] = lo;
+    }
+    return s;
+}
+
+// A 16-bit operand's bf16 parts (f16: two, exactly).
+template <int DT>
+struct LoraParts {
+    u32x4 p[LoraNum<DT>::PARTS];
+    __device__ __forceinline__ explicit LoraParts(u32x4 w) {
+        if constexpr (DT == SPC_F16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t hi, lo;
+                lora_split(lora_value<DT>(w, 2 * q), lora_value<DT>(w, 2 * q + 1), hi, lo);
+                p[0][q] = hi;
+                p[1][q] = lo;
+            }
+        } else {
+            p[0] = w;
+        }
+    }
+    LoraParts() = default;
+};
+
+// 16-bit operand times F32 values, the small products first.
+template <int DT>
+__device__ __forceinline__ floatx4 lora_mma_split(const LoraParts<DT>& a, const LoraSplit& b, floatx4 c) {
+    if constexpr (DT == SPC_F16) {
+        c = lora_mma<SPC_BF16>(a.p[1], b.lo, c);
+        c = lora_mma<SPC_BF16>(a.p[1], b.hi, c);
+    }
+    c = lora_mma<SPC_BF16>(a.p[0], b.lo, c);
+    return lora_mma<SPC_BF16>(a.p[0], b.hi, c);
+}
+
+// Dropout of V elements of a row: bit e of `bits` set where column e is kept.
+template <int DT>
+__device__ __forceinline__ uint32_t lora_keep(DropKey key, uint32_t drop, int64_t row, int col, int c) {
+    constexpr int V = LoraNum<DT>::V;
+    const u32x4 w = philox7(key, (uint64_t)(row * ((c + 7) / 8) + col / 8));
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits |= (uint32_t)drop_keeps(w, e, drop) << e;
+    return V == 8 ? bits : bits >> (col & 4);
+}
+template <int DT>
+__device__ __forceinline__ u32x4 lora_masked(u32x4 w, uint32_t bits) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if constexpr (DT == SPC_F32) w[q] = bits >> q & 1 ? w[q] : 0;
+        else w[q] &= (bits >> (2 * q) & 1 ? 0xffffu : 0) | (bits >> (2 * q + 1) & 1 ? 0xffff0000u : 0);
+    }
+    return w;
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// The F32 operand (hidden rows; ranks are the summed index) of a row tile: steps
+// of V lane-groups of ranks.  Rank up to 16 under 16-bit rows: lanes 0..31 hold the
+// high parts of ranks 8 (lane / 16 % 2) on, lanes 32..63 the low parts, so that
+// one matrix instruction takes both.
+template <int DT, int RT>
+struct LoraRanks {
+    static constexpr bool F = DT == SPC_F32, ONE = !F && RT == 1;
+    static constexpr int V = LoraNum<DT>::V;
+    static constexpr int STEPS = F ? RT : RT == 1 ? 1 : RT / 2;
+    // first rank of lane group g in step s
+    __device__ static __forceinline__ int rank(int s, int g) { return ONE ? 8 * (g & 1) : 4 * V * s + V * g; }
+
+    // row operand: the weights' parts
+    struct W {
+        LoraParts<DT> w[STEPS];
+        // element (rank j) at q + j stride
+        __device__ __forceinline__ void load(const typename LoraNum<DT>::S* q, int64_t stride, int r, int g) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int j = rank(s, g);
+                const u32x4 v = stride == 1 ? lora_load(q + j, r - j) : lora_gather(q + j * stride, stride, r - j);
+                if constexpr (F) w[s].p[0] = v;
+                else w[s] = LoraParts<DT>(v);
+            }
+        }
+    };
+    // column operand
+    struct H {
+        u32x4 hi[STEPS], lo[F || ONE ? 1 : STEPS];
+        // q: the row's F32 values in LDS, zeros past the rank
+        __device__ __forceinline__ void load(const float* q, int g) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const float* f = q + rank(s, g);
+                if constexpr (F) {
+                    hi[s] = *reinterpret_cast<const u32x4*>(f);
+                } else {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = f[e];
+                    const LoraSplit t = lora_split8(v);
+                    if constexpr (ONE) {
+                        hi[s] = g < 2 ? t.hi : t.lo;
+                    } else {
+                        hi[s] = t.hi;
+                        lo[s] = t.lo;
+                    }
+                }
+            }
+        }
+    };
+    __device__ static __forceinline__ floatx4 mma(const W& w, const H& h, floatx4 c) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if constexpr (F) {
+                c = lora_mma<SPC_F32>(w.w[s].p[0], h.hi[s], c);
+            } else if constexpr (ONE) {
+                if constexpr (DT == SPC_F16) c = lora_mma<SPC_BF16>(w.w[s].p[1], h.hi[s], c);
+                c = lora_mma<SPC_BF16>(w.w[s].p[0], h.hi[s], c);
+            } else {
+                c = lora_mma_split<DT>(w.w[s], LoraSplit{h.hi[s], h.lo[s]}, c);
+            }
+        }
+        return c;
+    }
+};
+
+// Column of a 16-column tile's row operand index m, tile t of the group at `col`:
+// 16-bit rows take two tiles at once, interleaved so that a lane's results are
+// eight consecutive columns V (lane / 16) on, as one 16-byte store wants them.
+template <int DT>
+__device__ __forceinline__ int lora_col(int col, int t, int m) {
+    if constexpr (DT == SPC_F32) return col + m;
+    else return col + 8 * (m >> 2) + 4 * t + (m & 3);
+}
+
+struct LoraTile {
+    int64_t row0, a;
+    int m;  // rows
+};
+
+constexpr int lora_pitch(int rp) { return rp + 4; }
+
+// Sums of the block's four waves over columns [k0, k1) of rows: red[wave][row]
+// [rank] in LDS.  Rows past the tile's and ranks past r hold what a valid one
+// does (they are not read).
+template <int DT, int RT, int MT, bool DROP>
+__device__ __forceinline__ void lora_shrink(const LoraArgs& p, const LoraTile& t, int k0, int k1, float* red) {
+    using N = LoraNum<DT>;
+    using S = typename N::S;
+    constexpr int V = N::V, UN = 2;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    const S* xr[MT];
+    const S* wr[RT];
+    int64_t row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        row[i] = t.row0 + min(16 * i + n16, t.m - 1);
+        xr[i] = static_cast<const S*>(p.x) + row[i] * p.xs;
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+        wr[j] = static_cast<const S*>(p.down) + (t.a * p.r + min(16 * j + n16, p.r - 1)) * p.c;
+    floatx4 acc[MT][RT] = {};
+    const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
+    for (int k = k0 + w * UN * N::STEP; k < k1; k += 4 * UN * N::STEP) {
+        u32x4 xv[UN][MT], wv[UN][RT];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int col = k + u * N::STEP + V * g, left = min(k1, p.c) - col;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[u][i] = lora_load(xr[i] + col, left);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) wv[u][j] = lora_load(wr[j] + col, left);
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (DROP) {
+                const int col = k + u * N::STEP + V * g;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    xv[u][i] = lora_masked<DT>(xv[u][i], lora_keep<DT>(key, p.drop, row[i], col, p.c));
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[i][j] = lora_mma<DT>(wv[u][j], xv[u][i], acc[i][j]);
+        }
+    }
+    constexpr int P = lora_pitch(16 * RT);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j)
+            *reinterpret_cast<floatx4*>(red + (w * 16 * MT + 16 * i + n16) * P + 16 * j + 4 * g) = acc[i][j];
+}
+
+// y's columns [c0, c1) of the tile's rows from their hidden rows in LDS.
+template <int DT, int RT, int MT>
+__device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t, int c0, int c1, const float* hid) {
+    using N = LoraNum<DT>;
+    using S = typename N::S;
+    using K = LoraRanks<DT, RT>;
+    constexpr int V = N::V, T = V / 4, P = lora_pitch(16 * RT);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    typename K::H h[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) h[i].load(hid + (16 * i + n16) * P, g);
+    const float s = p.scale ? p.scale[t.a] : 1.0f;
+    const S* up = static_cast<const S*>(p.up) + t.a * p.o * p.r;
+    for (int cg = c0 + w * N::STEP; cg < c1; cg += 4 * N::STEP) {
+        typename K::W wt[T];
+        u32x4 b[MT];
+        const int col = cg + V * g, left = p.o - col;
+#pragma unroll
+        for (int q = 0; q < T; ++q)
+            wt[q].load(up + (int64_t)min(lora_col<DT>(cg, q, n16), p.o - 1) * p.r, 1, p.r, g);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            b[i] = u32x4{0, 0, 0, 0};
+            if (p.base && 16 * i + n16 < t.m)
+                b[i] = lora_load(static_cast<const S*>(p.base) + (t.row0 + 16 * i + n16) * p.bs + col, left);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            float v[V];
+#pragma unroll
+            for (int q = 0; q < T; ++q) {
+                floatx4 z = {0, 0, 0, 0};
+                z = K::mma(wt[q], h[i], z);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * q + e] = s * z[e];
+            }
+            if (p.base)
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] += lora_value<DT>(b[i], e);
+            if (16 * i + n16 < t.m)
+                lora_store(static_cast<S*>(p.y) + (t.row0 + 16 * i + n16) * p.o + col, lora_round<DT>(v), left);
+        }
+    }
+}
+
+// Columns [c0, c1) of rows without an adapter: the base, or zeros.
+template <int DT>
+__device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base, int64_t bs, int64_t row0, int m, int c0,
+                                          int c1) {
+    using S = typename LoraNum<DT>::S;
+    constexpr int V = LoraNum<DT>::V;
+    const int groups = (c1 - c0 + V - 1) / V;
+    for (int i = threadIdx.x; i < m * groups; i += kLoraThreads) {
+        const int64_t row = row0 + i / groups;
+        const int col = c0 + i % groups * V;
+        u32x4 w = {0, 0, 0, 0};
+        if (base) w = lora_load(static_cast<const S*>(base) + row * bs + col, c1 - col);
+        lora_store(static_cast<S*>(y) + row * ys + col, w, c1 - col);
+    }
+}
+
+// A block takes a tile of 16 MT rows of one segment (tile numbers begin at
+// begin / rows + segment, so that no segment's meet another's whatever their
+// lengths) and, by MODE, forms their hidden rows and from them `col_per` columns
+// of y (kLoraFused), writes its hidden sums over `k_per` columns of x
+// (kLoraShrink), or adds those and forms y (kLoraExpand).
+template <int DT, int RT, int MT, int MODE, bool DROP>
+__global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) {
+    constexpr int R = 16 * MT, P = lora_pitch(16 * RT);
+    __shared__ __attribute__((aligned(16))) float red[MODE == kLoraExpand ? 1 : 4 * R * P];
+    __shared__ __attribute__((aligned(16))) float hid[MODE == kLoraShrink ? 4 : R * P];
+    const LoraItems& it = p.it;
+    const int64_t v = it.template find<R>(blockIdx.x, 1);
+    const int64_t row0 = it.begin(v) + (blockIdx.x - it.begin(v) / R - v) * R, end = it.end(v);
+    if (row0 >= end || row0 < 0) return;
+    const LoraTile t = {row0, it.adapter(v), (int)min((int64_t)R, end - row0)};
+    const int c0 = MODE == kLoraShrink ? 0 : blockIdx.y * p.col_per;
+    const int c1 = min(c0 + p.col_per, p.o);
+    if (t.a < 0) {
+        if (MODE != kLoraShrink) lora_pass<DT>(p.y, p.o, p.base, p.bs, row0, t.m, c0, c1);
+        if (MODE != kLoraShrink && p.hidden && blockIdx.y == 0)
+            for (int i = threadIdx.x; i < t.m * p.r; i += kLoraThreads) p.hidden[row0 * p.r + i] = 0.0f;
+        return;
+    }
+    if constexpr (MODE != kLoraExpand) {
+        const int k0 = MODE == kLoraShrink ? blockIdx.y * p.k_per : 0;
+        const int k1 = MODE == kLoraShrink ? min(k0 + p.k_per, p.c) : p.c;
+        lora_shrink<DT, RT, MT, DROP>(p, t, k0, k1, red);
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < R * 16 * RT; i += kLoraThreads) {
+        const int m = i / (16 * RT), j = i % (16 * RT);
+        float s = 0.0f;
+        if (m < t.m && j < p.r) {
+            if constexpr (MODE == kLoraExpand) {
+                for (int q = 0; q < p.splits; ++q) s += p.part[((int64_t)q * it.n + row0 + m) * p.r + j];
+            } else {
+                const float* f = red + m * P + j;
+                s = (f[0] + f[R * P]) + (f[2 * R * P] + f[3 * R * P]);
+                if (DROP) s *= p.factor;
+            }
+            if constexpr (MODE == kLoraShrink) p.part[((int64_t)blockIdx.y * it.n + row0 + m) * p.r + j] = s;
+            else if (p.hidden && blockIdx.y == 0) p.hidden[(row0 + m) * p.r + j] = s;
+        }
+        if constexpr (MODE != kLoraShrink) hid[m * P + j] = s;
+    }
+    if constexpr (MODE != kLoraShrink) {
+        __syncthreads();
+        lora_expand<DT, RT, MT>(p, t, c0, c1, hid);
+    }
+}
+
+template <int DT, int RT, int MT>
+void lora_forward_mode(hipStream_t s, const LoraArgs& p, int mode, dim3 grid) {
+    if (mode == kLoraExpand) lora_forward_kernel<DT, RT, MT, kLoraExpand, false><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (mode == kLoraShrink && p.drop)
+        lora_forward_kernel<DT, RT, MT, kLoraShrink, true><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (mode == kLoraShrink) lora_forward_kernel<DT, RT, MT, kLoraShrink, false><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (p.drop) lora_forward_kernel<DT, RT, MT, kLoraFused, true><<<grid, kLoraThreads, 0, s>>>(p);
+    else lora_forward_kernel<DT, RT, MT, kLoraFused, false><<<grid, kLoraThreads, 0, s>>>(p);
+}
+
+template <int DT>
+hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid) {
+    const int rt = lora_rank_tiles(p.r);
+    if (rt == 1) mt == 1 ? lora_forward_mode<DT, 1, 1>(s, p, mode, grid) : lora_forward_mode<DT, 1, 4>(s, p, mode, grid);
+    else if (rt == 2) mt == 1 ? lora_forward_mode<DT, 2, 1>(s, p, mode, grid) : lora_forward_mode<DT, 2, 4>(s, p, mode, grid);
+    else if (rt == 4) mt == 1 ? lora_forward_mode<DT, 4, 1>(s, p, mode, grid) : lora_forward_mode<DT, 4, 2>(s, p, mode, grid);
+    else mt == 1 ? lora_forward_mode<DT, 8, 1>(s, p, mode, grid) : lora_forward_mode<DT, 8, 2>(s, p, mode, grid);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
+// Both kernels take chunks of rows_per rows by blocks of columns: a wave holds
+// 32 rows x 16 V columns of them at a time, lane l rows 8 (l / 16) .. + 7 of columns
+// V (l % 16) on (16 bytes a row).  That is the row operand of the weights'
+// gradients (columns by summed rows; 16-bit elements are exchanged between the
+// lane's registers to bring a column's eight rows together), whose sums stay in
+// registers until the chunk or the segment ends.  Waves stand along the columns
+// and, from rank 33 on, along ranks of 32 each.
+constexpr int kLoraRows = 32;
+
+template <int DT>
+struct LoraRaw {
+    u32x4 v[8];
+    // rows row0 + 8 g .. that are below `end`, `left` columns; the rest zeros
+    __device__ __forceinline__ void load(const void* base, int64_t stride, int64_t row0, int64_t end, int col, int c) {
+        using S = typename LoraNum<DT>::S;
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t row = row0 + 8 * g + j;
+            v[j] = u32x4{0, 0, 0, 0};
+            if (row < end && col < c) v[j] = lora_load(static_cast<const S*>(base) + row * stride + col, c - col);
+        }
+    }
+    // column e's eight rows (16-bit elements)
+    __device__ __forceinline__ u32x4 column(int e) const {
+        u32x4 w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            w[q] = __builtin_amdgcn_perm(v[2 * q + 1][e / 2], v[2 * q][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+        return w;
+    }
+};
+
+// acc[e][j] += rows of column e times F32 values b[j][row] (rank tile j).
+template <int DT, int RW>
+__device__ __forceinline__ void lora_outer(const LoraRaw<DT>& raw, const float (&b)[RW][8],
+                                           floatx4 (&acc)[LoraNum<DT>::V][RW]) {
+    if constexpr (DT == SPC_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+                    acc[e][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(raw.v[i][e]), b[j][i], acc[e][j],
+                                                                     0, 0, 0);
+    } else {
+        LoraSplit s[RW];
+#pragma unroll
+        for (int j = 0; j < RW; ++j) s[j] = lora_split8(b[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const LoraParts<DT> w(raw.column(e));
+#pragma unroll
+            for (int j = 0; j < RW; ++j) acc[e][j] = lora_mma_split<DT>(w, s[j], acc[e][j]);
+        }
+    }
+}
+
+// Writes (or leaves out) a wave's sums: element (col + V (4 g + i) + e, rank) at
+// dst[col ci + rank ri].
+template <int DT, int RW>
+__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* dst, int64_t ci, int64_t ri, int col,
+                                           int c, int rank0, int r, float f) {
+    constexpr int V = LoraNum<DT>::V;
+    const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+        const int rank = rank0 + 16 * j + n16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int k = col + V * (4 * g + i) + e;
+                if (rank < r && k < c) dst[k * ci + rank * ri] = f * acc[e][j][i];
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+#pragma unroll
+        for (int j = 0; j < RW; ++j) acc[e][j] = floatx4{0, 0, 0, 0};
+}
+
+__device__ __forceinline__ void lora_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+// The pass over dy: u of the block's columns (one of u_parts shares of the sum),
+// and the sums of dup.  RW: rank tiles of a wave, WR: waves along the ranks.
+template <int DT, int RW, int WR>
+__global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBackArgs p) {
+    using N = LoraNum<DT>;
+    using S = typename N::S;
+    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, RP = 16 * RW * WR, P = lora_pitch(RP);
+    constexpr int TP = CW + V;  // pitch of a wave's tile
+    __shared__ __attribute__((aligned(16))) S tile[4][kLoraRows * TP];
+    __shared__ __attribute__((aligned(16))) float red[WC > 1 ? 2 * WC * kLoraRows * P : 4];
+    const LoraItems& it = p.it;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
+    const int col0 = (blockIdx.x * WC + wc) * CW, mine = col0 + V * n16;
+    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
+    floatx4 acc[V][RW] = {};
+    int turn = 0;
+    for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
+        const int64_t b0 = it.begin(v);
+        if (b0 >= hi) break;
+        const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
+        if (r0 >= r1 || a < 0) continue;
+        const float s = p.scale ? p.scale[a] : 1.0f;
+        u32x4 wt[4][RW];
+        if (p.u) {
+            const S* up = static_cast<const S*>(p.up) + a * p.o * p.r;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < RW; ++j) {
+                    const int col = col0 + q * N::STEP + V * g;
+                    wt[q][j] = lora_gather(up + (int64_t)min(col, p.o - 1) * p.r + min(rank0 + 16 * j + n16, p.r - 1),
+                                           p.r, p.o - col);
+                }
+        }
+        LoraRaw<DT> raw;
+        raw.load(p.dy, p.dys, r0, r1, mine, p.o);
+        for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+            LoraRaw<DT> next;
+            next.load(p.dy, p.dys, row0 + kLoraRows, r1, mine, p.o);
+            if (p.u) {
+                S* t = tile[w];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) *reinterpret_cast<u32x4*>(t + (8 * g + j) * TP + V * n16) = raw.v[j];
+                lora_wave_sync();
+                floatx4 u[2][RW] = {};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const u32x4 d = *reinterpret_cast<const u32x4*>(t + (16 * i + n16) * TP + q * N::STEP + V * g);
+#pragma unroll
+                        for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[q][j], d, u[i][j]);
+                    }
+                lora_wave_sync();
+                if constexpr (WC > 1) {
+                    float* f = red + (turn * WC + wc) * kLoraRows * P;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < RW; ++j)
+                            *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + rank0 + 16 * j + 4 * g) = u[i][j];
+                    lds_barrier();
+                    f = red + turn * WC * kLoraRows * P;
+                    for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
+                        const int m = i / RP, j = i % RP;
+                        float z = f[m * P + j];
+#pragma unroll
+                        for (int q = 1; q < WC; ++q) z += f[q * kLoraRows * P + m * P + j];
+                        if (row0 + m < r1 && j < p.r)
+                            p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
+                    }
+                    turn ^= 1;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < RW; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int64_t row = row0 + 16 * i + n16;
+                                const int rank = rank0 + 16 * j + 4 * g + e;
+                                if (row < r1 && rank < p.r)
+                                    p.u[((int64_t)blockIdx.x * it.n + row) * p.r + rank] = s * u[i][j][e];
+                            }
+                }
+            }
+            if (p.pu) {
+                float h[RW][8];
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int64_t row = row0 + 8 * g + i;
+                        const int rank = rank0 + 16 * j + n16;
+                        h[j][i] = row < r1 && rank < p.r ? p.hidden[row * p.r + rank] : 0.0f;
+                    }
+                lora_outer<DT, RW>(raw, h, acc);
+            }
+            raw = next;
+        }
+        if (p.pu)
+            lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * (int64_t)p.o * p.r, p.r, 1, col0, p.o, rank0, p.r, s);
+    }
+}
+
+// The pass over x: dx of the block's columns and the sums of ddown.
+template <int DT, int RW, int WR, bool DROP>
+__global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackArgs p) {
+    using N = LoraNum<DT>;
+    using S = typename N::S;
+    using K = LoraRanks<DT, RW * WR>;
+    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, RP = 16 * RW * WR, P = lora_pitch(RP), T = V / 4;
+    constexpr int QN = 4 / WR;       // steps of columns whose dx the wave forms
+    constexpr int G = CW / 8;        // groups of eight columns
+    __shared__ __attribute__((aligned(16))) float ub[2][kLoraRows * P];
+    __shared__ uint8_t keep[DROP ? 4 : 1][kLoraRows * G];
+    const LoraItems& it = p.it;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
+    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
+    const int col0 = (blockIdx.x * WC + wc) * CW, mine = col0 + V * n16;
+    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
+    const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
+    floatx4 acc[V][RW] = {};
+    int turn = 0;
+    for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
+        const int64_t b0 = it.begin(v);
+        if (b0 >= hi) break;
+        const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
+        if (r0 >= r1) continue;
+        if (a < 0) {
+            const int c0 = blockIdx.x * WC * CW;
+            if (p.dx && c0 < p.c)
+                for (int64_t row = r0; row < r1; row += kLoraRows)
+                    lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, (int)min((int64_t)kLoraRows, r1 - row), c0,
+                                  min(c0 + WC * CW, p.c));
+            continue;
+        }
+        typename K::W wt[QN][T];
+        if (p.dx) {
+            const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
+#pragma unroll
+            for (int q = 0; q < QN; ++q)
+#pragma unroll
+                for (int k = 0; k < T; ++k)
+                    wt[q][k].load(down + min(lora_col<DT>(col0 + (wr * QN + q) * N::STEP, k, n16), p.c - 1), p.c, p.r, g);
+        }
+        LoraRaw<DT> raw = {};
+        if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
+        for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+            LoraRaw<DT> next;
+            if (p.pd) next.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
+            float* f = ub[turn];
+            turn ^= 1;
+            for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
+                const int m = i / RP, j = i % RP;
+                float z = 0.0f;
+                if (row0 + m < r1 && j < p.r)
+                    for (int q = 0; q < p.u_parts; ++q) z += p.u[((int64_t)q * it.n + row0 + m) * p.r + j];
+                f[m * P + j] = z;
+            }
+            if (DROP) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t bits = lora_keep<DT>(key, p.drop, row0 + 8 * g + i, mine, p.c);
+                    raw.v[i] = lora_masked<DT>(raw.v[i], bits);
+                    if constexpr (V == 8) {
+                        keep[w][(8 * g + i) * G + n16] = (uint8_t)bits;
+                    } else {
+                        const uint32_t other = __shfl_xor(bits & 15, 1);
+                        if (!(n16 & 1)) keep[w][(8 * g + i) * G + n16 / 2] = (uint8_t)((bits & 15) | other << 4);
+                    }
+                }
+            }
+            lds_barrier();
+            if (p.dx) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    typename K::H h;
+                    h.load(f + (16 * i + n16) * P, g);
+                    const int64_t row = row0 + 16 * i + n16;
+#pragma unroll
+                    for (int q = 0; q < QN; ++q) {
+                        const int at = (wr * QN + q) * N::STEP + V * g, col = col0 + at, left = p.c - col;
+                        float z[V];
+#pragma unroll
+                        for (int k = 0; k < T; ++k) {
+                            floatx4 d = {0, 0, 0, 0};
+                            d = K::mma(wt[q][k], h, d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
+                        }
+                        if (DROP) {
+                            const uint32_t bits = keep[w][(16 * i + n16) * G + at / 8] >> (V == 8 ? 0 : at & 4);
+#pragma unroll
+                            for (int e = 0; e < V; ++e) z[e] = bits >> e & 1 ? z[e] * p.factor : 0.0f;
+                        }
+                        if (row < r1 && left > 0) {
+                            if (p.base) {
+                                const u32x4 b = lora_load(static_cast<const S*>(p.base) + row * p.bs + col, left);
+#pragma unroll
+                                for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(b, e);
+                            }
+                            lora_store(static_cast<S*>(p.dx) + row * p.c + col, lora_round<DT>(z), left);
+                        }
+                    }
+                }
+            }
+            if (p.pd) {
+                float b[RW][8];
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
+                lora_outer<DT, RW>(raw, b, acc);
+                raw = next;
+            }
+        }
+        if (p.pd)
+            lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * (int64_t)p.c * p.r, 1, p.c, col0, p.c, rank0, p.r,
+                               DROP ? p.factor : 1.0f);
+    }
+}
+
+template <int DT>
+hipError_t lora_back_out(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
+    const int rt = lora_rank_tiles(p.r);
+    if (rt == 1) lora_back_out_kernel<DT, 1, 1><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_out_kernel<DT, 2, 1><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_out_kernel<DT, 2, 2><<<grid, kLoraThreads, 0, s>>>(p);
+    else lora_back_out_kernel<DT, 2, 4><<<grid, kLoraThreads, 0, s>>>(p);
+    return hipGetLastError();
+}
+
+template <int DT, bool DROP>
+void lora_back_in_rank(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
+    const int rt = lora_rank_tiles(p.r);
+    if (rt == 1) lora_back_in_kernel<DT, 1, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_in_kernel<DT, 2, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_in_kernel<DT, 2, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else lora_back_in_kernel<DT, 2, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+}
+
+template <int DT>
+hipError_t lora_back_in(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
+    if (p.drop) lora_back_in_rank<DT, true>(s, p, grid);
+    else lora_back_in_rank<DT, false>(s, p, grid);
+    return hipGetLastError();
+}
+
+}  // namespace spc
