@@ -36,13 +36,12 @@ __global__ __launch_bounds__(kDropThreads) void drop_kernel(DropArgs p) {
         R x, r;
         x.load(static_cast<const S*>(p.x) + row * p.x_stride + 8 * g, left);
         if (RES) r.load(static_cast<const S*>(p.res) + row * p.res_stride + 8 * g, left);
-        u32x4 words = {~0u, ~0u, ~0u, ~0u};
-        if (p.drop) words = philox7(key, (uint64_t)(row * p.groups + g));
+        // (a dropped value counts as zero even if it is not finite)
+        if (p.drop) x.mask(drop_ones(philox7(key, (uint64_t)(row * p.groups + g)), p.drop));
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            // (a dropped value counts as zero even if it is not finite)
-            const float k = p.drop && !drop_keeps(words, e, p.drop) ? 0.0f : x.get(e) * p.factor;
+            const float k = x.get(e) * p.factor;
             v[e] = RES ? k + r.get(e) : k;
         }
         x.set(v);

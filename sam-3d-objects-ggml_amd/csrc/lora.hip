@@ -174,7 +174,9 @@ size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t i
         out_features > kLoraMaxWidth)
         return 0;
     size_t floats = 0;
-    if (backward) {
+    if (lora_small(in_features, out_features)) {
+        floats = (size_t)n * rank;
+    } else if (backward) {
         const LoraBackPlan b = lora_back_plan(dtype, n, n_items, in_features, out_features, rank);
         floats = lora_round_up(b.u) + lora_round_up(b.pu) + b.pd;
     } else {
@@ -231,7 +233,9 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
                                   : lora_forward_f32(s, p, mode, f.mt, grid);
     };
     hipError_t err = hipSuccess;
-    if (f.mode == kLoraFused) {
+    if (lora_small(p.c, p.o)) {
+        err = lora_small_forward(s, dtype, p);
+    } else if (f.mode == kLoraFused) {
         err = launch(kLoraFused, f.col_blocks);
     } else {
         err = launch(kLoraShrink, f.splits);
@@ -286,6 +290,10 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     p.seed = q.seed;
     p.factor = drop_factor(p.drop);
     hipError_t err = hipSuccess;
+    if (lora_small(p.c, p.o)) {
+        err = lora_small_backward(s, dtype, p, ddown, dup);
+        return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
+    }
     if (n > 0) {
         const dim3 out((unsigned)b.blocks_o, (unsigned)b.chunks_o), in((unsigned)b.blocks_c, (unsigned)b.chunks_c);
         p.rows_per = b.rows_o;

@@ -119,6 +119,11 @@ LORA_LAUNCHERS(f16)
 LORA_LAUNCHERS(f32)
 #undef LORA_LAUNCHERS
 
+// Widths below eight (lora_small.hip).
+inline bool lora_small(int64_t c, int64_t o) { return c < 8 || o < 8; }
+hipError_t lora_small_forward(hipStream_t s, int dt, const LoraArgs& p);
+hipError_t lora_small_backward(hipStream_t s, int dt, const LoraBackArgs& p, void* ddown, void* dup);
+
 // ranks in tiles of 16: 1, 2, 4 or 8
 inline int lora_rank_tiles(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 inline int lora_row_tiles(int64_t r) { return r <= 32 ? 4 : 2; }
@@ -138,48 +143,66 @@ struct LoraNum {
     static constexpr int PARTS = DT == SPC_F16 ? 2 : 1;   // of a weight or row that meets F32 values
 };
 
-// V elements, those from `left` on zeros.
+// V elements of a row (c >= V of them, at any address) from `col` on, in two steps:
+// 16 bytes that lie inside the row, without a branch, and, only in blocks that hold
+// a row's end, what moves them into place and clears what is past it.  (With a
+// branch at each load the backward kernels spilled the masks of all of them.)
 template <typename S>
-__device__ __forceinline__ u32x4 lora_load(const S* q, int left) {
+__device__ __forceinline__ u32x4 lora_shift(u32x4 w, int by) {
     constexpr int V = 16 / (int)sizeof(S);
-    if (left >= V) return *reinterpret_cast<const u32x4_rows*>(q);
-    u32x4 w = {0, 0, 0, 0};
+    if constexpr (V == 8)
+        w = by & 1 ? u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16} : w;
+    w = by & (V / 4) ? u32x4{w[1], w[2], w[3], 0} : w;
+    w = by & (V / 2) ? u32x4{w[2], w[3], 0, 0} : w;
+    return by >= V ? u32x4{0, 0, 0, 0} : w;
+}
+template <typename S>
+__device__ __forceinline__ u32x4 lora_fetch(const S* row, int col, int c) {
+    return *reinterpret_cast<const u32x4_rows*>(row + min(col, c - 16 / (int)sizeof(S)));
+}
+template <typename S>
+__device__ __forceinline__ u32x4 lora_edge(u32x4 w, int col, int c) {
+    return lora_shift<S>(w, max(col - (c - 16 / (int)sizeof(S)), 0));
+}
+template <typename S>
+__device__ __forceinline__ u32x4 lora_load(const S* row, int col, int c) {
+    return lora_edge<S>(lora_fetch(row, col, c), col, c);
+}
+// The same of a short row, r elements at `at` of an array of `all` >= V: the 16
+// bytes lie inside the array, and what is not the row's is cleared.
+template <typename S>
+__device__ __forceinline__ u32x4 lora_fetch_short(const S* array, int64_t at, int64_t all) {
+    return *reinterpret_cast<const u32x4_rows*>(array + min(at, all - 16 / (int)sizeof(S)));
+}
+template <typename S>
+__device__ __forceinline__ u32x4 lora_edge_short(u32x4 w, int64_t at, int64_t all, int left) {
+    constexpr int V = 16 / (int)sizeof(S);
+    w = lora_shift<S>(w, (int)max(at - (all - V), (int64_t)0));
 #pragma unroll
-    for (int e = 0; e < V - 1; ++e) {
-        if (e >= left) continue;
-        if constexpr (sizeof(S) == 4) w[e] = q[e];
-        else w[e / 2] |= (uint32_t)q[e] << (16 * (e & 1));
+    for (int q = 0; q < 4; ++q) {
+        if constexpr (V == 4) w[q] = q < left ? w[q] : 0;
+        else w[q] = 2 * q + 1 < left ? w[q] : 2 * q < left ? w[q] & 0xffff : 0;
     }
     return w;
 }
 
+// Stores V elements at q, `left` of which are the row's.
 template <typename S>
 __device__ __forceinline__ void lora_store(S* q, u32x4 w, int left) {
     constexpr int V = 16 / (int)sizeof(S);
     if (left >= V) {
         *reinterpret_cast<u32x4_rows*>(q) = w;
-        return;
+    } else {
+        for (int e = 0; e < left; ++e) {
+            if constexpr (V == 4) {
+                q[e] = w[0];
+                w = u32x4{w[1], w[2], w[3], 0};
+            } else {
+                q[e] = (uint16_t)w[0];
+                w = u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+            }
+        }
     }
-#pragma unroll
-    for (int e = 0; e < V - 1; ++e) {
-        if (e >= left) continue;
-        if constexpr (sizeof(S) == 4) q[e] = w[e];
-        else q[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-    }
-}
-
-// V elements `stride` apart, those from `left` on zeros.
-template <typename S>
-__device__ __forceinline__ u32x4 lora_gather(const S* q, int64_t stride, int left) {
-    constexpr int V = 16 / (int)sizeof(S);
-    u32x4 w = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const S v = e < left ? q[e * stride] : (S)0;
-        if constexpr (sizeof(S) == 4) w[e] = v;
-        else w[e / 2] |= (uint32_t)v << (16 * (e & 1));
-    }
-    return w;
 }
 
 template <int DT>
@@ -196,8 +219,7 @@ __device__ __forceinline__ u32x4 lora_round(const float (&v)[LoraNum<DT>::V]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (DT == SPC_F32) w[i] = __float_as_uint(v[i]);
-        else if constexpr (DT == SPC_BF16) w[i] = f32_to_bf16_bits(v[2 * i]) | (uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16;
-        else w[i] = f32_to_f16_bits(v[2 * i]) | (uint32_t)f32_to_f16_bits(v[2 * i + 1]) << 16;
+        else w[i] = round_pair<DT>(v[2 * i], v[2 * i + 1]);
     }
     return w;
 }
@@ -226,8 +248,7 @@ __device__ __forceinline__ floatx4 lora_mma(u32x4 a, u32x4 b, floatx4 c) {
 __device__ __forceinline__ void lora_split(float a, float b, uint32_t& hi, uint32_t& lo) {
     const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
     hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
-    lo = f32_to_bf16_bits(a - __uint_as_float(ia & 0xffff0000u)) |
-         (uint32_t)f32_to_bf16_bits(b - __uint_as_float(ib & 0xffff0000u)) << 16;
+    lo = round_pair<SPC_BF16>(a - __uint_as_float(ia & 0xffff0000u), b - __uint_as_float(ib & 0xffff0000u));
 }
 
 // F32 values h and u as column operand: 16-bit rows two bf16 parts.
@@ -277,22 +298,20 @@ __device__ __forceinline__ floatx4 lora_mma_split(const LoraParts<DT>& a, const 
     return lora_mma<SPC_BF16>(a.p[0], b.hi, c);
 }
 
-// Dropout of V elements of a row: bit e of `bits` set where column e is kept.
-template <int DT>
-__device__ __forceinline__ uint32_t lora_keep(DropKey key, uint32_t drop, int64_t row, int col, int c) {
-    constexpr int V = LoraNum<DT>::V;
-    const u32x4 w = philox7(key, (uint64_t)(row * ((c + 7) / 8) + col / 8));
-    uint32_t bits = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bits |= (uint32_t)drop_keeps(w, e, drop) << e;
-    return V == 8 ? bits : bits >> (col & 4);
+// Dropout of V elements of a row from column `col` on: the group's mask (words of
+// halves), and the elements with zeros where dropped.
+__device__ __forceinline__ u32x4 lora_ones(DropKey key, uint32_t drop, int64_t row, int col, int c) {
+    return drop_ones(philox7(key, (uint64_t)(row * ((c + 7) / 8) + col / 8)), drop);
 }
 template <int DT>
-__device__ __forceinline__ u32x4 lora_masked(u32x4 w, uint32_t bits) {
+__device__ __forceinline__ u32x4 lora_masked(u32x4 w, u32x4 ones, int col) {
+    if constexpr (DT == SPC_F32) {
+        const bool second = col & 4;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        if constexpr (DT == SPC_F32) w[q] = bits >> q & 1 ? w[q] : 0;
-        else w[q] &= (bits >> (2 * q) & 1 ? 0xffffu : 0) | (bits >> (2 * q + 1) & 1 ? 0xffff0000u : 0);
+        for (int e = 0; e < 4; ++e) w[e] = drop_word(w[e], second ? ones[2 + e / 2] : ones[e / 2], 16 * (e & 1));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = drop_pair(w[q], ones[q]);
     }
     return w;
 }
@@ -315,15 +334,15 @@ struct LoraRanks {
     // row operand: the weights' parts
     struct W {
         LoraParts<DT> w[STEPS];
-        // element (rank j) at q + j stride
-        __device__ __forceinline__ void load(const typename LoraNum<DT>::S* q, int64_t stride, int r, int g) {
+        // from 16 bytes of a column's ranks a step
+        __device__ __forceinline__ void set(const u32x4 (&raw)[STEPS]) {
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const int j = rank(s, g);
-                const u32x4 v = stride == 1 ? lora_load(q + j, r - j) : lora_gather(q + j * stride, stride, r - j);
-                if constexpr (F) w[s].p[0] = v;
-                else w[s] = LoraParts<DT>(v);
-            }
+            for (int s = 0; s < STEPS; ++s) w[s] = LoraParts<DT>(raw[s]);
+        }
+        // q: the same in LDS, zeros past the rank
+        __device__ __forceinline__ void load_lds(const typename LoraNum<DT>::S* q, int g) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) w[s] = LoraParts<DT>(*reinterpret_cast<const u32x4*>(q + rank(s, g)));
         }
     };
     // column operand
@@ -409,11 +428,21 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& p, const LoraTile& t
         u32x4 xv[UN][MT], wv[UN][RT];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int col = k + u * N::STEP + V * g, left = min(k1, p.c) - col;
+            const int col = k + u * N::STEP + V * g;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xv[u][i] = lora_load(xr[i] + col, left);
+            for (int i = 0; i < MT; ++i) xv[u][i] = lora_fetch(xr[i], col, k1);
 #pragma unroll
-            for (int j = 0; j < RT; ++j) wv[u][j] = lora_load(wr[j] + col, left);
+            for (int j = 0; j < RT; ++j) wv[u][j] = lora_fetch(wr[j], col, k1);
+        }
+        if (k + UN * N::STEP > k1) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int col = k + u * N::STEP + V * g;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) xv[u][i] = lora_edge<S>(xv[u][i], col, k1);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) wv[u][j] = lora_edge<S>(wv[u][j], col, k1);
+            }
         }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
@@ -421,7 +450,7 @@ __device__ __forceinline__ void lora_shrink(const LoraArgs& p, const LoraTile& t
                 const int col = k + u * N::STEP + V * g;
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
-                    xv[u][i] = lora_masked<DT>(xv[u][i], lora_keep<DT>(key, p.drop, row[i], col, p.c));
+                    xv[u][i] = lora_masked<DT>(xv[u][i], lora_ones(key, p.drop, row[i], col, p.c), col);
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -449,20 +478,33 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
 #pragma unroll
     for (int i = 0; i < MT; ++i) h[i].load(hid + (16 * i + n16) * P, g);
     const float s = p.scale ? p.scale[t.a] : 1.0f;
-    const S* up = static_cast<const S*>(p.up) + t.a * p.o * p.r;
+    const S* up = static_cast<const S*>(p.up);
+    const int64_t all = p.it.adapters * p.o * p.r;
     for (int cg = c0 + w * N::STEP; cg < c1; cg += 4 * N::STEP) {
-        typename K::W wt[T];
-        u32x4 b[MT];
+        u32x4 wr[T][K::STEPS], b[MT];
         const int col = cg + V * g, left = p.o - col;
+        const bool edge = cg + N::STEP > p.o;
 #pragma unroll
-        for (int q = 0; q < T; ++q)
-            wt[q].load(up + (int64_t)min(lora_col<DT>(cg, q, n16), p.o - 1) * p.r, 1, p.r, g);
+        for (int q = 0; q < T; ++q) {
+            const int64_t at = (t.a * p.o + min(lora_col<DT>(cg, q, n16), p.o - 1)) * p.r;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            b[i] = u32x4{0, 0, 0, 0};
-            if (p.base && 16 * i + n16 < t.m)
-                b[i] = lora_load(static_cast<const S*>(p.base) + (t.row0 + 16 * i + n16) * p.bs + col, left);
+            for (int k = 0; k < K::STEPS; ++k) wr[q][k] = lora_fetch_short(up, at + K::rank(k, g), all);
         }
+        if (p.base)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                b[i] = lora_fetch(static_cast<const S*>(p.base) + (t.row0 + min(16 * i + n16, t.m - 1)) * p.bs, col, p.o);
+        if (p.r < 16 * RT)
+#pragma unroll
+            for (int q = 0; q < T; ++q) {
+                const int64_t at = (t.a * p.o + min(lora_col<DT>(cg, q, n16), p.o - 1)) * p.r;
+#pragma unroll
+                for (int k = 0; k < K::STEPS; ++k)
+                    wr[q][k] = lora_edge_short<S>(wr[q][k], at + K::rank(k, g), all, p.r - K::rank(k, g));
+            }
+        typename K::W wt[T];
+#pragma unroll
+        for (int q = 0; q < T; ++q) wt[q].set(wr[q]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             float v[V];
@@ -473,11 +515,16 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[4 * q + e] = s * z[e];
             }
-            if (p.base)
+            if (p.base) {
+                if (edge) b[i] = lora_edge<S>(b[i], col, p.o);
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[e] += lora_value<DT>(b[i], e);
-            if (16 * i + n16 < t.m)
-                lora_store(static_cast<S*>(p.y) + (t.row0 + 16 * i + n16) * p.o + col, lora_round<DT>(v), left);
+            }
+            if (16 * i + n16 < t.m) {
+                S* q = static_cast<S*>(p.y) + (t.row0 + 16 * i + n16) * p.o + col;
+                if (!edge) *reinterpret_cast<u32x4_rows*>(q) = lora_round<DT>(v);
+                else lora_store(q, lora_round<DT>(v), left);
+            }
         }
     }
 }
@@ -493,7 +540,7 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
         const int64_t row = row0 + i / groups;
         const int col = c0 + i % groups * V;
         u32x4 w = {0, 0, 0, 0};
-        if (base) w = lora_load(static_cast<const S*>(base) + row * bs + col, c1 - col);
+        if (base) w = lora_load(static_cast<const S*>(base) + row * bs, col, c1);
         lora_store(static_cast<S*>(y) + row * ys + col, w, c1 - col);
     }
 }
@@ -584,16 +631,36 @@ constexpr int kLoraRows = 32;
 template <int DT>
 struct LoraRaw {
     u32x4 v[8];
-    // rows row0 + 8 g .. that are below `end`, `left` columns; the rest zeros
+    // Rows row0 + 8 g on, from `col` on (lora_fetch; rows past `end` are its last).
     __device__ __forceinline__ void load(const void* base, int64_t stride, int64_t row0, int64_t end, int col, int c) {
         using S = typename LoraNum<DT>::S;
-        const int g = (threadIdx.x & 63) >> 4;
+        if (row0 >= end) return;
+        const int g8 = (threadIdx.x & 63) / 16 * 8;
+        if (row0 + kLoraRows <= end) {
+            const S* q = static_cast<const S*>(base) + (row0 + g8) * stride;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t row = row0 + 8 * g + j;
-            v[j] = u32x4{0, 0, 0, 0};
-            if (row < end && col < c) v[j] = lora_load(static_cast<const S*>(base) + row * stride + col, c - col);
+            for (int j = 0; j < 8; ++j) {
+                v[j] = lora_fetch(q, col, c);
+                q += stride;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = lora_fetch(static_cast<const S*>(base) + min(row0 + g8 + j, end - 1) * stride, col, c);
         }
+    }
+    // Zeros for what is past the end of the rows, and, at the row's end, of the columns.
+    __device__ __forceinline__ void trim(int64_t row0, int64_t end, bool edge, int col, int c) {
+        using S = typename LoraNum<DT>::S;
+        if (row0 + kLoraRows > end) {
+            const int rows = (int)(end - row0) - (threadIdx.x & 63) / 16 * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j >= rows) v[j] = u32x4{0, 0, 0, 0};
+        }
+        if (edge)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = lora_edge<S>(v[j], col, c);
     }
     // column e's eight rows (16-bit elements)
     __device__ __forceinline__ u32x4 column(int e) const {
@@ -631,23 +698,30 @@ __device__ __forceinline__ void lora_outer(const LoraRaw<DT>& raw, const float (
     }
 }
 
-// Writes (or leaves out) a wave's sums: element (col + V (4 g + i) + e, rank) at
-// dst[col ci + rank ri].
-template <int DT, int RW>
-__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* dst, int64_t ci, int64_t ri, int col,
-                                           int c, int rank0, int r, float f) {
+// Writes a wave's sums times f and clears them: column col + V (4 g + i) + e, rank
+// rank0 + 16 j + lane % 16.  ALONG: dst [r][c], so that a lane's V columns are a run;
+// else [c][r].  (The addresses are made here: hoisted out of the segments' loop
+// they would fill the registers.)
+template <int DT, int RW, bool ALONG>
+__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* dst, int col, int c, int rank0, int r,
+                                           float f) {
     constexpr int V = LoraNum<DT>::V;
-    const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int n16 = lane & 15, k0 = col + 4 * V * (lane >> 4), left = c - k0;
+    float* q = dst + (ALONG ? (int64_t)(rank0 + n16) * c + k0 : (int64_t)k0 * r + rank0 + n16);
 #pragma unroll
     for (int j = 0; j < RW; ++j) {
-        const int rank = rank0 + 16 * j + n16;
+        const bool on = rank0 + 16 * j + n16 < r;
+        float* t = q + (ALONG ? (int64_t)16 * j * c : 16 * j);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int k = col + V * (4 * g + i) + e;
-                if (rank < r && k < c) dst[k * ci + rank * ri] = f * acc[e][j][i];
+                if (on && V * i + e < left) *t = f * acc[e][j][i];
+                t += ALONG ? 1 : r;
             }
+        }
     }
 #pragma unroll
     for (int e = 0; e < V; ++e)
@@ -663,44 +737,65 @@ __device__ __forceinline__ void lora_wave_sync() {
 
 // The pass over dy: u of the block's columns (one of u_parts shares of the sum),
 // and the sums of dup.  RW: rank tiles of a wave, WR: waves along the ranks.
+// u sums along a row, so its operand is read back from the wave's tile in LDS,
+// and the waves' shares meet there too, in the tiles' place; the adapter's columns
+// lie in LDS by rank.
 template <int DT, int RW, int WR>
 __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBackArgs p) {
     using N = LoraNum<DT>;
     using S = typename N::S;
-    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, RP = 16 * RW * WR, P = lora_pitch(RP);
-    constexpr int TP = CW + V;  // pitch of a wave's tile
+    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RW * WR, P = lora_pitch(16 * RW);
+    constexpr int TP = CW + V, WP = CB + V;  // pitches of a wave's tile and of the weights
     __shared__ __attribute__((aligned(16))) S tile[4][kLoraRows * TP];
-    __shared__ __attribute__((aligned(16))) float red[WC > 1 ? 2 * WC * kLoraRows * P : 4];
+    __shared__ __attribute__((aligned(16))) S wl[RP * WP];
+    static_assert(kLoraRows * P * sizeof(float) <= sizeof(tile[0]), "a wave's share of u in its tile's place");
     const LoraItems& it = p.it;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
     const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
-    const int col0 = (blockIdx.x * WC + wc) * CW, mine = col0 + V * n16;
+    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW, mine = col0 + V * n16;
+    const bool edge = block0 + CB > p.o;
     const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     floatx4 acc[V][RW] = {};
-    int turn = 0;
     for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
         const int64_t b0 = it.begin(v);
         if (b0 >= hi) break;
         const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
         if (r0 >= r1 || a < 0) continue;
         const float s = p.scale ? p.scale[a] : 1.0f;
-        u32x4 wt[4][RW];
-        if (p.u) {
-            const S* up = static_cast<const S*>(p.up) + a * p.o * p.r;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int j = 0; j < RW; ++j) {
-                    const int col = col0 + q * N::STEP + V * g;
-                    wt[q][j] = lora_gather(up + (int64_t)min(col, p.o - 1) * p.r + min(rank0 + 16 * j + n16, p.r - 1),
-                                           p.r, p.o - col);
-                }
-        }
         LoraRaw<DT> raw;
         raw.load(p.dy, p.dys, r0, r1, mine, p.o);
+        if (p.u) {
+            const S* up = static_cast<const S*>(p.up);
+            const int64_t all = it.adapters * p.o * p.r;
+            lds_barrier();
+            for (int i = threadIdx.x; i < CB * (RP / V); i += kLoraThreads) {
+                const int k = i % CB, j = i / CB * V, col = block0 + k;
+                const int64_t at = (a * p.o + min(col, p.o - 1)) * p.r + j;
+                const u32x4 q = lora_edge_short<S>(lora_fetch_short(up, at, all), at, all, col < p.o ? p.r - j : 0);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    if constexpr (V == 4) wl[(j + e) * WP + k] = q[e];
+                    else wl[(j + e) * WP + k] = (S)(q[e / 2] >> (16 * (e & 1)));
+                }
+            }
+            lds_barrier();
+        }
         for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
-            LoraRaw<DT> next;
+            LoraRaw<DT> next = raw;
             next.load(p.dy, p.dys, row0 + kLoraRows, r1, mine, p.o);
+            float h[RW][8];
+            if (p.pu) {
+                const bool full = row0 + kLoraRows <= r1;
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int64_t row = row0 + 8 * g + i;
+                        h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
+                        if (!full && row >= r1) h[j][i] = 0.0f;
+                    }
+            }
+            raw.trim(row0, r1, edge, mine, p.o);
             if (p.u) {
                 S* t = tile[w];
 #pragma unroll
@@ -708,81 +803,68 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                 lora_wave_sync();
                 floatx4 u[2][RW] = {};
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q) {
+                    u32x4 wt[RW];
+#pragma unroll
+                    for (int j = 0; j < RW; ++j)
+                        wt[j] = *reinterpret_cast<const u32x4*>(wl + (rank0 + 16 * j + n16) * WP + wc * CW + q * N::STEP +
+                                                                V * g);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const u32x4 d = *reinterpret_cast<const u32x4*>(t + (16 * i + n16) * TP + q * N::STEP + V * g);
 #pragma unroll
-                        for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[q][j], d, u[i][j]);
+                        for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[j], d, u[i][j]);
                     }
+                }
                 lora_wave_sync();
-                if constexpr (WC > 1) {
-                    float* f = red + (turn * WC + wc) * kLoraRows * P;
+                float* f = reinterpret_cast<float*>(t);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                        for (int j = 0; j < RW; ++j)
-                            *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + rank0 + 16 * j + 4 * g) = u[i][j];
-                    lds_barrier();
-                    f = red + turn * WC * kLoraRows * P;
-                    for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
-                        const int m = i / RP, j = i % RP;
-                        float z = f[m * P + j];
+                    for (int j = 0; j < RW; ++j)
+                        *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + 16 * j + 4 * g) = u[i][j];
+                lds_barrier();
+                // (the waves of a rank group stand WC apart)
+                for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
+                    const int m = i / RP, j = i % RP;
+                    float z = 0.0f;
 #pragma unroll
-                        for (int q = 1; q < WC; ++q) z += f[q * kLoraRows * P + m * P + j];
-                        if (row0 + m < r1 && j < p.r)
-                            p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
-                    }
-                    turn ^= 1;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < RW; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int64_t row = row0 + 16 * i + n16;
-                                const int rank = rank0 + 16 * j + 4 * g + e;
-                                if (row < r1 && rank < p.r)
-                                    p.u[((int64_t)blockIdx.x * it.n + row) * p.r + rank] = s * u[i][j][e];
-                            }
+                    for (int q = 0; q < WC; ++q)
+                        z += reinterpret_cast<const float*>(tile[j / (16 * RW) * WC + q])[m * P + j % (16 * RW)];
+                    if (row0 + m < r1 && j < p.r) p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
                 }
             }
-            if (p.pu) {
-                float h[RW][8];
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int64_t row = row0 + 8 * g + i;
-                        const int rank = rank0 + 16 * j + n16;
-                        h[j][i] = row < r1 && rank < p.r ? p.hidden[row * p.r + rank] : 0.0f;
-                    }
-                lora_outer<DT, RW>(raw, h, acc);
-            }
+            if (p.pu) lora_outer<DT, RW>(raw, h, acc);
             raw = next;
+            if (p.u) lds_barrier();
         }
         if (p.pu)
-            lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * (int64_t)p.o * p.r, p.r, 1, col0, p.o, rank0, p.r, s);
+            lora_flush<DT, RW, false>(acc, p.pu + (blockIdx.y + v) * (int64_t)p.o * p.r, col0, p.o, rank0, p.r, s);
     }
 }
 
-// The pass over x: dx of the block's columns and the sums of ddown.
+// The pass over x: dx of the block's columns and the sums of ddown.  The
+// adapter's columns lie in LDS by column.
 template <int DT, int RW, int WR, bool DROP>
 __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackArgs p) {
     using N = LoraNum<DT>;
     using S = typename N::S;
-    using K = LoraRanks<DT, RW * WR>;
-    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, RP = 16 * RW * WR, P = lora_pitch(RP), T = V / 4;
+    constexpr int RT = RW * WR;
+    using K = LoraRanks<DT, RT>;
+    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RT, P = lora_pitch(RP), T = V / 4;
+    constexpr int WP = RP + V;       // pitch of the weights
     constexpr int QN = 4 / WR;       // steps of columns whose dx the wave forms
     constexpr int G = CW / 8;        // groups of eight columns
+    constexpr int NU = kLoraRows * RP / kLoraThreads;  // values of u a thread
     __shared__ __attribute__((aligned(16))) float ub[2][kLoraRows * P];
+    __shared__ __attribute__((aligned(16))) S wl[CB * WP];
     __shared__ uint8_t keep[DROP ? 4 : 1][kLoraRows * G];
     const LoraItems& it = p.it;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
     const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
-    const int col0 = (blockIdx.x * WC + wc) * CW, mine = col0 + V * n16;
+    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW, mine = col0 + V * n16;
     const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
+    const bool edge = block0 + CB > p.c;
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
     floatx4 acc[V][RW] = {};
     int turn = 0;
@@ -792,83 +874,78 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
         const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
         if (r0 >= r1) continue;
         if (a < 0) {
-            const int c0 = blockIdx.x * WC * CW;
-            if (p.dx && c0 < p.c)
+            if (p.dx && block0 < p.c)
                 for (int64_t row = r0; row < r1; row += kLoraRows)
-                    lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, (int)min((int64_t)kLoraRows, r1 - row), c0,
-                                  min(c0 + WC * CW, p.c));
+                    lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, (int)min((int64_t)kLoraRows, r1 - row), block0,
+                                  min(block0 + CB, p.c));
             continue;
         }
-        typename K::W wt[QN][T];
+        LoraRaw<DT> raw = {};
+        u32x4 base[2][QN] = {};
+        float un[2][NU];
+        // the tile's rows of u (two shares, the first of which takes the rest), and of dx_base
+        auto load_u = [&](int64_t row0) {
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
+                un[0][i] = un[1][i] = 0.0f;
+                if (row0 + m < r1 && j < p.r) {
+                    const float* q = p.u + (row0 + m) * p.r + j;
+                    const int64_t part = it.n * p.r;
+                    un[0][i] = q[0];
+                    if (p.u_parts > 1) un[1][i] = q[part];
+                    for (int k = 2; k < p.u_parts; ++k) un[0][i] += q[k * part];
+                }
+            }
+        };
+        auto load_base = [&](int64_t row0) {
+            if (row0 >= r1) return;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int64_t row = min(row0 + 16 * i + n16, r1 - 1);
+#pragma unroll
+                for (int q = 0; q < QN; ++q) {
+                    const int col = col0 + (wr * QN + q) * N::STEP + V * g;
+                    base[i][q] = lora_fetch(static_cast<const S*>(p.base) + row * p.bs, col, p.c);
+                }
+            }
+        };
+        load_u(r0);
+        if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
+        if (p.dx && p.base) load_base(r0);
         if (p.dx) {
             const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
+            lds_barrier();
+            for (int i = threadIdx.x; i < RP * (CB / V); i += kLoraThreads) {
+                const int j = i % RP, k = i / RP * V, col = block0 + k;
+                const u32x4 w = lora_load(down + (int64_t)min(j, p.r - 1) * p.c, col, p.c);
+                const u32x4 q = j < p.r ? w : u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int q = 0; q < QN; ++q)
-#pragma unroll
-                for (int k = 0; k < T; ++k)
-                    wt[q][k].load(down + min(lora_col<DT>(col0 + (wr * QN + q) * N::STEP, k, n16), p.c - 1), p.c, p.r, g);
+                for (int e = 0; e < V; ++e) {
+                    if constexpr (V == 4) wl[(k + e) * WP + j] = q[e];
+                    else wl[(k + e) * WP + j] = (S)(q[e / 2] >> (16 * (e & 1)));
+                }
+            }
         }
-        LoraRaw<DT> raw = {};
-        if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
         for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
-            LoraRaw<DT> next;
-            if (p.pd) next.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
             float* f = ub[turn];
             turn ^= 1;
-            for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
-                const int m = i / RP, j = i % RP;
-                float z = 0.0f;
-                if (row0 + m < r1 && j < p.r)
-                    for (int q = 0; q < p.u_parts; ++q) z += p.u[((int64_t)q * it.n + row0 + m) * p.r + j];
-                f[m * P + j] = z;
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
+                f[m * P + j] = un[0][i] + un[1][i];
             }
+            if (p.pd) raw.trim(row0, r1, edge, mine, p.c);
             if (DROP) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t bits = lora_keep<DT>(key, p.drop, row0 + 8 * g + i, mine, p.c);
-                    raw.v[i] = lora_masked<DT>(raw.v[i], bits);
-                    if constexpr (V == 8) {
-                        keep[w][(8 * g + i) * G + n16] = (uint8_t)bits;
-                    } else {
-                        const uint32_t other = __shfl_xor(bits & 15, 1);
-                        if (!(n16 & 1)) keep[w][(8 * g + i) * G + n16 / 2] = (uint8_t)((bits & 15) | other << 4);
-                    }
+                    const u32x4 ones = lora_ones(key, p.drop, row0 + 8 * g + i, mine, p.c);
+                    raw.v[i] = lora_masked<DT>(raw.v[i], ones, mine);
+                    if (V == 8 || !(n16 & 1)) keep[w][(8 * g + i) * G + n16 * V / 8] = (uint8_t)drop_bits(ones);
                 }
             }
             lds_barrier();
-            if (p.dx) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    typename K::H h;
-                    h.load(f + (16 * i + n16) * P, g);
-                    const int64_t row = row0 + 16 * i + n16;
-#pragma unroll
-                    for (int q = 0; q < QN; ++q) {
-                        const int at = (wr * QN + q) * N::STEP + V * g, col = col0 + at, left = p.c - col;
-                        float z[V];
-#pragma unroll
-                        for (int k = 0; k < T; ++k) {
-                            floatx4 d = {0, 0, 0, 0};
-                            d = K::mma(wt[q][k], h, d);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
-                        }
-                        if (DROP) {
-                            const uint32_t bits = keep[w][(16 * i + n16) * G + at / 8] >> (V == 8 ? 0 : at & 4);
-#pragma unroll
-                            for (int e = 0; e < V; ++e) z[e] = bits >> e & 1 ? z[e] * p.factor : 0.0f;
-                        }
-                        if (row < r1 && left > 0) {
-                            if (p.base) {
-                                const u32x4 b = lora_load(static_cast<const S*>(p.base) + row * p.bs + col, left);
-#pragma unroll
-                                for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(b, e);
-                            }
-                            lora_store(static_cast<S*>(p.dx) + row * p.c + col, lora_round<DT>(z), left);
-                        }
-                    }
-                }
-            }
+            load_u(row0 + kLoraRows);
             if (p.pd) {
                 float b[RW][8];
 #pragma unroll
@@ -876,12 +953,61 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
 #pragma unroll
                     for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
                 lora_outer<DT, RW>(raw, b, acc);
-                raw = next;
+                raw.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
+            }
+            if (p.dx) {
+                if (p.base && edge)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < QN; ++q)
+                            base[i][q] = lora_edge<S>(base[i][q], col0 + (wr * QN + q) * N::STEP + V * g, p.c);
+                typename K::H h[2];
+                if constexpr (RT < 8) {
+                    h[0].load(f + n16 * P, g);
+                    h[1].load(f + (16 + n16) * P, g);
+                }
+#pragma unroll
+                for (int q = 0; q < QN; ++q) {
+                    const int at = (wr * QN + q) * N::STEP, col = col0 + at + V * g, left = p.c - col;
+                    typename K::W wt[T];
+#pragma unroll
+                    for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if constexpr (RT == 8) h[i].load(f + (16 * i + n16) * P, g);
+                        const int64_t row = row0 + 16 * i + n16;
+                        float z[V];
+#pragma unroll
+                        for (int k = 0; k < T; ++k) {
+                            floatx4 d = {0, 0, 0, 0};
+                            d = K::mma(wt[k], h[i], d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
+                        }
+                        if (DROP) {
+                            const uint32_t bits = keep[w][(16 * i + n16) * G + (at + V * g) / 8] >> (V == 8 ? 0 : 2 * (g & 1));
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
+                        }
+                        if (p.base) {
+#pragma unroll
+                            for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(base[i][q], e);
+                        }
+                        if (row < r1) {
+                            S* d = static_cast<S*>(p.dx) + row * p.c + col;
+                            if (!edge) *reinterpret_cast<u32x4_rows*>(d) = lora_round<DT>(z);
+                            else lora_store(d, lora_round<DT>(z), left);
+                        }
+                    }
+                }
+                if (p.base) load_base(row0 + kLoraRows);
             }
         }
         if (p.pd)
-            lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * (int64_t)p.c * p.r, 1, p.c, col0, p.c, rank0, p.r,
-                               DROP ? p.factor : 1.0f);
+            lora_flush<DT, RW, true>(acc, p.pd + (blockIdx.y + v) * (int64_t)p.c * p.r, col0, p.c, rank0, p.r,
+                                     DROP ? p.factor : 1.0f);
     }
 }
 
