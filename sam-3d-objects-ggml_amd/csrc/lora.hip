@@ -18,6 +18,8 @@ struct LoraSum {
     int rows_per;
 };
 
+typedef floatx4 floatx4_any __attribute__((aligned(4)));
+
 template <int DT>
 __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, LoraSum first, LoraSum second) {
     __shared__ float ls[16][64];
@@ -44,9 +46,15 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
 #pragma unroll 4
                 for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16) {
                     const float* q = p.part + j * p.elements + e0;
+                    if (left == 4) {
+                        const floatx4 w = *reinterpret_cast<const floatx4_any*>(q);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < left) s[e] += q[e];
+                        for (int e = 0; e < 4; ++e) s[e] += w[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (e < left) s[e] += q[e];
+                    }
                 }
             }
         }

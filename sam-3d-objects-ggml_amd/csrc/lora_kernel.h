@@ -763,6 +763,21 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
         if (r0 >= r1 || a < 0) continue;
         const float s = p.scale ? p.scale[a] : 1.0f;
         LoraRaw<DT> raw;
+        float h[RW][8];
+        // a tile's hidden rows, a wave's ranks: one tile ahead as dy is, and before it
+        // (loads return in order)
+        auto load_h = [&](int64_t row0, float (&h)[RW][8]) {
+            if (!p.pu || row0 >= r1) return;
+            const bool full = row0 + kLoraRows <= r1;
+#pragma unroll
+            for (int j = 0; j < RW; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t row = row0 + 8 * g + i;
+                    h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
+                }
+        };
+        load_h(r0, h);
         raw.load(p.dy, p.dys, r0, r1, mine, p.o);
         if (p.u) {
             const S* up = static_cast<const S*>(p.up);
@@ -782,19 +797,9 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
         }
         for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
             LoraRaw<DT> next = raw;
+            float hn[RW][8];
+            load_h(row0 + kLoraRows, hn);
             next.load(p.dy, p.dys, row0 + kLoraRows, r1, mine, p.o);
-            float h[RW][8];
-            if (p.pu) {
-                const bool full = row0 + kLoraRows <= r1;
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int64_t row = row0 + 8 * g + i;
-                        h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
-                        if (!full && row >= r1) h[j][i] = 0.0f;
-                    }
-            }
             raw.trim(row0, r1, edge, mine, p.o);
             if (p.u) {
                 S* t = tile[w];
@@ -834,7 +839,19 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                     if (row0 + m < r1 && j < p.r) p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
                 }
             }
-            if (p.pu) lora_outer<DT, RW>(raw, h, acc);
+            if (p.pu) {
+                if (row0 + kLoraRows > r1)
+#pragma unroll
+                    for (int j = 0; j < RW; ++j)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (row0 + 8 * g + i >= r1) h[j][i] = 0.0f;
+                lora_outer<DT, RW>(raw, h, acc);
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) h[j][i] = hn[j][i];
+            }
             raw = next;
             if (p.u) lds_barrier();
         }

@@ -64,14 +64,16 @@ __device__ __forceinline__ u32x4 philox7(DropKey key, uint64_t k) {
 // from 1 to 65536; u >= drop as a saturating difference, both halves at once).
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x4 drop_ones(u32x4 words, uint32_t drop) {
-    const u16x2 one = {1, 1}, d = {(uint16_t)(drop - 1), (uint16_t)(drop - 1)};
+    const u16x2 d = {(uint16_t)(drop - 1), (uint16_t)(drop - 1)};
+    uint32_t one = 0x00010001u;
+    asm("" : "+s"(one));  // (known, the halves would be compared one by one)
     u32x4 r;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const uint32_t w = words[q];  // (a bit cast of a vector's element itself takes element 0)
-        uint32_t m = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w), d));
-        asm("" : "+v"(m));  // (or the halves are compared one by one)
-        r[q] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, m), one));
+        r[q] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
+                                                __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w), d),
+                                                __builtin_bit_cast(u16x2, one)));
     }
     return r;
 }
