@@ -10,27 +10,27 @@ namespace {
 
 // Gradients from the slots that the row passes left: adapter a's is the sum over
 // its items and their chunks (slot = chunk + segment), in a fixed order.  A block
-// takes 64 elements, sixteen slots at a time.
+// takes 64 of a slot's floats, sixteen slots at a time.
 struct LoraSum {
     const float* part;
     void* dst;
-    int64_t elements;  // of an adapter
+    int64_t slot;  // floats
+    int c;         // columns
+    int along;     // dst [r][c], else [c][r]
     int rows_per;
 };
 
-typedef floatx4 floatx4_any __attribute__((aligned(4)));
-
 template <int DT>
-__global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, LoraSum first, LoraSum second) {
-    __shared__ float ls[16][64];
+__global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, LoraSum first, LoraSum second, int r, int rt) {
+    constexpr int V = LoraNum<DT>::V;
+    __shared__ floatx4 ls[16][16];
     const LoraSum p = blockIdx.y ? second : first;
     if (!p.dst) return;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x & 63;
-    const int64_t blocks = (p.elements + 63) / 64;
+    const int64_t blocks = p.slot / 64;
     for (int64_t w = blockIdx.x; w < blocks * it.adapters; w += gridDim.x) {
-        const int64_t a = w / blocks, first_e = w % blocks * 64, e0 = first_e + 4 * tx;
-        const int left = (int)min(p.elements - e0, (int64_t)4);
-        float s[4] = {0, 0, 0, 0};
+        const int64_t a = w / blocks, e0 = w % blocks * 64 + 4 * tx;
+        floatx4 s = {0, 0, 0, 0};
         for (int64_t i0 = 0; i0 < it.items; i0 += 64) {
             const int64_t i = i0 + lane, v = it.off ? i + 1 : 0;
             int64_t b = 0, e = 0;
@@ -38,38 +38,32 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
                 b = it.begin(v);
                 e = it.end(v);
             }
-            const int mine0 = (int)(b / p.rows_per), mine1 = (int)((e - 1) / p.rows_per);
+            const int mine0 = (int)b / p.rows_per, mine1 = (int)(e - 1) / p.rows_per;
             for (uint64_t m = __ballot(b < e); m; m &= m - 1) {
                 const int k = __builtin_ctzll(m);
                 const int64_t seg = it.off ? i0 + k + 1 : 0;
                 const int64_t j0 = __shfl(mine0, k) + seg, j1 = __shfl(mine1, k) + seg;
 #pragma unroll 4
-                for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16) {
-                    const float* q = p.part + j * p.elements + e0;
-                    if (left == 4) {
-                        const floatx4 w = *reinterpret_cast<const floatx4_any*>(q);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[e] += w[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 3; ++e)
-                            if (e < left) s[e] += q[e];
-                    }
-                }
+                for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16)
+                    s += *reinterpret_cast<const floatx4*>(p.part + j * p.slot + e0);
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ls[ty][4 * tx + e] = s[e];
+        ls[ty][tx] = s;
         __syncthreads();
-        const int64_t at = first_e + threadIdx.x;
-        if (threadIdx.x < 64 && at < p.elements) {
+        if (threadIdx.x < 64) {
+            const int64_t at = w % blocks * 64 + threadIdx.x, tile = at >> 8;
+            const int i = threadIdx.x & 3, n = (int)(at >> 2) & 63;
+            const int64_t col = tile / (V * rt) * (16 * V) + V * (4 * (n >> 4) + i) + tile % V;
+            const int rank = (int)(tile / V % rt) * 16 + (n & 15);
             float z = 0.0f;
 #pragma unroll
-            for (int q = 0; q < 16; ++q) z += ls[q][threadIdx.x];
-            using S = typename LoraNum<DT>::S;
-            S* d = static_cast<S*>(p.dst) + a * p.elements + at;
-            if constexpr (DT == SPC_F32) *d = __float_as_uint(z);
-            else *d = DT == SPC_BF16 ? f32_to_bf16_bits(z) : f32_to_f16_bits(z);
+            for (int q = 0; q < 16; ++q) z += ls[q][threadIdx.x >> 2][i];
+            if (col < p.c && rank < r) {
+                using S = typename LoraNum<DT>::S;
+                S* d = static_cast<S*>(p.dst) + a * p.c * r + (p.along ? rank * (int64_t)p.c + col : col * r + rank);
+                if constexpr (DT == SPC_F32) *d = __float_as_uint(z);
+                else *d = DT == SPC_BF16 ? f32_to_bf16_bits(z) : f32_to_f16_bits(z);
+            }
         }
         __syncthreads();
     }
@@ -85,10 +79,17 @@ struct LoraPlan {
 LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
     LoraPlan q{};
     const int step = dt == SPC_F32 ? 16 : 32;
-    q.mt = n / items >= 32 ? lora_row_tiles(r) : 1;
-    const int64_t rows = 16 * q.mt, busy = std::max(ceil_div(n, rows), std::min(items, n));
+    // Tiles of 32 rows halve the adapters' traffic, tiles of 16 give twice the blocks
+    // (us in a graph, 1024 -> 1024 rank 16 bf16, 32 / 16: 4096 rows 15.2 / 9.5, 16,384
+    // 21.3 / 22.3; 30,000 rank 32 38.6 / 45.2).
+    q.mt = n / items >= 32 && n >= 384 * 32 ? kLoraRowTiles : 1;
+    const int64_t rows = 16 * q.mt, busy = std::max<int64_t>(1, std::max(ceil_div(n, rows), std::min(items, n)));
     q.tiles = items > 1 ? n / rows + items + 3 : ceil_div(n, rows) + 3;
-    q.mode = busy >= 256 || r * c <= 32768 ? kLoraFused : kLoraShrink;
+    // One kernel, each of whose column blocks forms the tile's hidden rows again, or two:
+    // one where the tiles fill the device or are little work (us, one / two: 1024 x 1024 ->
+    // 1024 rank 16 8.0 / 9.0, 4 items 1024 -> 4096 rank 64 8.2 / 8.4, 1024 x 4096 -> 1024
+    // rank 32 27 / 18, 8 items 8192 -> 16,384 rank 64 f16 69 / 12.3).
+    q.mode = busy >= 256 || c * (16 + r) * float_size(dt) <= 200000 ? kLoraFused : kLoraShrink;
     auto share = [&](int64_t width, int64_t unit, int64_t want) {  // columns a block
         const int64_t blocks = std::min(std::max<int64_t>(want / busy, 1), ceil_div(width, unit));
         return ceil_div(ceil_div(width, blocks), unit) * unit;
@@ -99,7 +100,7 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
         q.k_per = (int)share(c, 8 * step, 512);
         q.splits = (int)ceil_div(c, q.k_per);
     }
-    q.col_per = (int)share(o, 4 * step, 512);
+    q.col_per = (int)share(o, 8 * step, q.mode == kLoraShrink ? 512 : 384);
     q.col_blocks = (int)ceil_div(o, q.col_per);
     return q;
 }
@@ -107,7 +108,8 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
 struct LoraBackPlan {
     int rows_o, rows_c;         // rows of a chunk
     int64_t chunks_o, chunks_c, blocks_o, blocks_c;
-    size_t u, pu, pd;           // floats
+    int64_t slot_o, slot_c;     // floats
+    size_t u, pu, pd;
 };
 
 LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
@@ -125,8 +127,10 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t
     q.chunks_o = ceil_div(n, q.rows_o);
     q.chunks_c = ceil_div(n, q.rows_c);
     q.u = (size_t)(q.blocks_o * n * r);
-    q.pu = (size_t)((q.chunks_o + items + 2) * o * r);
-    q.pd = (size_t)((q.chunks_c + items + 2) * c * r);
+    q.slot_o = lora_slot(o, lora_wave_cols(dt), lora_rank_tiles(r));
+    q.slot_c = lora_slot(c, lora_wave_cols(dt), lora_rank_tiles(r));
+    q.pu = (size_t)((q.chunks_o + items + 2) * q.slot_o);
+    q.pd = (size_t)((q.chunks_c + items + 2) * q.slot_c);
     return q;
 }
 
@@ -315,11 +319,12 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
                                      : lora_back_in_f32(s, p, in);
     }
     if (err == hipSuccess && (ddown || dup)) {
-        const LoraSum d = {p.pd, ddown, q.in_features * q.rank, b.rows_c}, u = {p.pu, dup, q.out_features * q.rank, b.rows_o};
-        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(std::max(d.elements, u.elements), 64) * q.n_adapters, 1 << 20), 2);
-        if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
-        else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
-        else lora_sum_kernel<SPC_F32><<<grid, kLoraThreads, 0, s>>>(p.it, d, u);
+        const LoraSum d = {p.pd, ddown, b.slot_c, p.c, 1, b.rows_c}, u = {p.pu, dup, b.slot_o, p.o, 0, b.rows_o};
+        const dim3 grid((unsigned)std::min<int64_t>(std::max(d.slot, u.slot) / 64 * q.n_adapters, 1 << 20), 2);
+        const int rt = lora_rank_tiles(q.rank);
+        if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+        else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+        else lora_sum_kernel<SPC_F32><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
         err = hipGetLastError();
     }
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");

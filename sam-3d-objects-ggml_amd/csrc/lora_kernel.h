@@ -98,8 +98,8 @@ struct LoraBackArgs {
     void* dx;
     float* u;          // [u_parts][n][r]
     int u_parts;
-    float* pd;         // [slots][r][c], null: not wanted
-    float* pu;         // [slots][o][r]
+    float* pd;         // slots of ddown (lora_slot), null: not wanted
+    float* pu;         // of dup
     int c, o, r;
     int rows_per;
     const int64_t* seed;
@@ -108,7 +108,7 @@ struct LoraBackArgs {
 };
 
 // Launches, one for each of the rows' dtypes (lora_bf16.hip, ...).  mt: row tiles
-// of 16 in a block's tile, 1 or lora_row_tiles(rank).
+// of 16 in a block's tile, 1 or kLoraRowTiles.
 enum { kLoraFused, kLoraShrink, kLoraExpand };
 #define LORA_LAUNCHERS(D)                                                                             \
     hipError_t lora_forward_##D(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid);       \
@@ -126,7 +126,7 @@ hipError_t lora_small_backward(hipStream_t s, int dt, const LoraBackArgs& p, voi
 
 // ranks in tiles of 16: 1, 2, 4 or 8
 inline int lora_rank_tiles(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
-inline int lora_row_tiles(int64_t r) { return r <= 32 ? 4 : 2; }
+constexpr int kLoraRowTiles = 2;
 // waves of a block along the ranks in the backward kernels (the others along columns)
 inline int lora_rank_waves(int64_t r) { return r <= 32 ? 1 : r <= 64 ? 2 : 4; }
 // columns of one such wave
@@ -150,6 +150,7 @@ struct LoraNum {
 template <typename S>
 __device__ __forceinline__ u32x4 lora_shift(u32x4 w, int by) {
     constexpr int V = 16 / (int)sizeof(S);
+    asm volatile("" : "+v"(by));  // (or its comparisons' masks are kept through the loops)
     if constexpr (V == 8)
         w = by & 1 ? u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16} : w;
     w = by & (V / 4) ? u32x4{w[1], w[2], w[3], 0} : w;
@@ -395,6 +396,29 @@ __device__ __forceinline__ int lora_col(int col, int t, int m) {
     else return col + 8 * (m >> 2) + 4 * t + (m & 3);
 }
 
+// Stores a tile of 16 rows x 2 STEP columns whose results lie as lora_mma leaves
+// them, rows below m of it: a lane has V columns from V (lane / 16) on of row lane %
+// 16, of the first step in a and of the second in b.  Eight lanes a row take 128
+// bytes of it in one store, after lanes 8 apart have exchanged one of the two
+// (rows of 1024, read and written: 64 bytes of a row in a store 102 us, 128 76).
+template <typename S>
+__device__ __forceinline__ void lora_store_pair(S* at, int64_t stride, u32x4 a, u32x4 b, int m) {
+    constexpr int V = 16 / (int)sizeof(S);
+    const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
+    const bool high = n16 & 8;
+    u32x4 first, second;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t mine = high ? a[q] : b[q];
+        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0x128, 0xf, 0xf, true);  // lane ^ 8
+        first[q] = high ? other : a[q];
+        second[q] = high ? b[q] : other;
+    }
+    S* q = at + (n16 & 7) * stride + V * g + (high ? 4 * V : 0);
+    if ((n16 & 7) < m) __builtin_nontemporal_store(first, reinterpret_cast<u32x4_rows*>(q));
+    if ((n16 & 7) + 8 < m) __builtin_nontemporal_store(second, reinterpret_cast<u32x4_rows*>(q + 8 * stride));
+}
+
 struct LoraTile {
     int64_t row0, a;
     int m;  // rows
@@ -409,7 +433,8 @@ template <int DT, int RT, int MT, bool DROP>
 __device__ __forceinline__ void lora_shrink(const LoraArgs& p, const LoraTile& t, int k0, int k1, float* red) {
     using N = LoraNum<DT>;
     using S = typename N::S;
-    constexpr int V = N::V, UN = 2;
+    // (steps in flight: few rows are bound by the latency of their loads)
+    constexpr int V = N::V, UN = RT <= 2 ? 4 : 2;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
     const S* xr[MT];
     const S* wr[RT];
@@ -480,51 +505,74 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
     const float s = p.scale ? p.scale[t.a] : 1.0f;
     const S* up = static_cast<const S*>(p.up);
     const int64_t all = p.it.adapters * p.o * p.r;
-    for (int cg = c0 + w * N::STEP; cg < c1; cg += 4 * N::STEP) {
-        u32x4 wr[T][K::STEPS], b[MT];
-        const int col = cg + V * g, left = p.o - col;
-        const bool edge = cg + N::STEP > p.o;
+    // two steps of columns at a time
+    for (int cb = c0 + w * 2 * N::STEP; cb < c1; cb += 8 * N::STEP) {
+        u32x4 wr[2][T][K::STEPS], b[2][MT];
+        const bool edge = cb + 2 * N::STEP > p.o;
 #pragma unroll
-        for (int q = 0; q < T; ++q) {
-            const int64_t at = (t.a * p.o + min(lora_col<DT>(cg, q, n16), p.o - 1)) * p.r;
+        for (int x = 0; x < 2; ++x) {
 #pragma unroll
-            for (int k = 0; k < K::STEPS; ++k) wr[q][k] = lora_fetch_short(up, at + K::rank(k, g), all);
+            for (int q = 0; q < T; ++q) {
+                const int64_t at = (t.a * p.o + min(lora_col<DT>(cb + x * N::STEP, q, n16), p.o - 1)) * p.r;
+#pragma unroll
+                for (int k = 0; k < K::STEPS; ++k) wr[x][q][k] = lora_fetch_short(up, at + K::rank(k, g), all);
+            }
+            if (p.base)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    b[x][i] = lora_fetch(static_cast<const S*>(p.base) + (t.row0 + min(16 * i + n16, t.m - 1)) * p.bs,
+                                         cb + x * N::STEP + V * g, p.o);
         }
-        if (p.base)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                b[i] = lora_fetch(static_cast<const S*>(p.base) + (t.row0 + min(16 * i + n16, t.m - 1)) * p.bs, col, p.o);
         if (p.r < 16 * RT)
 #pragma unroll
-            for (int q = 0; q < T; ++q) {
-                const int64_t at = (t.a * p.o + min(lora_col<DT>(cg, q, n16), p.o - 1)) * p.r;
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int k = 0; k < K::STEPS; ++k)
-                    wr[q][k] = lora_edge_short<S>(wr[q][k], at + K::rank(k, g), all, p.r - K::rank(k, g));
+                for (int q = 0; q < T; ++q) {
+                    const int64_t at = (t.a * p.o + min(lora_col<DT>(cb + x * N::STEP, q, n16), p.o - 1)) * p.r;
+#pragma unroll
+                    for (int k = 0; k < K::STEPS; ++k)
+                        wr[x][q][k] = lora_edge_short<S>(wr[x][q][k], at + K::rank(k, g), all, p.r - K::rank(k, g));
+                }
+        if (p.base && edge)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) b[x][i] = lora_edge<S>(b[x][i], cb + x * N::STEP + V * g, p.o);
+        u32x4 out[2][MT];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            typename K::W wt[T];
+#pragma unroll
+            for (int q = 0; q < T; ++q) wt[q].set(wr[x][q]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float v[V];
+#pragma unroll
+                for (int q = 0; q < T; ++q) {
+                    floatx4 z = {0, 0, 0, 0};
+                    z = K::mma(wt[q], h[i], z);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[4 * q + e] = s * z[e];
+                }
+                if (p.base)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] += lora_value<DT>(b[x][i], e);
+                out[x][i] = lora_round<DT>(v);
             }
-        typename K::W wt[T];
+        }
+        S* y = static_cast<S*>(p.y) + t.row0 * p.o + cb;
+        if (!edge) {
 #pragma unroll
-        for (int q = 0; q < T; ++q) wt[q].set(wr[q]);
+            for (int i = 0; i < MT; ++i)
+                lora_store_pair(y + (int64_t)16 * i * p.o, p.o, out[0][i], out[1][i], t.m - 16 * i);
+        } else {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            float v[V];
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int q = 0; q < T; ++q) {
-                floatx4 z = {0, 0, 0, 0};
-                z = K::mma(wt[q], h[i], z);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * q + e] = s * z[e];
-            }
-            if (p.base) {
-                if (edge) b[i] = lora_edge<S>(b[i], col, p.o);
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[e] += lora_value<DT>(b[i], e);
-            }
-            if (16 * i + n16 < t.m) {
-                S* q = static_cast<S*>(p.y) + (t.row0 + 16 * i + n16) * p.o + col;
-                if (!edge) *reinterpret_cast<u32x4_rows*>(q) = lora_round<DT>(v);
-                else lora_store(q, lora_round<DT>(v), left);
-            }
+                for (int i = 0; i < MT; ++i) {
+                    const int at = x * N::STEP + V * g;
+                    if (16 * i + n16 < t.m) lora_store(y + (int64_t)(16 * i + n16) * p.o + at, out[x][i], p.o - cb - at);
+                }
         }
     }
 }
@@ -553,7 +601,7 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
 template <int DT, int RT, int MT, int MODE, bool DROP>
 __global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) {
     constexpr int R = 16 * MT, P = lora_pitch(16 * RT);
-    __shared__ __attribute__((aligned(16))) float red[MODE == kLoraExpand ? 1 : 4 * R * P];
+    __shared__ __attribute__((aligned(16))) float red[4 * R * P];
     __shared__ __attribute__((aligned(16))) float hid[MODE == kLoraShrink ? 4 : R * P];
     const LoraItems& it = p.it;
     const int64_t v = it.template find<R>(blockIdx.x, 1);
@@ -572,19 +620,25 @@ __global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) 
         const int k0 = MODE == kLoraShrink ? blockIdx.y * p.k_per : 0;
         const int k1 = MODE == kLoraShrink ? min(k0 + p.k_per, p.c) : p.c;
         lora_shrink<DT, RT, MT, DROP>(p, t, k0, k1, red);
-        __syncthreads();
+    } else {
+        // a wave takes every fourth share, so that few rows wait for few of them in turn
+        const int w = threadIdx.x >> 6;
+        for (int i = threadIdx.x & 63; i < t.m * p.r; i += 64) {
+            const float* q = p.part + row0 * p.r + i;
+            float s = 0.0f;
+#pragma unroll 8
+            for (int k = w; k < p.splits; k += 4) s += q[(int64_t)k * it.n * p.r];
+            red[(w * R + i / p.r) * P + i % p.r] = s;
+        }
     }
+    __syncthreads();
     for (int i = threadIdx.x; i < R * 16 * RT; i += kLoraThreads) {
         const int m = i / (16 * RT), j = i % (16 * RT);
         float s = 0.0f;
         if (m < t.m && j < p.r) {
-            if constexpr (MODE == kLoraExpand) {
-                for (int q = 0; q < p.splits; ++q) s += p.part[((int64_t)q * it.n + row0 + m) * p.r + j];
-            } else {
-                const float* f = red + m * P + j;
-                s = (f[0] + f[R * P]) + (f[2 * R * P] + f[3 * R * P]);
-                if (DROP) s *= p.factor;
-            }
+            const float* f = red + m * P + j;
+            s = (f[0] + f[R * P]) + (f[2 * R * P] + f[3 * R * P]);
+            if (DROP) s *= p.factor;
             if constexpr (MODE == kLoraShrink) p.part[((int64_t)blockIdx.y * it.n + row0 + m) * p.r + j] = s;
             else if (p.hidden && blockIdx.y == 0) p.hidden[(row0 + m) * p.r + j] = s;
         }
@@ -609,10 +663,11 @@ void lora_forward_mode(hipStream_t s, const LoraArgs& p, int mode, dim3 grid) {
 template <int DT>
 hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid) {
     const int rt = lora_rank_tiles(p.r);
-    if (rt == 1) mt == 1 ? lora_forward_mode<DT, 1, 1>(s, p, mode, grid) : lora_forward_mode<DT, 1, 4>(s, p, mode, grid);
-    else if (rt == 2) mt == 1 ? lora_forward_mode<DT, 2, 1>(s, p, mode, grid) : lora_forward_mode<DT, 2, 4>(s, p, mode, grid);
-    else if (rt == 4) mt == 1 ? lora_forward_mode<DT, 4, 1>(s, p, mode, grid) : lora_forward_mode<DT, 4, 2>(s, p, mode, grid);
-    else mt == 1 ? lora_forward_mode<DT, 8, 1>(s, p, mode, grid) : lora_forward_mode<DT, 8, 2>(s, p, mode, grid);
+    constexpr int M = kLoraRowTiles;
+    if (rt == 1) mt == 1 ? lora_forward_mode<DT, 1, 1>(s, p, mode, grid) : lora_forward_mode<DT, 1, M>(s, p, mode, grid);
+    else if (rt == 2) mt == 1 ? lora_forward_mode<DT, 2, 1>(s, p, mode, grid) : lora_forward_mode<DT, 2, M>(s, p, mode, grid);
+    else if (rt == 4) mt == 1 ? lora_forward_mode<DT, 4, 1>(s, p, mode, grid) : lora_forward_mode<DT, 4, M>(s, p, mode, grid);
+    else mt == 1 ? lora_forward_mode<DT, 8, 1>(s, p, mode, grid) : lora_forward_mode<DT, 8, M>(s, p, mode, grid);
     return hipGetLastError();
 }
 
@@ -698,35 +753,25 @@ __device__ __forceinline__ void lora_outer(const LoraRaw<DT>& raw, const float (
     }
 }
 
-// Writes a wave's sums times f and clears them: column col + V (4 g + i) + e, rank
-// rank0 + 16 j + lane % 16.  ALONG: dst [r][c], so that a lane's V columns are a run;
-// else [c][r].  (The addresses are made here: hoisted out of the segments' loop
-// they would fill the registers.)
-template <int DT, int RW, bool ALONG>
-__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* dst, int col, int c, int rank0, int r,
+// A slot of the weights' gradients holds its sums as the waves' registers do: for
+// each tile of 16 V columns, rank tile and e, a lane's four (columns V (4 (lane / 16)
+// + i) + e, rank lane % 16), so that a wave writes and the sum over the slots reads
+// whole lines (by rank and column, four bytes a lane and line, the writes alone
+// were 20 us of 62,710 x 1024).
+constexpr int64_t lora_slot(int64_t c, int cw, int rt) { return (c + cw - 1) / cw * cw * 16 * rt; }
+
+template <int DT, int RW>
+__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* slot, int tile, int rt, int rank_tile,
                                            float f) {
     constexpr int V = LoraNum<DT>::V;
-    int lane = threadIdx.x & 63;
-    asm volatile("" : "+v"(lane));
-    const int n16 = lane & 15, k0 = col + 4 * V * (lane >> 4), left = c - k0;
-    float* q = dst + (ALONG ? (int64_t)(rank0 + n16) * c + k0 : (int64_t)k0 * r + rank0 + n16);
+    float* q = slot + ((int64_t)tile * rt + rank_tile) * V * 256 + 4 * (threadIdx.x & 63);
 #pragma unroll
-    for (int j = 0; j < RW; ++j) {
-        const bool on = rank0 + 16 * j + n16 < r;
-        float* t = q + (ALONG ? (int64_t)16 * j * c : 16 * j);
+    for (int j = 0; j < RW; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (on && V * i + e < left) *t = f * acc[e][j][i];
-                t += ALONG ? 1 : r;
-            }
+        for (int e = 0; e < V; ++e) {
+            *reinterpret_cast<floatx4*>(q + (j * V + e) * 256) = f * acc[e][j];
+            acc[e][j] = floatx4{0, 0, 0, 0};
         }
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-#pragma unroll
-        for (int j = 0; j < RW; ++j) acc[e][j] = floatx4{0, 0, 0, 0};
 }
 
 __device__ __forceinline__ void lora_wave_sync() {
@@ -796,6 +841,11 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             lds_barrier();
         }
         for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+            // (what follows from the lane is formed anew each time: kept through the loops it
+            // would not fit the registers)
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
             LoraRaw<DT> next = raw;
             float hn[RW][8];
             load_h(row0 + kLoraRows, hn);
@@ -855,8 +905,8 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             raw = next;
             if (p.u) lds_barrier();
         }
-        if (p.pu)
-            lora_flush<DT, RW, false>(acc, p.pu + (blockIdx.y + v) * (int64_t)p.o * p.r, col0, p.o, rank0, p.r, s);
+        if (p.pu && col0 < p.o)
+            lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
     }
 }
 
@@ -870,7 +920,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     using K = LoraRanks<DT, RT>;
     constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RT, P = lora_pitch(RP), T = V / 4;
     constexpr int WP = RP + V;       // pitch of the weights
-    constexpr int QN = 4 / WR;       // steps of columns whose dx the wave forms
+    constexpr int QN = 4 / WR, QP = QN > 1 ? 2 : 1;  // steps of columns whose dx the wave forms, at a time
     constexpr int G = CW / 8;        // groups of eight columns
     constexpr int NU = kLoraRows * RP / kLoraThreads;  // values of u a thread
     __shared__ __attribute__((aligned(16))) float ub[2][kLoraRows * P];
@@ -915,8 +965,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 }
             }
         };
-        auto load_base = [&](int64_t row0) {
-            if (row0 >= r1) return;
+        auto load_base = [&](int64_t row0, int n16, int g) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int64_t row = min(row0 + 16 * i + n16, r1 - 1);
@@ -929,7 +978,6 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
         };
         load_u(r0);
         if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
-        if (p.dx && p.base) load_base(r0);
         if (p.dx) {
             const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
             lds_barrier();
@@ -945,6 +993,11 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
             }
         }
         for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+            // (what follows from the lane is formed anew each time: kept through the loops it
+            // would not fit the registers)
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
             float* f = ub[turn];
             turn ^= 1;
 #pragma unroll
@@ -952,7 +1005,14 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
                 f[m * P + j] = un[0][i] + un[1][i];
             }
-            if (p.pd) raw.trim(row0, r1, edge, mine, p.c);
+            // (loads return in order: u, wanted first, before dx_base and the next rows)
+            LoraRaw<DT> next = raw;
+            load_u(row0 + kLoraRows);
+            if (p.dx && p.base) load_base(row0, n16, g);
+            if (p.pd) {
+                next.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
+                raw.trim(row0, r1, edge, mine, p.c);
+            }
             if (DROP) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -962,7 +1022,6 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 }
             }
             lds_barrier();
-            load_u(row0 + kLoraRows);
             if (p.pd) {
                 float b[RW][8];
 #pragma unroll
@@ -970,7 +1029,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
 #pragma unroll
                     for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
                 lora_outer<DT, RW>(raw, b, acc);
-                raw.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
+                raw = next;
             }
             if (p.dx) {
                 if (p.base && edge)
@@ -984,47 +1043,62 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                     h[0].load(f + n16 * P, g);
                     h[1].load(f + (16 + n16) * P, g);
                 }
+                const int rows = (int)min(r1 - row0, (int64_t)kLoraRows);
+                S* d = static_cast<S*>(p.dx) + row0 * p.c + col0 + wr * QN * N::STEP;
 #pragma unroll
-                for (int q = 0; q < QN; ++q) {
-                    const int at = (wr * QN + q) * N::STEP, col = col0 + at + V * g, left = p.c - col;
-                    typename K::W wt[T];
+                for (int q = 0; q < QN; q += QP) {
+                    u32x4 out[2][QP];
 #pragma unroll
-                    for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
+                    for (int x = 0; x < QP; ++x) {
+                        const int at = (wr * QN + q + x) * N::STEP;
+                        typename K::W wt[T];
+#pragma unroll
+                        for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            if constexpr (RT == 8) h[i].load(f + (16 * i + n16) * P, g);
+                            float z[V];
+#pragma unroll
+                            for (int k = 0; k < T; ++k) {
+                                floatx4 d = {0, 0, 0, 0};
+                                d = K::mma(wt[k], h[i], d);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
+                            }
+                            if (DROP) {
+                                const uint32_t bits =
+                                    keep[w][(16 * i + n16) * G + (at + V * g) / 8] >> (V == 8 ? 0 : 2 * (g & 1));
+#pragma unroll
+                                for (int e = 0; e < V; ++e)
+                                    z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
+                            }
+                            if (p.base)
+#pragma unroll
+                                for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(base[i][q + x], e);
+                            out[i][x] = lora_round<DT>(z);
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if constexpr (RT == 8) h[i].load(f + (16 * i + n16) * P, g);
-                        const int64_t row = row0 + 16 * i + n16;
-                        float z[V];
+                        S* t = d + (int64_t)16 * i * p.c + q * N::STEP;
+                        if (QP == 2 && !edge) {
+                            lora_store_pair(t, p.c, out[i][0], out[i][QP - 1], rows - 16 * i);
+                        } else {
 #pragma unroll
-                        for (int k = 0; k < T; ++k) {
-                            floatx4 d = {0, 0, 0, 0};
-                            d = K::mma(wt[k], h[i], d);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
-                        }
-                        if (DROP) {
-                            const uint32_t bits = keep[w][(16 * i + n16) * G + (at + V * g) / 8] >> (V == 8 ? 0 : 2 * (g & 1));
-#pragma unroll
-                            for (int e = 0; e < V; ++e)
-                                z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
-                        }
-                        if (p.base) {
-#pragma unroll
-                            for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(base[i][q], e);
-                        }
-                        if (row < r1) {
-                            S* d = static_cast<S*>(p.dx) + row * p.c + col;
-                            if (!edge) *reinterpret_cast<u32x4_rows*>(d) = lora_round<DT>(z);
-                            else lora_store(d, lora_round<DT>(z), left);
+                            for (int x = 0; x < QP; ++x) {
+                                const int at = x * N::STEP + V * g;
+                                if (16 * i + n16 < rows)
+                                    lora_store(t + n16 * (int64_t)p.c + at, out[i][x],
+                                               p.c - col0 - (wr * QN + q) * N::STEP - at);
+                            }
                         }
                     }
                 }
-                if (p.base) load_base(row0 + kLoraRows);
             }
         }
-        if (p.pd)
-            lora_flush<DT, RW, true>(acc, p.pd + (blockIdx.y + v) * (int64_t)p.c * p.r, col0, p.c, rank0, p.r,
-                                     DROP ? p.factor : 1.0f);
+        if (p.pd && col0 < p.c)
+            lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
+                               DROP ? p.factor : 1.0f);
     }
 }
 

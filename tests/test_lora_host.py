@@ -119,6 +119,8 @@ def test_host_validation_lora(spc):
         assert need > 0
         assert (fwd, bwd)[b](n=1000, wsb=need - 1) == nat.BAD_ARG
     assert b"workspace" in L.spc_last_error()
+    for items in (1, 7, 65535):  # no rows: an answer, not a division
+        assert all(L.spc_lora_workspace_bytes(nat.F16, 0, items, 64, 48, 8, b) > 0 for b in (0, 1))
     assert L.spc_lora_workspace_bytes(nat.BF16, 4, 1, 64, 48, 129, 0) == 0
     assert L.spc_lora_workspace_bytes(nat.Q8_0, 4, 1, 64, 48, 8, 0) == 0
     assert L.spc_lora_workspace_bytes(nat.BF16, 4, 0, 64, 48, 8, 1) == 0
