@@ -722,7 +722,7 @@ int spc_dropout(spc_stream_t stream, int dtype, const void* x, int64_t x_stride,
 
 /* Low-rank adapters, by the batch item (request) that a row belongs to: item
  * i's rows are [offsets[i], offsets[i + 1]) (device int64 [n_items + 1],
- * ascending; NULL with n_items 1: every row), its adapter is adapters[i]
+ * ascending; NULL: n / n_items rows each, n a multiple), its adapter is adapters[i]
  * (device int32 [n_items]; NULL with n_adapters 1: adapter 0), values outside
  * [0, n_adapters) naming none.  down [n_adapters, rank, in_features], up
  * [n_adapters, out_features, rank] (contiguous, the rows' dtype), scale f32
@@ -749,7 +749,7 @@ typedef struct {
  * rows x_stride and base_stride elements apart, y contiguous (may be base where
  * that is).  hidden: f32 [n, rank], dropout(x) down_a^T (zeros for rows without
  * an adapter), what the gradient reads, or NULL.  Sums are F32, the hidden rows
- * are kept in F32; one rounding to dtype.  rank 1 to 128, in_features and
+ * are kept in F32; one rounding to dtype.  n up to 2^27, rank 1 to 128, in_features and
  * out_features to 2^24, n_items and n_adapters to 65535.  workspace:
  * spc_lora_workspace_bytes, 16-byte aligned. */
 size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t in_features,

@@ -1164,8 +1164,8 @@ def _lora_params(x, down, up, scale, offsets, adapters, p, seed):
         if offsets.dtype != torch.int64 or offsets.shape != (items + 1,):
             raise ValueError(f"offsets must be int64 [{items + 1}]")
         offsets = offsets.contiguous()
-    elif items != 1:
-        raise ValueError("more than one item needs offsets")
+    elif not items or x.shape[0] % items:
+        raise ValueError("items of unequal rows need offsets")
     seed = _dropout_seed(p, seed)
     keep = (down, up, scale, offsets, adapters, seed)
     return LoraParams(*map(_ptr, keep), k, items, i, o, r, p), keep
@@ -1178,7 +1178,7 @@ def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tens
     """base + scale_a (dropout(x) down_a^T) up_a^T [n, out] for rows x [n, in]
     (spc_lora), a the adapter of the row's batch item: down [k, rank, in], up
     [k, out, rank], scale float32 [k] (None: 1); item i's rows are offsets[i] ..
-    offsets[i+1] (device int64; None: one item of all rows), its adapter
+    offsets[i+1] (device int64; None: equally many rows each), its adapter
     adapters[i] (device int32 [n_items], outside 0 .. k - 1: none; may be left
     out with one adapter).  Rows without an adapter are base (None: zeros).  p,
     seed: dropout in front of the adapters, as dropout(x, p, seed).  F32
@@ -1188,8 +1188,8 @@ def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tens
     adapters are."""
     dev = _one_device(x, down, up, base, scale, offsets, adapters, seed, out)
     dt = dtype_code(x.dtype)
-    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
     x, n, c, stride = _strided_rows(x, "x")
+    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
     o, r, bs = q.out_features, q.rank, 0
     if c != q.in_features:
         raise ValueError(f"expected x [n, {q.in_features}], got {tuple(x.shape)}")
@@ -1226,8 +1226,8 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, hidden: torch.Tensor | None
     Deterministic."""
     dev = _one_device(x, dy, hidden, down, up, dx_base, scale, offsets, adapters, seed)
     dt = dtype_code(x.dtype)
-    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
     x, n, c, xs = _strided_rows(x, "x")
+    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
     o, r, bs = q.out_features, q.rank, 0
     if c != q.in_features or dy.shape != (n, o) or dy.dtype != x.dtype:
         raise ValueError(f"expected x [n, {q.in_features}] and dy [n, {o}] of one dtype, got "

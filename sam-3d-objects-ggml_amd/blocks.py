@@ -94,13 +94,25 @@ class SparseResBlock3d(nn.Module):
             x = self.updown(x)
         return x
 
-    def forward(self, x: SparseTensor, emb: torch.Tensor) -> SparseTensor:
-        emb_out = self.emb_layers(emb).type(x.dtype)
+    def _skip(self, x: SparseTensor, adapters) -> SparseTensor:
+        if adapters is None or not getattr(self.skip_connection, "has_adapters", False):
+            return self.skip_connection(x)
+        return self.skip_connection(x, adapters)
+
+    def forward(self, x: SparseTensor, emb: torch.Tensor,
+                adapters: Optional[torch.Tensor] = None) -> SparseTensor:
+        """adapters (int32 [B] on the device, -1 for none): each item's, for those of
+        the block's Linears that have any (Q4Linear.add_adapters)."""
+        act, modulation = self.emb_layers
+        if adapters is None or not getattr(modulation, "has_adapters", False):
+            emb_out = self.emb_layers(emb).type(x.dtype)
+        else:
+            emb_out = modulation(act(emb), adapters).type(x.dtype)
         # the halves as F32 in one pass (chunk and two conversions take two)
         scale, shift = emb_out.reshape(emb_out.shape[0], 2, -1).transpose(0, 1).to(
             torch.float32, memory_format=torch.contiguous_format).contiguous().unbind(0)
         if self.upsample and self.coarse_rows:
-            return self._forward_upsample(x, scale, shift)
+            return self._forward_upsample(x, scale, shift, adapters)
         x = self._updown(x)
         h = x.replace(nat.layernorm_silu(x.feats, self.norm1.weight, self.norm1.bias,
                                          eps=self.norm1.eps))
@@ -114,14 +126,14 @@ class SparseResBlock3d(nn.Module):
             h = self.conv1(h)
             h = h.replace(nat.layernorm_mod_silu(h.feats, scale, shift, h.coords,
                                                  eps=self.norm2.eps))
-        skip = self.skip_connection(x)
+        skip = self._skip(x, adapters)
         if self.out_channels % 32 == 0:
             return self.conv2.forward_fused(h, residual=skip.feats)
         return self.conv2(h) + skip
 
 
-    def _forward_upsample(self, x: SparseTensor, scale: torch.Tensor,
-                          shift: torch.Tensor) -> SparseTensor:
+    def _forward_upsample(self, x: SparseTensor, scale: torch.Tensor, shift: torch.Tensor,
+                          adapters: Optional[torch.Tensor]) -> SparseTensor:
         """forward() with upsampling.  The reference upsamples first (fine
         row f is a copy of coarse row up[f]) and normalises the copies; norm1,
         SiLU and the skip Linear are row-wise, so they run on the coarse rows
@@ -159,7 +171,7 @@ class SparseResBlock3d(nn.Module):
             y1 = nat.layernorm_mod_silu(y1, scale, shift, fine.coords,
                                         eps=self.norm2.eps)
         h = fine.replace(y1)
-        skip = self.skip_connection(x).feats
+        skip = self._skip(x, adapters).feats
         if self.out_channels % 32 == 0:
             return self.conv2.forward_fused(h, residual=skip, residual_rows=rows)
         return self.conv2(h) + h.replace(nat.gather_rows(skip, rows))

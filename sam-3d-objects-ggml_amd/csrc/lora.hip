@@ -32,7 +32,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
         const int64_t a = w / blocks, e0 = w % blocks * 64 + 4 * tx;
         floatx4 s = {0, 0, 0, 0};
         for (int64_t i0 = 0; i0 < it.items; i0 += 64) {
-            const int64_t i = i0 + lane, v = it.off ? i + 1 : 0;
+            const int64_t i = i0 + lane, v = it.off ? i + 1 : i;
             int64_t b = 0, e = 0;
             if (i < it.items && it.adapter(v) == a) {
                 b = it.begin(v);
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
             const int mine0 = (int)b / p.rows_per, mine1 = (int)(e - 1) / p.rows_per;
             for (uint64_t m = __ballot(b < e); m; m &= m - 1) {
                 const int k = __builtin_ctzll(m);
-                const int64_t seg = it.off ? i0 + k + 1 : 0;
+                const int64_t seg = i0 + k + (it.off ? 1 : 0);
                 const int64_t j0 = __shfl(mine0, k) + seg, j1 = __shfl(mine1, k) + seg;
 #pragma unroll 4
                 for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16)
@@ -84,7 +84,7 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
     // 21.3 / 22.3; 30,000 rank 32 38.6 / 45.2).
     q.mt = n / items >= 32 && n >= 384 * 32 ? kLoraRowTiles : 1;
     const int64_t rows = 16 * q.mt, busy = std::max<int64_t>(1, std::max(ceil_div(n, rows), std::min(items, n)));
-    q.tiles = items > 1 ? n / rows + items + 3 : ceil_div(n, rows) + 3;
+    q.tiles = n / rows + items + 3;
     // One kernel, each of whose column blocks forms the tile's hidden rows again, or two:
     // one where the tiles fill the device or are little work (us, one / two: 1024 x 1024 ->
     // 1024 rank 16 8.0 / 9.0, 4 items 1024 -> 4096 rank 64 8.2 / 8.4, 1024 x 4096 -> 1024
@@ -155,8 +155,8 @@ int lora_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_
         set_last_error("%s: p must lie in [0, 1]", fn);
         return SPC_BAD_ARG;
     }
-    if ((!q->offsets && q->n_items != 1) || (!q->adapters && q->n_adapters != 1)) {
-        set_last_error("%s: more than one item needs offsets, more than one adapter the items' adapters", fn);
+    if ((!q->offsets && n % q->n_items) || (!q->adapters && q->n_adapters != 1)) {
+        set_last_error("%s: items of unequal rows need offsets, more than one adapter the items' adapters", fn);
         return SPC_BAD_ARG;
     }
     const int64_t e = float_size(dtype);
@@ -167,7 +167,7 @@ int lora_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_
         set_last_error("%s: null or misaligned pointer", fn);
         return SPC_BAD_ARG;
     }
-    *it = LoraItems{q->offsets, q->adapters, q->n_items, q->n_adapters, n};
+    *it = LoraItems{q->offsets, q->adapters, q->n_items, q->n_adapters, n, n / q->n_items};
     return SPC_OK;
 }
 

@@ -25,19 +25,20 @@ constexpr int64_t kLoraMaxRank = 128, kLoraMaxItems = 65535, kLoraMaxAdapters = 
 constexpr int64_t kLoraMaxWidth = 1 << 24, kLoraMaxRows = 1 << 27;
 constexpr int kLoraThreads = 256;
 
-// Where the items' rows and adapters are.  Segment 0 is the rows before the
-// first item, segment i + 1 item i's, the last the rows behind the items.
+// Where the items' rows and adapters are.  Without offsets segment i is item i's
+// rows, `per` of them; with them segment 0 is the rows before the first item,
+// segment i + 1 item i's, the last the rows behind the items.
 struct LoraItems {
-    const int64_t* off;    // [items + 1] or null: one item of all rows
+    const int64_t* off;    // [items + 1] or null
     const int32_t* which;  // [items] or null: adapter 0
-    int64_t items, adapters, n;
+    int64_t items, adapters, n, per;
 
-    __device__ __forceinline__ int64_t segments() const { return off ? items + 2 : 1; }
+    __device__ __forceinline__ int64_t segments() const { return off ? items + 2 : items; }
     __device__ __forceinline__ int64_t begin(int64_t v) const {
-        return v == 0 ? 0 : min(max(off[v - 1], (int64_t)0), n);
+        return !off ? v * per : v == 0 ? 0 : min(max(off[v - 1], (int64_t)0), n);
     }
     __device__ __forceinline__ int64_t end(int64_t v) const {
-        return v + 1 == segments() ? n : min(max(off[v], (int64_t)0), n);
+        return !off ? (v + 1) * per : v == items + 1 ? n : min(max(off[v], (int64_t)0), n);
     }
     // the segment's adapter, -1 for none
     __device__ __forceinline__ int64_t adapter(int64_t v) const {

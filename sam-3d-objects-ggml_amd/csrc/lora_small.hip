@@ -97,7 +97,7 @@ __global__ __launch_bounds__(256) void lora_weight_kernel(LoraItems it, const vo
     const int64_t i = t / r, j = t % r;
     double sum = 0.0;
     for (int64_t k = 0; k < it.items; ++k) {
-        const int64_t v = it.off ? k + 1 : 0;
+        const int64_t v = it.off ? k + 1 : k;
         if (it.adapter(v) != a) continue;
         for (int64_t row = it.begin(v); row < it.end(v); ++row)
             sum += (double)d.apply(lora_get<DT>(x, row * stride + i), row, i, c) * g[row * r + j];

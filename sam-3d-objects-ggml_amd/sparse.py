@@ -45,7 +45,7 @@ __all__ = [
     "SparseTensor", "SparseTensorData", "sparse_batch_broadcast", "sparse_batch_op",
     "sparse_cat", "sparse_unbind", "SparseConv3d", "SparseInverseConv3d",
     "SparseDownsample", "SparseUpsample", "SparseSubdivide", "SparseLinear",
-    "Q4Linear", "SparseGroupNorm32", "SparseLayerNorm32", "SparseSiLU",
+    "Q4Linear", "SparseGroupNorm32", "SparseLayerNorm32", "SparseDropout", "SparseSiLU",
 ]
 
 BACKEND = "hip"
@@ -885,6 +885,56 @@ class _Q4LinearFn(torch.autograd.Function):
         return dx, db, None
 
 
+class _LoraFn(torch.autograd.Function):
+    """nat.lora with the gradients of the rows, the base, down and up."""
+
+    @staticmethod
+    def forward(ctx, x, down, up, base, scale, offsets, adapters, p, seed):
+        y, hidden = nat.lora(x, down, up, base, scale=scale, offsets=offsets, adapters=adapters, p=p,
+                             seed=seed, return_hidden=True)
+        ctx.save_for_backward(x, hidden, down, up, scale, offsets, adapters, seed)
+        ctx.p = p
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, hidden, down, up, scale, offsets, adapters, seed = ctx.saved_tensors
+        grads = nat.lora_backward(dy, x, hidden, down, up, scale=scale, offsets=offsets,
+                                  adapters=adapters, p=ctx.p, seed=seed, need=ctx.needs_input_grad[:3])
+        return (*grads, dy if ctx.needs_input_grad[3] else None, *[None] * 5)
+
+
+class _Q4LoraFn(torch.autograd.Function):
+    """nat.linear_q4_0 with adapters on top, and the gradients of the rows (both
+    in one), the bias, down and up."""
+
+    @staticmethod
+    def forward(ctx, x, down, up, bias, linear, scale, offsets, adapters, p, seed):
+        base = nat.linear_q4_0(x, linear._q4_operand(x.device, False), bias)
+        y, hidden = nat.lora(x, down, up, base, scale=scale, offsets=offsets, adapters=adapters, p=p,
+                             seed=seed, return_hidden=True, out=base)
+        ctx.save_for_backward(x, hidden, down, up, scale, offsets, adapters, seed)
+        ctx.linear, ctx.blocks, ctx.p = linear, linear._q4, p
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, hidden, down, up, scale, offsets, adapters, seed = ctx.saved_tensors
+        need, dxb, db = ctx.needs_input_grad, None, None
+        if need[0]:
+            if ctx.linear._q4 is not ctx.blocks:
+                raise RuntimeError("the Q4_0 weights were replaced between forward and backward")
+            dxb = nat.linear_q4_0_input_grad(dy, ctx.linear._q4_operand(dy.device, True))
+        if need[3]:
+            db = nat.linear_q4_0_bias_grad(dy, ctx.bias_dtype)
+        grads = nat.lora_backward(dy, x, hidden, down, up, dxb, scale=scale, offsets=offsets,
+                                  adapters=adapters, p=ctx.p, seed=seed, need=need[:3])
+        return (*grads, db, *[None] * 6)
+
+
 class Q4Linear(nn.Linear):
     """nn.Linear whose weight may be Q4_0 blocks (load_q4_0, quantize_q4_0):
     without them nn.Linear itself; with them spc_linear_q4_0 on GPU rows of
@@ -896,9 +946,79 @@ class Q4Linear(nn.Linear):
     leave the key out).  Made for few rows: a modulation, a token.  The
     blocks are laid out by the first call and the first backward pass; a
     captured graph reads that memory, so load and drop blocks only once such
-    graphs are done with.  Capturing a backward pass: as SparseLayerNorm32."""
+    graphs are done with.  Capturing a backward pass: as SparseLayerNorm32.
+
+    add_adapters puts low-rank adapters beside the weight, whichever it is
+    (spc_lora); a call names each item's, forward(input, adapters): int32
+    [input.shape[0]] on the input's device, an item being input[i] (for
+    SparseLinear, a batch item's rows), -1 for none.  Without that argument
+    the Linear is what it is without adapters."""
 
     _q4 = None          # blocks, uint8 [out_features, in_features / 32 * 18]
+
+    def add_adapters(self, count: int, rank: int, alpha: Optional[float] = None,
+                     dropout: float = 0.0) -> None:
+        """`count` adapters of the given rank (at most 128), in place of any there
+        are: parameters adapter_down [count, rank, in_features], drawn as a Linear's
+        weight, and adapter_up [count, out_features, rank], zeros, so that they change
+        nothing yet, of the weight's dtype and device; a buffer adapter_scale [count],
+        alpha / rank (alpha: rank if not given).  All three are part of the state dict.
+        dropout: of the rows in front of the adapters, in training.  The other
+        parameters stay trainable or frozen as they are."""
+        if count < 1 or not 1 <= rank <= 128:
+            raise ValueError(f"adapters need a count of at least 1 and a rank of 1 to 128, got {count} "
+                             f"and {rank}")
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"dropout must lie in [0, 1], got {dropout}")
+        w = self.weight
+        self.drop_adapters()
+        down = torch.empty((count, rank, self.in_features), dtype=w.dtype, device=w.device)
+        if not w.is_meta:
+            nn.init.uniform_(down, -self.in_features ** -0.5, self.in_features ** -0.5)
+        self.adapter_down = nn.Parameter(down)
+        self.adapter_up = nn.Parameter(torch.zeros((count, self.out_features, rank), dtype=w.dtype,
+                                                   device=w.device))
+        self.register_buffer("adapter_scale", torch.full((count,), 1.0 if alpha is None else alpha / rank,
+                                                         dtype=torch.float32, device=w.device))
+        self.adapter_dropout = float(dropout)
+
+    def drop_adapters(self) -> None:
+        """Back to the weight alone."""
+        for name in ("adapter_down", "adapter_up", "adapter_scale"):
+            self._parameters.pop(name, None)
+            self._buffers.pop(name, None)
+
+    @property
+    def has_adapters(self) -> bool:
+        return "adapter_down" in self._parameters
+
+    def _adapted(self, x: torch.Tensor, adapters: torch.Tensor, offsets, leaf) -> torch.Tensor:
+        """The Linear of rows x [n, in_features] (of the leaf, if it is one) with
+        adapters, one for each of the offsets' items (None: of equally many rows)."""
+        if not self.has_adapters:
+            raise RuntimeError("this Linear has no adapters: call add_adapters first")
+        nat._need_gpu(leaf)
+        down, up, q4 = self.adapter_down, self.adapter_up, self._q4 is not None
+        leaves = (leaf, down, up, self.bias, None if q4 else self.weight)
+        held = _eager_leaves(*leaves) if _recorded(*leaves) else None  # (before any view or cast)
+        x = x()
+        if not x.shape[0]:  # no row meets an adapter
+            return Q4Linear.forward(self, x)
+        p = self.adapter_dropout if self.training else 0.0
+        kw = dict(scale=self.adapter_scale.float(), offsets=offsets, adapters=adapters, p=p,
+                  seed=dropout_seed(x.device) if p else None)
+        base = None
+        if not q4:
+            base = nn.functional.linear(x, self.weight, self.bias)
+            x = x.to(base.dtype)  # (autocast)
+        down, up = down.to(x.dtype), up.to(x.dtype)
+        if held is None:
+            if q4:
+                base = nat.linear_q4_0(x, self._q4_operand(x.device, False), self.bias)
+            return nat.lora(x, down, up, base, out=base, **kw)
+        if q4:
+            return _Q4LoraFn.apply(x, down, up, self.bias, self, *kw.values())
+        return _LoraFn.apply(x, down, up, base, *kw.values())
 
     def load_q4_0(self, blocks: torch.Tensor) -> None:
         """Uses Q4_0 blocks (uint8, 18 bytes each, rows [out_features,
@@ -954,7 +1074,14 @@ class Q4Linear(nn.Linear):
         else:
             super()._load_from_state_dict(state_dict, prefix, *args)
 
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: torch.Tensor, adapters: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if adapters is not None:
+            if input.dim() < 2 or adapters.shape != input.shape[:1] or \
+                    input.shape[-1] != self.in_features:
+                raise ValueError(f"expected input [n, ..., {self.in_features}] and adapters [n], got "
+                                 f"{tuple(input.shape)} and {tuple(adapters.shape)}")
+            y = self._adapted(lambda: input.reshape(-1, self.in_features), adapters, None, input)
+            return y.view(*input.shape[:-1], self.out_features)
         if self._q4 is None:
             return super().forward(input)
         nat._need_gpu(input)
@@ -972,10 +1099,17 @@ class Q4Linear(nn.Linear):
 
 
 class SparseLinear(Q4Linear):
-    """nn.Linear over the feats of a SparseTensor (SP/linear.py:9-15)."""
+    """nn.Linear over the feats of a SparseTensor (SP/linear.py:9-15); adapters,
+    if given, by batch item (rows outside the layout have none)."""
 
-    def forward(self, input: SparseTensor) -> SparseTensor:
-        return input.replace(super().forward(input.feats))
+    def forward(self, input: SparseTensor, adapters: Optional[torch.Tensor] = None) -> SparseTensor:
+        if adapters is None:
+            return input.replace(super().forward(input.feats))
+        x = input.feats
+        if x.dim() != 2 or x.shape[1] != self.in_features or adapters.shape != (input.shape[0],):
+            raise ValueError(f"expected feats [N, {self.in_features}] and adapters [{input.shape[0]}], got "
+                             f"{tuple(x.shape)} and {tuple(adapters.shape)}")
+        return input.replace(self._adapted(lambda: x, adapters, _item_offsets(input), x))
 
 
 def batch_offsets(x: SparseTensor) -> torch.Tensor:
@@ -1084,6 +1218,63 @@ class SparseLayerNorm32(nn.LayerNorm):
             return input.replace(y)
         return input.replace(nat.layer_norm(x, self.weight, self.bias, self.eps, scale=scale,
                                             shift=shift, offsets=offsets, silu=silu))
+
+
+def dropout_seed(device) -> torch.Tensor:
+    """A seed of nat.dropout's (int64 [2] on the device) from torch's generator: as
+    reproducible as its other numbers, and new in each replay of a captured graph."""
+    return torch.empty(2, dtype=torch.int64, device=device).random_()
+
+
+class _DropoutFn(torch.autograd.Function):
+    """nat.dropout; its gradient is the same call with the same seed."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, seed):
+        ctx.save_for_backward(seed)
+        ctx.p = p
+        return nat.dropout(x, p, seed, residual=residual)
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _DropoutFn.apply(dy, None, ctx.p, *ctx.saved_tensors)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None
+
+
+class SparseDropout(nn.Dropout):
+    """Dropout of the feats (spc_dropout), forward(x, residual) added to a
+    residual's feats in the same pass.  The mask is computed from a seed, in the
+    backward pass again, and never stored; the seed (dropout_seed) is what a call
+    draws, keeps for its backward pass and takes from a caller that has one (int64
+    [2] on the device).  In evaluation the feats themselves (plus the residual).
+    Differentiable any number of times; capturing a backward pass: as
+    SparseLayerNorm32."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__(p)
+
+    def forward(self, input: SparseTensor, residual: Optional[SparseTensor] = None,
+                seed: Optional[torch.Tensor] = None) -> SparseTensor:
+        x, r = input.feats, None if residual is None else residual.feats
+        if r is not None and r.shape != x.shape:
+            raise ValueError(f"residual feats must be {list(x.shape)}, got {list(r.shape)}")
+        if not self.training or self.p == 0:
+            return input if r is None else input.replace(x + r)
+        nat._need_gpu(x)
+        held = _eager_leaves(x, r) if _recorded(x, r) else None
+        if seed is None:
+            seed = dropout_seed(x.device)
+        shape = x.shape
+        if x.dim() != 2:
+            flat = (shape[0], shape[1:].numel())
+            x, r = x.reshape(flat), None if r is None else r.reshape(flat)
+        if held is not None:
+            y = _DropoutFn.apply(x, r, self.p, seed)
+        else:
+            y = nat.dropout(x, self.p, seed, residual=r)
+        return input.replace(y.view(shape))
 
 
 class SparseSiLU(nn.SiLU):

@@ -53,8 +53,10 @@ def factors(seed, rows, c, p, first=0):
 
 def adapter_of_rows(n, k, offsets=None, adapters=None):
     """int64 [n], -1 for rows without one."""
-    off = [0, n] if offsets is None else [int(v) for v in offsets]
-    ids = [0] * (len(off) - 1) if adapters is None else [int(v) for v in adapters]
+    ids = None if adapters is None else [int(v) for v in adapters]
+    items = 1 if ids is None else len(ids)
+    off = range(0, n + 1, max(n // items, 1)) if offsets is None else [int(v) for v in offsets]
+    ids = [0] * (len(off) - 1) if ids is None else ids
     of = torch.full((n,), -1, dtype=torch.int64)
     for lo, hi, a in zip(off, off[1:], ids):
         if 0 <= a < k:

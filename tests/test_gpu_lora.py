@@ -84,6 +84,19 @@ def test_items(spc, dev, dt, layout, c, o, r):
     Case(dev, dt, n, c, o, r, k=4, offsets=off, adapters=ids, p=0.2, base=False).check(spc._native)
 
 
+@pytest.mark.parametrize("n,k", [(40, 40), (7, 7), (60, 3), (2000, 4), (1, 1), (128, 64)])
+@pytest.mark.parametrize("dt", list(DT))
+def test_items_of_equal_rows(spc, dev, dt, n, k):
+    """Without offsets, as with them."""
+    nat, ids = spc._native, [(3 * i + 1) % 5 - 1 for i in range(k)]
+    q = Case(dev, dt, n, 136, 264, 16, k=4, adapters=ids, p=0.1)
+    q.check(nat)
+    y, h = nat.lora(q.x, q.down, q.up, q.base, return_hidden=True, **q.kw)
+    kw = {**q.kw, "offsets": torch.arange(0, n + 1, n // k, device=dev)}
+    y1, h1 = nat.lora(q.x, q.down, q.up, q.base, return_hidden=True, **kw)
+    assert torch.equal(y, y1) and torch.equal(h, h1)
+
+
 @pytest.mark.parametrize("dt", list(DT))
 def test_strides_and_alignment(spc, dev, dt):
     """Views at any element of wider rows, weights that are slices."""
@@ -255,7 +268,7 @@ def test_refusals(spc, dev):
     q = Case(dev, "bf16", 6, 32, 24, 4, k=2, offsets=[0, 2, 6], adapters=[0, 1], p=0.1)
     h = nat.lora(q.x, q.down, q.up, return_hidden=True, **q.kw)[1]
     kw = q.kw
-    bad = [dict(adapters=None), dict(adapters=kw["adapters"].long()), dict(offsets=None), dict(offsets=kw["offsets"][:2]),
+    bad = [dict(adapters=None), dict(adapters=kw["adapters"].long()), dict(offsets=None, adapters=torch.zeros(4, dtype=torch.int32, device=dev)), dict(offsets=kw["offsets"][:2]),
            dict(offsets=kw["offsets"].int()), dict(scale=kw["scale"][:1]), dict(scale=kw["scale"].half()),
            dict(seed=None), dict(p=2.0), dict(seed=kw["seed"].cpu())]
     for b in bad:

@@ -108,7 +108,7 @@ def test_host_validation_lora(spc):
                     dict(n_items=0), dict(n_items=65536)):
             assert run(**bad) == nat.BAD_SHAPE, bad
         for bad in (dict(dtype=nat.Q8_0), dict(p=-1.0), dict(p=float("nan")), dict(x=None), dict(down=None), dict(up=None),
-                    dict(seed=None), dict(offsets=None), dict(adapters=None), dict(offsets=fake + 4),
+                    dict(seed=None), dict(offsets=None, n_items=3), dict(adapters=None), dict(offsets=fake + 4),
                     dict(adapters=fake + 2), dict(scale=fake + 2), dict(down=fake + 1), dict(base=fake + 1), dict(bs=-1),
                     dict(ws=None), dict(ws=fake + 4), dict(wsb=0), dict(hidden=fake + 2), dict(x=fake + 1)):
             assert run(**bad) == nat.BAD_ARG, bad
@@ -135,3 +135,33 @@ def test_cpu_tensors_are_rejected(spc):
         nat.lora(x, torch.zeros(1, 4, 64), torch.zeros(1, 8, 4))
     with pytest.raises(RuntimeError, match="GPU only"):
         nat.lora_backward(torch.zeros(4, 8), x, torch.zeros(4, 4), torch.zeros(1, 4, 64), torch.zeros(1, 8, 4))
+
+
+def test_modules_without_a_gpu(spc):
+    """Construction, state and refusals need none; a call does."""
+    torch.manual_seed(1)
+    lin = spc.sparse.Q4Linear(64, 20)
+    x = torch.randn(3, 64)
+    want = lin(x)
+    assert list(lin.state_dict()) == ["weight", "bias"] and not lin.has_adapters
+    lin.add_adapters(3, 4, alpha=8, dropout=0.1)
+    assert lin.adapter_down.shape == (3, 4, 64) and lin.adapter_up.shape == (3, 20, 4)
+    assert lin.adapter_scale.tolist() == [2.0] * 3 and not lin.adapter_up.any() and lin.adapter_down.any()
+    assert torch.equal(lin(x), want)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        lin(x, torch.zeros(3, dtype=torch.int32))
+    for bad in (dict(count=0, rank=4), dict(count=1, rank=0), dict(count=1, rank=129), dict(count=1, rank=4, dropout=1.5)):
+        with pytest.raises(ValueError):
+            lin.add_adapters(**bad)
+    assert lin.has_adapters
+    lin.add_adapters(1, 2)
+    assert lin.adapter_down.shape == (1, 2, 64) and lin.adapter_scale.tolist() == [1.0]
+    lin.drop_adapters()
+    assert list(lin.state_dict()) == ["weight", "bias"]
+    t = spc.sparse.SparseTensor(x, torch.tensor([[0, i, 0, 0] for i in range(3)], dtype=torch.int32))
+    drop = spc.sparse.SparseDropout(0.5)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        drop(t)
+    assert drop.eval()(t) is t and torch.equal(drop(t, t).feats, x + x)
+    with pytest.raises(ValueError):
+        spc.sparse.SparseDropout(1.5)
