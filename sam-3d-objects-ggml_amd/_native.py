@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -1137,38 +1138,52 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, *,
     return out
 
 
-def _lora_params(x, down, up, scale, offsets, adapters, p, seed):
-    """(spc_lora_params, tensors it points into)."""
-    if down.dim() != 3 or up.dim() != 3 or down.shape[0] != up.shape[0] or \
-            down.shape[1] != up.shape[2]:
-        raise ValueError(f"down / up must be [k, rank, in] and [k, out, rank], got "
-                         f"{tuple(down.shape)} and {tuple(up.shape)}")
-    if down.dtype != x.dtype or up.dtype != x.dtype:
+def _lora_params(x, c, o, down, up, scale, offsets, adapters, p, seed):
+    """(spc_lora_params, tensors it points into, (n_items, in, out, rank)); c or o
+    None: taken from down or up."""
+    ds, us = down.shape, up.shape
+    if len(ds) != 3 or len(us) != 3 or ds[0] != us[0] or ds[1] != us[2]:
+        raise ValueError(f"down / up must be [k, rank, in] and [k, out, rank], got {tuple(ds)} and "
+                         f"{tuple(us)}")
+    (k, r, i), o_up = ds, us[1]
+    if i != c or (o is not None and o != o_up):
+        raise ValueError(f"down / up of {i} to {o_up} features do not fit the rows ({c}, {o})")
+    dt = x.dtype
+    if down.dtype is not dt or up.dtype is not dt:
         raise ValueError("down and up must have the rows' dtype")
-    (k, r, i), o = down.shape, up.shape[1]
     down, up = down.contiguous(), up.contiguous()
+    sp = op = ap = None
     if scale is not None:
-        if scale.shape != (k,) or scale.dtype != torch.float32:
+        if scale.shape != (k,) or scale.dtype is not torch.float32:
             raise ValueError(f"scale must be float32 [{k}]")
         scale = scale.contiguous()
+        sp = scale.data_ptr()
     items = 1
     if adapters is not None:
-        if adapters.dtype != torch.int32 or adapters.dim() != 1:
+        if adapters.dtype is not torch.int32 or adapters.dim() != 1:
             raise ValueError("adapters must be int32 [n_items]")
-        adapters, items = adapters.contiguous(), adapters.shape[0]
+        adapters = adapters.contiguous()
+        items, ap = adapters.shape[0], adapters.data_ptr()
     elif k != 1:
         raise ValueError("more than one adapter needs the items' adapters")
     elif offsets is not None:
         items = offsets.numel() - 1
     if offsets is not None:
-        if offsets.dtype != torch.int64 or offsets.shape != (items + 1,):
+        if offsets.dtype is not torch.int64 or offsets.shape != (items + 1,):
             raise ValueError(f"offsets must be int64 [{items + 1}]")
         offsets = offsets.contiguous()
+        op = offsets.data_ptr()
     elif not items or x.shape[0] % items:
         raise ValueError("items of unequal rows need offsets")
-    seed = _dropout_seed(p, seed)
-    keep = (down, up, scale, offsets, adapters, seed)
-    return LoraParams(*map(_ptr, keep), k, items, i, o, r, p), keep
+    if p or seed is not None:
+        seed = _dropout_seed(p, seed)
+    return (LoraParams(down.data_ptr(), up.data_ptr(), sp, op, ap, _ptr(seed), k, items, i, o_up, r, p),
+            (down, up, scale, offsets, adapters, seed), (items, i, o_up, r))
+
+
+@lru_cache(maxsize=4096)
+def _lora_workspace(dt: int, n: int, items: int, c: int, o: int, r: int, backward: int) -> int:
+    return lib().spc_lora_workspace_bytes(dt, n, items, c, o, r, backward)
 
 
 def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tensor | None = None, *,
@@ -1189,12 +1204,10 @@ def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tens
     dev = _one_device(x, down, up, base, scale, offsets, adapters, seed, out)
     dt = dtype_code(x.dtype)
     x, n, c, stride = _strided_rows(x, "x")
-    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
-    o, r, bs = q.out_features, q.rank, 0
-    if c != q.in_features:
-        raise ValueError(f"expected x [n, {q.in_features}], got {tuple(x.shape)}")
+    q, keep, (items, c, o, r) = _lora_params(x, c, None, down, up, scale, offsets, adapters, p, seed)
+    bs = 0
     if base is not None:
-        if base.shape != (n, o) or base.dtype != x.dtype:
+        if base.shape != (n, o) or base.dtype is not x.dtype:
             raise ValueError(f"base must be [{n}, {o}], of x's dtype")
         base, _, _, bs = _strided_rows(base, "base")
     if out is None:
@@ -1202,11 +1215,10 @@ def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tens
     else:
         _into(out, ((n, o), x.dtype), "x", (x, False), (base, True))
     hidden = torch.empty((n, r), dtype=torch.float32, device=dev) if return_hidden else None
-    L = lib()
-    nbytes = L.spc_lora_workspace_bytes(dt, n, q.n_items, c, o, r, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    st = _launch(L.spc_lora, dev, dt, x.data_ptr(), stride, n, q, _ptr(base), bs, out.data_ptr(),
-                 _ptr(hidden), ws.data_ptr(), nbytes)
+    nbytes = _lora_workspace(dt, n, items, c, o, r, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    st = _launch(lib().spc_lora, dev, dt, x.data_ptr(), stride, n, q, _ptr(base), bs, out.data_ptr(),
+                 _ptr(hidden), _ptr(ws), nbytes)
     if st:
         _check("spc_lora", st)
     del keep  # alive until queued
@@ -1227,28 +1239,28 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, hidden: torch.Tensor | None
     dev = _one_device(x, dy, hidden, down, up, dx_base, scale, offsets, adapters, seed)
     dt = dtype_code(x.dtype)
     x, n, c, xs = _strided_rows(x, "x")
-    q, keep = _lora_params(x, down, up, scale, offsets, adapters, p, seed)
-    o, r, bs = q.out_features, q.rank, 0
-    if c != q.in_features or dy.shape != (n, o) or dy.dtype != x.dtype:
-        raise ValueError(f"expected x [n, {q.in_features}] and dy [n, {o}] of one dtype, got "
-                         f"{tuple(x.shape)} and {tuple(dy.shape)}")
-    dy, _, _, dys = _strided_rows(dy, "dy")
+    if dy.dtype is not x.dtype or dy.dim() != 2 or dy.shape[0] != n:
+        raise ValueError(f"expected x [n, in] and dy [n, out] of one dtype, got {tuple(x.shape)} and "
+                         f"{tuple(dy.shape)}")
+    dy, _, o, dys = _strided_rows(dy, "dy")
+    q, keep, (items, c, o, r) = _lora_params(x, c, o, down, up, scale, offsets, adapters, p, seed)
     if hidden is not None:
-        if hidden.shape != (n, r) or hidden.dtype != torch.float32 or not hidden.is_contiguous():
+        if hidden.shape != (n, r) or hidden.dtype is not torch.float32 or not hidden.is_contiguous():
             raise ValueError(f"hidden must be contiguous float32 [{n}, {r}]")
     elif need[2]:
         raise ValueError("the gradient of up needs the hidden rows")
+    bs = 0
     if dx_base is not None:
-        if dx_base.shape != x.shape or dx_base.dtype != x.dtype:
+        if dx_base.shape != (n, c) or dx_base.dtype is not x.dtype:
             raise ValueError("dx_base must have x's shape and dtype")
         dx_base, _, _, bs = _strided_rows(dx_base, "dx_base")
     dx = x.new_empty((n, c)) if need[0] else None
-    ddown, dup = (torch.empty_like(t) if k else None for t, k in zip(keep[:2], need[1:]))
-    L = lib()
-    nbytes = L.spc_lora_workspace_bytes(dt, n, q.n_items, c, o, r, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    st = _launch(L.spc_lora_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs, _ptr(hidden), n,
-                 q, _ptr(dx_base), bs, _ptr(dx), _ptr(ddown), _ptr(dup), ws.data_ptr(), nbytes)
+    ddown = torch.empty_like(keep[0]) if need[1] else None
+    dup = torch.empty_like(keep[1]) if need[2] else None
+    nbytes = _lora_workspace(dt, n, items, c, o, r, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    st = _launch(lib().spc_lora_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs, _ptr(hidden), n,
+                 q, _ptr(dx_base), bs, _ptr(dx), _ptr(ddown), _ptr(dup), _ptr(ws), nbytes)
     if st:
         _check("spc_lora_backward", st)
     del keep  # alive until queued

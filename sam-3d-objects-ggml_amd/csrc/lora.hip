@@ -195,7 +195,7 @@ size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t i
         const LoraPlan f = lora_plan(dtype, n, n_items, in_features, out_features, rank);
         if (f.mode == kLoraShrink) floats = (size_t)f.splits * n * rank;
     }
-    return std::max<size_t>(floats, 4) * sizeof(float);
+    return floats * sizeof(float);
 }
 
 int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
@@ -214,8 +214,8 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
         set_last_error("%s: null or misaligned pointer, or a negative stride", fn);
         return SPC_BAD_ARG;
     }
-    if (!workspace || off(workspace, 16) ||
-        workspace_bytes < spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 0)) {
+    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 0);
+    if (need && (!workspace || off(workspace, 16) || workspace_bytes < need)) {
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
@@ -274,8 +274,8 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         return SPC_BAD_ARG;
     }
     if (!dx && !ddown && !dup) return SPC_OK;
-    if (!workspace || off(workspace, 16) ||
-        workspace_bytes < spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 1)) {
+    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 1);
+    if (need && (!workspace || off(workspace, 16) || workspace_bytes < need)) {
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }

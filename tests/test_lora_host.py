@@ -110,17 +110,20 @@ def test_host_validation_lora(spc):
         for bad in (dict(dtype=nat.Q8_0), dict(p=-1.0), dict(p=float("nan")), dict(x=None), dict(down=None), dict(up=None),
                     dict(seed=None), dict(offsets=None, n_items=3), dict(adapters=None), dict(offsets=fake + 4),
                     dict(adapters=fake + 2), dict(scale=fake + 2), dict(down=fake + 1), dict(base=fake + 1), dict(bs=-1),
-                    dict(ws=None), dict(ws=fake + 4), dict(wsb=0), dict(hidden=fake + 2), dict(x=fake + 1)):
+                    dict(hidden=fake + 2), dict(x=fake + 1)):
             assert run(**bad) == nat.BAD_ARG, bad
     assert fwd(y=None) == fwd(y=fake + 1) == nat.BAD_ARG
     assert bwd(dy=None) == bwd(hidden=None) == bwd(dys=-1) == bwd(du=fake + 1) == nat.BAD_ARG
-    for b in (0, 1):
-        need = L.spc_lora_workspace_bytes(nat.BF16, 1000, 2, 64, 48, 8, b)
+    # few wide rows: the forward pass in two kernels; the backward pass's shares
+    for b, n, wide in ((0, 8, 8192), (1, 5000, 64)):
+        need = L.spc_lora_workspace_bytes(nat.BF16, n, 2, wide, 48, 64, b)
         assert need > 0
-        assert (fwd, bwd)[b](n=1000, wsb=need - 1) == nat.BAD_ARG
+        kw = dict(n=n, in_features=wide, rank=64, **({"xs": wide} if b == 0 else {}))
+        for bad in (dict(wsb=need - 1), dict(ws=None), dict(ws=fake + 4)):
+            assert (fwd, bwd)[b](**kw, **bad) == nat.BAD_ARG
     assert b"workspace" in L.spc_last_error()
     for items in (1, 7, 65535):  # no rows: an answer, not a division
-        assert all(L.spc_lora_workspace_bytes(nat.F16, 0, items, 64, 48, 8, b) > 0 for b in (0, 1))
+        assert all(L.spc_lora_workspace_bytes(nat.F16, 0, items, 64, 48, 8, b) >= 0 for b in (0, 1))
     assert L.spc_lora_workspace_bytes(nat.BF16, 4, 1, 64, 48, 129, 0) == 0
     assert L.spc_lora_workspace_bytes(nat.Q8_0, 4, 1, 64, 48, 8, 0) == 0
     assert L.spc_lora_workspace_bytes(nat.BF16, 4, 0, 64, 48, 8, 1) == 0
