@@ -106,6 +106,8 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
 }
 
 struct LoraBackPlan {
+    bool few;                   // lora_few.hip, u in `shares` of o_per outputs
+    int shares, o_per;
     int rows_o, rows_c;         // rows of a chunk
     int64_t chunks_o, chunks_c, blocks_o, blocks_c;
     int64_t slot_o, slot_c;     // floats
@@ -114,6 +116,16 @@ struct LoraBackPlan {
 
 LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
     LoraBackPlan q{};
+    q.few = n <= 32 * items;
+    if (q.few) {
+        int64_t chunks = 1;
+        while (chunks * (dt == SPC_F32 ? 4 : 8) < r) chunks *= 2;
+        const int64_t lines = kLoraThreads / chunks;
+        q.shares = (int)std::min({(int64_t)8, ceil_div(o, lines * 8), std::max<int64_t>(1, 128 / std::max<int64_t>(n, 1))});
+        q.o_per = (int)ceil_div(o, q.shares);
+        q.u = (size_t)(q.shares * n * r);
+        return q;
+    }
     const int64_t cols = 4 / lora_rank_waves(r) * lora_wave_cols(dt);
     q.blocks_o = ceil_div(o, cols);
     q.blocks_c = ceil_div(c, cols);
@@ -293,7 +305,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     p.bs = dx_base_stride;
     p.dx = dx;
     p.u = dx || ddown ? ws : nullptr;
-    p.u_parts = (int)b.blocks_o;
+    p.u_parts = b.few ? b.shares : (int)b.blocks_o;
     p.pu = dup ? ws + lora_round_up(b.u) : nullptr;
     p.pd = ddown ? ws + lora_round_up(b.u) + lora_round_up(b.pu) : nullptr;
     p.c = (int)q.in_features;
@@ -304,6 +316,10 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     hipError_t err = hipSuccess;
     if (lora_small(p.c, p.o)) {
         err = lora_small_backward(s, dtype, p, ddown, dup);
+        return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
+    }
+    if (b.few) {
+        err = lora_few_backward(s, dtype, p, b.o_per, ddown, dup);
         return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
     }
     if (n > 0) {

@@ -133,6 +133,10 @@ inline int lora_rank_waves(int64_t r) { return r <= 32 ? 1 : r <= 64 ? 2 : 4; }
 // columns of one such wave
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
 
+
+// The gradients of few rows (lora_few.hip); u in u_parts shares of o_per outputs.
+hipError_t lora_few_backward(hipStream_t s, int dt, const LoraBackArgs& p, int o_per, void* ddown, void* dup);
+
 // ---------------------------------------------------------------------------
 // operands
 // ---------------------------------------------------------------------------
