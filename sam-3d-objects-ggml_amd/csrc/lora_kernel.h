@@ -401,6 +401,20 @@ __device__ __forceinline__ int lora_col(int col, int t, int m) {
     else return col + 8 * (m >> 2) + 4 * t + (m & 3);
 }
 
+// Lanes 8 apart exchange one of two words: lora_mma's layout of two steps of columns
+// (V columns from V (lane / 16) on of row lane % 16, the first step's in a, the second's
+// in b) becomes eight lanes a row, rows 0 to 7 in a and 8 to 15 in b, and back.
+__device__ __forceinline__ void lora_turn_pair(u32x4& a, u32x4& b) {
+    const bool high = threadIdx.x & 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t mine = high ? a[q] : b[q];
+        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0x128, 0xf, 0xf, true);  // lane ^ 8
+        a[q] = high ? other : a[q];
+        b[q] = high ? b[q] : other;
+    }
+}
+
 // Stores a tile of 16 rows x 2 STEP columns whose results lie as lora_mma leaves
 // them, rows below m of it: a lane has V columns from V (lane / 16) on of row lane %
 // 16, of the first step in a and of the second in b.  Eight lanes a row take 128
@@ -410,20 +424,21 @@ template <typename S>
 __device__ __forceinline__ void lora_store_pair(S* at, int64_t stride, u32x4 a, u32x4 b, int m) {
     constexpr int V = 16 / (int)sizeof(S);
     const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4;
-    const bool high = n16 & 8;
-    u32x4 first, second;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const uint32_t mine = high ? a[q] : b[q];
-        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0x128, 0xf, 0xf, true);  // lane ^ 8
-        first[q] = high ? other : a[q];
-        second[q] = high ? b[q] : other;
-    }
-    S* q = at + (n16 & 7) * stride + V * g + (high ? 4 * V : 0);
-    if ((n16 & 7) < m) __builtin_nontemporal_store(first, reinterpret_cast<u32x4_rows*>(q));
-    if ((n16 & 7) + 8 < m) __builtin_nontemporal_store(second, reinterpret_cast<u32x4_rows*>(q + 8 * stride));
+    lora_turn_pair(a, b);
+    S* q = at + (n16 & 7) * stride + V * g + (n16 & 8 ? 4 * V : 0);
+    if ((n16 & 7) < m) __builtin_nontemporal_store(a, reinterpret_cast<u32x4_rows*>(q));
+    if ((n16 & 7) + 8 < m) __builtin_nontemporal_store(b, reinterpret_cast<u32x4_rows*>(q + 8 * stride));
 }
 
+// Such a tile's elements, rows past m as the last (lora_turn_pair for lora_mma's layout).
+template <typename S>
+__device__ __forceinline__ void lora_fetch_pair(u32x4& first, u32x4& second, const S* at, int64_t stride, int m) {
+    constexpr int V = 16 / (int)sizeof(S);
+    const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4, row = n16 & 7;
+    const S* q = at + V * g + (n16 & 8 ? 4 * V : 0);
+    first = *reinterpret_cast<const u32x4_rows*>(q + min(row, m - 1) * stride);
+    second = *reinterpret_cast<const u32x4_rows*>(q + min(row + 8, m - 1) * stride);
+}
 struct LoraTile {
     int64_t row0, a;
     int m;  // rows
@@ -522,11 +537,19 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
 #pragma unroll
                 for (int k = 0; k < K::STEPS; ++k) wr[x][q][k] = lora_fetch_short(up, at + K::rank(k, g), all);
             }
-            if (p.base)
+        }
+        if (p.base) {
+            const S* base = static_cast<const S*>(p.base) + t.row0 * p.bs;
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    b[x][i] = lora_fetch(static_cast<const S*>(p.base) + (t.row0 + min(16 * i + n16, t.m - 1)) * p.bs,
-                                         cb + x * N::STEP + V * g, p.o);
+            for (int i = 0; i < MT; ++i) {
+                if (!edge) {
+                    lora_fetch_pair(b[0][i], b[1][i], base + min(16 * i, t.m - 1) * p.bs + cb, p.bs, max(t.m - 16 * i, 1));
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        b[x][i] = lora_fetch(base + min(16 * i + n16, t.m - 1) * p.bs, cb + x * N::STEP + V * g, p.o);
+                }
+            }
         }
         if (p.r < 16 * RT)
 #pragma unroll
@@ -538,11 +561,16 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
                     for (int k = 0; k < K::STEPS; ++k)
                         wr[x][q][k] = lora_edge_short<S>(wr[x][q][k], at + K::rank(k, g), all, p.r - K::rank(k, g));
                 }
-        if (p.base && edge)
+        if (p.base)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int i = 0; i < MT; ++i) {
+                if (!edge) {
+                    lora_turn_pair(b[0][i], b[1][i]);
+                } else {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) b[x][i] = lora_edge<S>(b[x][i], cb + x * N::STEP + V * g, p.o);
+                    for (int x = 0; x < 2; ++x) b[x][i] = lora_edge<S>(b[x][i], cb + x * N::STEP + V * g, p.o);
+                }
+            }
         u32x4 out[2][MT];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -971,15 +999,22 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
             }
         };
         auto load_base = [&](int64_t row0, int n16, int g) {
+            const int rows = (int)min(r1 - row0, (int64_t)kLoraRows);
+            const S* from = static_cast<const S*>(p.base) + row0 * p.bs;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int64_t row = min(row0 + 16 * i + n16, r1 - 1);
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int q = 0; q < QN; ++q) {
-                    const int col = col0 + (wr * QN + q) * N::STEP + V * g;
-                    base[i][q] = lora_fetch(static_cast<const S*>(p.base) + row * p.bs, col, p.c);
+                for (int q = 0; q < QN; q += QP) {
+                    const int col = col0 + (wr * QN + q) * N::STEP;
+                    if (QP == 2 && !edge) {
+                        lora_fetch_pair(base[i][q], base[i][q + QP - 1], from + min(16 * i, rows - 1) * p.bs + col, p.bs,
+                                        max(rows - 16 * i, 1));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < QP; ++x)
+                            base[i][q + x] = lora_fetch(from + min(16 * i + n16, rows - 1) * p.bs, col + x * N::STEP + V * g, p.c);
+                    }
                 }
-            }
         };
         load_u(r0);
         if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
@@ -1037,12 +1072,18 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 raw = next;
             }
             if (p.dx) {
-                if (p.base && edge)
+                if (p.base && edge) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int q = 0; q < QN; ++q)
                             base[i][q] = lora_edge<S>(base[i][q], col0 + (wr * QN + q) * N::STEP + V * g, p.c);
+                } else if (p.base && QP == 2) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < QN; q += QP) lora_turn_pair(base[i][q], base[i][q + QP - 1]);
+                }
                 typename K::H h[2];
                 if constexpr (RT < 8) {
                     h[0].load(f + n16 * P, g);
