@@ -129,7 +129,7 @@ hipError_t lora_small_backward(hipStream_t s, int dt, const LoraBackArgs& p, voi
 inline int lora_rank_tiles(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
 constexpr int kLoraRowTiles = 2;
 // waves of a block along the ranks in the backward kernels (the others along columns)
-inline int lora_rank_waves(int64_t r) { return r <= 32 ? 1 : r <= 64 ? 2 : 4; }
+inline int lora_rank_waves(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 // columns of one such wave
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
 
@@ -712,43 +712,61 @@ hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3
 // V (l % 16) on (16 bytes a row).  That is the row operand of the weights'
 // gradients (columns by summed rows; 16-bit elements are exchanged between the
 // lane's registers to bring a column's eight rows together), whose sums stay in
-// registers until the chunk or the segment ends.  Waves stand along the columns
-// and, from rank 33 on, along ranks of 32 each.
+// registers until the chunk or the segment ends.  WC waves stand along the columns
+// and WR along the ranks (16 RW each): those of the same columns load, and mask, a
+// share of the rows each and pass them on through LDS.
 constexpr int kLoraRows = 32;
 
-template <int DT>
-struct LoraRaw {
-    u32x4 v[8];
+// NR of a lane's eight rows, from j0 on.
+template <int DT, int NR>
+struct LoraRows {
+    u32x4 v[NR];
     // Rows row0 + 8 g on, from `col` on (lora_fetch; rows past `end` are its last).
-    __device__ __forceinline__ void load(const void* base, int64_t stride, int64_t row0, int64_t end, int col, int c) {
+    __device__ __forceinline__ void load(const void* base, int64_t stride, int64_t row0, int64_t end, int j0, int col,
+                                         int c) {
         using S = typename LoraNum<DT>::S;
         if (row0 >= end) return;
-        const int g8 = (threadIdx.x & 63) / 16 * 8;
+        const int first = (threadIdx.x & 63) / 16 * 8 + j0;
         if (row0 + kLoraRows <= end) {
-            const S* q = static_cast<const S*>(base) + (row0 + g8) * stride;
+            const S* q = static_cast<const S*>(base) + (row0 + first) * stride;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < NR; ++j) {
                 v[j] = lora_fetch(q, col, c);
                 q += stride;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[j] = lora_fetch(static_cast<const S*>(base) + min(row0 + g8 + j, end - 1) * stride, col, c);
+            for (int j = 0; j < NR; ++j)
+                v[j] = lora_fetch(static_cast<const S*>(base) + min(row0 + first + j, end - 1) * stride, col, c);
         }
     }
     // Zeros for what is past the end of the rows, and, at the row's end, of the columns.
-    __device__ __forceinline__ void trim(int64_t row0, int64_t end, bool edge, int col, int c) {
+    __device__ __forceinline__ void trim(int64_t row0, int64_t end, int j0, bool edge, int col, int c) {
         using S = typename LoraNum<DT>::S;
         if (row0 + kLoraRows > end) {
-            const int rows = (int)(end - row0) - (threadIdx.x & 63) / 16 * 8;
+            const int rows = (int)(end - row0) - ((threadIdx.x & 63) / 16 * 8 + j0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < NR; ++j)
                 if (j >= rows) v[j] = u32x4{0, 0, 0, 0};
         }
         if (edge)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = lora_edge<S>(v[j], col, c);
+            for (int j = 0; j < NR; ++j) v[j] = lora_edge<S>(v[j], col, c);
+    }
+    // A tile of rows `pitch` apart in LDS.
+    template <typename S>
+    __device__ __forceinline__ void put(S* tile, int pitch, int j0) const {
+        const int lane = threadIdx.x & 63;
+        S* q = tile + (8 * (lane >> 4) + j0) * pitch + LoraNum<DT>::V * (lane & 15);
+#pragma unroll
+        for (int j = 0; j < NR; ++j) *reinterpret_cast<u32x4*>(q + j * pitch) = v[j];
+    }
+    template <typename S>
+    __device__ __forceinline__ void get(const S* tile, int pitch) {
+        const int lane = threadIdx.x & 63;
+        const S* q = tile + 8 * (lane >> 4) * pitch + LoraNum<DT>::V * (lane & 15);
+#pragma unroll
+        for (int j = 0; j < NR; ++j) v[j] = *reinterpret_cast<const u32x4*>(q + j * pitch);
     }
     // column e's eight rows (16-bit elements)
     __device__ __forceinline__ u32x4 column(int e) const {
@@ -762,7 +780,7 @@ struct LoraRaw {
 
 // acc[e][j] += rows of column e times F32 values b[j][row] (rank tile j).
 template <int DT, int RW>
-__device__ __forceinline__ void lora_outer(const LoraRaw<DT>& raw, const float (&b)[RW][8],
+__device__ __forceinline__ void lora_outer(const LoraRows<DT, 8>& raw, const float (&b)[RW][8],
                                            floatx4 (&acc)[LoraNum<DT>::V][RW]) {
     if constexpr (DT == SPC_F32) {
 #pragma unroll
@@ -814,38 +832,40 @@ __device__ __forceinline__ void lora_wave_sync() {
 }
 
 // The pass over dy: u of the block's columns (one of u_parts shares of the sum),
-// and the sums of dup.  RW: rank tiles of a wave, WR: waves along the ranks.
-// u sums along a row, so its operand is read back from the wave's tile in LDS,
-// and the waves' shares meet there too, in the tiles' place; the adapter's columns
-// lie in LDS by rank.
+// and the sums of dup.  u sums along a row, so its operand is read back from the
+// tile in LDS, and the waves' shares meet there too; the adapter's columns lie in
+// LDS by rank.
 template <int DT, int RW, int WR>
 __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBackArgs p) {
     using N = LoraNum<DT>;
     using S = typename N::S;
     constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RW * WR, P = lora_pitch(16 * RW);
-    constexpr int TP = CW + V, WP = CB + V;  // pitches of a wave's tile and of the weights
-    __shared__ __attribute__((aligned(16))) S tile[4][kLoraRows * TP];
+    constexpr int TP = CW + V, WP = CB + V;  // pitches of a tile and of the weights
+    constexpr int NR = 8 / WR;               // rows a lane loads
+    __shared__ __attribute__((aligned(16))) S tile[WC][kLoraRows * TP];
     __shared__ __attribute__((aligned(16))) S wl[RP * WP];
-    static_assert(kLoraRows * P * sizeof(float) <= sizeof(tile[0]), "a wave's share of u in its tile's place");
+    __shared__ __attribute__((aligned(16))) float red[2][4][kLoraRows * P];
     const LoraItems& it = p.it;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
-    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
-    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW, mine = col0 + V * n16;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr, j0 = NR * wr;
+    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.o;
     const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     floatx4 acc[V][RW] = {};
+    int turn = 0;
     for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
         const int64_t b0 = it.begin(v);
         if (b0 >= hi) break;
         const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
         if (r0 >= r1 || a < 0) continue;
         const float s = p.scale ? p.scale[a] : 1.0f;
-        LoraRaw<DT> raw;
+        LoraRows<DT, NR> rows;
         float h[RW][8];
         // a tile's hidden rows, a wave's ranks: one tile ahead as dy is, and before it
         // (loads return in order)
         auto load_h = [&](int64_t row0, float (&h)[RW][8]) {
             if (!p.pu || row0 >= r1) return;
+            const int n16 = lane & 15, g = lane >> 4;
             const bool full = row0 + kLoraRows <= r1;
 #pragma unroll
             for (int j = 0; j < RW; ++j)
@@ -856,7 +876,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                 }
         };
         load_h(r0, h);
-        raw.load(p.dy, p.dys, r0, r1, mine, p.o);
+        rows.load(p.dy, p.dys, r0, r1, j0, col0 + V * (lane & 15), p.o);
         if (p.u) {
             const S* up = static_cast<const S*>(p.up);
             const int64_t all = it.adapters * p.o * p.r;
@@ -879,16 +899,21 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
-            LoraRaw<DT> next = raw;
+            const S* t = tile[wc];
+            LoraRows<DT, 8> raw;
+            rows.trim(row0, r1, j0, edge, mine, p.o);
+            if (p.u || WR > 1) rows.put(tile[wc], TP, j0);
+            if constexpr (WR == 1) {
+                raw = rows;
+                lora_wave_sync();
+            } else {
+                lds_barrier();
+            }
             float hn[RW][8];
             load_h(row0 + kLoraRows, hn);
-            next.load(p.dy, p.dys, row0 + kLoraRows, r1, mine, p.o);
-            raw.trim(row0, r1, edge, mine, p.o);
+            rows.load(p.dy, p.dys, row0 + kLoraRows, r1, j0, mine, p.o);
+            if constexpr (WR > 1) raw.get(t, TP);
             if (p.u) {
-                S* t = tile[w];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) *reinterpret_cast<u32x4*>(t + (8 * g + j) * TP + V * n16) = raw.v[j];
-                lora_wave_sync();
                 floatx4 u[2][RW] = {};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -904,23 +929,25 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                         for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[j], d, u[i][j]);
                     }
                 }
-                lora_wave_sync();
-                float* f = reinterpret_cast<float*>(t);
+                float* f = red[turn][w];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < RW; ++j)
                         *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + 16 * j + 4 * g) = u[i][j];
-                lds_barrier();
-                // (the waves of a rank group stand WC apart)
+            }
+            // (also: the tile has been read; red is not written again before the next one)
+            if (p.u || WR > 1) lds_barrier();
+            if (p.u) {
+                // (the waves of a rank group stand together)
                 for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
                     const int m = i / RP, j = i % RP;
                     float z = 0.0f;
 #pragma unroll
-                    for (int q = 0; q < WC; ++q)
-                        z += reinterpret_cast<const float*>(tile[j / (16 * RW) * WC + q])[m * P + j % (16 * RW)];
+                    for (int q = 0; q < WC; ++q) z += red[turn][j / (16 * RW) * WC + q][m * P + j % (16 * RW)];
                     if (row0 + m < r1 && j < p.r) p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
                 }
+                turn ^= 1;
             }
             if (p.pu) {
                 if (row0 + kLoraRows > r1)
@@ -935,12 +962,22 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
 #pragma unroll
                     for (int i = 0; i < 8; ++i) h[j][i] = hn[j][i];
             }
-            raw = next;
-            if (p.u) lds_barrier();
         }
         if (p.pu && col0 < p.o)
             lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
     }
+}
+
+// u's shares, where there are more than two: their sum in the first one's place.
+constexpr int kLoraShares = 2;
+__global__ __launch_bounds__(kLoraThreads) static void lora_add_u_kernel(float* u, int64_t n, int parts) {
+    for (int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kLoraThreads * 4)
+        for (int e = 0; e < 4 && i + e < n; ++e) {
+            float s = u[i + e];
+#pragma unroll 4
+            for (int q = 1; q < parts; ++q) s += u[q * n + i + e];
+            u[i + e] = s;
+        }
 }
 
 // The pass over x: dx of the block's columns and the sums of ddown.  The
@@ -952,19 +989,24 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     constexpr int RT = RW * WR;
     using K = LoraRanks<DT, RT>;
     constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RT, P = lora_pitch(RP), T = V / 4;
-    constexpr int WP = RP + V;       // pitch of the weights
-    constexpr int QN = 4 / WR, QP = QN > 1 ? 2 : 1;  // steps of columns whose dx the wave forms, at a time
-    constexpr int G = CW / 8;        // groups of eight columns
+    constexpr int TP = CW + V, WP = RP + V;  // pitches of a tile and of the weights
+    constexpr int NR = 8 / WR;               // rows a lane loads
+    constexpr int BUF = RT == 8 ? 1 : 2;     // (room for two blocks a CU)
+    // of the 4 steps of columns x 2 halves of rows of dx, a wave forms QN x NI
+    constexpr int QN = WR == 1 ? 4 : 2, NI = WR == 4 ? 1 : 2;
+    constexpr int G = CW / 8;                // groups of eight columns
     constexpr int NU = kLoraRows * RP / kLoraThreads;  // values of u a thread
-    __shared__ __attribute__((aligned(16))) float ub[2][kLoraRows * P];
+    __shared__ __attribute__((aligned(16))) float ub[BUF][kLoraRows * P];
     __shared__ __attribute__((aligned(16))) S wl[CB * WP];
-    __shared__ uint8_t keep[DROP ? 4 : 1][kLoraRows * G];
+    __shared__ __attribute__((aligned(16))) S tile[WR > 1 ? BUF : 1][WR > 1 ? WC : 1][WR > 1 ? kLoraRows * TP : 8];
+    __shared__ uint8_t kept[DROP ? BUF : 1][DROP ? WC : 1][kLoraRows * G];
     const LoraItems& it = p.it;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n16 = lane & 15, g = lane >> 4;
-    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr;
-    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW, mine = col0 + V * n16;
-    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr, j0 = NR * wr;
+    const int q0 = WR == 1 ? 0 : WR == 2 ? 2 * wr : wr / 2 * 2, i0 = WR == 4 ? wr & 1 : 0;
+    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.c;
+    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
     floatx4 acc[V][RW] = {};
     int turn = 0;
@@ -980,10 +1022,10 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                                   min(block0 + CB, p.c));
             continue;
         }
-        LoraRaw<DT> raw = {};
-        u32x4 base[2][QN] = {};
+        LoraRows<DT, NR> rows = {};
+        u32x4 base[NI][QN] = {};
         float un[2][NU];
-        // the tile's rows of u (two shares, the first of which takes the rest), and of dx_base
+        // the tile's rows of u (one share or two), and of dx_base
         auto load_u = [&](int64_t row0) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
@@ -991,36 +1033,34 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 un[0][i] = un[1][i] = 0.0f;
                 if (row0 + m < r1 && j < p.r) {
                     const float* q = p.u + (row0 + m) * p.r + j;
-                    const int64_t part = it.n * p.r;
                     un[0][i] = q[0];
-                    if (p.u_parts > 1) un[1][i] = q[part];
-                    for (int k = 2; k < p.u_parts; ++k) un[0][i] += q[k * part];
+                    if (p.u_parts > 1) un[1][i] = q[it.n * p.r];
                 }
             }
         };
         auto load_base = [&](int64_t row0, int n16, int g) {
-            const int rows = (int)min(r1 - row0, (int64_t)kLoraRows);
+            const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
             const S* from = static_cast<const S*>(p.base) + row0 * p.bs;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int q = 0; q < QN; q += QP) {
-                    const int col = col0 + (wr * QN + q) * N::STEP;
-                    if (QP == 2 && !edge) {
-                        lora_fetch_pair(base[i][q], base[i][q + QP - 1], from + min(16 * i, rows - 1) * p.bs + col, p.bs,
-                                        max(rows - 16 * i, 1));
+                for (int q = 0; q < QN; q += 2) {
+                    const int col = col0 + (q0 + q) * N::STEP, first = 16 * (i0 + i);
+                    if (!edge) {
+                        lora_fetch_pair(base[i][q], base[i][q + 1], from + min(first, m - 1) * p.bs + col, p.bs,
+                                        max(m - first, 1));
                     } else {
 #pragma unroll
-                        for (int x = 0; x < QP; ++x)
-                            base[i][q + x] = lora_fetch(from + min(16 * i + n16, rows - 1) * p.bs, col + x * N::STEP + V * g, p.c);
+                        for (int x = 0; x < 2; ++x)
+                            base[i][q + x] = lora_fetch(from + min(first + n16, m - 1) * p.bs, col + x * N::STEP + V * g, p.c);
                     }
                 }
         };
         load_u(r0);
-        if (p.pd) raw.load(p.x, p.xs, r0, r1, mine, p.c);
+        if (p.pd) rows.load(p.x, p.xs, r0, r1, j0, col0 + V * (lane & 15), p.c);
+        lds_barrier();
         if (p.dx) {
             const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
-            lds_barrier();
             for (int i = threadIdx.x; i < RP * (CB / V); i += kLoraThreads) {
                 const int j = i % RP, k = i / RP * V, col = block0 + k;
                 const u32x4 w = lora_load(down + (int64_t)min(j, p.r - 1) * p.c, col, p.c);
@@ -1039,70 +1079,74 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
             asm volatile("" : "+v"(ln));
             const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
             float* f = ub[turn];
-            turn ^= 1;
+            S* t = tile[WR > 1 ? turn : 0][WR > 1 ? wc : 0];
+            uint8_t* keep = kept[DROP ? turn : 0][DROP ? wc : 0];
+            turn = BUF == 2 ? turn ^ 1 : 0;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
                 f[m * P + j] = un[0][i] + un[1][i];
             }
             // (loads return in order: u, wanted first, before dx_base and the next rows)
-            LoraRaw<DT> next = raw;
             load_u(row0 + kLoraRows);
             if (p.dx && p.base) load_base(row0, n16, g);
+            LoraRows<DT, 8> raw;
+            LoraRows<DT, NR> now = rows;
             if (p.pd) {
-                next.load(p.x, p.xs, row0 + kLoraRows, r1, mine, p.c);
-                raw.trim(row0, r1, edge, mine, p.c);
+                rows.load(p.x, p.xs, row0 + kLoraRows, r1, j0, mine, p.c);
+                now.trim(row0, r1, j0, edge, mine, p.c);
             }
             if (DROP) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const u32x4 ones = lora_ones(key, p.drop, row0 + 8 * g + i, mine, p.c);
-                    raw.v[i] = lora_masked<DT>(raw.v[i], ones, mine);
-                    if (V == 8 || !(n16 & 1)) keep[w][(8 * g + i) * G + n16 * V / 8] = (uint8_t)drop_bits(ones);
+                for (int i = 0; i < NR; ++i) {
+                    const u32x4 ones = lora_ones(key, p.drop, row0 + 8 * g + j0 + i, mine, p.c);
+                    now.v[i] = lora_masked<DT>(now.v[i], ones, mine);
+                    if (V == 8 || !(n16 & 1)) keep[(8 * g + j0 + i) * G + n16 * V / 8] = (uint8_t)drop_bits(ones);
                 }
             }
+            if constexpr (WR == 1) raw = now;
+            else if (p.pd) now.put(t, TP, j0);
             lds_barrier();
             if (p.pd) {
+                if constexpr (WR > 1) raw.get(t, TP);
                 float b[RW][8];
 #pragma unroll
                 for (int j = 0; j < RW; ++j)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
                 lora_outer<DT, RW>(raw, b, acc);
-                raw = next;
             }
             if (p.dx) {
-                if (p.base && edge) {
+                if (p.base)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int i = 0; i < NI; ++i)
 #pragma unroll
-                        for (int q = 0; q < QN; ++q)
-                            base[i][q] = lora_edge<S>(base[i][q], col0 + (wr * QN + q) * N::STEP + V * g, p.c);
-                } else if (p.base && QP == 2) {
+                        for (int q = 0; q < QN; q += 2) {
+                            if (!edge) {
+                                lora_turn_pair(base[i][q], base[i][q + 1]);
+                            } else {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                                for (int x = 0; x < 2; ++x)
+                                    base[i][q + x] =
+                                        lora_edge<S>(base[i][q + x], col0 + (q0 + q + x) * N::STEP + V * g, p.c);
+                            }
+                        }
+                typename K::H h[NI];
 #pragma unroll
-                        for (int q = 0; q < QN; q += QP) lora_turn_pair(base[i][q], base[i][q + QP - 1]);
-                }
-                typename K::H h[2];
-                if constexpr (RT < 8) {
-                    h[0].load(f + n16 * P, g);
-                    h[1].load(f + (16 + n16) * P, g);
-                }
-                const int rows = (int)min(r1 - row0, (int64_t)kLoraRows);
-                S* d = static_cast<S*>(p.dx) + row0 * p.c + col0 + wr * QN * N::STEP;
+                for (int i = 0; i < NI; ++i) h[i].load(f + (16 * (i0 + i) + n16) * P, g);
+                const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
+                S* d = static_cast<S*>(p.dx) + row0 * p.c + col0 + q0 * N::STEP;
 #pragma unroll
-                for (int q = 0; q < QN; q += QP) {
-                    u32x4 out[2][QP];
+                for (int q = 0; q < QN; q += 2) {
+                    u32x4 out[NI][2];
 #pragma unroll
-                    for (int x = 0; x < QP; ++x) {
-                        const int at = (wr * QN + q + x) * N::STEP;
+                    for (int x = 0; x < 2; ++x) {
+                        const int at = (q0 + q + x) * N::STEP;
                         typename K::W wt[T];
 #pragma unroll
                         for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            if constexpr (RT == 8) h[i].load(f + (16 * i + n16) * P, g);
+                        for (int i = 0; i < NI; ++i) {
                             float z[V];
 #pragma unroll
                             for (int k = 0; k < T; ++k) {
@@ -1112,8 +1156,8 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                                 for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
                             }
                             if (DROP) {
-                                const uint32_t bits =
-                                    keep[w][(16 * i + n16) * G + (at + V * g) / 8] >> (V == 8 ? 0 : 2 * (g & 1));
+                                const uint32_t bits = keep[(16 * (i0 + i) + n16) * G + (at + V * g) / 8] >>
+                                                      (V == 8 ? 0 : 2 * (g & 1));
 #pragma unroll
                                 for (int e = 0; e < V; ++e)
                                     z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
@@ -1125,22 +1169,23 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        S* t = d + (int64_t)16 * i * p.c + q * N::STEP;
-                        if (QP == 2 && !edge) {
-                            lora_store_pair(t, p.c, out[i][0], out[i][QP - 1], rows - 16 * i);
+                    for (int i = 0; i < NI; ++i) {
+                        S* to = d + (int64_t)16 * (i0 + i) * p.c + q * N::STEP;
+                        const int left = m - 16 * (i0 + i);
+                        if (!edge) {
+                            lora_store_pair(to, p.c, out[i][0], out[i][1], left);
                         } else {
 #pragma unroll
-                            for (int x = 0; x < QP; ++x) {
+                            for (int x = 0; x < 2; ++x) {
                                 const int at = x * N::STEP + V * g;
-                                if (16 * i + n16 < rows)
-                                    lora_store(t + n16 * (int64_t)p.c + at, out[i][x],
-                                               p.c - col0 - (wr * QN + q) * N::STEP - at);
+                                if (n16 < left)
+                                    lora_store(to + n16 * (int64_t)p.c + at, out[i][x], p.c - col0 - (q0 + q) * N::STEP - at);
                             }
                         }
                     }
                 }
             }
+            if (BUF == 1) lds_barrier();
         }
         if (p.pd && col0 < p.c)
             lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
@@ -1152,9 +1197,13 @@ template <int DT>
 hipError_t lora_back_out(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
     const int rt = lora_rank_tiles(p.r);
     if (rt == 1) lora_back_out_kernel<DT, 1, 1><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 2) lora_back_out_kernel<DT, 2, 1><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 4) lora_back_out_kernel<DT, 2, 2><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_out_kernel<DT, 1, 2><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_out_kernel<DT, 1, 4><<<grid, kLoraThreads, 0, s>>>(p);
     else lora_back_out_kernel<DT, 2, 4><<<grid, kLoraThreads, 0, s>>>(p);
+    if (p.u && p.u_parts > kLoraShares) {
+        const int64_t n = p.it.n * p.r, blocks = (n + 4 * kLoraThreads - 1) / (4 * kLoraThreads);
+        lora_add_u_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), kLoraThreads, 0, s>>>(p.u, n, p.u_parts);
+    }
     return hipGetLastError();
 }
 
@@ -1162,8 +1211,8 @@ template <int DT, bool DROP>
 void lora_back_in_rank(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
     const int rt = lora_rank_tiles(p.r);
     if (rt == 1) lora_back_in_kernel<DT, 1, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 2) lora_back_in_kernel<DT, 2, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 4) lora_back_in_kernel<DT, 2, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_in_kernel<DT, 1, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_in_kernel<DT, 1, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
     else lora_back_in_kernel<DT, 2, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
 }
 
