@@ -859,10 +859,10 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
         const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
         if (r0 >= r1 || a < 0) continue;
         const float s = p.scale ? p.scale[a] : 1.0f;
-        LoraRows<DT, NR> rows;
-        float h[RW][8];
-        // a tile's hidden rows, a wave's ranks: one tile ahead as dy is, and before it
-        // (loads return in order)
+        // dy and the hidden rows (a wave's ranks) two tiles ahead: with u's way through LDS a
+        // tile takes longer than a load (one tile ahead 40 us of 62,710 x 1024)
+        LoraRows<DT, NR> even, odd;
+        float heven[RW][8], hodd[RW][8];
         auto load_h = [&](int64_t row0, float (&h)[RW][8]) {
             if (!p.pu || row0 >= r1) return;
             const int n16 = lane & 15, g = lane >> 4;
@@ -875,8 +875,8 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                     h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
                 }
         };
-        load_h(r0, h);
-        rows.load(p.dy, p.dys, r0, r1, j0, col0 + V * (lane & 15), p.o);
+        load_h(r0, heven);
+        even.load(p.dy, p.dys, r0, r1, j0, col0 + V * (lane & 15), p.o);
         if (p.u) {
             const S* up = static_cast<const S*>(p.up);
             const int64_t all = it.adapters * p.o * p.r;
@@ -893,7 +893,9 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             }
             lds_barrier();
         }
-        for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+        load_h(r0 + kLoraRows, hodd);
+        odd.load(p.dy, p.dys, r0 + kLoraRows, r1, j0, col0 + V * (lane & 15), p.o);
+        auto step = [&](int64_t row0, LoraRows<DT, NR>& rows, float (&h)[RW][8]) {
             // (what follows from the lane is formed anew each time: kept through the loops it
             // would not fit the registers)
             int ln = lane;
@@ -909,9 +911,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             } else {
                 lds_barrier();
             }
-            float hn[RW][8];
-            load_h(row0 + kLoraRows, hn);
-            rows.load(p.dy, p.dys, row0 + kLoraRows, r1, j0, mine, p.o);
+            rows.load(p.dy, p.dys, row0 + 2 * kLoraRows, r1, j0, mine, p.o);
             if constexpr (WR > 1) raw.get(t, TP);
             if (p.u) {
                 floatx4 u[2][RW] = {};
@@ -957,11 +957,12 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                         for (int i = 0; i < 8; ++i)
                             if (row0 + 8 * g + i >= r1) h[j][i] = 0.0f;
                 lora_outer<DT, RW>(raw, h, acc);
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) h[j][i] = hn[j][i];
+                load_h(row0 + 2 * kLoraRows, h);
             }
+        };
+        for (int64_t row0 = r0; row0 < r1; row0 += 2 * kLoraRows) {
+            step(row0, even, heven);
+            if (row0 + kLoraRows < r1) step(row0 + kLoraRows, odd, hodd);
         }
         if (p.pu && col0 < p.o)
             lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
