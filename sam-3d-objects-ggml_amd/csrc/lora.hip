@@ -329,7 +329,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
               : dtype == SPC_F16 ? lora_back_out_f16(s, p, out)
                                  : lora_back_out_f32(s, p, out);
         p.rows_per = b.rows_c;
-        if (p.u_parts > kLoraShares) p.u_parts = 1;  // (they have been added)
+        if (p.u_parts > lora_shares(lora_rank_tiles(p.r))) p.u_parts = 1;  // (they have been added)
         if (err == hipSuccess && p.u)
             err = dtype == SPC_BF16  ? lora_back_in_bf16(s, p, in)
                   : dtype == SPC_F16 ? lora_back_in_f16(s, p, in)

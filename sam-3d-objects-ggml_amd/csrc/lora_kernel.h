@@ -969,8 +969,9 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
     }
 }
 
-// u's shares, where there are more than two: their sum in the first one's place.
-constexpr int kLoraShares = 2;
+// u's shares, where there are more than the pass over x takes (four at 16 ranks, two
+// from there on: registers): their sum in the first one's place.
+constexpr int lora_shares(int rt) { return rt == 1 ? 4 : 2; }
 __global__ __launch_bounds__(kLoraThreads) static void lora_add_u_kernel(float* u, int64_t n, int parts) {
     for (int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kLoraThreads * 4)
         for (int e = 0; e < 4 && i + e < n; ++e) {
@@ -997,6 +998,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     constexpr int QN = WR == 1 ? 4 : 2, NI = WR == 4 ? 1 : 2;
     constexpr int G = CW / 8;                // groups of eight columns
     constexpr int NU = kLoraRows * RP / kLoraThreads;  // values of u a thread
+    constexpr int SH = lora_shares(RT);                // and the shares of each
     __shared__ __attribute__((aligned(16))) float ub[BUF][kLoraRows * P];
     __shared__ __attribute__((aligned(16))) S wl[CB * WP];
     __shared__ __attribute__((aligned(16))) S tile[WR > 1 ? BUF : 1][WR > 1 ? WC : 1][WR > 1 ? kLoraRows * TP : 8];
@@ -1025,18 +1027,16 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
         }
         LoraRows<DT, NR> rows = {};
         u32x4 base[NI][QN] = {};
-        float un[2][NU];
-        // the tile's rows of u (one share or two), and of dx_base
+        float un[SH][NU];
+        // the tile's rows of u (its shares), and of dx_base
         auto load_u = [&](int64_t row0) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
-                un[0][i] = un[1][i] = 0.0f;
-                if (row0 + m < r1 && j < p.r) {
-                    const float* q = p.u + (row0 + m) * p.r + j;
-                    un[0][i] = q[0];
-                    if (p.u_parts > 1) un[1][i] = q[it.n * p.r];
-                }
+                const bool on = row0 + m < r1 && j < p.r;
+                const float* q = p.u + (row0 + m) * p.r + j;
+#pragma unroll
+                for (int k = 0; k < SH; ++k) un[k][i] = on && k < p.u_parts ? q[k * it.n * p.r] : 0.0f;
             }
         };
         auto load_base = [&](int64_t row0, int n16, int g) {
@@ -1086,7 +1086,9 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
-                f[m * P + j] = un[0][i] + un[1][i];
+                float z = un[0][i] + un[1][i];
+                if constexpr (SH == 4) z += un[2][i] + un[3][i];
+                f[m * P + j] = z;
             }
             // (loads return in order: u, wanted first, before dx_base and the next rows)
             load_u(row0 + kLoraRows);
@@ -1201,7 +1203,7 @@ hipError_t lora_back_out(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
     else if (rt == 2) lora_back_out_kernel<DT, 1, 2><<<grid, kLoraThreads, 0, s>>>(p);
     else if (rt == 4) lora_back_out_kernel<DT, 1, 4><<<grid, kLoraThreads, 0, s>>>(p);
     else lora_back_out_kernel<DT, 2, 4><<<grid, kLoraThreads, 0, s>>>(p);
-    if (p.u && p.u_parts > kLoraShares) {
+    if (p.u && p.u_parts > lora_shares(rt)) {
         const int64_t n = p.it.n * p.r, blocks = (n + 4 * kLoraThreads - 1) / (4 * kLoraThreads);
         lora_add_u_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), kLoraThreads, 0, s>>>(p.u, n, p.u_parts);
     }
