@@ -173,7 +173,9 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
                     kept |= (uint32_t)k << t;
                     xs[8 * w + t][lane] = k ? xv[t] : 0.0f;
                 }
-                __syncthreads();
+            }
+            __syncthreads();  // (for rows without an adapter too: the list has been read)
+            if (!none) {
                 for (int t = 0; t < count; ++t) {
                     const float xt = xs[t][lane];
                     float d = 0.0f;

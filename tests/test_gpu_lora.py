@@ -4,7 +4,7 @@ dropout, values that are not finite, streams, graphs, refusals."""
 import pytest
 import torch
 
-from lora_reference import Adapters, adapter_of_rows
+from lora_reference import Adapters, adapter_of_rows, factors
 from norm_reference import check
 
 pytestmark = pytest.mark.gpu
@@ -158,6 +158,48 @@ def test_large_values_beside_small(spc, dev, dt):
     q.dy[:, 5], q.up[0, 5] = big, 0
     q.up[0, 5, 7], q.down[0, 7] = 1, 0
     q.check(nat)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_many_rows_without_an_adapter(spc, dev, dt):
+    """Hundreds of them in short items, gathered in several rounds, and behind the
+    items."""
+    n = 900
+    q = Case(dev, dt, n, 70, 200, 12, k=3, offsets=list(range(10, 811, 20)),
+             adapters=[i // 13 if i % 13 == 0 and i < 39 else -1 for i in range(40)], p=0.3)
+    q.check(spc._native)
+    dx = spc._native.lora_backward(q.dy, q.x, None, q.down, q.up, q.dx_base, need=(1, 0, 0), **q.kw)[0]
+    rest = (adapter_of_rows(n, 3, q.kw["offsets"], q.kw["adapters"]) < 0).to(dev)
+    assert int(rest.sum()) == 840 and torch.equal(dx[rest], q.dx_base[rest])
+
+
+def test_more_elements_than_32_bits_count(spc, dev):
+    """Rows past 2^31 elements of x, dy, dx and y are as in calls of their own; the
+    gradients are those of the rows that are not zero."""
+    nat = spc._native
+    g = torch.Generator().manual_seed(1)
+    n, c, r = (1 << 21) + 77, 1040, 8
+    f = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)  # noqa: E731
+    down, up = f(2, r, c) * 0.03, f(2, c, r) * 0.3
+    ids = torch.tensor([1, -1, 0], dtype=torch.int32, device=dev)
+    off = torch.tensor([0, 100, n - 90, n - 3], device=dev)
+    x = torch.zeros((n, c), dtype=torch.bfloat16, device=dev)
+    x[:100], x[n - 90:] = f(100, c), f(90, c)
+    kw = dict(adapters=ids, p=0.25, seed=torch.tensor(SEED, device=dev))
+    y, h = nat.lora(x, down, up, x, offsets=off, return_hidden=True, **kw)
+    dx, dd, du = nat.lora_backward(x, x, h, down, up, x, offsets=off, **kw)
+    for rows, a, first in ((slice(0, 100), 1, 0), (slice(n - 90, n - 3), 0, n - 90)):
+        k = rows.stop - rows.start
+        q = Adapters(x[rows], down[a:a + 1], up[a:a + 1])
+        q.f = factors(SEED, k, c, 0.25, first=first)
+        q.x = q.x * q.f
+        (wy, ey), (wh, eh) = q.forward(x[rows])
+        check("y", y[rows], wy, ey), check("hidden", h[rows], wh, eh)
+        (wx, ex), (wd, ed), (wu, eu) = q.backward(x[rows], h[rows], x[rows])
+        check("dx", dx[rows], wx, ex), check("ddown", dd[a:a + 1], wd, ed), check("dup", du[a:a + 1], wu, eu)
+    for t in (y, dx):
+        assert torch.equal(t[n - 3:], x[n - 3:]) and not t[100:n - 90].any()
+    assert not h[100:n - 90].any() and not h[n - 3:].any()
 
 
 def test_in_place_and_partial_gradients(spc, dev):
