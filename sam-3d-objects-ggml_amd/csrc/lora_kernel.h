@@ -49,19 +49,34 @@ struct LoraItems {
         const int64_t a = which ? which[v] : 0;
         return a >= 0 && a < adapters ? a : -1;
     }
-    // The last segment v with begin(v) / R + per v <= t (64 probes at a time, by
-    // a whole wave; inside the segments' range whatever the offsets hold).
+    // The last segment v with begin(v) / R + per v <= t, its rows and adapter (64 probes
+    // at a time, by a whole wave; inside the segments' range whatever the offsets hold).
+    // What the last probes' lanes need is read in one go: a wait of its own for each of
+    // them is a good part of what few rows take.
+    struct Found {
+        int64_t v, begin, end, adapter;
+    };
     template <int R>
-    __device__ __forceinline__ int64_t find(int64_t t, int64_t per) const {
+    __device__ __forceinline__ Found find(int64_t t, int64_t per) const {
+        const int lane = threadIdx.x & 63;
         int64_t lo = 0, size = segments();
-        while (size > 1) {
-            const int64_t step = (size + 63) / 64, at = (int64_t)(threadIdx.x & 63) * step;
+        while (size > 64) {
+            const int64_t step = (size + 63) / 64, at = lane * step;
             const bool ok = at < size && begin(lo + at) / R + per * (lo + at) <= t;
             const int64_t past = max(__popcll(__ballot(ok)), 1) - 1;
             lo += past * step;
             size = min(step, size - past * step);
         }
-        return lo;
+        const int64_t v = lo + min((int64_t)lane, size - 1);
+        const int64_t b = begin(v), e = end(v);
+        const int a = (int)adapter(v);
+        const bool ok = lane < size && b / R + per * v <= t;
+        const int k = max(__popcll(__ballot(ok)), 1) - 1;
+        auto pick = [&](int64_t x) {
+            return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), k) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane((int)x, k));
+        };
+        return {lo + k, pick(b), pick(e), __builtin_amdgcn_readlane(a, k)};
     }
 };
 
@@ -637,10 +652,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) 
     __shared__ __attribute__((aligned(16))) float red[4 * R * P];
     __shared__ __attribute__((aligned(16))) float hid[MODE == kLoraShrink ? 4 : R * P];
     const LoraItems& it = p.it;
-    const int64_t v = it.template find<R>(blockIdx.x, 1);
-    const int64_t row0 = it.begin(v) + (blockIdx.x - it.begin(v) / R - v) * R, end = it.end(v);
-    if (row0 >= end || row0 < 0) return;
-    const LoraTile t = {row0, it.adapter(v), (int)min((int64_t)R, end - row0)};
+    const LoraItems::Found seg = it.template find<R>(blockIdx.x, 1);
+    const int64_t row0 = seg.begin + (blockIdx.x - seg.begin / R - seg.v) * R;
+    if (row0 >= seg.end || row0 < 0) return;
+    const LoraTile t = {row0, seg.adapter, (int)min((int64_t)R, seg.end - row0)};
     const int c0 = MODE == kLoraShrink ? 0 : blockIdx.y * p.col_per;
     const int c1 = min(c0 + p.col_per, p.o);
     if (t.a < 0) {
@@ -853,10 +868,11 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
     const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     floatx4 acc[V][RW] = {};
     int turn = 0;
-    for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
-        const int64_t b0 = it.begin(v);
-        if (b0 >= hi) break;
-        const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
+    LoraItems::Found seg = it.template find<1>(lo, 0);
+    for (int64_t v = seg.v; v < it.segments(); ++v) {
+        if (v != seg.v) seg = {v, it.begin(v), it.end(v), it.adapter(v)};
+        if (seg.begin >= hi) break;
+        const int64_t r0 = max(seg.begin, lo), r1 = min(seg.end, hi), a = seg.adapter;
         if (r0 >= r1 || a < 0) continue;
         const float s = p.scale ? p.scale[a] : 1.0f;
         // dy and the hidden rows (a wave's ranks) two tiles ahead: with u's way through LDS a
@@ -1013,10 +1029,11 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
     floatx4 acc[V][RW] = {};
     int turn = 0;
-    for (int64_t v = it.template find<1>(lo, 0); v < it.segments(); ++v) {
-        const int64_t b0 = it.begin(v);
-        if (b0 >= hi) break;
-        const int64_t r0 = max(b0, lo), r1 = min(it.end(v), hi), a = it.adapter(v);
+    LoraItems::Found seg = it.template find<1>(lo, 0);
+    for (int64_t v = seg.v; v < it.segments(); ++v) {
+        if (v != seg.v) seg = {v, it.begin(v), it.end(v), it.adapter(v)};
+        if (seg.begin >= hi) break;
+        const int64_t r0 = max(seg.begin, lo), r1 = min(seg.end, hi), a = seg.adapter;
         if (r0 >= r1) continue;
         if (a < 0) {
             if (p.dx && block0 < p.c)

@@ -10,11 +10,6 @@ namespace spc {
 
 namespace {
 
-// The adapter of a row, -1 for none.
-__device__ int64_t lora_of_row(const LoraItems& it, int64_t row) {
-    return it.adapter(it.find<1>(row, 0));
-}
-
 template <int DT>
 __device__ __forceinline__ float lora_get(const void* p, int64_t i) {
     if constexpr (DT == SPC_F32) return static_cast<const float*>(p)[i];
@@ -48,7 +43,7 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraItems it, const vo
                                                           int64_t r, const float* scale, LoraDrop d,
                                                           float* out) {
     for (int64_t row = blockIdx.x; row < it.n; row += gridDim.x) {
-        const int64_t a = lora_of_row(it, row);
+        const int64_t a = it.find<1>(row, 0).adapter;
         for (int64_t j = threadIdx.x / 64; j < r; j += 4) {
             float sum = 0.0f;
             if (a >= 0)
@@ -69,7 +64,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraItems it, const fl
                                                           const float* scale, LoraDrop d, const void* base,
                                                           int64_t base_stride, int64_t c, void* y) {
     for (int64_t row = blockIdx.x; row < it.n; row += gridDim.x) {
-        const int64_t a = lora_of_row(it, row);
+        const int64_t a = it.find<1>(row, 0).adapter;
         for (int64_t i = threadIdx.x; i < c; i += 256) {
             float sum = 0.0f;
             if (a >= 0) {
