@@ -181,6 +181,13 @@ template <typename S>
 __device__ __forceinline__ u32x4 lora_fetch(const S* row, int col, int c) {
     return *reinterpret_cast<const u32x4_rows*>(row + min(col, c - 16 / (int)sizeof(S)));
 }
+// The same of rows that a call reads once, past the caches. With inputs that change from call to call it measured 32.4 us
+// against 35.1 at 11,774 x 2048 to 1024 of rank 32, BF16, and 134.8 against 139 for the gradients of 62,710 x 1024 of rank 16.
+// The same 96 MB over and over, which then stay in the memory's own cache, are faster kept: 29 us against 32.3.
+template <typename S>
+__device__ __forceinline__ u32x4 lora_stream(const S* row, int col, int c) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_rows*>(row + min(col, c - 16 / (int)sizeof(S))));
+}
 template <typename S>
 __device__ __forceinline__ u32x4 lora_edge(u32x4 w, int col, int c) {
     return lora_shift<S>(w, max(col - (c - 16 / (int)sizeof(S)), 0));
@@ -451,8 +458,8 @@ __device__ __forceinline__ void lora_fetch_pair(u32x4& first, u32x4& second, con
     constexpr int V = 16 / (int)sizeof(S);
     const int lane = threadIdx.x & 63, n16 = lane & 15, g = lane >> 4, row = n16 & 7;
     const S* q = at + V * g + (n16 & 8 ? 4 * V : 0);
-    first = *reinterpret_cast<const u32x4_rows*>(q + min(row, m - 1) * stride);
-    second = *reinterpret_cast<const u32x4_rows*>(q + min(row + 8, m - 1) * stride);
+    first = __builtin_nontemporal_load(reinterpret_cast<const u32x4_rows*>(q + min(row, m - 1) * stride));
+    second = __builtin_nontemporal_load(reinterpret_cast<const u32x4_rows*>(q + min(row + 8, m - 1) * stride));
 }
 struct LoraTile {
     int64_t row0, a;
@@ -746,13 +753,13 @@ struct LoraRows {
             const S* q = static_cast<const S*>(base) + (row0 + first) * stride;
 #pragma unroll
             for (int j = 0; j < NR; ++j) {
-                v[j] = lora_fetch(q, col, c);
+                v[j] = lora_stream(q, col, c);
                 q += stride;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < NR; ++j)
-                v[j] = lora_fetch(static_cast<const S*>(base) + min(row0 + first + j, end - 1) * stride, col, c);
+                v[j] = lora_stream(static_cast<const S*>(base) + min(row0 + first + j, end - 1) * stride, col, c);
         }
     }
     // Zeros for what is past the end of the rows, and, at the row's end, of the columns.
