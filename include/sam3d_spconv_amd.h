@@ -752,8 +752,9 @@ typedef struct {
  * are kept in F32; one rounding to dtype.  n up to 2^27, rank 1 to 128, in_features and
  * out_features to 2^24, n_items and n_adapters to 65535.  workspace:
  * spc_lora_workspace_bytes (which may be none), 16-byte aligned. */
-size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t in_features,
-                                int64_t out_features, int64_t rank, int backward);
+size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t n_adapters,
+                                int64_t in_features, int64_t out_features, int64_t rank,
+                                int backward);
 int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
              const spc_lora_params* params, const void* base, int64_t base_stride, void* y,
              float* hidden, void* workspace, size_t workspace_bytes);

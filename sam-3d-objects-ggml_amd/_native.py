@@ -136,7 +136,7 @@ def lib() -> ctypes.CDLL:
     L.spc_linear_q4_0_bias_grad.argtypes = [_P, _INT, _P, _I64, _I64, _I64, _INT, _P, _P, _SZ]
     L.spc_dropout.argtypes = [_P, _INT, _P, _I64, _I64, _I64, ctypes.c_double, _P, _P, _I64, _P]
     L.spc_lora_workspace_bytes.restype = _SZ
-    L.spc_lora_workspace_bytes.argtypes = [_INT, _I64, _I64, _I64, _I64, _I64, _INT]
+    L.spc_lora_workspace_bytes.argtypes = [_INT, _I64, _I64, _I64, _I64, _I64, _I64, _INT]
     L.spc_lora.argtypes = [_P, _INT, _P, _I64, _I64, ctypes.POINTER(LoraParams), _P, _I64, _P, _P, _P,
                            _SZ]
     L.spc_lora_backward.argtypes = [_P, _INT, _P, _I64, _P, _I64, _P, _I64,
@@ -1182,8 +1182,8 @@ def _lora_params(x, c, o, down, up, scale, offsets, adapters, p, seed):
 
 
 @lru_cache(maxsize=4096)
-def _lora_workspace(dt: int, n: int, items: int, c: int, o: int, r: int, backward: int) -> int:
-    return lib().spc_lora_workspace_bytes(dt, n, items, c, o, r, backward)
+def _lora_workspace(dt: int, n: int, items: int, adapters: int, c: int, o: int, r: int, backward: int) -> int:
+    return lib().spc_lora_workspace_bytes(dt, n, items, adapters, c, o, r, backward)
 
 
 def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tensor | None = None, *,
@@ -1215,7 +1215,7 @@ def lora(x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, base: torch.Tens
     else:
         _into(out, ((n, o), x.dtype), "x", (x, False), (base, True))
     hidden = torch.empty((n, r), dtype=torch.float32, device=dev) if return_hidden else None
-    nbytes = _lora_workspace(dt, n, items, c, o, r, 0)
+    nbytes = _lora_workspace(dt, n, items, q.n_adapters, c, o, r, 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     st = _launch(lib().spc_lora, dev, dt, x.data_ptr(), stride, n, q, _ptr(base), bs, out.data_ptr(),
                  _ptr(hidden), _ptr(ws), nbytes)
@@ -1257,7 +1257,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, hidden: torch.Tensor | None
     dx = x.new_empty((n, c)) if need[0] else None
     ddown = torch.empty_like(keep[0]) if need[1] else None
     dup = torch.empty_like(keep[1]) if need[2] else None
-    nbytes = _lora_workspace(dt, n, items, c, o, r, 1)
+    nbytes = _lora_workspace(dt, n, items, q.n_adapters, c, o, r, 1)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     st = _launch(lib().spc_lora_backward, dev, dt, dy.data_ptr(), dys, x.data_ptr(), xs, _ptr(hidden), n,
                  q, _ptr(dx_base), bs, _ptr(dx), _ptr(ddown), _ptr(dup), _ptr(ws), nbytes)

@@ -114,13 +114,21 @@ struct LoraBackPlan {
     size_t u, pu, pd;
 };
 
-LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64_t r) {
+LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, int64_t c, int64_t o, int64_t r) {
     LoraBackPlan q{};
-    q.few = n <= 32 * items;
+    // Tiles of 32 rows of one item cost some 0.2 us an item, however short, and the sums
+    // behind them; gathered, an adapter's rows wait one after the other, some 8 us for each
+    // 32 of them (us, gathered / tiles, 1024 -> 1024 rank 16 bf16: 32 rows of one item 19 /
+    // 21, 128 of one 42 / 21; 512 of 256 items and 8 adapters 41 / 78, of 16 items 41 / 28,
+    // of 16 items and 2 adapters 69 / 23; 1024 of 512 and 8 67 / 124, of 64 and 8 56 / 50;
+    // 8192 of 2048 and 8 378 / 431, of 1024 and 8 332 / 223; 4096 one-row items of one
+    // adapter 1886 / 1272, of eight 318 / 892, of 1024 1489 / 9199).
+    q.few = n <= std::min(32 * items, std::min(items, adapters) * (64 + items / 2));
     if (q.few) {
         int64_t chunks = 1;
         while (chunks * (dt == SPC_F32 ? 4 : 8) < r) chunks *= 2;
         const int64_t lines = kLoraThreads / chunks;
+        // (u of few rows is one wait after the other along the outputs, of many enough blocks)
         q.shares = (int)std::min({(int64_t)8, ceil_div(o, lines * 8), std::max<int64_t>(1, 128 / std::max<int64_t>(n, 1))});
         q.o_per = (int)ceil_div(o, q.shares);
         q.u = (size_t)(q.shares * n * r);
@@ -129,6 +137,9 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t
     const int64_t cols = 4 / lora_rank_waves(r) * lora_wave_cols(dt);
     q.blocks_o = ceil_div(o, cols);
     q.blocks_c = ceil_div(c, cols);
+    // Some two blocks a CU: the registers hold no more of them at once, and every further
+    // chunk is a slot to write and add (us of 62,710 x 1024 rank 16 bf16 by blocks: 256 155,
+    // 384 157, 512 138, 640 166, 768 157, 1024 144).
     auto rows = [&](int64_t blocks) {
         int64_t per = std::max<int64_t>(1, ceil_div(n, std::max<int64_t>(1, 512 / blocks)));
         if (n / items >= kLoraRows || per >= kLoraRows) per = ceil_div(per, kLoraRows) * kLoraRows;
@@ -191,17 +202,17 @@ using namespace spc;
 
 extern "C" {
 
-size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t in_features,
+size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t n_adapters, int64_t in_features,
                                 int64_t out_features, int64_t rank, int backward) {
     if (!float_dtype(dtype) || n < 0 || n > kLoraMaxRows || rank < 1 || rank > kLoraMaxRank || n_items < 1 ||
-        n_items > kLoraMaxItems || in_features < 1 || in_features > kLoraMaxWidth || out_features < 1 ||
+        n_items > kLoraMaxItems || n_adapters < 1 || n_adapters > kLoraMaxAdapters || in_features < 1 || in_features > kLoraMaxWidth || out_features < 1 ||
         out_features > kLoraMaxWidth)
         return 0;
     size_t floats = 0;
     if (lora_small(in_features, out_features)) {
         floats = (size_t)n * rank;
     } else if (backward) {
-        const LoraBackPlan b = lora_back_plan(dtype, n, n_items, in_features, out_features, rank);
+        const LoraBackPlan b = lora_back_plan(dtype, n, n_items, n_adapters, in_features, out_features, rank);
         floats = lora_round_up(b.u) + lora_round_up(b.pu) + b.pd;
     } else {
         const LoraPlan f = lora_plan(dtype, n, n_items, in_features, out_features, rank);
@@ -226,7 +237,7 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
         set_last_error("%s: null or misaligned pointer, or a negative stride", fn);
         return SPC_BAD_ARG;
     }
-    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 0);
+    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.n_adapters, q.in_features, q.out_features, q.rank, 0);
     if (need && (!workspace || off(workspace, 16) || workspace_bytes < need)) {
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
@@ -286,12 +297,12 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         return SPC_BAD_ARG;
     }
     if (!dx && !ddown && !dup) return SPC_OK;
-    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.in_features, q.out_features, q.rank, 1);
+    const size_t need = spc_lora_workspace_bytes(dtype, n, q.n_items, q.n_adapters, q.in_features, q.out_features, q.rank, 1);
     if (need && (!workspace || off(workspace, 16) || workspace_bytes < need)) {
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
-    const LoraBackPlan b = lora_back_plan(dtype, n, q.n_items, q.in_features, q.out_features, q.rank);
+    const LoraBackPlan b = lora_back_plan(dtype, n, q.n_items, q.n_adapters, q.in_features, q.out_features, q.rank);
     float* ws = static_cast<float*>(workspace);
     p.dy = dy;
     p.dys = dy_stride;

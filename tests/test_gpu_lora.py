@@ -160,16 +160,27 @@ def test_large_values_beside_small(spc, dev, dt):
     q.check(nat)
 
 
+@pytest.mark.parametrize("n,rows,k", [(600, 5, 8), (600, 5, 3), (700, 1, 3), (512, 8, 8), (512, 32, 8), (2000, 2, 8)])
 @pytest.mark.parametrize("dt", list(DT))
-def test_many_rows_without_an_adapter(spc, dev, dt):
+def test_many_short_items(spc, dev, dt, n, rows, k):
+    """Few and many adapters, whose rows lie all over."""
+    ids = [(i * i + i // 7) % (k + 1) - 1 for i in range(n // rows)]
+    off = list(range(0, n // rows * rows + 1, rows))
+    Case(dev, dt, n, 136, 72, 16, k=k, offsets=off, adapters=ids).check(spc._native)
+    Case(dev, dt, n, 75, 136, 40, k=k, offsets=off, adapters=ids, p=0.2).check(spc._native)
+
+
+@pytest.mark.parametrize("k", [3, 12])
+@pytest.mark.parametrize("dt", list(DT))
+def test_many_rows_without_an_adapter(spc, dev, dt, k):
     """Hundreds of them in short items, gathered in several rounds, and behind the
     items."""
     n = 900
-    q = Case(dev, dt, n, 70, 200, 12, k=3, offsets=list(range(10, 811, 20)),
+    q = Case(dev, dt, n, 70, 200, 12, k=k, offsets=list(range(10, 811, 20)),
              adapters=[i // 13 if i % 13 == 0 and i < 39 else -1 for i in range(40)], p=0.3)
     q.check(spc._native)
     dx = spc._native.lora_backward(q.dy, q.x, None, q.down, q.up, q.dx_base, need=(1, 0, 0), **q.kw)[0]
-    rest = (adapter_of_rows(n, 3, q.kw["offsets"], q.kw["adapters"]) < 0).to(dev)
+    rest = (adapter_of_rows(n, k, q.kw["offsets"], q.kw["adapters"]) < 0).to(dev)
     assert int(rest.sum()) == 840 and torch.equal(dx[rest], q.dx_base[rest])
 
 

@@ -116,17 +116,18 @@ def test_host_validation_lora(spc):
     assert bwd(dy=None) == bwd(hidden=None) == bwd(dys=-1) == bwd(du=fake + 1) == nat.BAD_ARG
     # few wide rows: the forward pass in two kernels; the backward pass's shares
     for b, n, wide in ((0, 8, 8192), (1, 5000, 64)):
-        need = L.spc_lora_workspace_bytes(nat.BF16, n, 2, wide, 48, 64, b)
+        need = L.spc_lora_workspace_bytes(nat.BF16, n, 2, 3, wide, 48, 64, b)
         assert need > 0
         kw = dict(n=n, in_features=wide, rank=64, **({"xs": wide} if b == 0 else {}))
         for bad in (dict(wsb=need - 1), dict(ws=None), dict(ws=fake + 4)):
             assert (fwd, bwd)[b](**kw, **bad) == nat.BAD_ARG
     assert b"workspace" in L.spc_last_error()
     for items in (1, 7, 65535):  # no rows: an answer, not a division
-        assert all(L.spc_lora_workspace_bytes(nat.F16, 0, items, 64, 48, 8, b) >= 0 for b in (0, 1))
-    assert L.spc_lora_workspace_bytes(nat.BF16, 4, 1, 64, 48, 129, 0) == 0
-    assert L.spc_lora_workspace_bytes(nat.Q8_0, 4, 1, 64, 48, 8, 0) == 0
-    assert L.spc_lora_workspace_bytes(nat.BF16, 4, 0, 64, 48, 8, 1) == 0
+        assert all(L.spc_lora_workspace_bytes(nat.F16, 0, items, 2, 64, 48, 8, b) >= 0 for b in (0, 1))
+    assert L.spc_lora_workspace_bytes(nat.BF16, 4, 1, 1, 64, 48, 129, 0) == 0
+    assert L.spc_lora_workspace_bytes(nat.Q8_0, 4, 1, 1, 64, 48, 8, 0) == 0
+    assert L.spc_lora_workspace_bytes(nat.BF16, 4, 0, 1, 64, 48, 8, 1) == 0
+    assert L.spc_lora_workspace_bytes(nat.BF16, 4, 1, 0, 64, 48, 8, 1) == 0
 
 
 def test_cpu_tensors_are_rejected(spc):
