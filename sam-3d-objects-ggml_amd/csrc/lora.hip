@@ -159,6 +159,76 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
 
 inline size_t lora_round_up(size_t floats) { return (floats + 63) / 64 * 64; }
 
+// Widths below eight as the kernels take them: arrays of rows of eight behind the rest
+// of the workspace (`at`; null: their bytes are counted only).  A launch before and one
+// after, against plain sums over narrow rows (us of rank 8 bf16, so / plain: 21,766 x
+// 1024 to 4 17 / 174 forward, 49 / 12,276 backward; 100,000 x 4 to 64 20 / 175, 70 /
+// 56,246; 333 x 6 to 32 7.6 / 7.3, 21 / 131).
+struct LoraNarrow {
+    int dt;
+    char* at;
+    size_t bytes = 0;
+    LoraCopies in{}, out{};
+
+    LoraNarrow(int dt, void* at) : dt(dt), at(static_cast<char*>(at)) {}
+    static int64_t width(int64_t c) { return std::max<int64_t>(c, 8); }
+
+    void* take(int64_t elements) {
+        void* p = at ? at + bytes : nullptr;
+        bytes += lora_round_up((size_t)(elements * float_size(dt) + 3) / 4) * sizeof(float);
+        return p;
+    }
+    // Rows of `width` as rows of `fill`, in `dst`; and results back.
+    void* widen(void* dst, const void* src, int64_t rows, int64_t stride, int64_t width, int64_t fill) {
+        if (src) in.job[in.jobs++] = {src, dst, rows, stride, fill, (int)width, (int)fill};
+        return dst;
+    }
+    void narrow(void* dst, const void* src, int64_t rows, int64_t width, int64_t fill) {
+        if (dst) out.job[out.jobs++] = {src, dst, rows, fill, width, (int)width, (int)width};
+    }
+    const void* rows(const void* src, int64_t rows, int64_t* stride, int64_t width) {
+        const void* p = widen(take(rows * 8), src, rows, *stride, width, 8);
+        *stride = 8;
+        return p;
+    }
+
+    // The adapters, of c and o features.
+    void adapters(const void** down, const void** up, int64_t k, int64_t r, int64_t c, int64_t o) {
+        int64_t stride = c;
+        if (c < 8) *down = rows(*down, k * r, &stride, c);
+        if (o < 8) *up = widen(take(k * 8 * r), *up, k, o * r, o * r, 8 * r);
+    }
+    // y (dx), onto whose wide rows base is copied.
+    void sum(void** y, const void** base, int64_t* stride, int64_t n, int64_t width) {
+        void* wide = take(n * 8);
+        if (*base) *base = widen(wide, *base, n, *stride, width, 8);
+        *stride = 8;
+        narrow(*y, wide, n, width, 8);
+        if (*y) *y = wide;
+    }
+    void forward(LoraArgs* p, int64_t k, int64_t r, int64_t c, int64_t o) {
+        adapters(&p->down, &p->up, k, r, c, o);
+        if (c < 8) p->x = rows(p->x, p->it.n, &p->xs, c);
+        if (o < 8) sum(&p->y, &p->base, &p->bs, p->it.n, o);
+    }
+    void backward(LoraBackArgs* p, void** ddown, void** dup, int64_t k, int64_t r, int64_t c, int64_t o) {
+        adapters(&p->down, &p->up, k, r, c, o);
+        if (c < 8) {
+            p->x = rows(p->x, p->it.n, &p->xs, c);
+            sum(&p->dx, &p->base, &p->bs, p->it.n, c);
+            void* wide = take(k * r * 8);
+            narrow(*ddown, wide, k * r, c, 8);
+            if (*ddown) *ddown = wide;
+        }
+        if (o < 8) {
+            p->dy = rows(p->dy, p->it.n, &p->dys, o);
+            void* wide = take(k * 8 * r);
+            narrow(*dup, wide, k, o * r, 8 * r);
+            if (*dup) *dup = wide;
+        }
+    }
+};
+
 // Checks what both entry points share.
 int lora_args(const char* fn, int dtype, const void* x, int64_t x_stride, int64_t n,
               const spc_lora_params* q, LoraItems* it, uint32_t* drop) {
@@ -205,20 +275,27 @@ extern "C" {
 size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t n_adapters, int64_t in_features,
                                 int64_t out_features, int64_t rank, int backward) {
     if (!float_dtype(dtype) || n < 0 || n > kLoraMaxRows || rank < 1 || rank > kLoraMaxRank || n_items < 1 ||
-        n_items > kLoraMaxItems || n_adapters < 1 || n_adapters > kLoraMaxAdapters || in_features < 1 || in_features > kLoraMaxWidth || out_features < 1 ||
-        out_features > kLoraMaxWidth)
+        n_items > kLoraMaxItems || n_adapters < 1 || n_adapters > kLoraMaxAdapters || in_features < 1 ||
+        in_features > kLoraMaxWidth || out_features < 1 || out_features > kLoraMaxWidth)
         return 0;
+    const int64_t c = LoraNarrow::width(in_features), o = LoraNarrow::width(out_features);
+    LoraNarrow narrow(dtype, nullptr);
     size_t floats = 0;
-    if (lora_small(in_features, out_features)) {
-        floats = (size_t)n * rank;
-    } else if (backward) {
-        const LoraBackPlan b = lora_back_plan(dtype, n, n_items, n_adapters, in_features, out_features, rank);
+    if (backward) {
+        const LoraBackPlan b = lora_back_plan(dtype, n, n_items, n_adapters, c, o, rank);
         floats = lora_round_up(b.u) + lora_round_up(b.pu) + b.pd;
+        LoraBackArgs p{};
+        void *ddown = nullptr, *dup = nullptr;
+        p.it.n = n;
+        narrow.backward(&p, &ddown, &dup, n_adapters, rank, in_features, out_features);
     } else {
-        const LoraPlan f = lora_plan(dtype, n, n_items, in_features, out_features, rank);
+        const LoraPlan f = lora_plan(dtype, n, n_items, c, o, rank);
         if (f.mode == kLoraShrink) floats = (size_t)f.splits * n * rank;
+        LoraArgs p{};
+        p.it.n = n;
+        narrow.forward(&p, n_adapters, rank, in_features, out_features);
     }
-    return floats * sizeof(float);
+    return (narrow.bytes ? lora_round_up(floats) : floats) * sizeof(float) + narrow.bytes;
 }
 
 int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, int64_t n,
@@ -242,7 +319,8 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
-    const LoraPlan f = lora_plan(dtype, n, q.n_items, q.in_features, q.out_features, q.rank);
+    const int64_t c = LoraNarrow::width(q.in_features), o = LoraNarrow::width(q.out_features);
+    const LoraPlan f = lora_plan(dtype, n, q.n_items, c, o, q.rank);
     p.x = x;
     p.xs = x_stride;
     p.down = q.down;
@@ -253,8 +331,8 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
     p.y = y;
     p.hidden = hidden;
     p.part = static_cast<float*>(workspace);
-    p.c = (int)q.in_features;
-    p.o = (int)q.out_features;
+    p.c = (int)c;
+    p.o = (int)o;
     p.r = (int)q.rank;
     p.k_per = f.k_per;
     p.splits = f.splits;
@@ -267,15 +345,16 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
                : dtype == SPC_F16 ? lora_forward_f16(s, p, mode, f.mt, grid)
                                   : lora_forward_f32(s, p, mode, f.mt, grid);
     };
-    hipError_t err = hipSuccess;
-    if (lora_small(p.c, p.o)) {
-        err = lora_small_forward(s, dtype, p);
-    } else if (f.mode == kLoraFused) {
+    LoraNarrow narrow(dtype, p.part + (f.mode == kLoraShrink ? lora_round_up((size_t)f.splits * n * q.rank) : 0));
+    narrow.forward(&p, q.n_adapters, q.rank, q.in_features, q.out_features);
+    hipError_t err = lora_copy(s, dtype, narrow.in);
+    if (err == hipSuccess && f.mode == kLoraFused) {
         err = launch(kLoraFused, f.col_blocks);
-    } else {
+    } else if (err == hipSuccess) {
         err = launch(kLoraShrink, f.splits);
         if (err == hipSuccess) err = launch(kLoraExpand, f.col_blocks);
     }
+    if (err == hipSuccess) err = lora_copy(s, dtype, narrow.out);
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora launch");
 }
 
@@ -302,7 +381,8 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         set_last_error("%s: workspace missing, misaligned or too small", fn);
         return SPC_BAD_ARG;
     }
-    const LoraBackPlan b = lora_back_plan(dtype, n, q.n_items, q.n_adapters, q.in_features, q.out_features, q.rank);
+    const int64_t c = LoraNarrow::width(q.in_features), o = LoraNarrow::width(q.out_features);
+    const LoraBackPlan b = lora_back_plan(dtype, n, q.n_items, q.n_adapters, c, o, q.rank);
     float* ws = static_cast<float*>(workspace);
     p.dy = dy;
     p.dys = dy_stride;
@@ -319,21 +399,16 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     p.u_parts = b.few ? b.shares : (int)b.blocks_o;
     p.pu = dup ? ws + lora_round_up(b.u) : nullptr;
     p.pd = ddown ? ws + lora_round_up(b.u) + lora_round_up(b.pu) : nullptr;
-    p.c = (int)q.in_features;
-    p.o = (int)q.out_features;
+    p.c = (int)c;
+    p.o = (int)o;
     p.r = (int)q.rank;
     p.seed = q.seed;
     p.factor = drop_factor(p.drop);
-    hipError_t err = hipSuccess;
-    if (lora_small(p.c, p.o)) {
-        err = lora_small_backward(s, dtype, p, ddown, dup);
-        return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
-    }
-    if (b.few) {
-        err = lora_few_backward(s, dtype, p, b.o_per, ddown, dup);
-        return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
-    }
-    if (n > 0) {
+    LoraNarrow narrow(dtype, ws + lora_round_up(b.u) + lora_round_up(b.pu) + lora_round_up(b.pd));
+    narrow.backward(&p, &ddown, &dup, q.n_adapters, q.rank, q.in_features, q.out_features);
+    hipError_t err = lora_copy(s, dtype, narrow.in);
+    if (err == hipSuccess && b.few) err = lora_few_backward(s, dtype, p, b.o_per, ddown, dup);
+    if (err == hipSuccess && !b.few && n > 0) {
         const dim3 out((unsigned)b.blocks_o, (unsigned)b.chunks_o), in((unsigned)b.blocks_c, (unsigned)b.chunks_c);
         p.rows_per = b.rows_o;
         err = dtype == SPC_BF16  ? lora_back_out_bf16(s, p, out)
@@ -346,7 +421,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
                   : dtype == SPC_F16 ? lora_back_in_f16(s, p, in)
                                      : lora_back_in_f32(s, p, in);
     }
-    if (err == hipSuccess && (ddown || dup)) {
+    if (err == hipSuccess && !b.few && (ddown || dup)) {
         const LoraSum d = {p.pd, ddown, b.slot_c, p.c, 1, b.rows_c}, u = {p.pu, dup, b.slot_o, p.o, 0, b.rows_o};
         const dim3 grid((unsigned)std::min<int64_t>(std::max(d.slot, u.slot) / 64 * q.n_adapters, 1 << 20), 2);
         const int rt = lora_rank_tiles(q.rank);
@@ -355,6 +430,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         else lora_sum_kernel<SPC_F32><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
         err = hipGetLastError();
     }
+    if (err == hipSuccess) err = lora_copy(s, dtype, narrow.out);
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");
 }
 

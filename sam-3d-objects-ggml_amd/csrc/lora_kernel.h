@@ -135,10 +135,19 @@ LORA_LAUNCHERS(f16)
 LORA_LAUNCHERS(f32)
 #undef LORA_LAUNCHERS
 
-// Widths below eight (lora_small.hip).
-inline bool lora_small(int64_t c, int64_t o) { return c < 8 || o < 8; }
-hipError_t lora_small_forward(hipStream_t s, int dt, const LoraArgs& p);
-hipError_t lora_small_backward(hipStream_t s, int dt, const LoraBackArgs& p, void* ddown, void* dup);
+// Copies of rows (lora_narrow.hip): `width` elements of each, then zeros up to `fill`
+// (rows x fill < 2^31).
+struct LoraCopy {
+    const void* src;
+    void* dst;
+    int64_t rows, src_stride, dst_stride;
+    int width, fill;
+};
+struct LoraCopies {
+    LoraCopy job[5];
+    int jobs;
+};
+hipError_t lora_copy(hipStream_t s, int dt, const LoraCopies& q);
 
 // ranks in tiles of 16: 1, 2, 4 or 8
 inline int lora_rank_tiles(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8; }
@@ -147,7 +156,6 @@ constexpr int kLoraRowTiles = 2;
 inline int lora_rank_waves(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 // columns of one such wave
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
-
 
 // The gradients of few rows (lora_few.hip); u in u_parts shares of o_per outputs.
 hipError_t lora_few_backward(hipStream_t s, int dt, const LoraBackArgs& p, int o_per, void* ddown, void* dup);

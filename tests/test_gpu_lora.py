@@ -160,6 +160,30 @@ def test_large_values_beside_small(spc, dev, dt):
     q.check(nat)
 
 
+@pytest.mark.parametrize("c,o", [(1, 64), (4, 136), (7, 8), (8, 7), (200, 3), (520, 1), (5, 6), (1, 1)])
+@pytest.mark.parametrize("dt", list(DT))
+def test_narrow_rows(spc, dev, dt, c, o):
+    """Of fewer elements than 16 bytes hold: strides, bases in place, few rows and many,
+    nothing beside the results."""
+    nat, t = spc._native, DT[dt]
+    for n, off, ids in ((70, [0, 9, 40, 60], [2, 0, 1]), (900, [3, 400, 410, 880], [1, 2, -1])):
+        for r in (1, 12, 40):
+            q = Case(dev, dt, n, c, o, r, k=3, offsets=off, adapters=ids, p=0.25)
+            q.x = torch.randn(n, c + 3, device=dev).to(t)[:, 1:1 + c]
+            q.dy = torch.randn(n, o + 2, device=dev).to(t)[:, 2:]
+            q.check(nat)
+            y, h = nat.lora(q.x, q.down, q.up, q.base, return_hidden=True, **q.kw)
+            buf = torch.full((n + 2, o), 7.0, dtype=t, device=dev)
+            buf[1:-1] = q.base
+            nat.lora(q.x, q.down, q.up, buf[1:-1], out=buf[1:-1], **q.kw)
+            assert torch.equal(buf[1:-1], y) and (buf[[0, -1]] == 7).all()
+            whole = nat.lora_backward(q.dy, q.x, h, q.down, q.up, q.dx_base, **q.kw)
+            for i in range(3):
+                need = [i == k for k in range(3)]
+                part = nat.lora_backward(q.dy, q.x, h, q.down, q.up, q.dx_base, need=need, **q.kw)
+                assert torch.equal(part[i], whole[i]) and [p is None for p in part] == [not k for k in need]
+
+
 @pytest.mark.parametrize("n,rows,k", [(600, 5, 8), (600, 5, 3), (700, 1, 3), (512, 8, 8), (512, 32, 8), (2000, 2, 8)])
 @pytest.mark.parametrize("dt", list(DT))
 def test_many_short_items(spc, dev, dt, n, rows, k):
