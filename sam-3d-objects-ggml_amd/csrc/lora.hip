@@ -69,6 +69,17 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
     }
 }
 
+// The sum of u's shares in the first one's place.
+__global__ __launch_bounds__(kLoraThreads) void lora_add_u_kernel(float* u, int64_t n, int parts) {
+    for (int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kLoraThreads * 4)
+        for (int e = 0; e < 4 && i + e < n; ++e) {
+            float s = u[i + e];
+#pragma unroll 4
+            for (int q = 1; q < parts; ++q) s += u[q * n + i + e];
+            u[i + e] = s;
+        }
+}
+
 // How a call is split, from its sizes alone.
 struct LoraPlan {
     int mt, mode;     // mode: kLoraFused, or kLoraShrink and kLoraExpand
@@ -134,19 +145,19 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
         q.u = (size_t)(q.shares * n * r);
         return q;
     }
-    const int64_t cols = 4 / lora_rank_waves(r) * lora_wave_cols(dt);
-    q.blocks_o = ceil_div(o, cols);
-    q.blocks_c = ceil_div(c, cols);
+    q.blocks_o = ceil_div(o, (int64_t)lora_col_waves(dt, r, o) * lora_wave_cols(dt));
+    q.blocks_c = ceil_div(c, (int64_t)lora_col_waves(dt, r, c) * lora_wave_cols(dt));
     // Some two blocks a CU: the registers hold no more of them at once, and every further
     // chunk is a slot to write and add (us of 62,710 x 1024 rank 16 bf16 by blocks: 256 155,
     // 384 157, 512 138, 640 166, 768 157, 1024 144).
-    auto rows = [&](int64_t blocks) {
+    auto rows = [&](int64_t blocks, int64_t width) {
+        const int64_t tile = kLoraRows * lora_row_waves(dt, r, width);
         int64_t per = std::max<int64_t>(1, ceil_div(n, std::max<int64_t>(1, 512 / blocks)));
-        if (n / items >= kLoraRows || per >= kLoraRows) per = ceil_div(per, kLoraRows) * kLoraRows;
+        if (n / items >= tile || per >= tile) per = ceil_div(per, tile) * tile;
         return (int)per;
     };
-    q.rows_o = rows(q.blocks_o);
-    q.rows_c = rows(q.blocks_c);
+    q.rows_o = rows(q.blocks_o, o);
+    q.rows_c = rows(q.blocks_c, c);
     q.chunks_o = ceil_div(n, q.rows_o);
     q.chunks_c = ceil_div(n, q.rows_c);
     q.u = (size_t)(q.blocks_o * n * r);
@@ -415,7 +426,12 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
               : dtype == SPC_F16 ? lora_back_out_f16(s, p, out)
                                  : lora_back_out_f32(s, p, out);
         p.rows_per = b.rows_c;
-        if (p.u_parts > lora_shares(lora_rank_tiles(p.r))) p.u_parts = 1;  // (they have been added)
+        if (err == hipSuccess && p.u && p.u_parts > lora_shares(lora_rank_tiles(p.r), lora_row_waves(dtype, p.r, p.c))) {
+            const int64_t all = n * p.r, blocks = std::min<int64_t>(ceil_div(all, 4 * kLoraThreads), 4096);
+            lora_add_u_kernel<<<(unsigned)blocks, kLoraThreads, 0, s>>>(p.u, all, p.u_parts);
+            err = hipGetLastError();
+            p.u_parts = 1;
+        }
         if (err == hipSuccess && p.u)
             err = dtype == SPC_BF16  ? lora_back_in_bf16(s, p, in)
                   : dtype == SPC_F16 ? lora_back_in_f16(s, p, in)

@@ -156,6 +156,17 @@ constexpr int kLoraRowTiles = 2;
 inline int lora_rank_waves(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 // columns of one such wave
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
+// and the waves along columns: half of them where the rows are no wider than half of them
+// take, the others along rows (us of the gradients, so / all along columns: 200,000 x 64
+// to 64 rank 16 bf16 60 / 123, 62,710 x 96 to 160 f32 58 / 71)
+inline int lora_col_waves(int dt, int64_t r, int64_t width) {
+    int w = 4 / lora_rank_waves(r);
+    while (w > 1 && w / 2 * lora_wave_cols(dt) >= width) w /= 2;
+    return w;
+}
+inline int lora_row_waves(int dt, int64_t r, int64_t width) {
+    return 4 / lora_rank_waves(r) / lora_col_waves(dt, r, width);
+}
 
 // The gradients of few rows (lora_few.hip); u in u_parts shares of o_per outputs.
 hipError_t lora_few_backward(hipStream_t s, int dt, const LoraBackArgs& p, int o_per, void* ddown, void* dup);
@@ -751,9 +762,10 @@ hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3
 // V (l % 16) on (16 bytes a row).  That is the row operand of the weights'
 // gradients (columns by summed rows; 16-bit elements are exchanged between the
 // lane's registers to bring a column's eight rows together), whose sums stay in
-// registers until the chunk or the segment ends.  WC waves stand along the columns
-// and WR along the ranks (16 RW each): those of the same columns load, and mask, a
-// share of the rows each and pass them on through LDS.
+// registers until the chunk or the segment ends.  WC waves stand along the columns,
+// WR along the ranks (16 RW each) and WG along the rows, a tile of 32 each: those of
+// the same columns and rows load, and mask, a share of the rows each and pass them on
+// through LDS, those along the rows add their sums there at the end.
 constexpr int kLoraRows = 32;
 
 // NR of a lane's eight rows, from j0 on.
@@ -864,6 +876,29 @@ __device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], f
         }
 }
 
+// The sums of the waves along the rows (WAVES of each) added to the first ones', in
+// their order; ls: 64 V RW floatx4 for each of the others, which nobody else uses.
+template <int WAVES, int WG, int V, int RW>
+__device__ __forceinline__ void lora_gather(floatx4 (&acc)[V][RW], floatx4* ls) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    if (w >= WAVES)
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int j = 0; j < RW; ++j) {
+                ls[((w - WAVES) * V * RW + e * RW + j) * 64 + lane] = acc[e][j];
+                acc[e][j] = floatx4{0, 0, 0, 0};
+            }
+    lds_barrier();
+    if (w < WAVES)
+#pragma unroll
+        for (int q = 0; q < WG - 1; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+#pragma unroll
+                for (int j = 0; j < RW; ++j) acc[e][j] += ls[((q * WAVES + w) * V * RW + e * RW + j) * 64 + lane];
+}
+
 __device__ __forceinline__ void lora_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
@@ -874,22 +909,24 @@ __device__ __forceinline__ void lora_wave_sync() {
 // and the sums of dup.  u sums along a row, so its operand is read back from the
 // tile in LDS, and the waves' shares meet there too; the adapter's columns lie in
 // LDS by rank.
-template <int DT, int RW, int WR>
+template <int DT, int RW, int WR, int WC>
 __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBackArgs p) {
     using N = LoraNum<DT>;
     using S = typename N::S;
-    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RW * WR, P = lora_pitch(16 * RW);
+    constexpr int V = N::V, CW = 16 * V, CB = WC * CW, RP = 16 * RW * WR, P = lora_pitch(16 * RW);
     constexpr int TP = CW + V, WP = CB + V;  // pitches of a tile and of the weights
     constexpr int NR = 8 / WR;               // rows a lane loads
-    __shared__ __attribute__((aligned(16))) S tile[WC][kLoraRows * TP];
+    constexpr int WG = 4 / (WR * WC), ROWS = WG * kLoraRows;
+    __shared__ __attribute__((aligned(16))) S tile[WC * WG][kLoraRows * TP];
     __shared__ __attribute__((aligned(16))) S wl[RP * WP];
     __shared__ __attribute__((aligned(16))) float red[2][4][kLoraRows * P];
     const LoraItems& it = p.it;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr, j0 = NR * wr;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wc = w % WC, wr = w / WC % WR, first = WG == 1 ? 0 : w / (WC * WR) * kLoraRows, rank0 = 16 * RW * wr, j0 = NR * wr;
     const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.o;
     const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
+    static_assert(sizeof(tile) >= (WG - 1) * WC * WR * 64 * V * RW * 16, "the sums meet there");
     floatx4 acc[V][RW] = {};
     int turn = 0;
     LoraItems::Found seg = it.template find<1>(lo, 0);
@@ -915,8 +952,8 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                     h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
                 }
         };
-        load_h(r0, heven);
-        even.load(p.dy, p.dys, r0, r1, j0, col0 + V * (lane & 15), p.o);
+        load_h(r0 + first, heven);
+        even.load(p.dy, p.dys, r0 + first, r1, j0, col0 + V * (lane & 15), p.o);
         if (p.u) {
             const S* up = static_cast<const S*>(p.up);
             const int64_t all = it.adapters * p.o * p.r;
@@ -933,25 +970,26 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             }
             lds_barrier();
         }
-        load_h(r0 + kLoraRows, hodd);
-        odd.load(p.dy, p.dys, r0 + kLoraRows, r1, j0, col0 + V * (lane & 15), p.o);
-        auto step = [&](int64_t row0, LoraRows<DT, NR>& rows, float (&h)[RW][8]) {
+        load_h(r0 + ROWS + first, hodd);
+        odd.load(p.dy, p.dys, r0 + ROWS + first, r1, j0, col0 + V * (lane & 15), p.o);
+        auto step = [&](int64_t block_row, LoraRows<DT, NR>& rows, float (&h)[RW][8]) {
+            const int64_t row0 = block_row + first;  // the wave's
             // (what follows from the lane is formed anew each time: kept through the loops it
             // would not fit the registers)
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
-            const S* t = tile[wc];
+            const S* t = tile[w / (WC * WR) * WC + wc];
             LoraRows<DT, 8> raw;
             rows.trim(row0, r1, j0, edge, mine, p.o);
-            if (p.u || WR > 1) rows.put(tile[wc], TP, j0);
+            if (p.u || WR > 1) rows.put(const_cast<S*>(t), TP, j0);
             if constexpr (WR == 1) {
                 raw = rows;
                 lora_wave_sync();
             } else {
                 lds_barrier();
             }
-            rows.load(p.dy, p.dys, row0 + 2 * kLoraRows, r1, j0, mine, p.o);
+            rows.load(p.dy, p.dys, row0 + 2 * ROWS, r1, j0, mine, p.o);
             if constexpr (WR > 1) raw.get(t, TP);
             if (p.u) {
                 floatx4 u[2][RW] = {};
@@ -979,13 +1017,15 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
             // (also: the tile has been read; red is not written again before the next one)
             if (p.u || WR > 1) lds_barrier();
             if (p.u) {
-                // (the waves of a rank group stand together)
-                for (int i = threadIdx.x; i < kLoraRows * RP; i += kLoraThreads) {
+                // (the waves of the same rows and ranks stand together)
+                for (int i = threadIdx.x; i < ROWS * RP; i += kLoraThreads) {
                     const int m = i / RP, j = i % RP;
                     float z = 0.0f;
 #pragma unroll
-                    for (int q = 0; q < WC; ++q) z += red[turn][j / (16 * RW) * WC + q][m * P + j % (16 * RW)];
-                    if (row0 + m < r1 && j < p.r) p.u[((int64_t)blockIdx.x * it.n + row0 + m) * p.r + j] = s * z;
+                    for (int q = 0; q < WC; ++q)
+                        z += red[turn][(m / kLoraRows * WR + j / (16 * RW)) * WC + q][m % kLoraRows * P + j % (16 * RW)];
+                    if (block_row + m < r1 && j < p.r)
+                        p.u[((int64_t)blockIdx.x * it.n + block_row + m) * p.r + j] = s * z;
                 }
                 turn ^= 1;
             }
@@ -997,55 +1037,52 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
                         for (int i = 0; i < 8; ++i)
                             if (row0 + 8 * g + i >= r1) h[j][i] = 0.0f;
                 lora_outer<DT, RW>(raw, h, acc);
-                load_h(row0 + 2 * kLoraRows, h);
+                load_h(row0 + 2 * ROWS, h);
             }
         };
-        for (int64_t row0 = r0; row0 < r1; row0 += 2 * kLoraRows) {
+        for (int64_t row0 = r0; row0 < r1; row0 += 2 * ROWS) {
             step(row0, even, heven);
-            if (row0 + kLoraRows < r1) step(row0 + kLoraRows, odd, hodd);
+            if (row0 + ROWS < r1) step(row0 + ROWS, odd, hodd);
         }
-        if (p.pu && col0 < p.o)
+        if (WG > 1 && p.pu) {
+            lds_barrier();
+            lora_gather<WC * WR, WG>(acc, reinterpret_cast<floatx4*>(tile));
+            lds_barrier();  // (the tiles are written again)
+        }
+        if (p.pu && col0 < p.o && first == 0)
             lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
     }
 }
 
-// u's shares, where there are more than the pass over x takes (four at 16 ranks, two
-// from there on: registers): their sum in the first one's place.
-constexpr int lora_shares(int rt) { return rt == 1 ? 4 : 2; }
-__global__ __launch_bounds__(kLoraThreads) static void lora_add_u_kernel(float* u, int64_t n, int parts) {
-    for (int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kLoraThreads * 4)
-        for (int e = 0; e < 4 && i + e < n; ++e) {
-            float s = u[i + e];
-#pragma unroll 4
-            for (int q = 1; q < parts; ++q) s += u[q * n + i + e];
-            u[i + e] = s;
-        }
-}
+// Shares of u that the pass over x adds (registers); of more, their sum comes first.
+constexpr int lora_shares(int rt, int wg) { return wg > 1 ? 1 : rt == 1 ? 4 : 2; }
 
 // The pass over x: dx of the block's columns and the sums of ddown.  The
 // adapter's columns lie in LDS by column.
-template <int DT, int RW, int WR, bool DROP>
+template <int DT, int RW, int WR, int WC, bool DROP>
 __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackArgs p) {
     using N = LoraNum<DT>;
     using S = typename N::S;
     constexpr int RT = RW * WR;
     using K = LoraRanks<DT, RT>;
-    constexpr int V = N::V, CW = 16 * V, WC = 4 / WR, CB = WC * CW, RP = 16 * RT, P = lora_pitch(RP), T = V / 4;
+    constexpr int V = N::V, CW = 16 * V, CB = WC * CW, RP = 16 * RT, P = lora_pitch(RP), T = V / 4;
     constexpr int TP = CW + V, WP = RP + V;  // pitches of a tile and of the weights
     constexpr int NR = 8 / WR;               // rows a lane loads
+    constexpr int WG = 4 / (WR * WC), ROWS = WG * kLoraRows;
     constexpr int BUF = RT == 8 ? 1 : 2;     // (room for two blocks a CU)
     // of the 4 steps of columns x 2 halves of rows of dx, a wave forms QN x NI
     constexpr int QN = WR == 1 ? 4 : 2, NI = WR == 4 ? 1 : 2;
     constexpr int G = CW / 8;                // groups of eight columns
-    constexpr int NU = kLoraRows * RP / kLoraThreads;  // values of u a thread
-    constexpr int SH = lora_shares(RT);                // and the shares of each
-    __shared__ __attribute__((aligned(16))) float ub[BUF][kLoraRows * P];
+    constexpr int NU = ROWS * RP / kLoraThreads;  // values of u a thread
+    constexpr int SH = lora_shares(RT, WG);       // and the shares of each
+    __shared__ __attribute__((aligned(16))) float ub[BUF][ROWS * P];
     __shared__ __attribute__((aligned(16))) S wl[CB * WP];
-    __shared__ __attribute__((aligned(16))) S tile[WR > 1 ? BUF : 1][WR > 1 ? WC : 1][WR > 1 ? kLoraRows * TP : 8];
-    __shared__ uint8_t kept[DROP ? BUF : 1][DROP ? WC : 1][kLoraRows * G];
+    __shared__ __attribute__((aligned(16))) S tile[WR > 1 ? BUF : 1][WR > 1 ? WC * WG : 1][WR > 1 ? kLoraRows * TP : 8];
+    __shared__ uint8_t kept[DROP ? BUF : 1][DROP ? WC * WG : 1][kLoraRows * G];
+    __shared__ floatx4 sums[WG > 1 ? (WG - 1) * WC * WR * V * RW * 64 : 1];
     const LoraItems& it = p.it;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int wc = w % WC, wr = w / WC, rank0 = 16 * RW * wr, j0 = NR * wr;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wc = w % WC, wr = w / WC % WR, wg = WG == 1 ? 0 : w / (WC * WR), rank0 = 16 * RW * wr, j0 = NR * wr;
     const int q0 = WR == 1 ? 0 : WR == 2 ? 2 * wr : wr / 2 * 2, i0 = WR == 4 ? wr & 1 : 0;
     const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.c;
@@ -1069,7 +1106,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
         LoraRows<DT, NR> rows = {};
         u32x4 base[NI][QN] = {};
         float un[SH][NU];
-        // the tile's rows of u (its shares), and of dx_base
+        // the tiles' rows of u (its shares), and the wave's of dx_base
         auto load_u = [&](int64_t row0) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
@@ -1099,7 +1136,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 }
         };
         load_u(r0);
-        if (p.pd) rows.load(p.x, p.xs, r0, r1, j0, col0 + V * (lane & 15), p.c);
+        if (p.pd) rows.load(p.x, p.xs, r0 + wg * kLoraRows, r1, j0, col0 + V * (lane & 15), p.c);
         lds_barrier();
         if (p.dx) {
             const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
@@ -1114,30 +1151,33 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                 }
             }
         }
-        for (int64_t row0 = r0; row0 < r1; row0 += kLoraRows) {
+        for (int64_t block_row = r0; block_row < r1; block_row += ROWS) {
+            const int64_t row0 = block_row + wg * kLoraRows;  // the wave's
             // (what follows from the lane is formed anew each time: kept through the loops it
             // would not fit the registers)
             int ln = lane;
             asm volatile("" : "+v"(ln));
             const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
             float* f = ub[turn];
-            S* t = tile[WR > 1 ? turn : 0][WR > 1 ? wc : 0];
-            uint8_t* keep = kept[DROP ? turn : 0][DROP ? wc : 0];
+            S* t = tile[WR > 1 ? turn : 0][WR > 1 ? wg * WC + wc : 0];
+            uint8_t* keep = kept[DROP ? turn : 0][DROP ? wg * WC + wc : 0];
             turn = BUF == 2 ? turn ^ 1 : 0;
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
                 const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
-                float z = un[0][i] + un[1][i];
+                float z = un[0][i];
+                if constexpr (SH >= 2) z += un[1][i];
                 if constexpr (SH == 4) z += un[2][i] + un[3][i];
                 f[m * P + j] = z;
             }
+            f += wg * kLoraRows * P;
             // (loads return in order: u, wanted first, before dx_base and the next rows)
-            load_u(row0 + kLoraRows);
-            if (p.dx && p.base) load_base(row0, n16, g);
+            load_u(block_row + ROWS);
+            if (p.dx && p.base && (WG == 1 || row0 < r1)) load_base(row0, n16, g);
             LoraRows<DT, 8> raw;
             LoraRows<DT, NR> now = rows;
             if (p.pd) {
-                rows.load(p.x, p.xs, row0 + kLoraRows, r1, j0, mine, p.c);
+                rows.load(p.x, p.xs, row0 + ROWS, r1, j0, mine, p.c);
                 now.trim(row0, r1, j0, edge, mine, p.c);
             }
             if (DROP) {
@@ -1160,7 +1200,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                     for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
                 lora_outer<DT, RW>(raw, b, acc);
             }
-            if (p.dx) {
+            if (p.dx && (WG == 1 || row0 < r1)) {
                 if (p.base)
 #pragma unroll
                     for (int i = 0; i < NI; ++i)
@@ -1231,7 +1271,8 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
             }
             if (BUF == 1) lds_barrier();
         }
-        if (p.pd && col0 < p.c)
+        if (WG > 1 && p.pd) lora_gather<WC * WR, WG>(acc, sums);
+        if (p.pd && col0 < p.c && wg == 0)
             lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
                                DROP ? p.factor : 1.0f);
     }
@@ -1239,25 +1280,27 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
 
 template <int DT>
 hipError_t lora_back_out(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
-    const int rt = lora_rank_tiles(p.r);
-    if (rt == 1) lora_back_out_kernel<DT, 1, 1><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 2) lora_back_out_kernel<DT, 1, 2><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 4) lora_back_out_kernel<DT, 1, 4><<<grid, kLoraThreads, 0, s>>>(p);
-    else lora_back_out_kernel<DT, 2, 4><<<grid, kLoraThreads, 0, s>>>(p);
-    if (p.u && p.u_parts > lora_shares(rt)) {
-        const int64_t n = p.it.n * p.r, blocks = (n + 4 * kLoraThreads - 1) / (4 * kLoraThreads);
-        lora_add_u_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), kLoraThreads, 0, s>>>(p.u, n, p.u_parts);
-    }
+    const int rt = lora_rank_tiles(p.r), wc = lora_col_waves(DT, p.r, p.o);
+    if (rt == 1 && wc == 4) lora_back_out_kernel<DT, 1, 1, 4><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 1 && wc == 2) lora_back_out_kernel<DT, 1, 1, 2><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 1) lora_back_out_kernel<DT, 1, 1, 1><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2 && wc == 2) lora_back_out_kernel<DT, 1, 2, 2><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_out_kernel<DT, 1, 2, 1><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_out_kernel<DT, 1, 4, 1><<<grid, kLoraThreads, 0, s>>>(p);
+    else lora_back_out_kernel<DT, 2, 4, 1><<<grid, kLoraThreads, 0, s>>>(p);
     return hipGetLastError();
 }
 
 template <int DT, bool DROP>
 void lora_back_in_rank(hipStream_t s, const LoraBackArgs& p, dim3 grid) {
-    const int rt = lora_rank_tiles(p.r);
-    if (rt == 1) lora_back_in_kernel<DT, 1, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 2) lora_back_in_kernel<DT, 1, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (rt == 4) lora_back_in_kernel<DT, 1, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
-    else lora_back_in_kernel<DT, 2, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    const int rt = lora_rank_tiles(p.r), wc = lora_col_waves(DT, p.r, p.c);
+    if (rt == 1 && wc == 4) lora_back_in_kernel<DT, 1, 1, 4, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 1 && wc == 2) lora_back_in_kernel<DT, 1, 1, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 1) lora_back_in_kernel<DT, 1, 1, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2 && wc == 2) lora_back_in_kernel<DT, 1, 2, 2, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 2) lora_back_in_kernel<DT, 1, 2, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else if (rt == 4) lora_back_in_kernel<DT, 1, 4, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
+    else lora_back_in_kernel<DT, 2, 4, 1, DROP><<<grid, kLoraThreads, 0, s>>>(p);
 }
 
 template <int DT>
