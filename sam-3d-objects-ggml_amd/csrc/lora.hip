@@ -1,6 +1,7 @@
 // lora.hip -- entry points of the low-rank adapters and their gradients
 // (kernels: lora_kernel.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "lora_kernel.h"
 
@@ -10,7 +11,7 @@ namespace {
 
 // Gradients from the slots that the row passes left: adapter a's is the sum over
 // its items and their chunks (slot = chunk + segment), in a fixed order.  A block
-// takes 64 of a slot's floats, sixteen slots at a time.
+// takes 1024 / G of a slot's floats, G slots at a time.
 struct LoraSum {
     const float* part;
     void* dst;
@@ -20,16 +21,16 @@ struct LoraSum {
     int rows_per;
 };
 
-template <int DT>
+template <int DT, int G>
 __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, LoraSum first, LoraSum second, int r, int rt) {
-    constexpr int V = LoraNum<DT>::V;
-    __shared__ floatx4 ls[16][16];
+    constexpr int V = LoraNum<DT>::V, T = kLoraThreads / G;
+    __shared__ floatx4 ls[G][T];
     const LoraSum p = blockIdx.y ? second : first;
     if (!p.dst) return;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, lane = threadIdx.x & 63;
-    const int64_t blocks = p.slot / 64;
+    const int tx = threadIdx.x % T, ty = threadIdx.x / T, lane = threadIdx.x & 63;
+    const int64_t blocks = p.slot / (4 * T);
     for (int64_t w = blockIdx.x; w < blocks * it.adapters; w += gridDim.x) {
-        const int64_t a = w / blocks, e0 = w % blocks * 64 + 4 * tx;
+        const int64_t a = w / blocks, e0 = w % blocks * (4 * T) + 4 * tx;
         floatx4 s = {0, 0, 0, 0};
         for (int64_t i0 = 0; i0 < it.items; i0 += 64) {
             const int64_t i = i0 + lane, v = it.off ? i + 1 : i;
@@ -44,20 +45,20 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
                 const int64_t seg = i0 + k + (it.off ? 1 : 0);
                 const int64_t j0 = __shfl(mine0, k) + seg, j1 = __shfl(mine1, k) + seg;
 #pragma unroll 4
-                for (int64_t j = j0 + ((ty - j0) & 15); j <= j1; j += 16)
+                for (int64_t j = j0 + ((ty - j0) & (G - 1)); j <= j1; j += G)
                     s += *reinterpret_cast<const floatx4*>(p.part + j * p.slot + e0);
             }
         }
         ls[ty][tx] = s;
         __syncthreads();
-        if (threadIdx.x < 64) {
-            const int64_t at = w % blocks * 64 + threadIdx.x, tile = at >> 8;
+        if (threadIdx.x < 4 * T) {
+            const int64_t at = w % blocks * (4 * T) + threadIdx.x, tile = at >> 8;
             const int i = threadIdx.x & 3, n = (int)(at >> 2) & 63;
             const int64_t col = tile / (V * rt) * (16 * V) + V * (4 * (n >> 4) + i) + tile % V;
             const int rank = (int)(tile / V % rt) * 16 + (n & 15);
             float z = 0.0f;
 #pragma unroll
-            for (int q = 0; q < 16; ++q) z += ls[q][threadIdx.x >> 2][i];
+            for (int q = 0; q < G; ++q) z += ls[q][threadIdx.x >> 2][i];
             if (col < p.c && rank < r) {
                 using S = typename LoraNum<DT>::S;
                 S* d = static_cast<S*>(p.dst) + a * p.c * r + (p.along ? rank * (int64_t)p.c + col : col * r + rank);
@@ -71,13 +72,12 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
 
 // The sum of u's shares in the first one's place.
 __global__ __launch_bounds__(kLoraThreads) void lora_add_u_kernel(float* u, int64_t n, int parts) {
-    for (int64_t i = ((int64_t)blockIdx.x * kLoraThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kLoraThreads * 4)
-        for (int e = 0; e < 4 && i + e < n; ++e) {
-            float s = u[i + e];
-#pragma unroll 4
-            for (int q = 1; q < parts; ++q) s += u[q * n + i + e];
-            u[i + e] = s;
-        }
+    for (int64_t i = (int64_t)blockIdx.x * kLoraThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kLoraThreads) {
+        float s = u[i];
+#pragma unroll 16
+        for (int q = 1; q < parts; ++q) s += u[q * n + i];
+        u[i] = s;
+    }
 }
 
 // How a call is split, from its sizes alone.
@@ -427,7 +427,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
                                  : lora_back_out_f32(s, p, out);
         p.rows_per = b.rows_c;
         if (err == hipSuccess && p.u && p.u_parts > lora_shares(lora_rank_tiles(p.r), lora_row_waves(dtype, p.r, p.c))) {
-            const int64_t all = n * p.r, blocks = std::min<int64_t>(ceil_div(all, 4 * kLoraThreads), 4096);
+            const int64_t all = n * p.r, blocks = std::min<int64_t>(ceil_div(all, kLoraThreads), 1 << 14);
             lora_add_u_kernel<<<(unsigned)blocks, kLoraThreads, 0, s>>>(p.u, all, p.u_parts);
             err = hipGetLastError();
             p.u_parts = 1;
@@ -439,11 +439,19 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     }
     if (err == hipSuccess && !b.few && (ddown || dup)) {
         const LoraSum d = {p.pd, ddown, b.slot_c, p.c, 1, b.rows_c}, u = {p.pu, dup, b.slot_o, p.o, 0, b.rows_o};
-        const dim3 grid((unsigned)std::min<int64_t>(std::max(d.slot, u.slot) / 64 * q.n_adapters, 1 << 20), 2);
         const int rt = lora_rank_tiles(q.rank);
-        if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
-        else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
-        else lora_sum_kernel<SPC_F32><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+        auto sum = [&](auto g) {
+            constexpr int G = g.value;
+            const dim3 grid((unsigned)std::min<int64_t>(std::max(d.slot, u.slot) / (1024 / G) * q.n_adapters, 1 << 20), 2);
+            if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+            else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+            else lora_sum_kernel<SPC_F32, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
+        };
+        // Few slots an adapter are wide work, many are long (us of the whole call, four groups
+        // of slots / sixteen: two slots of 8192 columns rank 64 33 / 48, eight 85 / 98, two of
+        // 16,384 rank 32 36 / 45, 490 of 64 rank 16 41 / 33).
+        if (std::max(b.chunks_o, b.chunks_c) + q.n_items <= 32 * q.n_adapters) sum(std::integral_constant<int, 4>{});
+        else sum(std::integral_constant<int, 16>{});
         err = hipGetLastError();
     }
     if (err == hipSuccess) err = lora_copy(s, dtype, narrow.out);
