@@ -128,13 +128,14 @@ struct LoraBackPlan {
 LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, int64_t c, int64_t o, int64_t r) {
     LoraBackPlan q{};
     // Tiles of 32 rows of one item cost some 0.2 us an item, however short, and the sums
-    // behind them; gathered, an adapter's rows wait one after the other, some 8 us for each
-    // 32 of them (us, gathered / tiles, 1024 -> 1024 rank 16 bf16: 32 rows of one item 19 /
-    // 21, 128 of one 42 / 21; 512 of 256 items and 8 adapters 41 / 78, of 16 items 41 / 28,
-    // of 16 items and 2 adapters 69 / 23; 1024 of 512 and 8 67 / 124, of 64 and 8 56 / 50;
-    // 8192 of 2048 and 8 378 / 431, of 1024 and 8 332 / 223; 4096 one-row items of one
-    // adapter 1886 / 1272, of eight 318 / 892, of 1024 1489 / 9199).
-    q.few = n <= std::min(32 * items, std::min(items, adapters) * (64 + items / 2));
+    // behind them; gathered, an adapter's rows wait one after the other, some 9 us for each
+    // 32 of them (us, gathered / tiles, 1024 -> 1024 rank 16 bf16: 32 rows of one item 16 /
+    // 18, 64 of one 22 / 18, 64 one-row items and four adapters 21 / 30; 512 rows of 256
+    // items and 8 adapters 42 / 76, of 16 and 8 46 / 22, of 16 and 2 70 / 22; 1024 of 512
+    // and 8 66 / 123, of 64 and 8 48 / 50; 8192 of 2048 and 8 386 / 442, of 1024 and 8 340 /
+    // 220; 4096 one-row items of one adapter 1890 / 1263, of eight 321 / 890, of 1024 1489 /
+    // 2619).
+    q.few = n <= std::min(32 * items, std::min(items, adapters) * (32 + items / 2));
     if (q.few) {
         int64_t chunks = 1;
         while (chunks * (dt == SPC_F32 ? 4 : 8) < r) chunks *= 2;

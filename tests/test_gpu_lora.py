@@ -194,7 +194,7 @@ def test_many_short_items(spc, dev, dt, n, rows, k):
     Case(dev, dt, n, 75, 136, 40, k=k, offsets=off, adapters=ids, p=0.2).check(spc._native)
 
 
-@pytest.mark.parametrize("k", [3, 12])
+@pytest.mark.parametrize("k", [3, 20])
 @pytest.mark.parametrize("dt", list(DT))
 def test_many_rows_without_an_adapter(spc, dev, dt, k):
     """Hundreds of them in short items, gathered in several rounds, and behind the
