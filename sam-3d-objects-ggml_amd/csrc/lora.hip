@@ -105,6 +105,10 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
         const int64_t blocks = std::min(std::max<int64_t>(want / busy, 1), ceil_div(width, unit));
         return ceil_div(ceil_div(width, blocks), unit) * unit;
     };
+    // Blocks that share a tile, each of 8 steps of columns or more (us in a graph): by 128 /
+    // 256 / 384 / 512 / 1024 of them 64 one-row requests 1024 -> 4096 rank 16 11.4 / 8.8 / 8.4
+    // / 8.7 / 10.4; in two kernels, 256 / 512 / 1024, 8 of 8192 -> 16,384 rank 64 13.8 / 12.5 /
+    // 12.5; one row of 1024 -> 2048, 8 steps / 16, 4.8 / 5.5.
     q.splits = 1;
     q.k_per = (int)c;
     if (q.mode == kLoraShrink) {
@@ -140,7 +144,9 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
         int64_t chunks = 1;
         while (chunks * (dt == SPC_F32 ? 4 : 8) < r) chunks *= 2;
         const int64_t lines = kLoraThreads / chunks;
-        // (u of few rows is one wait after the other along the outputs, of many enough blocks)
+        // A row's u by one block is one wait after the other along the outputs (us of the call by
+        // one block / 128 over the rows: 1 row 8192 -> 16,384 rank 64 109 / 28, 7 of 8192 -> 8192
+        // 63 / 24, 16 of 4096 -> 4096 rank 16 18.6 / 14.8).
         q.shares = (int)std::min({(int64_t)8, ceil_div(o, lines * 8), std::max<int64_t>(1, 128 / std::max<int64_t>(n, 1))});
         q.o_per = (int)ceil_div(o, q.shares);
         q.u = (size_t)(q.shares * n * r);

