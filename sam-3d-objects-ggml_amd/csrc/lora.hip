@@ -94,13 +94,17 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
     // (us in a graph, 1024 -> 1024 rank 16 bf16, 32 / 16: 4096 rows 15.2 / 9.5, 16,384
     // 21.3 / 22.3; 30,000 rank 32 38.6 / 45.2).
     q.mt = n / items >= 32 && n >= 384 * 32 ? kLoraRowTiles : 1;
+    // Ranks 33 to 64, whose adapters are most of a tile's traffic and whose sums still fit LDS
+    // twice (us, tiles of 64 / 32: 1024 -> 1024 rank 64 bf16 20,000 rows 41 / 41, 30,000 42 / 53,
+    // 50,000 81 / 97; 16,000 of 2048 -> 512 59 / 36, 25,000 49 / 63; f32 30,000 137 / 144).
+    if (lora_rank_tiles(r) == 4 && n / items >= 64 && n >= 384 * 64) q.mt = 2 * kLoraRowTiles;
     const int64_t rows = 16 * q.mt, busy = std::max<int64_t>(1, std::max(ceil_div(n, rows), std::min(items, n)));
     q.tiles = n / rows + items + 3;
     // One kernel, each of whose column blocks forms the tile's hidden rows again, or two:
     // one where the tiles fill the device or are little work (us, one / two: 1024 x 1024 ->
     // 1024 rank 16 8.0 / 9.0, 4 items 1024 -> 4096 rank 64 8.2 / 8.4, 1024 x 4096 -> 1024
     // rank 32 27 / 18, 8 items 8192 -> 16,384 rank 64 f16 69 / 12.3).
-    q.mode = busy >= 256 || c * (16 + r) * float_size(dt) <= 200000 ? kLoraFused : kLoraShrink;
+    q.mode = q.mt > 1 || busy >= 256 || c * (16 + r) * float_size(dt) <= 200000 ? kLoraFused : kLoraShrink;
     auto share = [&](int64_t width, int64_t unit, int64_t want) {  // columns a block
         const int64_t blocks = std::min(std::max<int64_t>(want / busy, 1), ceil_div(width, unit));
         return ceil_div(ceil_div(width, blocks), unit) * unit;

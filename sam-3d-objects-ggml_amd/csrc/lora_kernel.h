@@ -130,7 +130,7 @@ struct LoraBackArgs {
 };
 
 // Launches, one for each of the rows' dtypes (lora_bf16.hip, ...).  mt: row tiles
-// of 16 in a block's tile, 1 or kLoraRowTiles.
+// of 16 in a block's tile, 1 or kLoraRowTiles, of ranks 33 to 64 twice as many too.
 enum { kLoraFused, kLoraShrink, kLoraExpand };
 #define LORA_LAUNCHERS(D)                                                                             \
     hipError_t lora_forward_##D(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3 grid);       \
@@ -693,10 +693,10 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
 // dropout's mask; one row of 1024 to 2048 4.8 us in a graph, where an empty kernel is
 // some 2.5.
 template <int DT, int RT, int MT, int MODE, bool DROP>
-__global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) {
+__global__ __launch_bounds__(kLoraThreads, 2) void lora_forward_kernel(LoraArgs p) {
     constexpr int R = 16 * MT, P = lora_pitch(16 * RT);
     __shared__ __attribute__((aligned(16))) float red[4 * R * P];
-    __shared__ __attribute__((aligned(16))) float hid[MODE == kLoraShrink ? 4 : R * P];
+    float* hid = red;  // (the sums' own places)
     const LoraItems& it = p.it;
     const LoraItems::Found seg = it.template find<R>(blockIdx.x, 1);
     const int64_t row0 = seg.begin + (blockIdx.x - seg.begin / R - seg.v) * R;
@@ -744,13 +744,21 @@ __global__ __launch_bounds__(kLoraThreads) void lora_forward_kernel(LoraArgs p) 
     }
 }
 
+// (Tiles of more than 16 rows are of so many rows that they go in one kernel.)
 template <int DT, int RT, int MT>
 void lora_forward_mode(hipStream_t s, const LoraArgs& p, int mode, dim3 grid) {
-    if (mode == kLoraExpand) lora_forward_kernel<DT, RT, MT, kLoraExpand, false><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (mode == kLoraShrink && p.drop)
-        lora_forward_kernel<DT, RT, MT, kLoraShrink, true><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (mode == kLoraShrink) lora_forward_kernel<DT, RT, MT, kLoraShrink, false><<<grid, kLoraThreads, 0, s>>>(p);
-    else if (p.drop) lora_forward_kernel<DT, RT, MT, kLoraFused, true><<<grid, kLoraThreads, 0, s>>>(p);
+    if constexpr (MT == 1) {
+        if (mode == kLoraExpand) {
+            lora_forward_kernel<DT, RT, MT, kLoraExpand, false><<<grid, kLoraThreads, 0, s>>>(p);
+            return;
+        }
+        if (mode == kLoraShrink) {
+            if (p.drop) lora_forward_kernel<DT, RT, MT, kLoraShrink, true><<<grid, kLoraThreads, 0, s>>>(p);
+            else lora_forward_kernel<DT, RT, MT, kLoraShrink, false><<<grid, kLoraThreads, 0, s>>>(p);
+            return;
+        }
+    }
+    if (p.drop) lora_forward_kernel<DT, RT, MT, kLoraFused, true><<<grid, kLoraThreads, 0, s>>>(p);
     else lora_forward_kernel<DT, RT, MT, kLoraFused, false><<<grid, kLoraThreads, 0, s>>>(p);
 }
 
@@ -760,6 +768,7 @@ hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3
     constexpr int M = kLoraRowTiles;
     if (rt == 1) mt == 1 ? lora_forward_mode<DT, 1, 1>(s, p, mode, grid) : lora_forward_mode<DT, 1, M>(s, p, mode, grid);
     else if (rt == 2) mt == 1 ? lora_forward_mode<DT, 2, 1>(s, p, mode, grid) : lora_forward_mode<DT, 2, M>(s, p, mode, grid);
+    else if (rt == 4 && mt == 2 * M) lora_forward_mode<DT, 4, 2 * M>(s, p, mode, grid);
     else if (rt == 4) mt == 1 ? lora_forward_mode<DT, 4, 1>(s, p, mode, grid) : lora_forward_mode<DT, 4, M>(s, p, mode, grid);
     else mt == 1 ? lora_forward_mode<DT, 8, 1>(s, p, mode, grid) : lora_forward_mode<DT, 8, M>(s, p, mode, grid);
     return hipGetLastError();

@@ -160,6 +160,15 @@ def test_large_values_beside_small(spc, dev, dt):
     q.check(nat)
 
 
+@pytest.mark.parametrize("r", [33, 64])
+@pytest.mark.parametrize("dt", list(DT))
+def test_large_tiles(spc, dev, dt, r):
+    """So many rows of such ranks that a block takes 64 of them; few columns, so that the
+    64-bit form is quick."""
+    Case(dev, dt, 25_003, 40, 72, r, k=2, offsets=[5, 70, 12_000, 24_990], adapters=[1, -1, 0], p=0.2).check(spc._native)
+    Case(dev, dt, 24_576, 33, 8, r, base=False).check(spc._native)
+
+
 @pytest.mark.parametrize("c,o", [(1, 64), (4, 136), (7, 8), (8, 7), (200, 3), (520, 1), (5, 6), (1, 1)])
 @pytest.mark.parametrize("dt", list(DT))
 def test_narrow_rows(spc, dev, dt, c, o):
