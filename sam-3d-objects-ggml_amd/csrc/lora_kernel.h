@@ -13,7 +13,7 @@
 // large copy 5.15); its gradients' pass over dy 38 us (128 MB and 24 of u and sums,
 // 4.0 TB/s), over x 92 (385 MB, 4.2 TB/s; the dropout's mask is 8 of them), the sums 9.
 // Larger ranks cost the adapters' way through L2 for each tile of rows (30,000 x 1024, rank
-// 16 / 64 / 128: 35 / 53 / 104 us, gradients 69 / 123 / 203), rows of 16-bit elements at
+// 16 / 64 / 128: 35 / 44 / 81 us, gradients 69 / 123 / 203), rows of 16-bit elements at
 // odd addresses twice the time (1023 to 1021: 75, 106).
 //
 // 16-bit rows meet 16-bit weights exactly (F32 sums).  h and u stay F32, and
@@ -682,6 +682,11 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
     }
 }
 
+// Blocks a CU: two, or as many more as fit; one for F32 rows and the largest ranks, whose
+// registers for two cost more than the second gives (30,000 x 1024 rank 128, one / two:
+// 235 / 256 us; BF16 104 / 81).
+constexpr int lora_forward_blocks(int dt, int rt, int mt) { return dt == SPC_F32 && rt == 8 && mt > 1 ? 1 : 2; }
+
 // A block takes a tile of 16 MT rows of one segment (tile numbers begin at
 // begin / rows + segment, so that no segment's meet another's whatever their
 // lengths) and, by MODE, forms their hidden rows and from them `col_per` columns
@@ -693,7 +698,7 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
 // dropout's mask; one row of 1024 to 2048 4.8 us in a graph, where an empty kernel is
 // some 2.5.
 template <int DT, int RT, int MT, int MODE, bool DROP>
-__global__ __launch_bounds__(kLoraThreads, 2) void lora_forward_kernel(LoraArgs p) {
+__global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void lora_forward_kernel(LoraArgs p) {
     constexpr int R = 16 * MT, P = lora_pitch(16 * RT);
     __shared__ __attribute__((aligned(16))) float red[4 * R * P];
     float* hid = red;  // (the sums' own places)
