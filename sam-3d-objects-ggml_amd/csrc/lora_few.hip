@@ -29,6 +29,26 @@ __device__ __forceinline__ void few_put(void* p, int64_t i, float v) {
     else static_cast<uint16_t*>(p)[i] = DT == SPC_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
 }
 
+// RJ values times f, `left` of which are the row's.
+template <int DT, int RJ>
+__device__ __forceinline__ void few_put_ranks(void* p, int64_t at, const float (&v)[RJ], float f, int left) {
+    using S = typename LoraNum<DT>::S;
+    constexpr int V = LoraNum<DT>::V;
+    if constexpr (RJ >= V) {
+#pragma unroll
+        for (int i = 0; i < RJ; i += V) {
+            float z[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] = f * v[i + e];
+            if (i < left) lora_store(static_cast<S*>(p) + at + i, lora_round<DT>(z), left - i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RJ; ++i)
+            if (i < left) few_put<DT>(p, at + i, f * v[i]);
+    }
+}
+
 // Threads along the ranks (V each, to a power of two of them), the rest along the
 // outputs.
 template <int DT>
@@ -206,10 +226,14 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
         __syncthreads();
         if (none || !grad || !on) continue;
         const float f = in ? (drop ? p.factor : 1.0f) : p.scale ? p.scale[a] : 1.0f;
+        if (in) {
 #pragma unroll
-        for (int i = 0; i < RJ; ++i) {
-            const int j = j0 + i;
-            if (j < p.r) few_put<DT>(grad, in ? (a * p.r + j) * p.c + col : (a * p.o + col) * p.r + j, f * acc[i]);
+            for (int i = 0; i < RJ; ++i)
+                if (j0 + i < p.r) few_put<DT>(grad, (a * p.r + j0 + i) * p.c + col, f * acc[i]);
+        } else {
+            // (a column's ranks stand together: 16 bytes of them in a store, 34 one-row items of
+            // 17 to 3712, rank 128 and 16 adapters 79 us one by one, so 46)
+            few_put_ranks<DT, RJ>(grad, (a * p.o + col) * p.r + j0, acc, f, p.r - j0);
         }
     }
 }

@@ -192,6 +192,7 @@ struct LoraNum {
 // 16 bytes that lie inside the row, without a branch, and, only in blocks that hold
 // a row's end, what moves them into place and clears what is past it.  (With a
 // branch at each load the backward kernels spilled the masks of all of them.)
+typedef float floatx4_rows __attribute__((ext_vector_type(4), aligned(4)));  // (at any float)
 template <typename S>
 __device__ __forceinline__ u32x4 lora_shift(u32x4 w, int by) {
     constexpr int V = 16 / (int)sizeof(S);
@@ -720,14 +721,26 @@ __global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void
         const int k1 = MODE == kLoraShrink ? min(k0 + p.k_per, p.c) : p.c;
         lora_shrink<DT, RT, MT, DROP>(p, t, k0, k1, red);
     } else {
-        // a wave takes every fourth share, so that few rows wait for few of them in turn
-        const int w = threadIdx.x >> 6;
-        for (int i = threadIdx.x & 63; i < t.m * p.r; i += 64) {
-            const float* q = p.part + row0 * p.r + i;
-            float s = 0.0f;
+        // a wave takes every fourth share, so that few rows wait for few of them in turn, 16
+        // bytes a lane (a value a lane, 40 rows of F32 rank 128 to 2368 71 us, so 32)
+        const int w = threadIdx.x >> 6, all = t.m * p.r;
+        for (int i = 4 * (threadIdx.x & 63); i < all; i += 256) {
+            const int from = max(min(i, all - 4), 0);  // (a hidden row alone may hold fewer)
+            const float* q = p.part + row0 * p.r + from;
+            floatx4 s = {0, 0, 0, 0};
+            if (all >= 4) {
 #pragma unroll 8
-            for (int k = w; k < p.splits; k += 4) s += q[(int64_t)k * it.n * p.r];
-            red[(w * R + i / p.r) * P + i % p.r] = s;
+                for (int k = w; k < p.splits; k += 4)
+                    s += *reinterpret_cast<const floatx4_rows*>(q + (int64_t)k * it.n * p.r);
+            } else {
+                for (int k = w; k < p.splits; k += 4)
+                    for (int e = 0; e < all; ++e) s[e] += q[(int64_t)k * it.n * p.r + e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at = from + e;
+                if (at < all) red[(w * R + at / p.r) * P + at % p.r] = s[e];
+            }
         }
     }
     __syncthreads();
