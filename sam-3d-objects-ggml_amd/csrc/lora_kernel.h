@@ -162,13 +162,16 @@ constexpr int kLoraRowTiles = 2;
 inline int lora_rank_waves(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 // columns of one such wave
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
-// and the waves along columns: half of them where the rows are no wider than half of them
-// take, the others along rows (us of the gradients, so / all along columns: 200,000 x 64
-// to 64 rank 16 bf16 60 / 123, 62,710 x 96 to 160 f32 58 / 71)
+// and the waves along columns: half of them where the last block of all would use no
+// more, one for rows no wider than its own, the others along rows (us of the gradients, so /
+// all along columns, rank 16 bf16: 200,000 x 64 to 64 60 / 123, 53,333 x 576 77 / 85, 40,000 x
+// 768 71 / 74, 27,927 x 1100 86 / 90; where the last block uses more, 34,133 x 900 88 / 84,
+// 21,818 x 1408 75 / 76)
 inline int lora_col_waves(int dt, int64_t r, int64_t width) {
+    const int64_t tiles = (width + lora_wave_cols(dt) - 1) / lora_wave_cols(dt);
     int w = 4 / lora_rank_waves(r);
-    while (w > 1 && w / 2 * lora_wave_cols(dt) >= width) w /= 2;
-    return w;
+    if (w == 4 && (tiles - 1) % 4 < 2) w = 2;
+    return tiles == 1 ? 1 : w;
 }
 inline int lora_row_waves(int dt, int64_t r, int64_t width) {
     return 4 / lora_rank_waves(r) / lora_col_waves(dt, r, width);
@@ -1093,7 +1096,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
 }
 
 // Shares of u that the pass over x adds (registers); of more, their sum comes first.
-constexpr int lora_shares(int rt, int wg) { return wg > 1 ? 1 : rt == 1 ? 4 : 2; }
+constexpr int lora_shares(int rt, int wg) { return wg > 2 ? 1 : wg == 2 || rt > 1 ? 2 : 4; }
 
 // The pass over x: dx of the block's columns and the sums of ddown.  The
 // adapter's columns lie in LDS by column.
