@@ -739,10 +739,14 @@ __global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void
                 for (int k = w; k < p.splits; k += 4)
                     for (int e = 0; e < all; ++e) s[e] += q[(int64_t)k * it.n * p.r + e];
             }
+            int m = from / p.r, j = from - m * p.r;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int at = from + e;
-                if (at < all) red[(w * R + at / p.r) * P + at % p.r] = s[e];
+                if (from + e < all) red[(w * R + m) * P + j] = s[e];
+                if (++j == p.r) {
+                    j = 0;
+                    ++m;
+                }
             }
         }
     }
