@@ -10,7 +10,7 @@ namespace spc {
 namespace {
 
 // Gradients from the slots that the row passes left: adapter a's is the sum over
-// its items and their chunks (slot = chunk + segment), in a fixed order.  A block
+// its items and their chunks (lora_chunk_row), in a fixed order.  A block
 // takes 1024 / G of a slot's floats, G slots at a time.
 struct LoraSum {
     const float* part;
@@ -39,11 +39,11 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
                 b = it.begin(v);
                 e = it.end(v);
             }
-            const int mine0 = (int)b / p.rows_per, mine1 = (int)(e - 1) / p.rows_per;
+            const int mine0 = (int)b / p.rows_per, more = (int)(e - b - 1) / p.rows_per;
             for (uint64_t m = __ballot(b < e); m; m &= m - 1) {
                 const int k = __builtin_ctzll(m);
                 const int64_t seg = i0 + k + (it.off ? 1 : 0);
-                const int64_t j0 = __shfl(mine0, k) + seg, j1 = __shfl(mine1, k) + seg;
+                const int64_t j0 = __shfl(mine0, k) + seg, j1 = j0 + __shfl(more, k);
 #pragma unroll 4
                 for (int64_t j = j0 + ((ty - j0) & (G - 1)); j <= j1; j += G)
                     s += *reinterpret_cast<const floatx4*>(p.part + j * p.slot + e0);
@@ -161,21 +161,23 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
     // Some two blocks a CU: the registers hold no more of them at once, and every further
     // chunk is a slot to write and add (us of 62,710 x 1024 rank 16 bf16 by blocks: 256 155,
     // 384 157, 512 138, 640 166, 768 157, 1024 144).
+    // A block's chunk is of one item, whose last is shorter: some chunks fewer, so that those
+    // do not make a second round.
     auto rows = [&](int64_t blocks, int64_t width) {
         const int64_t tile = kLoraRows * lora_row_waves(dt, r, width);
-        int64_t per = std::max<int64_t>(1, ceil_div(n, std::max<int64_t>(1, 512 / blocks)));
-        if (n / items >= tile || per >= tile) per = ceil_div(per, tile) * tile;
+        const int64_t chunks = std::max<int64_t>(1, 512 / blocks), more = std::min(items, chunks / 2);
+        const int64_t per = ceil_div(ceil_div(n, chunks - more), tile) * tile;
         return (int)per;
     };
     q.rows_o = rows(q.blocks_o, o);
     q.rows_c = rows(q.blocks_c, c);
-    q.chunks_o = ceil_div(n, q.rows_o);
-    q.chunks_c = ceil_div(n, q.rows_c);
+    q.chunks_o = n / q.rows_o + items + 3;
+    q.chunks_c = n / q.rows_c + items + 3;
     q.u = (size_t)(q.blocks_o * n * r);
     q.slot_o = lora_slot(o, lora_wave_cols(dt), lora_rank_tiles(r));
     q.slot_c = lora_slot(c, lora_wave_cols(dt), lora_rank_tiles(r));
-    q.pu = (size_t)((q.chunks_o + items + 2) * q.slot_o);
-    q.pd = (size_t)((q.chunks_c + items + 2) * q.slot_c);
+    q.pu = (size_t)(q.chunks_o * q.slot_o);
+    q.pd = (size_t)(q.chunks_c * q.slot_c);
     return q;
 }
 
@@ -431,12 +433,19 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     hipError_t err = lora_copy(s, dtype, narrow.in);
     if (err == hipSuccess && b.few) err = lora_few_backward(s, dtype, p, b.o_per, ddown, dup);
     if (err == hipSuccess && !b.few && n > 0) {
-        const dim3 out((unsigned)b.blocks_o, (unsigned)b.chunks_o), in((unsigned)b.blocks_c, (unsigned)b.chunks_c);
+        const int64_t blocks = std::max(b.blocks_o * b.chunks_o, b.blocks_c * b.chunks_c);
+        if (blocks > INT32_MAX) {
+            set_last_error("%s: more than 2^31 blocks", fn);
+            return SPC_BAD_SHAPE;
+        }
+        const dim3 out((unsigned)(b.blocks_o * b.chunks_o)), in((unsigned)(b.blocks_c * b.chunks_c));
         p.rows_per = b.rows_o;
+        p.blocks = (int)b.blocks_o;
         err = dtype == SPC_BF16  ? lora_back_out_bf16(s, p, out)
               : dtype == SPC_F16 ? lora_back_out_f16(s, p, out)
                                  : lora_back_out_f32(s, p, out);
         p.rows_per = b.rows_c;
+        p.blocks = (int)b.blocks_c;
         if (err == hipSuccess && p.u && p.u_parts > lora_shares(lora_rank_tiles(p.r), lora_row_waves(dtype, p.r, p.c))) {
             const int64_t all = n * p.r, blocks = std::min<int64_t>(ceil_div(all, kLoraThreads), 1 << 14);
             lora_add_u_kernel<<<(unsigned)blocks, kLoraThreads, 0, s>>>(p.u, all, p.u_parts);
@@ -461,7 +470,7 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
         // Few slots an adapter are wide work, many are long (us of the whole call, four groups
         // of slots / sixteen: two slots of 8192 columns rank 64 33 / 48, eight 85 / 98, two of
         // 16,384 rank 32 36 / 45, 490 of 64 rank 16 41 / 33).
-        if (std::max(b.chunks_o, b.chunks_c) + q.n_items <= 32 * q.n_adapters) sum(std::integral_constant<int, 4>{});
+        if (std::max(b.chunks_o, b.chunks_c) <= 32 * q.n_adapters) sum(std::integral_constant<int, 4>{});
         else sum(std::integral_constant<int, 16>{});
         err = hipGetLastError();
     }

@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int
     constexpr int V = N::V, UN = 4;
     __shared__ float red[4][kLoraMaxRank];
     const LoraItems& it = p.it;
-    const int64_t row = blockIdx.x, a = it.template find<1>(row, 0).adapter;
+    const int64_t row = blockIdx.x, a = it.find(row, 1, 0).adapter;
     if (a < 0) return;
     const int chunks = few_chunks<DT>(p.r), lines = kLoraThreads / chunks, t = threadIdx.x;
     const int j = t % chunks * V, o1 = min((int)(blockIdx.y + 1) * o_per, p.o);

@@ -55,20 +55,20 @@ struct LoraItems {
         const int64_t a = which ? which[v] : 0;
         return a >= 0 && a < adapters ? a : -1;
     }
-    // The last segment v with begin(v) / R + per v <= t, its rows and adapter (64 probes
+    // The last segment v with begin(v) / rows + per v <= t, its rows and adapter (64 probes
     // at a time, by a whole wave; inside the segments' range whatever the offsets hold).
     // What the last probes' lanes need is read in one go: a wait of its own for each of
     // them is a good part of what few rows take.
     struct Found {
         int64_t v, begin, end, adapter;
     };
-    template <int R>
-    __device__ __forceinline__ Found find(int64_t t, int64_t per) const {
+    __device__ __forceinline__ Found find(int64_t t, int rows, int64_t per) const {
+        auto quotient = [&](int64_t b) { return (int64_t)((uint32_t)b / (uint32_t)rows); };
         const int lane = threadIdx.x & 63;
         int64_t lo = 0, size = segments();
         while (size > 64) {
             const int64_t step = (size + 63) / 64, at = lane * step;
-            const bool ok = at < size && begin(lo + at) / R + per * (lo + at) <= t;
+            const bool ok = at < size && quotient(begin(lo + at)) + per * (lo + at) <= t;
             const int64_t past = max(__popcll(__ballot(ok)), 1) - 1;
             lo += past * step;
             size = min(step, size - past * step);
@@ -76,7 +76,7 @@ struct LoraItems {
         const int64_t v = lo + min((int64_t)lane, size - 1);
         const int64_t b = begin(v), e = end(v);
         const int a = (int)adapter(v);
-        const bool ok = lane < size && b / R + per * v <= t;
+        const bool ok = lane < size && quotient(b) + per * v <= t;
         const int k = max(__popcll(__ballot(ok)), 1) - 1;
         auto pick = [&](int64_t x) {
             return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), k) << 32 |
@@ -123,7 +123,7 @@ struct LoraBackArgs {
     float* pd;         // slots of ddown (lora_slot), null: not wanted
     float* pu;         // of dup
     int c, o, r;
-    int rows_per;
+    int rows_per, blocks;  // rows of a chunk, blocks along columns
     const int64_t* seed;
     uint32_t drop;
     float factor;
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void
     __shared__ __attribute__((aligned(16))) float red[4 * R * P];
     float* hid = red;  // (the sums' own places)
     const LoraItems& it = p.it;
-    const LoraItems::Found seg = it.template find<R>(blockIdx.x, 1);
+    const LoraItems::Found seg = it.find(blockIdx.x, R, 1);
     const int64_t row0 = seg.begin + (blockIdx.x - seg.begin / R - seg.v) * R;
     if (row0 >= seg.end || row0 < 0) return;
     const LoraTile t = {row0, seg.adapter, (int)min((int64_t)R, seg.end - row0)};
@@ -950,6 +950,13 @@ __device__ __forceinline__ void lora_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
+// The first row of chunk number t of the segment that find(t, rows, 1) gave: a segment's
+// chunks of `rows` rows begin at number begin / rows + segment, so that no segment's meet
+// another's whatever their lengths.
+__device__ __forceinline__ int64_t lora_chunk_row(const LoraItems::Found& seg, int64_t t, int rows) {
+    return seg.begin + (t - (uint32_t)seg.begin / (uint32_t)rows - seg.v) * rows;
+}
+
 // The pass over dy: u of the block's columns (one of u_parts shares of the sum),
 // and the sums of dup.  u sums along a row, so its operand is read back from the
 // tile in LDS, and the waves' shares meet there too; the adapter's columns lie in
@@ -968,135 +975,130 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
     const LoraItems& it = p.it;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wc = w % WC, wr = w / WC % WR, first = WG == 1 ? 0 : w / (WC * WR) * kLoraRows, rank0 = 16 * RW * wr, j0 = NR * wr;
-    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
+    const int chunk = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
+    const int block0 = block * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.o;
-    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     static_assert(sizeof(tile) >= (WG - 1) * WC * WR * 64 * V * RW * 16, "the sums meet there");
     floatx4 acc[V][RW] = {};
     int turn = 0;
-    LoraItems::Found seg = it.template find<1>(lo, 0);
-    for (int64_t v = seg.v; v < it.segments(); ++v) {
-        if (v != seg.v) seg = {v, it.begin(v), it.end(v), it.adapter(v)};
-        if (seg.begin >= hi) break;
-        const int64_t r0 = max(seg.begin, lo), r1 = min(seg.end, hi), a = seg.adapter;
-        if (r0 >= r1 || a < 0) continue;
-        const float s = p.scale ? p.scale[a] : 1.0f;
-        // dy and the hidden rows (a wave's ranks) two tiles ahead: with u's way through LDS a
-        // tile takes longer than a load (one tile ahead 40 us of 62,710 x 1024)
-        LoraRows<DT, NR> even, odd;
-        float heven[RW][8], hodd[RW][8];
-        auto load_h = [&](int64_t row0, float (&h)[RW][8]) {
-            if (!p.pu || row0 >= r1) return;
-            const int n16 = lane & 15, g = lane >> 4;
-            const bool full = row0 + kLoraRows <= r1;
+    const LoraItems::Found seg = it.find(chunk, p.rows_per, 1);
+    const int64_t a = seg.adapter, r0 = lora_chunk_row(seg, chunk, p.rows_per), r1 = min(r0 + p.rows_per, seg.end);
+    if (r0 < seg.begin || r0 >= r1 || a < 0) return;
+    const float s = p.scale ? p.scale[a] : 1.0f;
+    // dy and the hidden rows (a wave's ranks) two tiles ahead: with u's way through LDS a
+    // tile takes longer than a load (one tile ahead 40 us of 62,710 x 1024)
+    LoraRows<DT, NR> even, odd;
+    float heven[RW][8], hodd[RW][8];
+    auto load_h = [&](int64_t row0, float (&h)[RW][8]) {
+        if (!p.pu || row0 >= r1) return;
+        const int n16 = lane & 15, g = lane >> 4;
+        const bool full = row0 + kLoraRows <= r1;
 #pragma unroll
-            for (int j = 0; j < RW; ++j)
+        for (int j = 0; j < RW; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t row = row0 + 8 * g + i;
-                    h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
-                }
-        };
-        load_h(r0 + first, heven);
-        even.load(p.dy, p.dys, r0 + first, r1, j0, col0 + V * (lane & 15), p.o);
-        if (p.u) {
-            const S* up = static_cast<const S*>(p.up);
-            const int64_t all = it.adapters * p.o * p.r;
-            lds_barrier();
-            for (int i = threadIdx.x; i < CB * (RP / V); i += kLoraThreads) {
-                const int k = i % CB, j = i / CB * V, col = block0 + k;
-                const int64_t at = (a * p.o + min(col, p.o - 1)) * p.r + j;
-                const u32x4 q = lora_edge_short<S>(lora_fetch_short(up, at, all), at, all, col < p.o ? p.r - j : 0);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if constexpr (V == 4) wl[(j + e) * WP + k] = q[e];
-                    else wl[(j + e) * WP + k] = (S)(q[e / 2] >> (16 * (e & 1)));
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int64_t row = row0 + 8 * g + i;
+                h[j][i] = p.hidden[(full ? row : min(row, r1 - 1)) * p.r + min(rank0 + 16 * j + n16, p.r - 1)];
             }
-            lds_barrier();
+    };
+    load_h(r0 + first, heven);
+    even.load(p.dy, p.dys, r0 + first, r1, j0, col0 + V * (lane & 15), p.o);
+    if (p.u) {
+        const S* up = static_cast<const S*>(p.up);
+        const int64_t all = it.adapters * p.o * p.r;
+        lds_barrier();
+        for (int i = threadIdx.x; i < CB * (RP / V); i += kLoraThreads) {
+            const int k = i % CB, j = i / CB * V, col = block0 + k;
+            const int64_t at = (a * p.o + min(col, p.o - 1)) * p.r + j;
+            const u32x4 q = lora_edge_short<S>(lora_fetch_short(up, at, all), at, all, col < p.o ? p.r - j : 0);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if constexpr (V == 4) wl[(j + e) * WP + k] = q[e];
+                else wl[(j + e) * WP + k] = (S)(q[e / 2] >> (16 * (e & 1)));
+            }
         }
-        load_h(r0 + ROWS + first, hodd);
-        odd.load(p.dy, p.dys, r0 + ROWS + first, r1, j0, col0 + V * (lane & 15), p.o);
-        auto step = [&](int64_t block_row, LoraRows<DT, NR>& rows, float (&h)[RW][8]) {
-            const int64_t row0 = block_row + first;  // the wave's
-            // (what follows from the lane is formed anew each time: kept through the loops it
-            // would not fit the registers)
-            int ln = lane;
-            asm volatile("" : "+v"(ln));
-            const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
-            const S* t = tile[w / (WC * WR) * WC + wc];
-            LoraRows<DT, 8> raw;
-            rows.trim(row0, r1, j0, edge, mine, p.o);
-            if (p.u || WR > 1) rows.put(const_cast<S*>(t), TP, j0);
-            if constexpr (WR == 1) {
-                raw = rows;
-                lora_wave_sync();
-            } else {
-                lds_barrier();
-            }
-            rows.load(p.dy, p.dys, row0 + 2 * ROWS, r1, j0, mine, p.o);
-            if constexpr (WR > 1) raw.get(t, TP);
-            if (p.u) {
-                floatx4 u[2][RW] = {};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    u32x4 wt[RW];
-#pragma unroll
-                    for (int j = 0; j < RW; ++j)
-                        wt[j] = *reinterpret_cast<const u32x4*>(wl + (rank0 + 16 * j + n16) * WP + wc * CW + q * N::STEP +
-                                                                V * g);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const u32x4 d = *reinterpret_cast<const u32x4*>(t + (16 * i + n16) * TP + q * N::STEP + V * g);
-#pragma unroll
-                        for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[j], d, u[i][j]);
-                    }
-                }
-                float* f = red[turn][w];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < RW; ++j)
-                        *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + 16 * j + 4 * g) = u[i][j];
-            }
-            // (also: the tile has been read; red is not written again before the next one)
-            if (p.u || WR > 1) lds_barrier();
-            if (p.u) {
-                // (the waves of the same rows and ranks stand together)
-                for (int i = threadIdx.x; i < ROWS * RP; i += kLoraThreads) {
-                    const int m = i / RP, j = i % RP;
-                    float z = 0.0f;
-#pragma unroll
-                    for (int q = 0; q < WC; ++q)
-                        z += red[turn][(m / kLoraRows * WR + j / (16 * RW)) * WC + q][m % kLoraRows * P + j % (16 * RW)];
-                    if (block_row + m < r1 && j < p.r)
-                        p.u[((int64_t)blockIdx.x * it.n + block_row + m) * p.r + j] = s * z;
-                }
-                turn ^= 1;
-            }
-            if (p.pu) {
-                if (row0 + kLoraRows > r1)
-#pragma unroll
-                    for (int j = 0; j < RW; ++j)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (row0 + 8 * g + i >= r1) h[j][i] = 0.0f;
-                lora_outer<DT, RW>(raw, h, acc);
-                load_h(row0 + 2 * ROWS, h);
-            }
-        };
-        for (int64_t row0 = r0; row0 < r1; row0 += 2 * ROWS) {
-            step(row0, even, heven);
-            if (row0 + ROWS < r1) step(row0 + ROWS, odd, hodd);
-        }
-        if (WG > 1 && p.pu) {
-            lds_barrier();
-            lora_gather<WC * WR, WG>(acc, reinterpret_cast<floatx4*>(tile));
-            lds_barrier();  // (the tiles are written again)
-        }
-        if (p.pu && col0 < p.o && first == 0)
-            lora_flush<DT, RW>(acc, p.pu + (blockIdx.y + v) * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
+        lds_barrier();
     }
+    load_h(r0 + ROWS + first, hodd);
+    odd.load(p.dy, p.dys, r0 + ROWS + first, r1, j0, col0 + V * (lane & 15), p.o);
+    auto step = [&](int64_t block_row, LoraRows<DT, NR>& rows, float (&h)[RW][8]) {
+        const int64_t row0 = block_row + first;  // the wave's
+        // (what follows from the lane is formed anew each time: kept through the loops it
+        // would not fit the registers)
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
+        const S* t = tile[w / (WC * WR) * WC + wc];
+        LoraRows<DT, 8> raw;
+        rows.trim(row0, r1, j0, edge, mine, p.o);
+        if (p.u || WR > 1) rows.put(const_cast<S*>(t), TP, j0);
+        if constexpr (WR == 1) {
+            raw = rows;
+            lora_wave_sync();
+        } else {
+            lds_barrier();
+        }
+        rows.load(p.dy, p.dys, row0 + 2 * ROWS, r1, j0, mine, p.o);
+        if constexpr (WR > 1) raw.get(t, TP);
+        if (p.u) {
+            floatx4 u[2][RW] = {};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                u32x4 wt[RW];
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+                    wt[j] = *reinterpret_cast<const u32x4*>(wl + (rank0 + 16 * j + n16) * WP + wc * CW + q * N::STEP +
+                                                            V * g);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const u32x4 d = *reinterpret_cast<const u32x4*>(t + (16 * i + n16) * TP + q * N::STEP + V * g);
+#pragma unroll
+                    for (int j = 0; j < RW; ++j) u[i][j] = lora_mma<DT>(wt[j], d, u[i][j]);
+                }
+            }
+            float* f = red[turn][w];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+                    *reinterpret_cast<floatx4*>(f + (16 * i + n16) * P + 16 * j + 4 * g) = u[i][j];
+        }
+        // (also: the tile has been read; red is not written again before the next one)
+        if (p.u || WR > 1) lds_barrier();
+        if (p.u) {
+            // (the waves of the same rows and ranks stand together)
+            for (int i = threadIdx.x; i < ROWS * RP; i += kLoraThreads) {
+                const int m = i / RP, j = i % RP;
+                float z = 0.0f;
+#pragma unroll
+                for (int q = 0; q < WC; ++q)
+                    z += red[turn][(m / kLoraRows * WR + j / (16 * RW)) * WC + q][m % kLoraRows * P + j % (16 * RW)];
+                if (block_row + m < r1 && j < p.r)
+                    p.u[((int64_t)block * it.n + block_row + m) * p.r + j] = s * z;
+            }
+            turn ^= 1;
+        }
+        if (p.pu) {
+            if (row0 + kLoraRows > r1)
+#pragma unroll
+                for (int j = 0; j < RW; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (row0 + 8 * g + i >= r1) h[j][i] = 0.0f;
+            lora_outer<DT, RW>(raw, h, acc);
+            load_h(row0 + 2 * ROWS, h);
+        }
+    };
+    for (int64_t row0 = r0; row0 < r1; row0 += 2 * ROWS) {
+        step(row0, even, heven);
+        if (row0 + ROWS < r1) step(row0 + ROWS, odd, hodd);
+    }
+    if (WG > 1 && p.pu) {
+        lds_barrier();
+        lora_gather<WC * WR, WG>(acc, reinterpret_cast<floatx4*>(tile));
+    }
+    if (p.pu && col0 < p.o && first == 0)
+        lora_flush<DT, RW>(acc, p.pu + chunk * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
 }
 
 // Shares of u that the pass over x adds (registers); of more, their sum comes first.
@@ -1129,198 +1131,193 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wc = w % WC, wr = w / WC % WR, wg = WG == 1 ? 0 : w / (WC * WR), rank0 = 16 * RW * wr, j0 = NR * wr;
     const int q0 = WR == 1 ? 0 : WR == 2 ? 2 * wr : wr / 2 * 2, i0 = WR == 4 ? wr & 1 : 0;
-    const int block0 = blockIdx.x * CB, col0 = block0 + wc * CW;
+    const int chunk = blockIdx.x / p.blocks, block0 = blockIdx.x % p.blocks * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.c;
-    const int64_t lo = (int64_t)blockIdx.y * p.rows_per, hi = min(lo + p.rows_per, it.n);
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
     floatx4 acc[V][RW] = {};
     int turn = 0;
-    LoraItems::Found seg = it.template find<1>(lo, 0);
-    for (int64_t v = seg.v; v < it.segments(); ++v) {
-        if (v != seg.v) seg = {v, it.begin(v), it.end(v), it.adapter(v)};
-        if (seg.begin >= hi) break;
-        const int64_t r0 = max(seg.begin, lo), r1 = min(seg.end, hi), a = seg.adapter;
-        if (r0 >= r1) continue;
-        if (a < 0) {
-            if (p.dx && block0 < p.c)
-                for (int64_t row = r0; row < r1; row += kLoraRows)
-                    lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, (int)min((int64_t)kLoraRows, r1 - row), block0,
-                                  min(block0 + CB, p.c));
-            continue;
+    const LoraItems::Found seg = it.find(chunk, p.rows_per, 1);
+    const int64_t a = seg.adapter, r0 = lora_chunk_row(seg, chunk, p.rows_per), r1 = min(r0 + p.rows_per, seg.end);
+    if (r0 < seg.begin || r0 >= r1) return;
+    if (a < 0) {
+        if (p.dx && block0 < p.c)
+            for (int64_t row = r0; row < r1; row += kLoraRows)
+                lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, (int)min((int64_t)kLoraRows, r1 - row), block0,
+                              min(block0 + CB, p.c));
+        return;
+    }
+    LoraRows<DT, NR> rows = {};
+    u32x4 base[NI][QN] = {};
+    float un[SH][NU];
+    // the tiles' rows of u (its shares), and the wave's of dx_base
+    auto load_u = [&](int64_t row0) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
+            const bool on = row0 + m < r1 && j < p.r;
+            const float* q = p.u + (row0 + m) * p.r + j;
+#pragma unroll
+            for (int k = 0; k < SH; ++k) un[k][i] = on && k < p.u_parts ? q[k * it.n * p.r] : 0.0f;
         }
-        LoraRows<DT, NR> rows = {};
-        u32x4 base[NI][QN] = {};
-        float un[SH][NU];
-        // the tiles' rows of u (its shares), and the wave's of dx_base
-        auto load_u = [&](int64_t row0) {
+    };
+    auto load_base = [&](int64_t row0, int n16, int g) {
+        const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
+        const S* from = static_cast<const S*>(p.base) + row0 * p.bs;
 #pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
-                const bool on = row0 + m < r1 && j < p.r;
-                const float* q = p.u + (row0 + m) * p.r + j;
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int k = 0; k < SH; ++k) un[k][i] = on && k < p.u_parts ? q[k * it.n * p.r] : 0.0f;
-            }
-        };
-        auto load_base = [&](int64_t row0, int n16, int g) {
-            const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
-            const S* from = static_cast<const S*>(p.base) + row0 * p.bs;
+            for (int q = 0; q < QN; q += 2) {
+                const int col = col0 + (q0 + q) * N::STEP, first = 16 * (i0 + i);
+                if (!edge) {
+                    lora_fetch_pair(base[i][q], base[i][q + 1], from + min(first, m - 1) * p.bs + col, p.bs,
+                                    max(m - first, 1));
+                } else {
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int q = 0; q < QN; q += 2) {
-                    const int col = col0 + (q0 + q) * N::STEP, first = 16 * (i0 + i);
-                    if (!edge) {
-                        lora_fetch_pair(base[i][q], base[i][q + 1], from + min(first, m - 1) * p.bs + col, p.bs,
-                                        max(m - first, 1));
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            base[i][q + x] = lora_fetch(from + min(first + n16, m - 1) * p.bs, col + x * N::STEP + V * g, p.c);
-                    }
+                    for (int x = 0; x < 2; ++x)
+                        base[i][q + x] = lora_fetch(from + min(first + n16, m - 1) * p.bs, col + x * N::STEP + V * g, p.c);
                 }
-        };
-        load_u(r0);
-        if (p.pd) rows.load(p.x, p.xs, r0 + wg * kLoraRows, r1, j0, col0 + V * (lane & 15), p.c);
+            }
+    };
+    load_u(r0);
+    if (p.pd) rows.load(p.x, p.xs, r0 + wg * kLoraRows, r1, j0, col0 + V * (lane & 15), p.c);
+    lds_barrier();
+    if (p.dx) {
+        const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
+        for (int i = threadIdx.x; i < RP * (CB / V); i += kLoraThreads) {
+            const int j = i % RP, k = i / RP * V, col = block0 + k;
+            const u32x4 w = lora_load(down + (int64_t)min(j, p.r - 1) * p.c, col, p.c);
+            const u32x4 q = j < p.r ? w : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if constexpr (V == 4) wl[(k + e) * WP + j] = q[e];
+                else wl[(k + e) * WP + j] = (S)(q[e / 2] >> (16 * (e & 1)));
+            }
+        }
+    }
+    for (int64_t block_row = r0; block_row < r1; block_row += ROWS) {
+        const int64_t row0 = block_row + wg * kLoraRows;  // the wave's
+        // (what follows from the lane is formed anew each time: kept through the loops it
+        // would not fit the registers)
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
+        float* f = ub[turn];
+        S* t = tile[WR > 1 ? turn : 0][WR > 1 ? wg * WC + wc : 0];
+        uint8_t* keep = kept[DROP ? turn : 0][DROP ? wg * WC + wc : 0];
+        turn = BUF == 2 ? turn ^ 1 : 0;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
+            float z = un[0][i];
+            if constexpr (SH >= 2) z += un[1][i];
+            if constexpr (SH == 4) z += un[2][i] + un[3][i];
+            f[m * P + j] = z;
+        }
+        f += wg * kLoraRows * P;
+        // (loads return in order: u, wanted first, before dx_base and the next rows)
+        load_u(block_row + ROWS);
+        if (p.dx && p.base && (WG == 1 || row0 < r1)) load_base(row0, n16, g);
+        LoraRows<DT, 8> raw;
+        LoraRows<DT, NR> now = rows;
+        if (p.pd) {
+            rows.load(p.x, p.xs, row0 + ROWS, r1, j0, mine, p.c);
+            now.trim(row0, r1, j0, edge, mine, p.c);
+        }
+        if (DROP) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const u32x4 ones = lora_ones(key, p.drop, row0 + 8 * g + j0 + i, mine, p.c);
+                now.v[i] = lora_masked<DT>(now.v[i], ones, mine);
+                if (V == 8 || !(n16 & 1)) keep[(8 * g + j0 + i) * G + n16 * V / 8] = (uint8_t)drop_bits(ones);
+            }
+        }
+        if constexpr (WR == 1) raw = now;
+        else if (p.pd) now.put(t, TP, j0);
         lds_barrier();
-        if (p.dx) {
-            const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
-            for (int i = threadIdx.x; i < RP * (CB / V); i += kLoraThreads) {
-                const int j = i % RP, k = i / RP * V, col = block0 + k;
-                const u32x4 w = lora_load(down + (int64_t)min(j, p.r - 1) * p.c, col, p.c);
-                const u32x4 q = j < p.r ? w : u32x4{0, 0, 0, 0};
+        if (p.pd) {
+            if constexpr (WR > 1) raw.get(t, TP);
+            float b[RW][8];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if constexpr (V == 4) wl[(k + e) * WP + j] = q[e];
-                    else wl[(k + e) * WP + j] = (S)(q[e / 2] >> (16 * (e & 1)));
-                }
-            }
+            for (int j = 0; j < RW; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
+            lora_outer<DT, RW>(raw, b, acc);
         }
-        for (int64_t block_row = r0; block_row < r1; block_row += ROWS) {
-            const int64_t row0 = block_row + wg * kLoraRows;  // the wave's
-            // (what follows from the lane is formed anew each time: kept through the loops it
-            // would not fit the registers)
-            int ln = lane;
-            asm volatile("" : "+v"(ln));
-            const int n16 = ln & 15, g = ln >> 4, mine = col0 + V * n16;
-            float* f = ub[turn];
-            S* t = tile[WR > 1 ? turn : 0][WR > 1 ? wg * WC + wc : 0];
-            uint8_t* keep = kept[DROP ? turn : 0][DROP ? wg * WC + wc : 0];
-            turn = BUF == 2 ? turn ^ 1 : 0;
+        if (p.dx && (WG == 1 || row0 < r1)) {
+            if (p.base)
 #pragma unroll
-            for (int i = 0; i < NU; ++i) {
-                const int at = threadIdx.x + i * kLoraThreads, m = at / RP, j = at % RP;
-                float z = un[0][i];
-                if constexpr (SH >= 2) z += un[1][i];
-                if constexpr (SH == 4) z += un[2][i] + un[3][i];
-                f[m * P + j] = z;
-            }
-            f += wg * kLoraRows * P;
-            // (loads return in order: u, wanted first, before dx_base and the next rows)
-            load_u(block_row + ROWS);
-            if (p.dx && p.base && (WG == 1 || row0 < r1)) load_base(row0, n16, g);
-            LoraRows<DT, 8> raw;
-            LoraRows<DT, NR> now = rows;
-            if (p.pd) {
-                rows.load(p.x, p.xs, row0 + ROWS, r1, j0, mine, p.c);
-                now.trim(row0, r1, j0, edge, mine, p.c);
-            }
-            if (DROP) {
+                for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    const u32x4 ones = lora_ones(key, p.drop, row0 + 8 * g + j0 + i, mine, p.c);
-                    now.v[i] = lora_masked<DT>(now.v[i], ones, mine);
-                    if (V == 8 || !(n16 & 1)) keep[(8 * g + j0 + i) * G + n16 * V / 8] = (uint8_t)drop_bits(ones);
-                }
-            }
-            if constexpr (WR == 1) raw = now;
-            else if (p.pd) now.put(t, TP, j0);
-            lds_barrier();
-            if (p.pd) {
-                if constexpr (WR > 1) raw.get(t, TP);
-                float b[RW][8];
-#pragma unroll
-                for (int j = 0; j < RW; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) b[j][i] = f[(8 * g + i) * P + rank0 + 16 * j + n16];
-                lora_outer<DT, RW>(raw, b, acc);
-            }
-            if (p.dx && (WG == 1 || row0 < r1)) {
-                if (p.base)
-#pragma unroll
-                    for (int i = 0; i < NI; ++i)
-#pragma unroll
-                        for (int q = 0; q < QN; q += 2) {
-                            if (!edge) {
-                                lora_turn_pair(base[i][q], base[i][q + 1]);
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 2; ++x)
-                                    base[i][q + x] =
-                                        lora_edge<S>(base[i][q + x], col0 + (q0 + q + x) * N::STEP + V * g, p.c);
-                            }
-                        }
-                typename K::H h[NI];
-#pragma unroll
-                for (int i = 0; i < NI; ++i) h[i].load(f + (16 * (i0 + i) + n16) * P, g);
-                const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
-                S* d = static_cast<S*>(p.dx) + row0 * p.c + col0 + q0 * N::STEP;
-#pragma unroll
-                for (int q = 0; q < QN; q += 2) {
-                    u32x4 out[NI][2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int at = (q0 + q + x) * N::STEP;
-                        typename K::W wt[T];
-#pragma unroll
-                        for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
-#pragma unroll
-                        for (int i = 0; i < NI; ++i) {
-                            float z[V];
-#pragma unroll
-                            for (int k = 0; k < T; ++k) {
-                                floatx4 d = {0, 0, 0, 0};
-                                d = K::mma(wt[k], h[i], d);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
-                            }
-                            if (DROP) {
-                                const uint32_t bits = keep[(16 * (i0 + i) + n16) * G + (at + V * g) / 8] >>
-                                                      (V == 8 ? 0 : 2 * (g & 1));
-#pragma unroll
-                                for (int e = 0; e < V; ++e)
-                                    z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
-                            }
-                            if (p.base)
-#pragma unroll
-                                for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(base[i][q + x], e);
-                            out[i][x] = lora_round<DT>(z);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < NI; ++i) {
-                        S* to = d + (int64_t)16 * (i0 + i) * p.c + q * N::STEP;
-                        const int left = m - 16 * (i0 + i);
+                    for (int q = 0; q < QN; q += 2) {
                         if (!edge) {
-                            lora_store_pair(to, p.c, out[i][0], out[i][1], left);
+                            lora_turn_pair(base[i][q], base[i][q + 1]);
                         } else {
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const int at = x * N::STEP + V * g;
-                                if (n16 < left)
-                                    lora_store(to + n16 * (int64_t)p.c + at, out[i][x], p.c - col0 - (q0 + q) * N::STEP - at);
-                            }
+                            for (int x = 0; x < 2; ++x)
+                                base[i][q + x] =
+                                    lora_edge<S>(base[i][q + x], col0 + (q0 + q + x) * N::STEP + V * g, p.c);
+                        }
+                    }
+            typename K::H h[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) h[i].load(f + (16 * (i0 + i) + n16) * P, g);
+            const int m = (int)min(r1 - row0, (int64_t)kLoraRows);
+            S* d = static_cast<S*>(p.dx) + row0 * p.c + col0 + q0 * N::STEP;
+#pragma unroll
+            for (int q = 0; q < QN; q += 2) {
+                u32x4 out[NI][2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int at = (q0 + q + x) * N::STEP;
+                    typename K::W wt[T];
+#pragma unroll
+                    for (int k = 0; k < T; ++k) wt[k].load_lds(wl + lora_col<DT>(wc * CW + at, k, n16) * WP, g);
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+                        float z[V];
+#pragma unroll
+                        for (int k = 0; k < T; ++k) {
+                            floatx4 d = {0, 0, 0, 0};
+                            d = K::mma(wt[k], h[i], d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
+                        }
+                        if (DROP) {
+                            const uint32_t bits = keep[(16 * (i0 + i) + n16) * G + (at + V * g) / 8] >>
+                                                  (V == 8 ? 0 : 2 * (g & 1));
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                z[e] = p.factor * __uint_as_float(drop_word(__float_as_uint(z[e]), bits, drop_bit(e)));
+                        }
+                        if (p.base)
+#pragma unroll
+                            for (int e = 0; e < V; ++e) z[e] += lora_value<DT>(base[i][q + x], e);
+                        out[i][x] = lora_round<DT>(z);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    S* to = d + (int64_t)16 * (i0 + i) * p.c + q * N::STEP;
+                    const int left = m - 16 * (i0 + i);
+                    if (!edge) {
+                        lora_store_pair(to, p.c, out[i][0], out[i][1], left);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int at = x * N::STEP + V * g;
+                            if (n16 < left)
+                                lora_store(to + n16 * (int64_t)p.c + at, out[i][x], p.c - col0 - (q0 + q) * N::STEP - at);
                         }
                     }
                 }
             }
-            if (BUF == 1) lds_barrier();
         }
-        if (WG > 1 && p.pd) lora_gather<WC * WR, WG>(acc, sums);
-        if (p.pd && col0 < p.c && wg == 0)
-            lora_flush<DT, RW>(acc, p.pd + (blockIdx.y + v) * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
-                               DROP ? p.factor : 1.0f);
+        if (BUF == 1) lds_barrier();
     }
+    if (WG > 1 && p.pd) lora_gather<WC * WR, WG>(acc, sums);
+    if (p.pd && col0 < p.c && wg == 0)
+        lora_flush<DT, RW>(acc, p.pd + chunk * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
+                           DROP ? p.factor : 1.0f);
 }
 
 template <int DT>
