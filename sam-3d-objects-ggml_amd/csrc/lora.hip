@@ -138,11 +138,11 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
     // Tiles of 32 rows of one item cost some 0.2 us an item, however short, and the sums
     // behind them; gathered, an adapter's rows wait one after the other, some 9 us for each
     // 32 of them (us, gathered / tiles, 1024 -> 1024 rank 16 bf16: 32 rows of one item 16 /
-    // 18, 64 of one 22 / 18, 64 one-row items and four adapters 21 / 30; 512 rows of 256
-    // items and 8 adapters 42 / 76, of 16 and 8 46 / 22, of 16 and 2 70 / 22; 1024 of 512
-    // and 8 66 / 123, of 64 and 8 48 / 50; 8192 of 2048 and 8 386 / 442, of 1024 and 8 340 /
-    // 220; 4096 one-row items of one adapter 1890 / 1263, of eight 321 / 890, of 1024 1489 /
-    // 2619).
+    // 17, 64 of one 22 / 17, 64 one-row items and four adapters 20 / 26; 512 rows of 256
+    // items and 8 adapters 40 / 79, of 64 and 8 32 / 26, of 16 and 8 35 / 20, of 16 and 2 59
+    // / 21; 1024 of 512 and 8 64 / 129, of 64 and 8 45 / 26; 8192 of 2048 and 8 372 / 431, of
+    // 1024 and 8 343 / 226; 4096 one-row items of one adapter 1946 / 1266, of eight 320 / 905,
+    // of 1024 1470 / 2643).
     q.few = n <= std::min(32 * items, std::min(items, adapters) * (32 + items / 2));
     if (q.few) {
         int64_t chunks = 1;
@@ -159,8 +159,9 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
     q.blocks_o = ceil_div(o, (int64_t)lora_col_waves(dt, r, o) * lora_wave_cols(dt));
     q.blocks_c = ceil_div(c, (int64_t)lora_col_waves(dt, r, c) * lora_wave_cols(dt));
     // Some two blocks a CU: the registers hold no more of them at once, and every further
-    // chunk is a slot to write and add (us of 62,710 x 1024 rank 16 bf16 by blocks: 256 155,
-    // 384 157, 512 138, 640 166, 768 157, 1024 144).
+    // chunk is a slot to write and add (us by 256 / 384 / 512 / 640 / 1024 blocks: 30,000 x 1024
+    // rank 16 bf16 67 / 63 / 59 / 71 / 70, rank 64 158 / 132 / 112 / 111 / 130, 21,766 x 768 rank 8
+    // f32 70 / 72 / 65 / 64 / 73).
     // A block's chunk is of one item, whose last is shorter: some chunks fewer, so that those
     // do not make a second round.
     auto rows = [&](int64_t blocks, int64_t width) {
