@@ -10,11 +10,11 @@
 // reads its rows once and the products run on the matrix instructions, which
 // are far from their limit (rank 16: some 50 operations a byte at most).  BF16,
 // inputs that change: y of 62,710 x 1024, rank 16, with a base 78 us (4.9 TB/s; a
-// large copy 5.15); its gradients' pass over dy 38 us (128 MB and 24 of u and sums,
-// 4.0 TB/s), over x 92 (385 MB, 4.2 TB/s; the dropout's mask is 8 of them), the sums 9.
+// large copy 5.15); its gradients' pass over dy 37 us (132 MB and 24 of u and sums,
+// 4.3 TB/s), over x 89 (401 MB, 4.5 TB/s; the dropout's mask is 8 of them), the sums 9.
 // Larger ranks cost the adapters' way through L2 for each tile of rows (30,000 x 1024, rank
-// 16 / 64 / 128: 35 / 44 / 81 us, gradients 69 / 123 / 203), rows of 16-bit elements at
-// odd addresses twice the time (1023 to 1021: 75, 106).
+// 16 / 64 / 128: 34 / 42 / 81 us, gradients 67 / 121 / 180), rows of 16-bit elements at
+// odd addresses twice the time (1023 to 1021: 74, 105).
 //
 // 16-bit rows meet 16-bit weights exactly (F32 sums).  h and u stay F32, and
 // meet 16-bit operands as two bf16 parts (their sum within 2^-17 of the value,
