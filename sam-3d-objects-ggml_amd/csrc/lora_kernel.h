@@ -807,10 +807,10 @@ hipError_t lora_forward(hipStream_t s, const LoraArgs& p, int mode, int mt, dim3
 // V (l % 16) on (16 bytes a row).  That is the row operand of the weights'
 // gradients (columns by summed rows; 16-bit elements are exchanged between the
 // lane's registers to bring a column's eight rows together), whose sums stay in
-// registers until the chunk or the segment ends.  WC waves stand along the columns,
-// WR along the ranks (16 RW each) and WG along the rows, a tile of 32 each: those of
-// the same columns and rows load, and mask, a share of the rows each and pass them on
-// through LDS, those along the rows add their sums there at the end.
+// registers until the chunk, whose rows are of one segment, ends.  WC waves stand
+// along the columns, WR along the ranks (16 RW each) and WG along the rows, a tile of
+// 32 each: those of the same columns and rows load, and mask, a share of the rows each
+// and pass them on through LDS, those along the rows add their sums there at the end.
 constexpr int kLoraRows = 32;
 
 // NR of a lane's eight rows, from j0 on.
@@ -908,17 +908,14 @@ __device__ __forceinline__ void lora_outer(const LoraRows<DT, 8>& raw, const flo
 constexpr int64_t lora_slot(int64_t c, int cw, int rt) { return (c + cw - 1) / cw * cw * 16 * rt; }
 
 template <int DT, int RW>
-__device__ __forceinline__ void lora_flush(floatx4 (&acc)[LoraNum<DT>::V][RW], float* slot, int tile, int rt, int rank_tile,
+__device__ __forceinline__ void lora_flush(const floatx4 (&acc)[LoraNum<DT>::V][RW], float* slot, int tile, int rt, int rank_tile,
                                            float f) {
     constexpr int V = LoraNum<DT>::V;
     float* q = slot + ((int64_t)tile * rt + rank_tile) * V * 256 + 4 * (threadIdx.x & 63);
 #pragma unroll
     for (int j = 0; j < RW; ++j)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            *reinterpret_cast<floatx4*>(q + (j * V + e) * 256) = f * acc[e][j];
-            acc[e][j] = floatx4{0, 0, 0, 0};
-        }
+        for (int e = 0; e < V; ++e) *reinterpret_cast<floatx4*>(q + (j * V + e) * 256) = f * acc[e][j];
 }
 
 // The sums of the waves along the rows (WAVES of each) added to the first ones', in
@@ -930,10 +927,7 @@ __device__ __forceinline__ void lora_gather(floatx4 (&acc)[V][RW], floatx4* ls) 
 #pragma unroll
         for (int e = 0; e < V; ++e)
 #pragma unroll
-            for (int j = 0; j < RW; ++j) {
-                ls[((w - WAVES) * V * RW + e * RW + j) * 64 + lane] = acc[e][j];
-                acc[e][j] = floatx4{0, 0, 0, 0};
-            }
+            for (int j = 0; j < RW; ++j) ls[((w - WAVES) * V * RW + e * RW + j) * 64 + lane] = acc[e][j];
     lds_barrier();
     if (w < WAVES)
 #pragma unroll
@@ -1006,7 +1000,6 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
     if (p.u) {
         const S* up = static_cast<const S*>(p.up);
         const int64_t all = it.adapters * p.o * p.r;
-        lds_barrier();
         for (int i = threadIdx.x; i < CB * (RP / V); i += kLoraThreads) {
             const int k = i % CB, j = i / CB * V, col = block0 + k;
             const int64_t at = (a * p.o + min(col, p.o - 1)) * p.r + j;
@@ -1180,7 +1173,6 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     };
     load_u(r0);
     if (p.pd) rows.load(p.x, p.xs, r0 + wg * kLoraRows, r1, j0, col0 + V * (lane & 15), p.c);
-    lds_barrier();
     if (p.dx) {
         const S* down = static_cast<const S*>(p.down) + a * p.c * p.r;
         for (int i = threadIdx.x; i < RP * (CB / V); i += kLoraThreads) {
