@@ -88,6 +88,17 @@ def test_more_elements_than_32_bits_count(spc, dev):
         assert torch.equal(x[first:first + 5].double().cpu(), want)
 
 
+def test_more_groups_than_threads(spc, dev):
+    """Of an odd number a row, so that a thread's next one begins elsewhere in its row."""
+    n, c = (1 << 28) // 3 + 1000, 17
+    x = _rows(1, c, "bf16", dev).expand(n, c)
+    y = spc._native.dropout(x, 0.25, _seed(dev))
+    for first in (0, n - 1003, n - 5):   # 2^28 groups of eight end in row n - 1000
+        want = x[:5].double().cpu() * factors(SEED, 5, c, 0.25, first=first)
+        # the factor's and the product's F32 steps, 2 x 2^-24, then the rounding of y
+        check(f"rows from {first}", y[first:first + 5], want, want.abs() * 2.0 ** -23, torch.bfloat16)
+
+
 def test_other_streams_graphs_and_two_seeds(spc, dev):
     """A replayed graph takes the seed that the tensor then holds, with eager
     work between the replays."""
