@@ -17,10 +17,11 @@
 // odd addresses twice the time (1023 to 1021: 74, 105).
 //
 // 16-bit rows meet 16-bit weights exactly (F32 sums).  h and u stay F32, and
-// meet 16-bit operands as two bf16 parts (their sum within 2^-17 of the value,
-// at any magnitude, where one part would be a rounding like the output's); f16
-// operands of those products are two bf16 parts as well, exactly, so that no
-// range but F32's bounds h and u.  F32 rows run on F32 matrix instructions.
+// meet 16-bit operands as three bf16 parts of eight bits each, whose sum is the
+// value itself (below 2^-110 but for what lies under 2^-133, bf16's last bit; two
+// parts, 2^-16 of the value, turned outputs' roundings over); f16 operands of those
+// products are two bf16 parts, exactly too, so that no range but F32's bounds h
+// and u.  F32 rows run on F32 matrix instructions.
 #pragma once
 
 #include "rows8.h"
@@ -300,26 +301,26 @@ __device__ __forceinline__ floatx4 lora_mma(u32x4 a, u32x4 b, floatx4 c) {
     }
 }
 
-// Two values as bf16 parts: hi cut, lo the nearest of what is left.  (An infinity's
-// rest is NaN, as is a product that it enters.)
-__device__ __forceinline__ void lora_split(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
-    hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
-    lo = round_pair<SPC_BF16>(a - __uint_as_float(ia & 0xffff0000u), b - __uint_as_float(ib & 0xffff0000u));
+// The upper halves of two values, a's below: their leading eight bits as bf16.
+__device__ __forceinline__ uint32_t lora_cut(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
+// What those leave, exactly.  (An infinity leaves NaN, as is a product that it enters.)
+__device__ __forceinline__ float lora_rest(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
 
-// F32 values h and u as column operand: 16-bit rows two bf16 parts.
+// F32 values h and u as column operand: 16-bit rows three bf16 parts, which hold all
+// 24 bits.
 struct LoraSplit {
-    u32x4 hi, lo;
+    u32x4 hi, mid, lo;
 };
 __device__ __forceinline__ LoraSplit lora_split8(const float (&v)[8]) {
     LoraSplit s;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        uint32_t hi, lo;
-        lora_split(v[2 * q], v[2 * q + 1], hi, lo);
-        s.hi[q] = hi;
-        s.lo[q] = lo;
+        const float a = v[2 * q], b = v[2 * q + 1], ra = lora_rest(a), rb = lora_rest(b);
+        s.hi[q] = lora_cut(a, b);
+        s.mid[q] = lora_cut(ra, rb);
+        s.lo[q] = lora_cut(lora_rest(ra), lora_rest(rb));
     }
     return s;
 }
@@ -332,10 +333,9 @@ struct LoraParts {
         if constexpr (DT == SPC_F16) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                uint32_t hi, lo;
-                lora_split(lora_value<DT>(w, 2 * q), lora_value<DT>(w, 2 * q + 1), hi, lo);
-                p[0][q] = hi;
-                p[1][q] = lo;
+                const float a = lora_value<DT>(w, 2 * q), b = lora_value<DT>(w, 2 * q + 1);
+                p[0][q] = lora_cut(a, b);
+                p[1][q] = lora_cut(lora_rest(a), lora_rest(b));
             }
         } else {
             p[0] = w;
@@ -349,9 +349,11 @@ template <int DT>
 __device__ __forceinline__ floatx4 lora_mma_split(const LoraParts<DT>& a, const LoraSplit& b, floatx4 c) {
     if constexpr (DT == SPC_F16) {
         c = lora_mma<SPC_BF16>(a.p[1], b.lo, c);
+        c = lora_mma<SPC_BF16>(a.p[1], b.mid, c);
         c = lora_mma<SPC_BF16>(a.p[1], b.hi, c);
     }
     c = lora_mma<SPC_BF16>(a.p[0], b.lo, c);
+    c = lora_mma<SPC_BF16>(a.p[0], b.mid, c);
     return lora_mma<SPC_BF16>(a.p[0], b.hi, c);
 }
 
@@ -378,8 +380,8 @@ __device__ __forceinline__ u32x4 lora_masked(u32x4 w, u32x4 ones, int col) {
 // ---------------------------------------------------------------------------
 // The F32 operand (hidden rows; ranks are the summed index) of a row tile: steps
 // of V lane-groups of ranks.  Rank up to 16 under 16-bit rows: lanes 0..31 hold the
-// high parts of ranks 8 (lane / 16 % 2) on, lanes 32..63 the low parts, so that
-// one matrix instruction takes both.
+// first parts of ranks 8 (lane / 16 % 2) on, lanes 32..63 the second, so that one
+// matrix instruction takes both, and another the third beside zeros.
 template <int DT, int RT>
 struct LoraRanks {
     static constexpr bool F = DT == SPC_F32, ONE = !F && RT == 1;
@@ -404,7 +406,7 @@ struct LoraRanks {
     };
     // column operand
     struct H {
-        u32x4 hi[STEPS], lo[F || ONE ? 1 : STEPS];
+        u32x4 hi[STEPS], mid[F || ONE ? 1 : STEPS], lo[F ? 1 : STEPS];
         // q: the row's F32 values in LDS, zeros past the rank
         __device__ __forceinline__ void load(const float* q, int g) {
 #pragma unroll
@@ -418,9 +420,11 @@ struct LoraRanks {
                     for (int e = 0; e < 8; ++e) v[e] = f[e];
                     const LoraSplit t = lora_split8(v);
                     if constexpr (ONE) {
-                        hi[s] = g < 2 ? t.hi : t.lo;
+                        hi[s] = g < 2 ? t.hi : t.mid;
+                        lo[s] = g < 2 ? t.lo : u32x4{0, 0, 0, 0};
                     } else {
                         hi[s] = t.hi;
+                        mid[s] = t.mid;
                         lo[s] = t.lo;
                     }
                 }
@@ -433,10 +437,14 @@ struct LoraRanks {
             if constexpr (F) {
                 c = lora_mma<SPC_F32>(w.w[s].p[0], h.hi[s], c);
             } else if constexpr (ONE) {
-                if constexpr (DT == SPC_F16) c = lora_mma<SPC_BF16>(w.w[s].p[1], h.hi[s], c);
+                if constexpr (DT == SPC_F16) {
+                    c = lora_mma<SPC_BF16>(w.w[s].p[1], h.lo[s], c);
+                    c = lora_mma<SPC_BF16>(w.w[s].p[1], h.hi[s], c);
+                }
+                c = lora_mma<SPC_BF16>(w.w[s].p[0], h.lo[s], c);
                 c = lora_mma<SPC_BF16>(w.w[s].p[0], h.hi[s], c);
             } else {
-                c = lora_mma_split<DT>(w.w[s], LoraSplit{h.hi[s], h.lo[s]}, c);
+                c = lora_mma_split<DT>(w.w[s], LoraSplit{h.hi[s], h.mid[s], h.lo[s]}, c);
             }
         }
         return c;
