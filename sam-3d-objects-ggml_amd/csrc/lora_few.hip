@@ -16,19 +16,6 @@ namespace {
 
 constexpr int kFewRows = 32;   // rows at a time
 
-template <int DT>
-__device__ __forceinline__ float few_get(const void* p, int64_t i) {
-    if constexpr (DT == SPC_F32) return static_cast<const float*>(p)[i];
-    else if constexpr (DT == SPC_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-    else return f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
-}
-
-template <int DT>
-__device__ __forceinline__ void few_put(void* p, int64_t i, float v) {
-    if constexpr (DT == SPC_F32) static_cast<float*>(p)[i] = v;
-    else static_cast<uint16_t*>(p)[i] = DT == SPC_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-}
-
 // RJ values times f, `left` of which are the row's.
 template <int DT, int RJ>
 __device__ __forceinline__ void few_put_ranks(void* p, int64_t at, const float (&v)[RJ], float f, int left) {
@@ -45,7 +32,7 @@ __device__ __forceinline__ void few_put_ranks(void* p, int64_t at, const float (
     } else {
 #pragma unroll
         for (int i = 0; i < RJ; ++i)
-            if (i < left) few_put<DT>(p, at + i, f * v[i]);
+            if (i < left) lora_put<DT>(p, at + i, f * v[i]);
     }
 }
 
@@ -80,7 +67,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int
         for (int k = 0; k < UN; ++k) {
             const int q = min(o + k * lines, o1 - 1);
             w[k] = lora_fetch_short(up, (a * p.o + q) * p.r + j, all);
-            d[k] = few_get<DT>(p.dy, row * p.dys + q);
+            d[k] = lora_get<DT>(p.dy, row * p.dys + q);
         }
 #pragma unroll
         for (int k = 0; k < UN; ++k) {
@@ -102,12 +89,6 @@ __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int
         const float z = (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]);
         p.u[(blockIdx.y * it.n + row) * p.r + t] = p.scale ? p.scale[a] * z : z;
     }
-}
-
-// Column e of the group: kept.
-__device__ __forceinline__ bool few_keeps(u32x4 ones, int col) {
-    const uint32_t q = col & 4 ? (col & 2 ? ones[3] : ones[2]) : (col & 2 ? ones[1] : ones[0]);
-    return q >> (16 * (col & 1)) & 1;
 }
 
 // Blocks along x: 64 columns of x (dx, ddown), then of dy (dup); along y: adapters,
@@ -136,7 +117,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
         if (dx && !none)
 #pragma unroll
             for (int i = 0; i < RJ; ++i)
-                wt[i] = few_get<DT>(p.down, (a * p.r + min(j0 + i, p.r - 1)) * p.c + at);
+                if (j0 + i < p.r) wt[i] = lora_get<DT>(p.down, (a * p.r + j0 + i) * p.c + at);
         int64_t v0 = -64;
         uint64_t m = 0;
         int b = 0, e = 0, row = 0, end = 0;
@@ -173,8 +154,8 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 rows[t] = list[min(8 * w + t, count - 1)];
-                bv[t] = dx && p.base ? few_get<DT>(p.base, rows[t] * p.bs + at) : 0.0f;
-                xv[t] = grad && !none ? few_get<DT>(x, rows[t] * stride + at) : 0.0f;
+                bv[t] = dx && p.base ? lora_get<DT>(p.base, rows[t] * p.bs + at) : 0.0f;
+                xv[t] = grad && !none ? lora_get<DT>(x, rows[t] * stride + at) : 0.0f;
             }
             if (!none) {
                 for (int i = threadIdx.x; i < kFewRows * 4 * RJ; i += kLoraThreads) {
@@ -190,7 +171,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
 #pragma unroll
                 for (int t = 0; t < 8; ++t) {
                     if (8 * w + t >= count) continue;
-                    const bool k = !drop || few_keeps(lora_ones(key, p.drop, rows[t], at, p.c), at);
+                    const bool k = !drop || lora_keeps(lora_ones(key, p.drop, rows[t], at, p.c), at);
                     kept |= (uint32_t)k << t;
                     xs[8 * w + t][lane] = k ? xv[t] : 0.0f;
                 }
@@ -220,7 +201,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
                     z = (part[0][q][lane] + part[1][q][lane]) + (part[2][q][lane] + part[3][q][lane]);
                     if (drop) z *= p.factor;
                 }
-                few_put<DT>(p.dx, rows[t] * p.c + col, z + bv[t]);
+                lora_put<DT>(p.dx, rows[t] * p.c + col, z + bv[t]);
             }
         }
         __syncthreads();
@@ -229,7 +210,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
         if (in) {
 #pragma unroll
             for (int i = 0; i < RJ; ++i)
-                if (j0 + i < p.r) few_put<DT>(grad, (a * p.r + j0 + i) * p.c + col, f * acc[i]);
+                if (j0 + i < p.r) lora_put<DT>(grad, (a * p.r + j0 + i) * p.c + col, f * acc[i]);
         } else {
             // (a column's ranks stand together: 16 bytes of them in a store, 34 one-row items of
             // 17 to 3712, rank 128 and 16 adapters 79 us one by one, so 46)

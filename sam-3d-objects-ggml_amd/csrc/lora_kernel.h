@@ -271,6 +271,19 @@ __device__ __forceinline__ float lora_value(u32x4 w, int e) {
     else return f16_bits_to_f32((uint16_t)(w[e / 2] >> (16 * (e & 1))));
 }
 
+// one element
+template <int DT>
+__device__ __forceinline__ float lora_get(const void* p, int64_t i) {
+    if constexpr (DT == SPC_F32) return static_cast<const float*>(p)[i];
+    else if constexpr (DT == SPC_BF16) return bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+    else return f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void lora_put(void* p, int64_t i, float v) {
+    if constexpr (DT == SPC_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = DT == SPC_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+}
+
 template <int DT>
 __device__ __forceinline__ u32x4 lora_round(const float (&v)[LoraNum<DT>::V]) {
     u32x4 w;
@@ -305,7 +318,8 @@ __device__ __forceinline__ floatx4 lora_mma(u32x4 a, u32x4 b, floatx4 c) {
 __device__ __forceinline__ uint32_t lora_cut(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
-// What those leave, exactly.  (An infinity leaves NaN, as is a product that it enters.)
+// What those leave, exactly.  (An infinity leaves NaN, and one that meets a part of zero
+// makes it: LoraRanks and lora_flush_plain put right what that would spoil.)
 __device__ __forceinline__ float lora_rest(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xffff0000u); }
 
 // F32 values h and u as column operand: 16-bit rows three bf16 parts, which hold all
@@ -362,6 +376,11 @@ __device__ __forceinline__ floatx4 lora_mma_split(const LoraParts<DT>& a, const 
 __device__ __forceinline__ u32x4 lora_ones(DropKey key, uint32_t drop, int64_t row, int col, int c) {
     return drop_ones(philox7(key, (uint64_t)(row * ((c + 7) / 8) + col / 8)), drop);
 }
+// Column `col` of its group: kept.
+__device__ __forceinline__ bool lora_keeps(u32x4 ones, int col) {
+    const uint32_t q = col & 4 ? (col & 2 ? ones[3] : ones[2]) : (col & 2 ? ones[1] : ones[0]);
+    return q >> (16 * (col & 1)) & 1;
+}
 template <int DT>
 __device__ __forceinline__ u32x4 lora_masked(u32x4 w, u32x4 ones, int col) {
     if constexpr (DT == SPC_F32) {
@@ -380,8 +399,11 @@ __device__ __forceinline__ u32x4 lora_masked(u32x4 w, u32x4 ones, int col) {
 // ---------------------------------------------------------------------------
 // The F32 operand (hidden rows; ranks are the summed index) of a row tile: steps
 // of V lane-groups of ranks.  Rank up to 16 under 16-bit rows: lanes 0..31 hold the
-// first parts of ranks 8 (lane / 16 % 2) on, lanes 32..63 the second, so that one
-// matrix instruction takes both, and another the third beside zeros.
+// second parts of ranks 8 (lane / 16 % 2) on, lanes 32..63 the third, so that one
+// matrix instruction takes both, and another the first beside zeros.
+// The first parts have a sum of their own.  Where a value or a weight is infinite it is
+// what the formula has, and the sum of the rest may be NaN, of a part that is zero or of an
+// infinity's: then it stands alone.
 template <int DT, int RT>
 struct LoraRanks {
     static constexpr bool F = DT == SPC_F32, ONE = !F && RT == 1;
@@ -393,20 +415,24 @@ struct LoraRanks {
     // row operand: the weights' parts
     struct W {
         LoraParts<DT> w[STEPS];
+        u32x4 first;  // (ONE: of the first parts, zeros in lanes 32..63)
         // from 16 bytes of a column's ranks a step
-        __device__ __forceinline__ void set(const u32x4 (&raw)[STEPS]) {
+        __device__ __forceinline__ void set(const u32x4 (&raw)[STEPS], int g) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) w[s] = LoraParts<DT>(raw[s]);
+            if constexpr (ONE) first = g < 2 ? w[0].p[0] : u32x4{0, 0, 0, 0};
         }
         // q: the same in LDS, zeros past the rank
         __device__ __forceinline__ void load_lds(const typename LoraNum<DT>::S* q, int g) {
+            u32x4 raw[STEPS];
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) w[s] = LoraParts<DT>(*reinterpret_cast<const u32x4*>(q + rank(s, g)));
+            for (int s = 0; s < STEPS; ++s) raw[s] = *reinterpret_cast<const u32x4*>(q + rank(s, g));
+            set(raw, g);
         }
     };
     // column operand
     struct H {
-        u32x4 hi[STEPS], mid[F || ONE ? 1 : STEPS], lo[F ? 1 : STEPS];
+        u32x4 hi[STEPS], mid[F ? 1 : STEPS], lo[F || ONE ? 1 : STEPS];
         // q: the row's F32 values in LDS, zeros past the rank
         __device__ __forceinline__ void load(const float* q, int g) {
 #pragma unroll
@@ -420,8 +446,8 @@ struct LoraRanks {
                     for (int e = 0; e < 8; ++e) v[e] = f[e];
                     const LoraSplit t = lora_split8(v);
                     if constexpr (ONE) {
-                        hi[s] = g < 2 ? t.hi : t.mid;
-                        lo[s] = g < 2 ? t.lo : u32x4{0, 0, 0, 0};
+                        hi[s] = g < 2 ? t.hi : u32x4{0, 0, 0, 0};
+                        mid[s] = g < 2 ? t.mid : t.lo;
                     } else {
                         hi[s] = t.hi;
                         mid[s] = t.mid;
@@ -431,21 +457,36 @@ struct LoraRanks {
             }
         }
     };
-    __device__ static __forceinline__ floatx4 mma(const W& w, const H& h, floatx4 c) {
+    __device__ static __forceinline__ floatx4 mma(const W& w, const H& h) {
+        floatx4 c = {0, 0, 0, 0}, rest = {0, 0, 0, 0};
+        if constexpr (F) {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            if constexpr (F) {
-                c = lora_mma<SPC_F32>(w.w[s].p[0], h.hi[s], c);
-            } else if constexpr (ONE) {
-                if constexpr (DT == SPC_F16) {
-                    c = lora_mma<SPC_BF16>(w.w[s].p[1], h.lo[s], c);
-                    c = lora_mma<SPC_BF16>(w.w[s].p[1], h.hi[s], c);
-                }
-                c = lora_mma<SPC_BF16>(w.w[s].p[0], h.lo[s], c);
-                c = lora_mma<SPC_BF16>(w.w[s].p[0], h.hi[s], c);
-            } else {
-                c = lora_mma_split<DT>(w.w[s], LoraSplit{h.hi[s], h.mid[s], h.lo[s]}, c);
+            for (int s = 0; s < STEPS; ++s) c = lora_mma<SPC_F32>(w.w[s].p[0], h.hi[s], c);
+            return c;
+        } else if constexpr (ONE) {
+            if constexpr (DT == SPC_F16) {
+                rest = lora_mma<SPC_BF16>(w.w[0].p[1], h.mid[0], rest);
+                rest = lora_mma<SPC_BF16>(w.w[0].p[1], h.hi[0], rest);
             }
+            rest = lora_mma<SPC_BF16>(w.w[0].p[0], h.mid[0], rest);
+            c = lora_mma<SPC_BF16>(w.first, h.hi[0], c);
+        } else {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                if constexpr (DT == SPC_F16) {
+                    rest = lora_mma<SPC_BF16>(w.w[s].p[1], h.lo[s], rest);
+                    rest = lora_mma<SPC_BF16>(w.w[s].p[1], h.mid[s], rest);
+                    rest = lora_mma<SPC_BF16>(w.w[s].p[1], h.hi[s], rest);
+                }
+                rest = lora_mma<SPC_BF16>(w.w[s].p[0], h.lo[s], rest);
+                rest = lora_mma<SPC_BF16>(w.w[s].p[0], h.mid[s], rest);
+                c = lora_mma<SPC_BF16>(w.w[s].p[0], h.hi[s], c);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float z = c[e] + rest[e];
+            c[e] = z == z ? z : c[e];
         }
         return c;
     }
@@ -644,14 +685,13 @@ __device__ __forceinline__ void lora_expand(const LoraArgs& p, const LoraTile& t
         for (int x = 0; x < 2; ++x) {
             typename K::W wt[T];
 #pragma unroll
-            for (int q = 0; q < T; ++q) wt[q].set(wr[x][q]);
+            for (int q = 0; q < T; ++q) wt[q].set(wr[x][q], g);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 float v[V];
 #pragma unroll
                 for (int q = 0; q < T; ++q) {
-                    floatx4 z = {0, 0, 0, 0};
-                    z = K::mma(wt[q], h[i], z);
+                    const floatx4 z = K::mma(wt[q], h[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[4 * q + e] = s * z[e];
                 }
@@ -926,6 +966,37 @@ __device__ __forceinline__ void lora_flush(const floatx4 (&acc)[LoraNum<DT>::V][
         for (int e = 0; e < V; ++e) *reinterpret_cast<floatx4*>(q + (j * V + e) * 256) = f * acc[e][j];
 }
 
+// Sums of 16-bit rows that lora_flush wrote as NaN are formed again without parts, to be
+// the infinity that the formula has, or NaN after all: term(row, column, rank) is what the
+// chunk's rows [r0, r1) add up.
+template <int DT, int RW, typename Term>
+__device__ __forceinline__ void lora_flush_plain(const floatx4 (&acc)[LoraNum<DT>::V][RW], float* slot, int tile, int rt,
+                                                 int rank_tile, float f, int64_t r0, int64_t r1, int c, int r, Term term) {
+    constexpr int V = LoraNum<DT>::V;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+#pragma unroll
+        for (int j = 0; j < RW; ++j)
+            nan |= __builtin_isunordered(acc[e][j][0], acc[e][j][1]) | __builtin_isunordered(acc[e][j][2], acc[e][j][3]);
+    if (DT == SPC_F32 || !__any(nan)) return;
+    const int lane = threadIdx.x & 63;
+    float* q = slot + ((int64_t)tile * rt + rank_tile) * V * 256 + 4 * lane;
+    for (int k = 0; k < V * RW; ++k) {
+        floatx4 z = *reinterpret_cast<const floatx4*>(q + k * 256);
+        const int rank = 16 * (rank_tile + k / V) + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = 16 * V * tile + V * (4 * (lane >> 4) + i) + k % V;
+            if (z[i] == z[i] || col >= c || rank >= r) continue;
+            float s = 0.0f;
+            for (int64_t row = r0; row < r1; ++row) s += term(row, col, rank);
+            z[i] = f * s;
+        }
+        *reinterpret_cast<floatx4*>(q + k * 256) = z;
+    }
+}
+
 // The sums of the waves along the rows (WAVES of each) added to the first ones', in
 // their order; ls: 64 V RW floatx4 for each of the others, which nobody else uses.
 template <int WAVES, int WG, int V, int RW>
@@ -1098,12 +1169,18 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
         lds_barrier();
         lora_gather<WC * WR, WG>(acc, reinterpret_cast<floatx4*>(tile));
     }
-    if (p.pu && col0 < p.o && first == 0)
-        lora_flush<DT, RW>(acc, p.pu + chunk * lora_slot(p.o, CW, RW * WR), col0 / CW, RW * WR, RW * wr, s);
+    if (p.pu && col0 < p.o && first == 0) {
+        float* slot = p.pu + chunk * lora_slot(p.o, CW, RW * WR);
+        lora_flush<DT, RW>(acc, slot, col0 / CW, RW * WR, RW * wr, s);
+        lora_flush_plain<DT, RW>(acc, slot, col0 / CW, RW * WR, RW * wr, s, r0, r1, p.o, p.r,
+                                 [&](int64_t row, int col, int rank) {
+                                     return lora_get<DT>(p.dy, row * p.dys + col) * p.hidden[row * p.r + rank];
+                                 });
+    }
 }
 
 // Shares of u that the pass over x adds (registers); of more, their sum comes first.
-constexpr int lora_shares(int rt, int wg) { return wg > 2 ? 1 : wg == 2 || rt > 1 ? 2 : 4; }
+constexpr int lora_shares(int rt, int wg) { return wg > 2 || rt == 8 ? 1 : wg == 2 || rt > 1 ? 2 : 4; }
 
 // The pass over x: dx of the block's columns and the sums of ddown.  The
 // adapter's columns lie in LDS by column.
@@ -1277,8 +1354,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
                         float z[V];
 #pragma unroll
                         for (int k = 0; k < T; ++k) {
-                            floatx4 d = {0, 0, 0, 0};
-                            d = K::mma(wt[k], h[i], d);
+                            const floatx4 d = K::mma(wt[k], h[i]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) z[4 * k + e] = d[e];
                         }
@@ -1315,9 +1391,18 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
         if (BUF == 1) lds_barrier();
     }
     if (WG > 1 && p.pd) lora_gather<WC * WR, WG>(acc, sums);
-    if (p.pd && col0 < p.c && wg == 0)
-        lora_flush<DT, RW>(acc, p.pd + chunk * lora_slot(p.c, CW, RT), col0 / CW, RT, RW * wr,
-                           DROP ? p.factor : 1.0f);
+    if (p.pd && col0 < p.c && wg == 0) {
+        float* slot = p.pd + chunk * lora_slot(p.c, CW, RT);
+        const float f = DROP ? p.factor : 1.0f;
+        lora_flush<DT, RW>(acc, slot, col0 / CW, RT, RW * wr, f);
+        lora_flush_plain<DT, RW>(acc, slot, col0 / CW, RT, RW * wr, f, r0, r1, p.c, p.r,
+                                 [&](int64_t row, int col, int rank) {
+                                     float u = 0.0f, x = lora_get<DT>(p.x, row * p.xs + col);
+                                     for (int k = 0; k < p.u_parts; ++k) u += p.u[(k * it.n + row) * p.r + rank];
+                                     if (DROP && !lora_keeps(lora_ones(key, p.drop, row, col, p.c), col)) x = 0.0f;
+                                     return u * x;
+                                 });
+    }
 }
 
 template <int DT>
