@@ -58,6 +58,20 @@ class LayerNorm32(nn.LayerNorm):
         return super().forward(x.float()).type(x.dtype)
 
 
+def _adapted(module: nn.Module) -> bool:
+    """Whether it, or a Linear in it, has adapters."""
+    return any(getattr(m, "has_adapters", False) for m in module.modules())
+
+
+class _Modulation(nn.Sequential):
+    """A Sequential whose adapted Linears take each row's adapter."""
+
+    def forward(self, input: torch.Tensor, adapters: Optional[torch.Tensor] = None) -> torch.Tensor:
+        for m in self:
+            input = m(input, adapters) if adapters is not None and _adapted(m) else m(input)
+        return input
+
+
 class SparseResBlock3d(nn.Module):
     def __init__(self, channels: int, emb_channels: int, out_channels: Optional[int] = None,
                  downsample: bool = False, upsample: bool = False):
@@ -75,8 +89,8 @@ class SparseResBlock3d(nn.Module):
         for p in self.conv2.parameters():  # zero_module (modules/utils.py)
             p.detach().zero_()
         # nn.Linear, or Q4_0 blocks once loaded (Q4Linear.load_q4_0)
-        self.emb_layers = nn.Sequential(nn.SiLU(), Q4Linear(emb_channels, 2 * self.out_channels,
-                                                            bias=True))
+        self.emb_layers = _Modulation(nn.SiLU(), Q4Linear(emb_channels, 2 * self.out_channels,
+                                                          bias=True))
         self.skip_connection = (SparseLinear(channels, self.out_channels)
                                 if channels != self.out_channels else nn.Identity())
         self.updown = None
@@ -95,7 +109,7 @@ class SparseResBlock3d(nn.Module):
         return x
 
     def _skip(self, x: SparseTensor, adapters) -> SparseTensor:
-        if adapters is None or not getattr(self.skip_connection, "has_adapters", False):
+        if adapters is None or not _adapted(self.skip_connection):
             return self.skip_connection(x)
         return self.skip_connection(x, adapters)
 
@@ -103,11 +117,10 @@ class SparseResBlock3d(nn.Module):
                 adapters: Optional[torch.Tensor] = None) -> SparseTensor:
         """adapters (int32 [B] on the device, -1 for none): each item's, for those of
         the block's Linears that have any (Q4Linear.add_adapters)."""
-        act, modulation = self.emb_layers
-        if adapters is None or not getattr(modulation, "has_adapters", False):
+        if adapters is None or not _adapted(self.emb_layers):
             emb_out = self.emb_layers(emb).type(x.dtype)
         else:
-            emb_out = modulation(act(emb), adapters).type(x.dtype)
+            emb_out = self.emb_layers(emb, adapters).type(x.dtype)
         # the halves as F32 in one pass (chunk and two conversions take two)
         scale, shift = emb_out.reshape(emb_out.shape[0], 2, -1).transpose(0, 1).to(
             torch.float32, memory_format=torch.contiguous_format).contiguous().unbind(0)
