@@ -116,7 +116,15 @@ class SparseResBlock3d(nn.Module):
     def forward(self, x: SparseTensor, emb: torch.Tensor,
                 adapters: Optional[torch.Tensor] = None) -> SparseTensor:
         """adapters (int32 [B] on the device, -1 for none): each item's, for those of
-        the block's Linears that have any (Q4Linear.add_adapters)."""
+        the block's Linears that have any (Q4Linear.add_adapters).  The block keeps no
+        gradients (its norms and convs are not recorded), so such a call is refused
+        where an adapter would need one; adapters are trained in a chain of modules."""
+        if adapters is not None and torch.is_grad_enabled() and any(
+                p.requires_grad for m in (self.emb_layers, self.skip_connection) for lin in m.modules()
+                if getattr(lin, "has_adapters", False) for p in (lin.adapter_down, lin.adapter_up)):
+            raise RuntimeError("SparseResBlock3d gives its adapters no gradients: call it under torch.no_grad(), "
+                               "or train the Linears in a chain of modules (SparseLayerNorm32, SparseLinear, "
+                               "SparseDropout)")
         if adapters is None or not _adapted(self.emb_layers):
             emb_out = self.emb_layers(emb).type(x.dtype)
         else:

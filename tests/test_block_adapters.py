@@ -54,3 +54,30 @@ def test_modulation_is_called_with_its_hooks(spc):
         block.emb_layers(emb, which)
     block.emb_layers = Wrapped(block.emb_layers)
     assert torch.equal(block.emb_layers(emb), plain)
+
+
+@pytest.mark.parametrize("where", ["emb_layers", "skip_connection"])
+def test_adapters_that_need_a_gradient_are_refused(spc, where):
+    """The block gives none: a call that would leave them without it, in training or
+    not, frozen convs or not, raises before any work; without adapters, under no_grad
+    and with frozen adapters nothing changes."""
+    block, x, emb = _block(spc)
+    which = torch.tensor([0, -1], dtype=torch.int32)
+    lin = block.emb_layers[1] if where == "emb_layers" else block.skip_connection
+    lin.add_adapters(1, 4)
+    for train in (True, False):
+        block.train(train)
+        for frozen in (False, True):
+            block.conv1.requires_grad_(not frozen), block.conv2.requires_grad_(not frozen)
+            with pytest.raises(RuntimeError, match="no gradients"):
+                block(x, emb, which)
+            with pytest.raises(RuntimeError, match="GPU only"):
+                block(x, emb)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="GPU only"):
+                block(x, emb, which)
+    lin.adapter_down.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        block(x, emb, which)
+    lin.adapter_up.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        block(x, emb, which)
