@@ -962,7 +962,7 @@ class Q4Linear(nn.Linear):
         are: parameters adapter_down [count, rank, in_features], drawn as a Linear's
         weight, and adapter_up [count, out_features, rank], zeros, so that they change
         nothing yet, of the weight's dtype and device; a buffer adapter_scale [count],
-        alpha / rank (alpha: rank if not given).  All three are part of the state dict.
+        alpha / rank (alpha: rank if not given), F32 in a module of any dtype.  All three are part of the state dict.
         dropout: of the rows in front of the adapters, in training.  The other
         parameters stay trainable or frozen as they are."""
         if count < 1 or not 1 <= rank <= 128:
@@ -987,6 +987,13 @@ class Q4Linear(nn.Linear):
         for name in ("adapter_down", "adapter_up", "adapter_scale"):
             self._parameters.pop(name, None)
             self._buffers.pop(name, None)
+
+    def _apply(self, fn, recurse=True):
+        scale = self._buffers.get("adapter_scale")
+        super()._apply(fn, recurse)
+        if scale is not None and self.adapter_scale.dtype != scale.dtype:
+            self.adapter_scale = scale.to(self.adapter_scale.device)  # (F32 whatever the weights become)
+        return self
 
     @property
     def has_adapters(self) -> bool:
