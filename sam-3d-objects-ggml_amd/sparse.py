@@ -1009,8 +1009,8 @@ class Q4Linear(nn.Linear):
         leaves = (leaf, down, up, self.bias, None if q4 else self.weight)
         held = _eager_leaves(*leaves) if _recorded(*leaves) else None  # (before any view or cast)
         x = x()
-        if not x.shape[0]:  # no row meets an adapter
-            return Q4Linear.forward(self, x)
+        if not adapters.shape[0]:  # (no item: one of no rows, so that gradients are zeros)
+            adapters = adapters.new_full((1,), -1)
         p = self.adapter_dropout if self.training else 0.0
         kw = dict(scale=self.adapter_scale.float(), offsets=offsets, adapters=adapters, p=p,
                   seed=dropout_seed(x.device) if p else None)
