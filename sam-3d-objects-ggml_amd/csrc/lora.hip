@@ -11,11 +11,14 @@ namespace {
 
 // Gradients from the slots that the row passes left: adapter a's is the sum over
 // its items and their chunks (lora_chunk_row), in a fixed order.  A block
-// takes 1024 / G of a slot's floats, G slots at a time.
+// takes 1024 / G of a slot's floats, G slots at a time.  Where the slots hold a part of
+// the chunks at a time (kLoraSlotBytes), sums are carried in F32 from part to part.
 struct LoraSum {
     const float* part;
     void* dst;
+    float* carry;  // like dst
     int64_t slot;  // floats
+    int64_t first, chunks, all;  // chunks of this part, and of all
     int c;         // columns
     int along;     // dst [r][c], else [c][r]
     int rows_per;
@@ -28,11 +31,18 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
     const LoraSum p = blockIdx.y ? second : first;
     if (!p.dst) return;
     const int tx = threadIdx.x % T, ty = threadIdx.x / T, lane = threadIdx.x & 63;
-    const int64_t blocks = p.slot / (4 * T);
+    const int64_t blocks = p.slot / (4 * T), last = p.first + p.chunks - 1;
+    const bool begins = p.first == 0, ends = last >= p.all - 1;
+    int64_t from = 0, to = it.items;  // items that may have chunks here
+    if (!begins || !ends) {
+        from = max(it.find(p.first, p.rows_per, 1).v - (it.off ? 1 : 0), (int64_t)0) & ~63;
+        to = min(it.find(last, p.rows_per, 1).v + 1, it.items);
+    }
     for (int64_t w = blockIdx.x; w < blocks * it.adapters; w += gridDim.x) {
         const int64_t a = w / blocks, e0 = w % blocks * (4 * T) + 4 * tx;
         floatx4 s = {0, 0, 0, 0};
-        for (int64_t i0 = 0; i0 < it.items; i0 += 64) {
+        uint64_t any = 0;
+        for (int64_t i0 = from; i0 < to; i0 += 64) {
             const int64_t i = i0 + lane, v = it.off ? i + 1 : i;
             int64_t b = 0, e = 0;
             if (i < it.items && it.adapter(v) == a) {
@@ -40,15 +50,18 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
                 e = it.end(v);
             }
             const int mine0 = (int)b / p.rows_per, more = (int)(e - b - 1) / p.rows_per;
-            for (uint64_t m = __ballot(b < e); m; m &= m - 1) {
+            uint64_t m = __ballot(b < e);
+            for (any |= m; m; m &= m - 1) {
                 const int k = __builtin_ctzll(m);
                 const int64_t seg = i0 + k + (it.off ? 1 : 0);
-                const int64_t j0 = __shfl(mine0, k) + seg, j1 = j0 + __shfl(more, k);
+                int64_t j0 = __shfl(mine0, k) + seg, j1 = min(j0 + __shfl(more, k), last) - p.first;
+                j0 = max(j0 - p.first, (int64_t)0);
 #pragma unroll 4
                 for (int64_t j = j0 + ((ty - j0) & (G - 1)); j <= j1; j += G)
                     s += *reinterpret_cast<const floatx4*>(p.part + j * p.slot + e0);
             }
         }
+        if (!any && !begins && !ends) continue;  // (what is carried stays as it is)
         ls[ty][tx] = s;
         __syncthreads();
         if (threadIdx.x < 4 * T) {
@@ -60,10 +73,10 @@ __global__ __launch_bounds__(kLoraThreads) void lora_sum_kernel(LoraItems it, Lo
 #pragma unroll
             for (int q = 0; q < G; ++q) z += ls[q][threadIdx.x >> 2][i];
             if (col < p.c && rank < r) {
-                using S = typename LoraNum<DT>::S;
-                S* d = static_cast<S*>(p.dst) + a * p.c * r + (p.along ? rank * (int64_t)p.c + col : col * r + rank);
-                if constexpr (DT == SPC_F32) *d = __float_as_uint(z);
-                else *d = DT == SPC_BF16 ? f32_to_bf16_bits(z) : f32_to_f16_bits(z);
+                const int64_t d = a * p.c * r + (p.along ? rank * (int64_t)p.c + col : col * r + rank);
+                if (!begins) z += p.carry[d];
+                if (ends) lora_put<DT>(p.dst, d, z);
+                else p.carry[d] = z;
             }
         }
         __syncthreads();
@@ -79,6 +92,8 @@ __global__ __launch_bounds__(kLoraThreads) void lora_add_u_kernel(float* u, int6
         u[i] = s;
     }
 }
+
+inline size_t lora_round_up(size_t floats) { return (floats + 63) / 64 * 64; }
 
 // How a call is split, from its sizes alone.
 struct LoraPlan {
@@ -124,13 +139,18 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
     return q;
 }
 
+// Of the slots of one weight's gradient; more chunks than they hold go in parts of 8192
+// blocks and more.  (65,535 one-row items would fill 4 GB at 1024 columns, rank 16.)
+constexpr int64_t kLoraSlotBytes = 1 << 29;
+
 struct LoraBackPlan {
     bool few;                   // lora_few.hip, u in `shares` of o_per outputs
     int shares, o_per;
     int rows_o, rows_c;         // rows of a chunk
     int64_t chunks_o, chunks_c, blocks_o, blocks_c;
     int64_t slot_o, slot_c;     // floats
-    size_t u, pu, pd;
+    int64_t held_o, held_c;     // chunks that the slots hold
+    size_t u, pu, pd;           // floats, with what is carried from part to part
 };
 
 LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, int64_t c, int64_t o, int64_t r) {
@@ -177,12 +197,19 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
     q.u = (size_t)(q.blocks_o * n * r);
     q.slot_o = lora_slot(o, lora_wave_cols(dt), lora_rank_tiles(r));
     q.slot_c = lora_slot(c, lora_wave_cols(dt), lora_rank_tiles(r));
-    q.pu = (size_t)(q.chunks_o * q.slot_o);
-    q.pd = (size_t)(q.chunks_c * q.slot_c);
+    auto held = [&](int64_t chunks, int64_t slot) {
+        return std::min(chunks, std::max<int64_t>(1, kLoraSlotBytes / (slot * (int64_t)sizeof(float))));
+    };
+    q.held_o = held(q.chunks_o, q.slot_o);
+    q.held_c = held(q.chunks_c, q.slot_c);
+    // (F32 gradients carry their own)
+    auto floats = [&](int64_t held, int64_t chunks, int64_t slot, int64_t width) {
+        return lora_round_up((size_t)(held * slot)) + (held < chunks && dt != SPC_F32 ? (size_t)(adapters * r * width) : 0);
+    };
+    q.pu = floats(q.held_o, q.chunks_o, q.slot_o, o);
+    q.pd = floats(q.held_c, q.chunks_c, q.slot_c, c);
     return q;
 }
-
-inline size_t lora_round_up(size_t floats) { return (floats + 63) / 64 * 64; }
 
 // Widths below eight as the kernels take them: arrays of rows of eight behind the rest
 // of the workspace (`at`; null: their bytes are counted only).  A launch before and one
@@ -433,47 +460,65 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
     narrow.backward(&p, &ddown, &dup, q.n_adapters, q.rank, q.in_features, q.out_features);
     hipError_t err = lora_copy(s, dtype, narrow.in);
     if (err == hipSuccess && b.few) err = lora_few_backward(s, dtype, p, b.o_per, ddown, dup);
-    if (err == hipSuccess && !b.few && n > 0) {
-        const int64_t blocks = std::max(b.blocks_o * b.chunks_o, b.blocks_c * b.chunks_c);
-        if (blocks > INT32_MAX) {
-            set_last_error("%s: more than 2^31 blocks", fn);
-            return SPC_BAD_SHAPE;
-        }
-        const dim3 out((unsigned)(b.blocks_o * b.chunks_o)), in((unsigned)(b.blocks_c * b.chunks_c));
-        p.rows_per = b.rows_o;
-        p.blocks = (int)b.blocks_o;
-        err = dtype == SPC_BF16  ? lora_back_out_bf16(s, p, out)
-              : dtype == SPC_F16 ? lora_back_out_f16(s, p, out)
-                                 : lora_back_out_f32(s, p, out);
-        p.rows_per = b.rows_c;
-        p.blocks = (int)b.blocks_c;
+    if (err == hipSuccess && !b.few) {
+        const int rt = lora_rank_tiles(q.rank);
+        auto carry = [&](float* part, void* dst, int64_t held, int64_t slot) {
+            return dtype == SPC_F32 ? static_cast<float*>(dst) : part + lora_round_up((size_t)(held * slot));
+        };
+        LoraSum d = {p.pd, ddown, carry(p.pd, ddown, b.held_c, b.slot_c), b.slot_c, 0, 0, b.chunks_c, p.c, 1, b.rows_c};
+        LoraSum u = {p.pu, dup, carry(p.pu, dup, b.held_o, b.slot_o), b.slot_o, 0, 0, b.chunks_o, p.o, 0, b.rows_o};
+        auto sum = [&](const LoraSum& first, const LoraSum& second) {
+            auto launch = [&](auto g) {
+                constexpr int G = g.value;
+                const dim3 grid((unsigned)std::min<int64_t>(std::max(first.slot, second.slot) / (1024 / G) * q.n_adapters, 1 << 20),
+                                second.dst ? 2 : 1);
+                if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16, G><<<grid, kLoraThreads, 0, s>>>(p.it, first, second, p.r, rt);
+                else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16, G><<<grid, kLoraThreads, 0, s>>>(p.it, first, second, p.r, rt);
+                else lora_sum_kernel<SPC_F32, G><<<grid, kLoraThreads, 0, s>>>(p.it, first, second, p.r, rt);
+            };
+            // Few slots an adapter are wide work, many are long (us of the whole call, four groups
+            // of slots / sixteen: two slots of 8192 columns rank 64 33 / 48, eight 85 / 98, two of
+            // 16,384 rank 32 36 / 45, 490 of 64 rank 16 41 / 33).
+            if (std::max(b.chunks_o, b.chunks_c) <= 32 * q.n_adapters) launch(std::integral_constant<int, 4>{});
+            else launch(std::integral_constant<int, 16>{});
+            return hipGetLastError();
+        };
+        // A pass over the rows, as many chunks at a time as its slots hold (without sums as
+        // many as a launch may have, 2^32 threads); the sums of a pass of several parts follow
+        // each of them.
+        auto pass = [&](bool out, LoraSum* z) {
+            const int64_t held = z->dst ? (out ? b.held_o : b.held_c) : z->all, blocks = out ? b.blocks_o : b.blocks_c;
+            const int64_t most = std::min<int64_t>(held, std::max<int64_t>(1, (1 << 23) / blocks));
+            for (z->first = 0; z->first < z->all && err == hipSuccess; z->first += z->chunks) {
+                z->chunks = std::min(most, z->all - z->first);
+                p.chunk0 = (int)z->first;
+                p.rows_per = z->rows_per;
+                p.blocks = (int)blocks;
+                const dim3 grid((unsigned)(blocks * z->chunks));
+                if (out)
+                    err = dtype == SPC_BF16  ? lora_back_out_bf16(s, p, grid)
+                          : dtype == SPC_F16 ? lora_back_out_f16(s, p, grid)
+                                             : lora_back_out_f32(s, p, grid);
+                else
+                    err = dtype == SPC_BF16  ? lora_back_in_bf16(s, p, grid)
+                          : dtype == SPC_F16 ? lora_back_in_f16(s, p, grid)
+                                             : lora_back_in_f32(s, p, grid);
+                if (err == hipSuccess && z->dst && z->chunks < z->all) err = sum(*z, LoraSum{});
+            }
+            z->first = 0;
+        };
+        if (p.u || dup) pass(true, &u);
         if (err == hipSuccess && p.u && p.u_parts > lora_shares(lora_rank_tiles(p.r), lora_row_waves(dtype, p.r, p.c))) {
             const int64_t all = n * p.r, blocks = std::min<int64_t>(ceil_div(all, kLoraThreads), 1 << 14);
             lora_add_u_kernel<<<(unsigned)blocks, kLoraThreads, 0, s>>>(p.u, all, p.u_parts);
             err = hipGetLastError();
             p.u_parts = 1;
         }
-        if (err == hipSuccess && p.u)
-            err = dtype == SPC_BF16  ? lora_back_in_bf16(s, p, in)
-                  : dtype == SPC_F16 ? lora_back_in_f16(s, p, in)
-                                     : lora_back_in_f32(s, p, in);
-    }
-    if (err == hipSuccess && !b.few && (ddown || dup)) {
-        const LoraSum d = {p.pd, ddown, b.slot_c, p.c, 1, b.rows_c}, u = {p.pu, dup, b.slot_o, p.o, 0, b.rows_o};
-        const int rt = lora_rank_tiles(q.rank);
-        auto sum = [&](auto g) {
-            constexpr int G = g.value;
-            const dim3 grid((unsigned)std::min<int64_t>(std::max(d.slot, u.slot) / (1024 / G) * q.n_adapters, 1 << 20), 2);
-            if (dtype == SPC_BF16) lora_sum_kernel<SPC_BF16, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
-            else if (dtype == SPC_F16) lora_sum_kernel<SPC_F16, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
-            else lora_sum_kernel<SPC_F32, G><<<grid, kLoraThreads, 0, s>>>(p.it, d, u, p.r, rt);
-        };
-        // Few slots an adapter are wide work, many are long (us of the whole call, four groups
-        // of slots / sixteen: two slots of 8192 columns rank 64 33 / 48, eight 85 / 98, two of
-        // 16,384 rank 32 36 / 45, 490 of 64 rank 16 41 / 33).
-        if (std::max(b.chunks_o, b.chunks_c) <= 32 * q.n_adapters) sum(std::integral_constant<int, 4>{});
-        else sum(std::integral_constant<int, 16>{});
-        err = hipGetLastError();
+        if (p.u) pass(false, &d);
+        // (of passes in one part together)
+        if (d.chunks < d.all) d.dst = nullptr;
+        if (u.chunks < u.all) u.dst = nullptr;
+        if (err == hipSuccess && (d.dst || u.dst)) err = d.dst ? sum(d, u) : sum(u, d);
     }
     if (err == hipSuccess) err = lora_copy(s, dtype, narrow.out);
     return err == hipSuccess ? SPC_OK : hip_status(err, "spc_lora_backward launch");

@@ -125,6 +125,7 @@ struct LoraBackArgs {
     float* pu;         // of dup
     int c, o, r;
     int rows_per, blocks;  // rows of a chunk, blocks along columns
+    int chunk0;            // the launch's first chunk, whose slot is the first
     const int64_t* seed;
     uint32_t drop;
     float factor;
@@ -1048,7 +1049,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
     const LoraItems& it = p.it;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wc = w % WC, wr = w / WC % WR, first = WG == 1 ? 0 : w / (WC * WR) * kLoraRows, rank0 = 16 * RW * wr, j0 = NR * wr;
-    const int chunk = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks;
+    const int slot_at = blockIdx.x / p.blocks, chunk = p.chunk0 + slot_at, block = blockIdx.x % p.blocks;
     const int block0 = block * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.o;
     static_assert(sizeof(tile) >= (WG - 1) * WC * WR * 64 * V * RW * 16, "the sums meet there");
@@ -1170,7 +1171,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_out_kernel(LoraBack
         lora_gather<WC * WR, WG>(acc, reinterpret_cast<floatx4*>(tile));
     }
     if (p.pu && col0 < p.o && first == 0) {
-        float* slot = p.pu + chunk * lora_slot(p.o, CW, RW * WR);
+        float* slot = p.pu + slot_at * lora_slot(p.o, CW, RW * WR);
         lora_flush<DT, RW>(acc, slot, col0 / CW, RW * WR, RW * wr, s);
         lora_flush_plain<DT, RW>(acc, slot, col0 / CW, RW * WR, RW * wr, s, r0, r1, p.o, p.r,
                                  [&](int64_t row, int col, int rank) {
@@ -1209,7 +1210,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wc = w % WC, wr = w / WC % WR, wg = WG == 1 ? 0 : w / (WC * WR), rank0 = 16 * RW * wr, j0 = NR * wr;
     const int q0 = WR == 1 ? 0 : WR == 2 ? 2 * wr : wr / 2 * 2, i0 = WR == 4 ? wr & 1 : 0;
-    const int chunk = blockIdx.x / p.blocks, block0 = blockIdx.x % p.blocks * CB, col0 = block0 + wc * CW;
+    const int slot_at = blockIdx.x / p.blocks, chunk = p.chunk0 + slot_at, block0 = blockIdx.x % p.blocks * CB, col0 = block0 + wc * CW;
     const bool edge = block0 + CB > p.c;
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
     floatx4 acc[V][RW] = {};
@@ -1392,7 +1393,7 @@ __global__ __launch_bounds__(kLoraThreads, 2) void lora_back_in_kernel(LoraBackA
     }
     if (WG > 1 && p.pd) lora_gather<WC * WR, WG>(acc, sums);
     if (p.pd && col0 < p.c && wg == 0) {
-        float* slot = p.pd + chunk * lora_slot(p.c, CW, RT);
+        float* slot = p.pd + slot_at * lora_slot(p.c, CW, RT);
         const float f = DROP ? p.factor : 1.0f;
         lora_flush<DT, RW>(acc, slot, col0 / CW, RT, RW * wr, f);
         lora_flush_plain<DT, RW>(acc, slot, col0 / CW, RT, RW * wr, f, r0, r1, p.c, p.r,
