@@ -45,7 +45,9 @@ __host__ __device__ inline int few_chunks(int r) {
     return c;
 }
 
-// u[share][row] = s_a sum over the share's outputs of dy[row] up_a.
+// u[share][row] = s_a sum over the share's outputs of dy[row] up_a; of a row without an
+// adapter dx, the base, a share of its columns.  (Left to few_columns_kernel, whose block of
+// 64 columns would gather such rows 32 at a time, 512 of them were 169 us of 1024 columns.)
 template <int DT>
 __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int o_per) {
     using N = LoraNum<DT>;
@@ -54,7 +56,11 @@ __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int
     __shared__ float red[4][kLoraMaxRank];
     const LoraItems& it = p.it;
     const int64_t row = blockIdx.x, a = it.find(row, 1, 0).adapter;
-    if (a < 0) return;
+    if (a < 0) {
+        const int per = (p.c / 8 / (int)gridDim.y + 1) * 8, c0 = min((int)blockIdx.y * per, p.c);
+        if (p.dx) lora_pass<DT>(p.dx, p.c, p.base, p.bs, row, 1, c0, min(c0 + per, p.c));
+        return;
+    }
     const int chunks = few_chunks<DT>(p.r), lines = kLoraThreads / chunks, t = threadIdx.x;
     const int j = t % chunks * V, o1 = min((int)(blockIdx.y + 1) * o_per, p.o);
     const S* up = static_cast<const S*>(p.up);
@@ -91,8 +97,8 @@ __global__ __launch_bounds__(kLoraThreads) void few_u_kernel(LoraBackArgs p, int
     }
 }
 
-// Blocks along x: 64 columns of x (dx, ddown), then of dy (dup); along y: adapters,
-// and after the last the rows without one.  The adapter's rows are gathered from
+// Blocks along x: 64 columns of x (dx, ddown), then of dy (dup); along y: adapters.
+// The adapter's rows are gathered from
 // the segments 32 at a time, so that one wait serves as many.  A wave loads eight
 // of them and holds RJ ranks' sums over all.
 template <int DT, int RJ, bool DROP>
@@ -110,11 +116,9 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
     const int64_t stride = in ? p.xs : p.dys;
     void* grad = in ? ddown : dup;
     const DropKey key = DROP ? drop_key(p.seed) : DropKey{};
-    for (int64_t a = blockIdx.y; a <= it.adapters; a += gridDim.y) {
-        const bool none = a == it.adapters;
-        if (none && !dx) continue;
+    for (int64_t a = blockIdx.y; a < it.adapters; a += gridDim.y) {
         float acc[RJ] = {}, wt[RJ] = {};
-        if (dx && !none)
+        if (dx)
 #pragma unroll
             for (int i = 0; i < RJ; ++i)
                 if (j0 + i < p.r) wt[i] = lora_get<DT>(p.down, (a * p.r + j0 + i) * p.c + at);
@@ -139,7 +143,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
                     if (v0 >= it.segments()) break;
                     const int64_t v = v0 + lane;
                     b = e = 0;
-                    if (v < it.segments() && it.adapter(v) == (none ? -1 : a)) {
+                    if (v < it.segments() && it.adapter(v) == a) {
                         b = (int)it.begin(v);
                         e = (int)it.end(v);
                     }
@@ -155,43 +159,39 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
             for (int t = 0; t < 8; ++t) {
                 rows[t] = list[min(8 * w + t, count - 1)];
                 bv[t] = dx && p.base ? lora_get<DT>(p.base, rows[t] * p.bs + at) : 0.0f;
-                xv[t] = grad && !none ? lora_get<DT>(x, rows[t] * stride + at) : 0.0f;
+                xv[t] = grad ? lora_get<DT>(x, rows[t] * stride + at) : 0.0f;
             }
-            if (!none) {
-                for (int i = threadIdx.x; i < kFewRows * 4 * RJ; i += kLoraThreads) {
-                    const int t = i / (4 * RJ), j = i % (4 * RJ);
-                    float z = 0.0f;
-                    if (t < count && j < p.r) {
-                        const int64_t f = (int64_t)list[t] * p.r + j;
-                        if (in) for (int q = 0; q < p.u_parts; ++q) z += p.u[(int64_t)q * it.n * p.r + f];
-                        else z = p.hidden[f];
-                    }
-                    us[t][j] = z;
+            for (int i = threadIdx.x; i < kFewRows * 4 * RJ; i += kLoraThreads) {
+                const int t = i / (4 * RJ), j = i % (4 * RJ);
+                float z = 0.0f;
+                if (t < count && j < p.r) {
+                    const int64_t f = (int64_t)list[t] * p.r + j;
+                    if (in) for (int q = 0; q < p.u_parts; ++q) z += p.u[(int64_t)q * it.n * p.r + f];
+                    else z = p.hidden[f];
                 }
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    if (8 * w + t >= count) continue;
-                    const bool k = !drop || lora_keeps(lora_ones(key, p.drop, rows[t], at, p.c), at);
-                    kept |= (uint32_t)k << t;
-                    xs[8 * w + t][lane] = k ? xv[t] : 0.0f;
-                }
+                us[t][j] = z;
             }
-            __syncthreads();  // (for rows without an adapter too: the list has been read)
-            if (!none) {
-                for (int t = 0; t < count; ++t) {
-                    const float xt = xs[t][lane];
-                    float d = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < RJ; ++i) {
-                        const float u = us[t][j0 + i];
-                        acc[i] += u * xt;
-                        d += u * wt[i];
-                    }
-                    if (dx) part[w][t][lane] = d;
+            for (int t = 0; t < 8; ++t) {
+                if (8 * w + t >= count) continue;
+                const bool k = !drop || lora_keeps(lora_ones(key, p.drop, rows[t], at, p.c), at);
+                kept |= (uint32_t)k << t;
+                xs[8 * w + t][lane] = k ? xv[t] : 0.0f;
+            }
+            __syncthreads();
+            for (int t = 0; t < count; ++t) {
+                const float xt = xs[t][lane];
+                float d = 0.0f;
+#pragma unroll
+                for (int i = 0; i < RJ; ++i) {
+                    const float u = us[t][j0 + i];
+                    acc[i] += u * xt;
+                    d += u * wt[i];
                 }
+                if (dx) part[w][t][lane] = d;
             }
             if (!dx) continue;
-            if (!none) __syncthreads();
+            __syncthreads();
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const int q = 8 * w + t;
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kLoraThreads) void few_columns_kernel(LoraBackArgs 
             }
         }
         __syncthreads();
-        if (none || !grad || !on) continue;
+        if (!grad || !on) continue;
         const float f = in ? (drop ? p.factor : 1.0f) : p.scale ? p.scale[a] : 1.0f;
         if (in) {
 #pragma unroll
@@ -230,7 +230,8 @@ void few_backward(hipStream_t s, const LoraBackArgs& p, int o_per, void* ddown, 
     if (p.it.n > 0 && p.u) few_u_kernel<DT><<<dim3((unsigned)p.it.n, (unsigned)p.u_parts), kLoraThreads, 0, s>>>(p, o_per);
     const int in_blocks = p.dx || ddown ? (int)ceil_div(p.c, 64) : 0, out_blocks = dup ? (int)ceil_div(p.o, 64) : 0;
     const int64_t x = in_blocks + out_blocks;
-    const dim3 grid((unsigned)x, (unsigned)std::min<int64_t>(p.it.adapters + 1, std::max<int64_t>(1, (1 << 18) / x)));
+    // (at most 65,535 along y, as the adapters)
+    const dim3 grid((unsigned)x, (unsigned)std::min<int64_t>(p.it.adapters, std::max<int64_t>(1, (1 << 18) / x)));
     const int rt = lora_rank_tiles(p.r);
     if (rt == 1) few_columns<DT, 4>(s, p, grid, in_blocks, ddown, dup);
     else if (rt == 2) few_columns<DT, 8>(s, p, grid, in_blocks, ddown, dup);
