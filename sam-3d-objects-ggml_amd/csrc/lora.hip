@@ -156,14 +156,16 @@ struct LoraBackPlan {
 LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, int64_t c, int64_t o, int64_t r) {
     LoraBackPlan q{};
     // Tiles of 32 rows of one item cost some 0.2 us an item, however short, and the sums
-    // behind them; gathered, an adapter's rows wait one after the other, some 9 us for each
-    // 32 of them (us, gathered / tiles, 1024 -> 1024 rank 16 bf16: 32 rows of one item 16 /
-    // 17, 64 of one 22 / 17, 64 one-row items and four adapters 20 / 26; 512 rows of 256
-    // items and 8 adapters 40 / 79, of 64 and 8 32 / 26, of 16 and 8 35 / 20, of 16 and 2 59
-    // / 21; 1024 of 512 and 8 64 / 129, of 64 and 8 45 / 26; 8192 of 2048 and 8 372 / 431, of
-    // 1024 and 8 343 / 226; 4096 one-row items of one adapter 1946 / 1266, of eight 320 / 905,
-    // of 1024 1470 / 2643).
-    q.few = n <= std::min(32 * items, std::min(items, adapters) * (32 + items / 2));
+    // behind them; gathered, an adapter's rows wait one after the other, some 14 us for each
+    // 32 of them.  How many those are is the device's to know, so that the rule stays where
+    // rows spread evenly over the adapters gain and all rows of one adapter lose less than
+    // twice (us, gathered / tiles, even; gathered / tiles, all of one; 1024 -> 1024 rank 16 bf16:
+    // 64 one-row items of 4 adapters 22 / 31; 42 / 39. 256 of 8 30 / 83; 130 / 112. 256 items of 2
+    // rows and 8 36 / 82; 178 / 113. 1024 of 2 and 64 79 / 198; 677 / 342. 4096 one-row items of 8
+    // 296 / 906; 1946 / 1501, of 1024 1333 / 2306; 2043 / 2202, and of one adapter 1940 / 1380.
+    // Left to tiles: 256 of 4 rows and 32 38 / 69; 279 / 105. 64 of 30 and 64 50 / 43; 401 / 49. 2048 of
+    // 4 and 8 350 / 459; 2404 / 749. 1024 of 8 and 1024 666 / 667; 2152 / 613. 16 of 32 and 8 27 / 24).
+    q.few = n <= std::min({32 * items, std::min(items, adapters) * (32 + items / 2), 180 + 2 * items});
     if (q.few) {
         int64_t chunks = 1;
         while (chunks * (dt == SPC_F32 ? 4 : 8) < r) chunks *= 2;

@@ -17,3 +17,13 @@ def test_backward_workspace_does_not_grow_with_the_items(spc, n, items, k, c, o,
         sums = 4 * k * r * (c + o)
         need = L.spc_lora_workspace_bytes(dt, n, items, k, c, o, r, 1)
         assert 0 < need <= u + 2 * (1 << 29) + sums + 4096
+
+
+@pytest.mark.parametrize("n,items,k", [(1920, 64, 64), (1024, 64, 64), (8192, 1024, 1024), (1024, 256, 32)])
+def test_route_does_not_trust_the_bank(spc, n, items, k):
+    """Rows that may all be one adapter's (some 14 us for each 32 of them, one after the
+    other, where they are gathered) take the tiles, whose workspace has the sums'
+    slots, whatever the number of adapters in the bank."""
+    L, nat = spc._native.lib(), spc._native
+    need = [L.spc_lora_workspace_bytes(nat.BF16, n, items, a, 1024, 1024, 16, 1) for a in (1, k)]
+    assert need[0] == need[1] > 4 * 2 * items * 1024 * 16
