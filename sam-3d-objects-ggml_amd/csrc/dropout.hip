@@ -34,8 +34,8 @@ template <int DT, bool RES>
 __global__ __launch_bounds__(kDropThreads) void drop_kernel(DropArgs p) {
     using R = Row8<DT>;
     using S = typename R::S;
-    // (2^28 threads at most: more groups than 32 bits count are one row's)
-    const uint32_t first = blockIdx.x * kDropThreads + threadIdx.x, groups = (uint32_t)min(p.groups, (int64_t)UINT32_MAX);
+    // (2^28 threads at most, and as many groups a row: spc_dropout's largest width)
+    const uint32_t first = blockIdx.x * kDropThreads + threadIdx.x, groups = (uint32_t)p.groups;
     const DropKey key = p.drop ? drop_key(p.seed) : DropKey{};
     int64_t row = first / groups, g = first % groups;
     while (row < p.n) {
