@@ -814,7 +814,12 @@ __global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void
     }
     if constexpr (MODE != kLoraShrink) {
         __syncthreads();
-        lora_expand<DT, RT, MT>(p, t, c0, c1, hid);
+        // (f16 tiles of 64 rows by halves: their parts and the weights' spill together, 30,000 x
+        // 1024 rank 64 66 us so, 75 at once; bf16's fit, rank 33 68 and 64)
+        constexpr int E = MT == 4 && DT == SPC_F16 ? 2 : MT;
+        for (int i = 0; i < MT; i += E)
+            if (16 * i < t.m)
+                lora_expand<DT, RT, E>(p, LoraTile{t.row0 + 16 * i, t.a, min(t.m - 16 * i, 16 * E)}, c0, c1, hid + 16 * i * P);
     }
 }
 
