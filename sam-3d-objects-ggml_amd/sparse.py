@@ -951,22 +951,24 @@ class Q4Linear(nn.Linear):
     add_adapters puts low-rank adapters beside the weight, whichever it is
     (spc_lora); a call names each item's, forward(input, adapters): int32
     [input.shape[0]] on the input's device, an item being input[i] (for
-    SparseLinear, a batch item's rows), -1 for none.  Without that argument
-    the Linear is what it is without adapters."""
+    SparseLinear, a batch item's rows), -1 for none.  At most 65,535 items;
+    one adapter for all rows of an input [n, in_features] is input[None] with
+    one, which is also the faster call.  Without that argument the Linear is
+    what it is without adapters."""
 
     _q4 = None          # blocks, uint8 [out_features, in_features / 32 * 18]
 
     def add_adapters(self, count: int, rank: int, alpha: Optional[float] = None,
                      dropout: float = 0.0) -> None:
-        """`count` adapters of the given rank (at most 128), in place of any there
+        """`count` adapters (at most 65,535) of the given rank (at most 128), in place of any there
         are: parameters adapter_down [count, rank, in_features], drawn as a Linear's
         weight, and adapter_up [count, out_features, rank], zeros, so that they change
         nothing yet, of the weight's dtype and device; a buffer adapter_scale [count],
         alpha / rank (alpha: rank if not given), F32 in a module of any dtype.  All three are part of the state dict.
         dropout: of the rows in front of the adapters, in training.  The other
         parameters stay trainable or frozen as they are."""
-        if count < 1 or not 1 <= rank <= 128:
-            raise ValueError(f"adapters need a count of at least 1 and a rank of 1 to 128, got {count} "
+        if not 1 <= count <= 65535 or not 1 <= rank <= 128:
+            raise ValueError(f"adapters need a count of 1 to 65535 and a rank of 1 to 128, got {count} "
                              f"and {rank}")
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f"dropout must lie in [0, 1], got {dropout}")

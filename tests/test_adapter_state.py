@@ -30,3 +30,12 @@ def test_scale_on_meta(spc):
     assert lin.adapter_scale.is_meta and lin.adapter_scale.dtype == torch.float32
     lin.to_empty(device="cpu")
     assert lin.adapter_scale.dtype == torch.float32 and lin.adapter_down.dtype == torch.float16
+
+
+def test_more_adapters_than_a_call_takes_are_refused(spc):
+    """When they are added, not by the first call; what was there stays."""
+    lin = spc.sparse.Q4Linear(8, 8)
+    lin.add_adapters(65_535, 1)
+    with pytest.raises(ValueError, match="65535"):
+        lin.add_adapters(65_536, 1)
+    assert lin.adapter_down.shape == (65_535, 1, 8)
