@@ -996,7 +996,7 @@ __device__ __forceinline__ void lora_flush_plain(const floatx4 (&acc)[LoraNum<DT
             const int col = 16 * V * tile + V * (4 * (lane >> 4) + i) + k % V;
             if (z[i] == z[i] || col >= c || rank >= r) continue;
             float s = 0.0f;
-            for (int64_t row = r0; row < r1; ++row) s += term(row, col, rank);
+            for (int64_t row = r0; row < r1 && s == s; ++row) s += term(row, col, rank);
             z[i] = f * s;
         }
         *reinterpret_cast<floatx4*>(q + k * 256) = z;
