@@ -749,7 +749,7 @@ typedef struct {
  * rows x_stride and base_stride elements apart, y contiguous (may be base where
  * that is).  hidden: f32 [n, rank], dropout(x) down_a^T (zeros for rows without
  * an adapter), what the gradient reads, or NULL.  Sums are F32, the hidden rows
- * are kept in F32; one rounding to dtype.  n up to 2^27, rank 1 to 128, in_features and
+ * are kept in F32 and enter y with all their bits; one rounding to dtype.  n up to 2^27, rank 1 to 128, in_features and
  * out_features to 2^24, n_items and n_adapters to 65535.  workspace:
  * spc_lora_workspace_bytes (which may be none), 16-byte aligned. */
 size_t spc_lora_workspace_bytes(int dtype, int64_t n, int64_t n_items, int64_t n_adapters,
@@ -766,7 +766,10 @@ int spc_lora(spc_stream_t stream, int dtype, const void* x, int64_t x_stride, in
  * down and up (zeros for adapters without rows), each NULL if not wanted
  * (hidden is read for dup only).  Rows without an adapter add to nothing.  Sums
  * are F32 in a fixed order: equal calls give equal bits.  workspace:
- * spc_lora_workspace_bytes with backward 1, 16-byte aligned. */
+ * spc_lora_workspace_bytes with backward 1, 16-byte aligned: shares of dy up_a in
+ * F32 (at most out_features / 128 of them, 64 for F32 rows, rounded up) and up to
+ * 512 MB of sums for each of ddown and dup (if those hold a part of the items at a
+ * time, F32 copies of ddown and dup too). */
 int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy_stride,
                       const void* x, int64_t x_stride, const float* hidden, int64_t n,
                       const spc_lora_params* params, const void* dx_base, int64_t dx_base_stride,

@@ -106,28 +106,29 @@ LoraPlan lora_plan(int dt, int64_t n, int64_t items, int64_t c, int64_t o, int64
     LoraPlan q{};
     const int step = dt == SPC_F32 ? 16 : 32;
     // Tiles of 32 rows halve the adapters' traffic, tiles of 16 give twice the blocks
-    // (us in a graph, 1024 -> 1024 rank 16 bf16, 32 / 16: 4096 rows 15.2 / 9.5, 16,384
-    // 21.3 / 22.3; 30,000 rank 32 38.6 / 45.2).
+    // (us in a graph, 1024 -> 1024 rank 16 bf16, 32 / 16: 4096 rows 14.8 / 10.9, 16,384
+    // 22.6 / 25.4; 30,000 rank 32 38.5 / 54.1).
     q.mt = n / items >= 32 && n >= 384 * 32 ? kLoraRowTiles : 1;
     // Ranks 33 to 64, whose adapters are most of a tile's traffic and whose sums still fit LDS
-    // twice (us, tiles of 64 / 32: 1024 -> 1024 rank 64 bf16 20,000 rows 41 / 41, 30,000 42 / 53,
-    // 50,000 81 / 97; 16,000 of 2048 -> 512 59 / 36, 25,000 49 / 63; f32 30,000 137 / 144).
+    // twice (us, tiles of 64 / 32: 1024 -> 1024 rank 64 bf16 20,000 rows 46 / 42, 30,000 48 / 55,
+    // 50,000 97 / 90; 16,000 of 2048 -> 512 33 / 37, 25,000 51 / 63; f16 20,000 56 / 52, 30,000 60 / 62,
+    // 50,000 106 / 105; f32 30,000 136 / 142).
     if (lora_rank_tiles(r) == 4 && n / items >= 64 && n >= 384 * 64) q.mt = 2 * kLoraRowTiles;
     const int64_t rows = 16 * q.mt, busy = std::max<int64_t>(1, std::max(ceil_div(n, rows), std::min(items, n)));
     q.tiles = n / rows + items + 3;
     // One kernel, each of whose column blocks forms the tile's hidden rows again, or two:
     // one where the tiles fill the device or are little work (us, one / two: 1024 x 1024 ->
-    // 1024 rank 16 8.0 / 9.0, 4 items 1024 -> 4096 rank 64 8.2 / 8.4, 1024 x 4096 -> 1024
-    // rank 32 27 / 18, 8 items 8192 -> 16,384 rank 64 f16 69 / 12.3).
+    // 1024 rank 16 8.1 / 8.5, 4 items 1024 -> 4096 rank 64 9.0 / 9.1, 1024 x 4096 -> 1024
+    // rank 32 27 / 14, 8 items 8192 -> 16,384 rank 64 f16 70 / 13.2).
     q.mode = q.mt > 1 || busy >= 256 || c * (16 + r) * float_size(dt) <= 200000 ? kLoraFused : kLoraShrink;
     auto share = [&](int64_t width, int64_t unit, int64_t want) {  // columns a block
         const int64_t blocks = std::min(std::max<int64_t>(want / busy, 1), ceil_div(width, unit));
         return ceil_div(ceil_div(width, blocks), unit) * unit;
     };
     // Blocks that share a tile, each of 8 steps of columns or more (us in a graph): by 128 /
-    // 256 / 384 / 512 / 1024 of them 64 one-row requests 1024 -> 4096 rank 16 11.4 / 8.8 / 8.4
-    // / 8.7 / 10.4; in two kernels, 256 / 512 / 1024, 8 of 8192 -> 16,384 rank 64 13.8 / 12.5 /
-    // 12.5; one row of 1024 -> 2048, 8 steps / 16, 4.8 / 5.5.
+    // 256 / 384 / 512 / 1024 of them 64 one-row requests 1024 -> 4096 rank 16 12.5 / 10.2 / 9.2
+    // / 9.3 / 10.5; in two kernels, 256 / 512 / 1024, 8 of 8192 -> 16,384 rank 64 14.7 / 13.3 /
+    // 13.2; one row of 1024 -> 2048, 8 steps / 16, 5.1 / 5.8.
     q.splits = 1;
     q.k_per = (int)c;
     if (q.mode == kLoraShrink) {
@@ -182,8 +183,8 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
     q.blocks_c = ceil_div(c, (int64_t)lora_col_waves(dt, r, c) * lora_wave_cols(dt));
     // Some two blocks a CU: the registers hold no more of them at once, and every further
     // chunk is a slot to write and add (us by 256 / 384 / 512 / 640 / 1024 blocks: 30,000 x 1024
-    // rank 16 bf16 67 / 63 / 59 / 71 / 70, rank 64 158 / 132 / 112 / 111 / 130, 21,766 x 768 rank 8
-    // f32 70 / 72 / 65 / 64 / 73).
+    // rank 16 bf16 without dx_base 73 / 66 / 60 / 74 / 77, rank 64 170 / 142 / 120 / 138 / 138, 21,766 x
+    // 768 rank 8 f32 71 / 73 / 65 / 65 / 73).
     // A block's chunk is of one item, whose last is shorter: some chunks fewer, so that those
     // do not make a second round.
     auto rows = [&](int64_t blocks, int64_t width) {
@@ -216,8 +217,8 @@ LoraBackPlan lora_back_plan(int dt, int64_t n, int64_t items, int64_t adapters, 
 // Widths below eight as the kernels take them: arrays of rows of eight behind the rest
 // of the workspace (`at`; null: their bytes are counted only).  A launch before and one
 // after, against plain sums over narrow rows (us of rank 8 bf16, so / plain: 21,766 x
-// 1024 to 4 17 / 174 forward, 49 / 12,276 backward; 100,000 x 4 to 64 20 / 175, 70 /
-// 56,246; 333 x 6 to 32 7.6 / 7.3, 21 / 131).
+// 1024 to 4 19 / 174 forward, 45 / 12,276 backward; 100,000 x 4 to 64 21 / 175, 41 /
+// 56,246; 333 x 6 to 32 7.5 / 7.3, 23 / 131).
 struct LoraNarrow {
     int dt;
     char* at;
@@ -479,8 +480,8 @@ int spc_lora_backward(spc_stream_t stream, int dtype, const void* dy, int64_t dy
                 else lora_sum_kernel<SPC_F32, G><<<grid, kLoraThreads, 0, s>>>(p.it, first, second, p.r, rt);
             };
             // Few slots an adapter are wide work, many are long (us of the whole call, four groups
-            // of slots / sixteen: two slots of 8192 columns rank 64 33 / 48, eight 85 / 98, two of
-            // 16,384 rank 32 36 / 45, 490 of 64 rank 16 41 / 33).
+            // of slots / sixteen: 40 x 8192 to 8192 rank 64 34 / 51, 200 of four items 50 / 77, 40 x
+            // 16,384 to 16,384 rank 32 34 / 51, 30,000 x 64 to 64 rank 16 27 / 23).
             if (std::max(b.chunks_o, b.chunks_c) <= 32 * q.n_adapters) launch(std::integral_constant<int, 4>{});
             else launch(std::integral_constant<int, 16>{});
             return hipGetLastError();

@@ -6,15 +6,19 @@
 //   u = s_a dy up_a,    dx = dx_base + d(u down_a)
 //   ddown_a = sum over a's rows of u^T d(x),  dup_a = s_a sum of dy^T h
 //
-// All of it is bound by the rows' bytes (few rows: the adapters'), so every pass
+// Up to rank 32 it is bound by the rows' bytes (few rows: the adapters'), so every pass
 // reads its rows once and the products run on the matrix instructions, which
 // are far from their limit (rank 16: some 50 operations a byte at most).  BF16,
-// inputs that change: y of 62,710 x 1024, rank 16, with a base 78 us (4.9 TB/s; a
-// large copy 5.15); its gradients' pass over dy 37 us (132 MB and 24 of u and sums,
-// 4.3 TB/s), over x 89 (401 MB, 4.5 TB/s; the dropout's mask is 8 of them), the sums 9.
-// Larger ranks cost the adapters' way through L2 for each tile of rows (30,000 x 1024, rank
-// 16 / 64 / 128: 34 / 42 / 81 us, gradients 67 / 121 / 180), rows of 16-bit elements at
-// odd addresses twice the time (1023 to 1021: 74, 105).
+// inputs that change: y of 62,710 x 1024, rank 16, with a base 79 us (4.8 TB/s; a
+// large copy 5.15); its gradients' pass over dy 38 us (132 MB and 24 of u and sums,
+// 4.1 TB/s), over x 100 by itself (401 MB, 4.0 TB/s; the dropout's mask is 8 of them), the
+// sums 9; the call 133.
+// Larger ranks cost the adapters' way through L2 for each tile of rows and, in the gradients,
+// where a block holds 128 columns (64 of F32), u's shares, their sum and the hidden rows by
+// every block: more than the rows themselves.  30,000 x 1024 with a base, kernels alone, rank 16
+// / 64 / 128: 41 / 57 / 101 us, gradients 71 / 146 / 223 (floors 36, 48 to 51); rank 100 F16 134
+// and 315; F32 rank 128 258 and 504 (72 and 99).  Rows of 16-bit elements at odd addresses
+// take twice the time (1023 to 1021: 79, 110).
 //
 // 16-bit rows meet 16-bit weights exactly (F32 sums).  h and u stay F32, and
 // meet 16-bit operands as three bf16 parts of eight bits each, whose sum is the
@@ -166,9 +170,9 @@ inline int lora_rank_waves(int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 inline int lora_wave_cols(int dt) { return dt == SPC_F32 ? 64 : 128; }
 // and the waves along columns: half of them where the last block of all would use no
 // more, one for rows no wider than its own, the others along rows (us of the gradients, so /
-// all along columns, rank 16 bf16: 200,000 x 64 to 64 60 / 123, 53,333 x 576 77 / 85, 40,000 x
-// 768 71 / 74, 27,927 x 1100 86 / 90; where the last block uses more, 34,133 x 900 88 / 84,
-// 21,818 x 1408 75 / 76)
+// all along columns, rank 16 bf16: 200,000 x 64 to 64 54 / 112, 53,333 x 576 68 / 75, 40,000 x
+// 768 64 / 66, 27,927 x 1100 74 / 78; where the last block would use more, all along columns
+// and half of them: 34,133 x 900 84 / 88, 21,818 x 1408 76 / 75)
 inline int lora_col_waves(int dt, int64_t r, int64_t width) {
     const int64_t tiles = (width + lora_wave_cols(dt) - 1) / lora_wave_cols(dt);
     int w = 4 / lora_rank_waves(r);
@@ -737,7 +741,7 @@ __device__ __forceinline__ void lora_pass(void* y, int64_t ys, const void* base,
 
 // Blocks a CU: two, or as many more as fit; one for F32 rows and the largest ranks, whose
 // registers for two cost more than the second gives (30,000 x 1024 rank 128, one / two:
-// 235 / 256 us; BF16 104 / 81).
+// 235 / 256 us; BF16's two take 84).
 constexpr int lora_forward_blocks(int dt, int rt, int mt) { return dt == SPC_F32 && rt == 8 && mt > 1 ? 1 : 2; }
 
 // A block takes a tile of 16 MT rows of one segment (tile numbers begin at
@@ -748,7 +752,7 @@ constexpr int lora_forward_blocks(int dt, int rt, int mt) { return dt == SPC_F32
 //
 // Where all tiles run at once, a tile's way through both products is what there is to
 // wait for: 11,774 x 2048 to 1024, rank 32 BF16 33 us for 98 MB, one of them the
-// dropout's mask; one row of 1024 to 2048 4.8 us in a graph, where an empty kernel is
+// dropout's mask; one row of 1024 to 2048 4.9 us in a graph, where an empty kernel is
 // some 2.5.
 template <int DT, int RT, int MT, int MODE, bool DROP>
 __global__ __launch_bounds__(kLoraThreads, lora_forward_blocks(DT, RT, MT)) void lora_forward_kernel(LoraArgs p) {
