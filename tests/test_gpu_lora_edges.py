@@ -53,18 +53,38 @@ def test_sums_in_parts(spc, dev, dt, n, rows, k, c, o, r, p):
         assert torch.equal(part[i], whole[i])
 
 
+def test_sums_in_parts_captured(spc, dev):
+    """Replays on new rows, with eager calls of another size between."""
+    nat = spc._native
+    q = Case(dev, "bf16", 2200, 1024, 1030, 100, k=2, offsets=list(range(0, 2201, 2)), adapters=[i % 3 - 1 for i in range(1100)], p=0.1)
+    h = torch.randn(2200, 100, device=dev)
+    run = lambda: nat.lora_backward(q.dy, q.x, h, q.down, q.up, q.dx_base, **q.kw)  # noqa: E731
+    run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for i in range(3):
+        q.x.copy_(torch.randn(2200, 1024))
+        q.kw["seed"].copy_(torch.tensor([i, 7]))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, run()))
+        nat.lora_backward(q.dy[:9], q.x[:9], h[:9], q.down[:1], q.up[:1])
+
+
 MOST = 65_535   # of items and of adapters
 
 
 @pytest.mark.parametrize("k,rows,name", [(MOST, 1, "each its own"), (MOST, 1, "the last"), (MOST, 1, "none"), (1, 2, "the last"),
                                          (3, 3, "in turn")])
+@pytest.mark.parametrize("c,o", [(8, 9), (4, 3)])
 @pytest.mark.parametrize("dt", list(DT))
-def test_largest_counts_of_items_and_adapters(spc, dev, dt, k, rows, name):
+def test_largest_counts_of_items_and_adapters(spc, dev, dt, c, o, k, rows, name):
     """Whole numbers, whose sums are exact (131,070 rows of at most 72 in one adapter's),
     so that results are the formulas', rounded once."""
     nat, t, g = spc._native, DT[dt], torch.Generator().manual_seed(k + rows)
     ints = lambda m, *s: torch.randint(-m, m + 1, s, generator=g).double()  # noqa: E731
-    n, c, o, r = MOST * rows + 5, 8, 9, 1
+    n, r = MOST * rows + 5, 1
     i = torch.arange(MOST)
     ids = {"each its own": torch.where(i % 10 == 3, -1, i * 7919 % MOST), "the last": torch.full((MOST,), k - 1),
            "none": torch.full((MOST,), -1), "in turn": i % 4}[name]
